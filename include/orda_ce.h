@@ -324,6 +324,129 @@ int orda_gemm(int32_t dtype, int32_t a_mn, int32_t b_mn, int64_t M, int64_t N, i
               int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, int32_t splits, void* workspace,
               size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * The projection, the gated feed-forward block and the norm of gradients: what
+ * stands in front of the loss in a student and behind its backward pass.  No
+ * counterpart in the reference, whose models call torch for them.  The
+ * conventions above hold: caller-owned memory, asynchronous, no allocation, no
+ * host synchronisation; every call may be captured into a graph. */
+
+/* Activations.  GELU is x Phi(x); GELU_TANH its tanh approximation. */
+enum orda_activation {
+  ORDA_ACT_NONE = 0,
+  ORDA_ACT_RELU = 1,
+  ORDA_ACT_GELU = 2,
+  ORDA_ACT_GELU_TANH = 3,
+  ORDA_ACT_SILU = 4,
+  ORDA_ACT_SIGMOID = 5
+};
+
+/* y = act(x W^T + bias) + residual.  Rows of x, weight and their gradients are
+ * ld* elements apart, a multiple of 8 (fp32: 4), and start 16-byte aligned; x
+ * and weight are zero from in_features up to the next such multiple, and their
+ * gradients are written up to it.  bias, residual, y and grad_output may have
+ * any alignment. */
+typedef struct orda_linear {
+  int32_t abi_version;   /* must equal ORDA_ABI_VERSION                      */
+  int32_t dtype;         /* enum orda_dtype, of every tensor                 */
+  int32_t activation;    /* enum orda_activation                             */
+  int32_t reserved;      /* 0                                                */
+  int64_t tokens;        /* rows of x, > 0                                   */
+  int64_t in_features;   /* columns of x                                     */
+  int64_t out_features;  /* rows of weight                                   */
+  int64_t ldx, ldw;      /* row pitches of x and weight in elements          */
+  int64_t ldr;           /* of residual                                      */
+  int64_t ldgx, ldgw;    /* of grad_x and grad_weight (backward only)        */
+} orda_linear_t;
+
+/* Elements between the rows of the pre-activations that orda_linear_forward
+ * keeps for the backward pass ([tokens x this], in dtype). */
+int64_t orda_linear_saved_pitch(const orda_linear_t* p);
+
+/* Scratch bytes of the forward (backward = 0) or the backward call (1). */
+size_t orda_linear_workspace_bytes(const orda_linear_t* p, int32_t backward);
+
+/* Writes y [tokens x out_features], dense.  bias [out_features] and residual
+ * may be NULL; z (saved pre-activations, 16-byte aligned) is written when not
+ * NULL. */
+int orda_linear_forward(const orda_linear_t* p, const void* x, const void* weight, const void* bias,
+                        const void* residual, void* y, void* z, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* dz = grad_output * act'(z) (grad_output [tokens x out_features], dense);
+ * grad_x = dz W [tokens x ldgx], grad_weight = dz^T x [out_features x ldgw] and
+ * grad_bias = sum of dz over the tokens; each may be NULL.  z may be NULL for
+ * ORDA_ACT_NONE.  The residual's gradient is grad_output itself. */
+int orda_linear_backward(const orda_linear_t* p, const void* x, const void* weight, const void* z,
+                         const void* grad_output, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* a = x Wg^T, b = x Wu^T, h = act(a) b, y = h Wd^T + residual, with w_gate and
+ * w_up [inner x hidden] and w_down [out_features x inner]; alignment and
+ * padding of x, the weights and their gradients as orda_linear's. */
+typedef struct orda_ffn {
+  int32_t abi_version;
+  int32_t dtype;
+  int32_t activation;
+  int32_t reserved;
+  int64_t tokens;
+  int64_t hidden;        /* columns of x, w_gate and w_up                    */
+  int64_t inner;         /* rows of w_gate and w_up, columns of w_down       */
+  int64_t out_features;  /* rows of w_down                                   */
+  int64_t ldx;           /* pitch of x                                       */
+  int64_t ldw;           /* of w_gate and w_up                               */
+  int64_t ldd;           /* of w_down                                        */
+  int64_t ldr;           /* of residual                                      */
+  int64_t ldg;           /* backward: of grad_output, a multiple of 8 (fp32:
+                            4), rows 16-byte aligned and zero-padded         */
+  int64_t ldgx;          /* backward: of grad_x                              */
+  int64_t ldgw;          /* backward: of grad_gate and grad_up               */
+  int64_t ldgd;          /* backward: of grad_down                           */
+} orda_ffn_t;
+
+/* Elements between the rows of h, a and b ([tokens x this] each, in dtype). */
+int64_t orda_ffn_inner_pitch(const orda_ffn_t* p);
+size_t orda_ffn_workspace_bytes(const orda_ffn_t* p, int32_t backward);
+
+/* Writes y [tokens x out_features], dense, and h; a and b too when not NULL
+ * (the three are what the backward call reads). */
+int orda_ffn_forward(const orda_ffn_t* p, const void* x, const void* w_gate, const void* w_up, const void* w_down,
+                     const void* residual, void* y, void* h, void* a, void* b, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* With dh = grad_output Wd: da = dh b act'(a), db = dh act(a), grad_x = da Wg +
+ * db Wu, grad_gate = da^T x, grad_up = db^T x, grad_down = grad_output^T h; each
+ * gradient may be NULL. */
+int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, const void* w_up, const void* w_down,
+                      const void* h, const void* a, const void* b, const void* grad_output, void* grad_x,
+                      void* grad_gate, void* grad_up, void* grad_down, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* One gradient: `rows` rows of `cols` elements, `ld` elements apart (a dense
+ * tensor is one row).  Any alignment.  The table is host memory, read before
+ * the call returns. */
+typedef struct orda_grad {
+  void* data;
+  void* out;             /* orda_clip_grads: where the result goes (NULL: in
+                            place), the same rows and cols                   */
+  int64_t rows, cols, ld, ld_out;
+  int32_t dtype;         /* enum orda_dtype                                  */
+  int32_t out_dtype;
+} orda_grad_t;
+
+/* Norm over all elements of n gradients: norm_type 1 (sum of magnitudes), 2 or
+ * infinity (HUGE_VAL: the largest magnitude, NaN if there is one).  Sums in
+ * fp64 in a fixed order; *total is a device fp32 scalar.  An empty table gives
+ * 0. */
+size_t orda_grad_norm_workspace_bytes(void);
+int orda_grad_norm(const orda_grad_t* grads, int64_t n, double norm_type, float* total, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* out = g * min(1, max_norm / (*total + 1e-6)), *total read on the device; a
+ * factor of 1 leaves gradients in place untouched.  Gradients written by one
+ * call must not overlap (ORDA_EINVAL). */
+int orda_clip_grads(const orda_grad_t* grads, int64_t n, const float* total, double max_norm, void* stream);
+
 /* Per-kernel-class timing, for benchmarks.  No counterpart in the reference,
  * whose benchmarks bracket whole steps with torch.cuda.Event
  * (test/benchmark/src/_train.py:410-419); this hook brackets each launch

@@ -1410,6 +1410,15 @@ int forward_with(const Plan& pl, const orda_problem_t* p, const orda_tensors_t* 
 
 }  // namespace
 
+// The message of a failed call of the entry points in ops_abi.hip (NULL: none).
+namespace orda {
+int set_last_error(int code, const char* msg) {
+  if (msg) g_err = msg;
+  else g_err.clear();
+  return code;
+}
+}  // namespace orda
+
 extern "C" {
 
 int orda_abi_version(void) { return ORDA_ABI_VERSION; }

@@ -1,0 +1,276 @@
+// epilogue.hpp -- what the products of the projection (orda_linear_*) and of
+// the gated feed-forward block (orda_ffn_*) do with their fp32 accumulators:
+// bias, activation, gate product and residual on the way out, or the
+// activation's derivative on the way back.  Every engine hands an epilogue W
+// consecutive columns of one row, in fp32; each output is rounded once.
+#pragma once
+#include "orda_core.hpp"
+
+namespace orda {
+
+__host__ __device__ __forceinline__ int64_t lmin(int64_t a, int64_t b) { return a < b ? a : b; }
+
+enum Act { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_SILU = 4, ACT_SIGMOID = 5, ACT_COUNT = 6 };
+
+// 1 / (1 + exp(-x)): in fp32 with the library's exp and an exact division,
+// for 16-bit outputs on the hardware's exp2 and reciprocal (errors of 1e-6,
+// far below half a step of the output).
+template <class T>
+__device__ __forceinline__ float sigmoid_of(float x) {
+  if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-x));
+  else return __builtin_amdgcn_rcpf(1.0f + fexp(-x));
+}
+
+// f = act(x), and with GRAD also df = act'(x).
+//   relu: a NaN stays one.  gelu: x Phi(x), Phi(x) = erfc(-x / sqrt 2) / 2,
+//   which keeps its relative accuracy where 1 + erf cancels.  gelu_tanh:
+//   (1 + tanh u) / 2 = sigmoid(2 u), u = sqrt(2 / pi) (x + 0.044715 x^3).
+// `kind` is uniform over the grid (a scalar branch).
+template <class T, bool GRAD, int W>
+__device__ __forceinline__ void act_eval(int kind, const float (&x)[W], float (&f)[W], float (&df)[W]) {
+  switch (kind) {
+    case ACT_RELU:
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        f[e] = x[e] < 0.0f ? 0.0f : x[e];
+        if constexpr (GRAD) df[e] = x[e] <= 0.0f ? 0.0f : 1.0f;
+      }
+      break;
+    case ACT_GELU:
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float phi = 0.5f * erfcf(x[e] * -0.70710678118654752f);
+        f[e] = x[e] * phi;
+        if constexpr (GRAD) {
+          const float g = -0.5f * x[e] * x[e];
+          const float d = 0.3989422804014327f * (sizeof(T) == 4 ? expf(g) : fexp(g));
+          df[e] = d == 0.0f ? phi : phi + x[e] * d;
+        }
+      }
+      break;
+    case ACT_GELU_TANH:
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float s = sigmoid_of<T>(1.5957691216057308f * (x[e] + 0.044715f * x[e] * x[e] * x[e]));
+        f[e] = x[e] * s;
+        if constexpr (GRAD) {
+          const float q = s * (1.0f - s);
+          df[e] = q == 0.0f ? s : s + x[e] * q * 1.5957691216057308f * (1.0f + 0.134145f * x[e] * x[e]);
+        }
+      }
+      break;
+    case ACT_SILU:
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float s = sigmoid_of<T>(x[e]);
+        f[e] = x[e] * s;
+        if constexpr (GRAD) df[e] = s + x[e] * s * (1.0f - s);
+      }
+      break;
+    case ACT_SIGMOID:
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        f[e] = sigmoid_of<T>(x[e]);
+        if constexpr (GRAD) df[e] = f[e] * (1.0f - f[e]);
+      }
+      break;
+    default:
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        f[e] = x[e];
+        if constexpr (GRAD) df[e] = 1.0f;
+      }
+  }
+}
+
+// W consecutive values; `wide`: the address is aligned to min(16, W sizeof(T))
+// bytes and all W are there.  Otherwise the first cnt, one by one (the rest
+// read as zero).
+template <class T, int W>
+__device__ __forceinline__ void ld_row(const T* p, float (&v)[W], bool wide, int cnt) {
+  constexpr int kB = W * (int)sizeof(T), kV = kB < 16 ? kB : 16, kE = kV / (int)sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(kE)));
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < W / kE; ++i) {
+      const vec x = *reinterpret_cast<const vec*>(p + i * kE);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) v[i * kE + e] = to_f32(x[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = e < cnt ? to_f32(p[e]) : 0.0f;
+  }
+}
+template <class T, int W>
+__device__ __forceinline__ void st_row(T* p, const float (&v)[W], bool wide, int cnt) {
+  constexpr int kB = W * (int)sizeof(T), kV = kB < 16 ? kB : 16, kE = kV / (int)sizeof(T);
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < W / kE; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        uint32_t u[kE / 2];
+#pragma unroll
+        for (int e = 0; e < kE / 2; ++e) u[e] = pack2<T>(v[i * kE + 2 * e], v[i * kE + 2 * e + 1]);
+        if constexpr (kE == 4) *reinterpret_cast<uint2*>(p + i * kE) = make_uint2(u[0], u[1]);
+        else *reinterpret_cast<uint4*>(p + i * kE) = make_uint4(u[0], u[1], u[2], u[3]);
+      } else {
+        *reinterpret_cast<float4*>(p + i * kE) = make_float4(v[i * 4], v[i * 4 + 1], v[i * 4 + 2], v[i * 4 + 3]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < W; ++e)
+      if (e < cnt) p[e] = from_f32<T>(v[e]);
+  }
+}
+
+// Epilogues: E(m, n, v[, u], cnt, wide) with cnt <= W valid columns; `cols` is
+// the number of columns written; kDual: v and u are the two products of the
+// same columns.  at(split): the epilogue of one K range (partials only).
+
+// y = act(v + bias) + residual; z, when given, keeps v + bias for the backward
+// pass (rounded to T as y is).
+template <class T>
+struct EpiLinear {
+  static constexpr bool kDual = false;
+  T* y;
+  T* z;
+  const T* bias;
+  const T* res;
+  int64_t ldy, ldz, ldr, cols;
+  int act;
+  int wide;  // every row of every tensor is 16-byte aligned
+  __device__ __forceinline__ const EpiLinear& at(int) const { return *this; }
+  template <int W>
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt) const {
+    const bool full = wide && cnt == W;
+    float t[W];
+    if (bias) {
+      ld_row<T, W>(bias + n, t, full, cnt);
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] += t[e];
+    }
+    if (z) st_row<T, W>(z + m * ldz + n, v, full, cnt);
+    if (act != ACT_NONE) {
+      float f[W];
+      act_eval<T, false, W>(act, v, f, t);
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] = f[e];
+    }
+    if (res) {
+      ld_row<T, W>(res + m * ldr + n, t, full, cnt);
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] += t[e];
+    }
+    st_row<T, W>(y + m * ldy + n, v, full, cnt);
+  }
+};
+
+// h = act(a) b; a and b are kept for the backward pass when asked for (all
+// three [M x ld], rounded to T: h is the next product's operand, which the
+// matrix cores take in T, and a, b are held as activations are between the
+// passes).
+template <class T>
+struct EpiGate {
+  static constexpr bool kDual = true;
+  T* h;
+  T* a;
+  T* b;
+  int64_t ld, cols;
+  int act;
+  int wide;
+  __device__ __forceinline__ const EpiGate& at(int) const { return *this; }
+  template <int W>
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&g)[W], float (&u)[W], int cnt) const {
+    const bool full = wide && cnt == W;
+    const int64_t o = m * ld + n;
+    if (a) {
+      st_row<T, W>(a + o, g, full, cnt);
+      st_row<T, W>(b + o, u, full, cnt);
+    }
+    float f[W], t[W];
+    act_eval<T, false, W>(act, g, f, t);
+#pragma unroll
+    for (int e = 0; e < W; ++e) f[e] *= u[e];
+    st_row<T, W>(h + o, f, full, cnt);
+  }
+};
+
+// From dh (fp32, never rounded): da = dh b act'(a), db = dh act(a), rounded to
+// T as the operands of the next products.  d is [M x 2 ld']: da in the first
+// `cols` columns of a row, db in the next.
+template <class T>
+struct EpiGateGrad {
+  static constexpr bool kDual = false;
+  T* d;
+  const T* a;
+  const T* b;
+  int64_t ldd, ld, cols;
+  int act;
+  int wide;
+  __device__ __forceinline__ const EpiGateGrad& at(int) const { return *this; }
+  template <int W>
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt) const {
+    const bool full = wide && cnt == W;
+    float av[W], bv[W], f[W], df[W];
+    ld_row<T, W>(a + m * ld + n, av, full, cnt);
+    ld_row<T, W>(b + m * ld + n, bv, full, cnt);
+    act_eval<T, true, W>(act, av, f, df);
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      bv[e] *= v[e] * df[e];
+      f[e] *= v[e];
+    }
+    st_row<T, W>(d + m * ldd + n, bv, full, cnt);
+    st_row<T, W>(d + m * ldd + cols + n, f, full, cnt);
+  }
+};
+
+// fp32 partial of one K range: [splits][M][ld], a dual product's second half
+// in columns cols .. of a row.  (ld a multiple of 4.)
+template <bool DUAL>
+struct EpiPart {
+  static constexpr bool kDual = DUAL;
+  float* p;
+  int64_t stride, ld, cols;
+  __device__ __forceinline__ EpiPart at(int split) const { return EpiPart{p + split * stride, stride, ld, cols}; }
+  template <int W>
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt) const {
+    st_row<float, W>(p + m * ld + n, v, cnt == W, cnt);
+  }
+  template <int W>
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], float (&u)[W], int cnt) const {
+    st_row<float, W>(p + m * ld + n, v, cnt == W, cnt);
+    st_row<float, W>(p + m * ld + cols + n, u, cnt == W, cnt);
+  }
+};
+
+// Sum of the partials in split order, then the epilogue; a thread takes 4
+// columns of a row.  cols a multiple of 4.
+template <class Epi>
+__global__ __launch_bounds__(256) void k_part_reduce(const float* __restrict__ part, int splits, int64_t stride,
+                                                     int64_t ld, int64_t M, int64_t cols, Epi E) {
+  const int64_t nq = cols / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= M * nq) return;
+  const int64_t m = i / nq, n = (i - m * nq) * 4;
+  float v[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+  const float* p = part + m * ld + n;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float4 x = *reinterpret_cast<const float4*>(p + s * stride);
+    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+    if constexpr (Epi::kDual) {
+      const float4 y = *reinterpret_cast<const float4*>(p + s * stride + cols);
+      u[0] += y.x; u[1] += y.y; u[2] += y.z; u[3] += y.w;
+    }
+  }
+  const int64_t rem = E.cols - n;
+  const int cnt = rem >= 4 ? 4 : (int)rem;
+  if (cnt <= 0) return;
+  if constexpr (Epi::kDual) E(m, n, v, u, cnt);
+  else E(m, n, v, cnt);
+}
+
+}  // namespace orda

@@ -1,0 +1,311 @@
+// norms.hip -- the norm over all elements of many tensors, and their clipping.
+//
+// A launch takes a table of tensors in its arguments (no copy to the device,
+// so it can be captured) and splits their rows into chunks; workgroup b of G
+// takes the b-th G-th of the chunks.  Both kernels are bound by memory: the
+// norm reads every element once, clipping reads and writes it once, in 16-byte
+// accesses from the first aligned address of a row on.  Squares and sums are
+// fp64, so neither tiny nor huge gradients lose anything, and every sum has a
+// fixed order: a thread's elements, the lanes of a wave, the waves, the
+// workgroups.
+#include <algorithm>
+
+#include "epilogue.hpp"
+#include "op_launch.hpp"
+
+namespace orda {
+
+constexpr int kSpanMax = 96;  // tensors of one launch (48 bytes each: the arguments hold 4 KiB)
+
+struct SpanTable {
+  int count;
+  int chunk;   // elements of a chunk (a multiple of 2048)
+  int chunks;  // in all
+  int pad;
+  struct Row {
+    const void* p;
+    void* out;
+    int64_t cols, ld, ld_out;
+    int per_row;  // chunks of a row
+    int first;    // the tensor's first chunk
+  } t[kSpanMax - 16];
+};
+constexpr int kSpanRows = kSpanMax - 16;
+static_assert(sizeof(SpanTable) <= 4000, "kernel arguments");
+
+// The chunks of workgroup b: f(tensor, first element of the row, elements
+// [lo, hi) of the row).  A row's chunks are cut at 16-byte aligned addresses.
+template <class T, class F>
+__device__ __forceinline__ void for_chunks(const SpanTable& S, const F& f) {
+  constexpr int VE = 16 / (int)sizeof(T);
+  const int c0 = (int)((int64_t)S.chunks * blockIdx.x / gridDim.x), c1 = (int)((int64_t)S.chunks * (blockIdx.x + 1) / gridDim.x);
+  if (c0 >= c1) return;
+  int i = 0, n = S.count;  // the last tensor that starts at or before c0
+  while (n - i > 1) {
+    const int m = (i + n) / 2;
+    if (S.t[m].first <= c0) i = m;
+    else n = m;
+  }
+  for (int c = c0; c < c1; ++c) {
+    while (i + 1 < S.count && S.t[i + 1].first <= c) ++i;
+    const int k = c - S.t[i].first, row = k / S.t[i].per_row, part = k - row * S.t[i].per_row;
+    const T* p = static_cast<const T*>(S.t[i].p) + row * S.t[i].ld;
+    const int skew = (int)((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));  // elements past an aligned address
+    const int64_t lo = (int64_t)part * S.chunk - skew, hi = lmin(lo + S.chunk, S.t[i].cols);
+    f(i, row, p, lo, hi);
+    (void)VE;
+  }
+}
+
+template <class T, int KIND>
+__device__ __forceinline__ void norm_add(double& s, float x) {
+  if constexpr (KIND == 2) s = fma((double)x, (double)x, s);
+  else if constexpr (KIND == 1) s += (double)fabsf(x);
+  else s = (fabsf(x) > s || x != x) ? (double)fabsf(x) : s;  // (a NaN stays: nothing compares above it)
+}
+template <int KIND>
+__device__ __forceinline__ double norm_join(double a, double b) {
+  if constexpr (KIND != 0) return a + b;
+  else return (b > a || b != b) ? b : a;
+}
+
+// A 16-byte vector of T as floats.
+template <class T>
+__device__ __forceinline__ void unpack16(const uint4& u, float (&v)[16 / sizeof(T)]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      v[2 * i] = lo16<T>(w[i]);
+      v[2 * i + 1] = hi16<T>(w[i]);
+    } else {
+      v[i] = __uint_as_float(w[i]);
+    }
+  }
+}
+
+// partials[b] (+)= workgroup b's share.
+template <class T, int KIND>
+__global__ __launch_bounds__(256) void k_grad_norm(SpanTable S, double* partials, int first) {
+  constexpr int VE = 16 / (int)sizeof(T), U = 4;
+  __shared__ double red[4];
+  double s = 0.0;
+  for_chunks<T>(S, [&](int, int, const T* p, int64_t lo, int64_t hi) {
+    int64_t e = lo + (int64_t)threadIdx.x * VE;
+    for (; e + (U - 1) * 256 * VE + VE <= hi && lo >= 0; e += U * 256 * VE) {
+      uint4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const uint4*>(p + e + u * 256 * VE);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x[VE];
+        unpack16<T>(v[u], x);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) norm_add<T, KIND>(s, x[i]);
+      }
+    }
+    for (; e < hi; e += 256 * VE) {
+      float x[VE];
+      if (e >= 0 && e + VE <= hi) {
+        unpack16<T>(*reinterpret_cast<const uint4*>(p + e), x);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) norm_add<T, KIND>(s, x[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+          if (e + i >= 0 && e + i < hi) norm_add<T, KIND>(s, to_f32(p[e + i]));
+      }
+    }
+  });
+  for (int m = 1; m < 64; m <<= 1) s = norm_join<KIND>(s, __shfl_xor(s, m));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 4; ++i) s = norm_join<KIND>(s, red[i]);
+  partials[blockIdx.x] = first ? s : norm_join<KIND>(partials[blockIdx.x], s);
+}
+
+template <int KIND>
+__global__ __launch_bounds__(256) void k_grad_total(const double* partials, int n, float* total) {
+  __shared__ double red[4];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += 256) s = norm_join<KIND>(s, partials[i]);
+  for (int m = 1; m < 64; m <<= 1) s = norm_join<KIND>(s, __shfl_xor(s, m));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 4; ++i) s = norm_join<KIND>(s, red[i]);
+  *total = (float)(KIND == 2 ? sqrt(s) : s);
+}
+
+// min(1, max_norm / (total + 1e-6)); a NaN norm gives a NaN factor.
+__device__ __forceinline__ float clip_factor(const float* total, float max_norm) {
+  const float f = max_norm / (*total + 1e-6f);
+  return f > 1.0f ? 1.0f : f;
+}
+
+template <class T, class O>
+__global__ __launch_bounds__(256) void k_clip(SpanTable S, const float* total, float max_norm, int in_place) {
+  constexpr int VE = 16 / (int)sizeof(T), U = 2;
+  const float f = clip_factor(total, max_norm);
+  if (in_place && f == 1.0f) return;
+  // (outputs at any element: the hardware's unaligned stores)
+  typedef O vec __attribute__((ext_vector_type(VE), aligned(sizeof(O))));
+  auto put = [&](O* o, const uint4& u) {
+    float x[VE];
+    unpack16<T>(u, x);
+    vec y;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) y[i] = from_f32<O>(x[i] * f);
+    *reinterpret_cast<vec*>(o) = y;
+  };
+  for_chunks<T>(S, [&](int t, int row, const T* p, int64_t lo, int64_t hi) {
+    O* o = static_cast<O*>(S.t[t].out) + row * S.t[t].ld_out;
+    int64_t e = lo + (int64_t)threadIdx.x * VE;
+    for (; e + (U - 1) * 256 * VE + VE <= hi && lo >= 0; e += U * 256 * VE) {
+      uint4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const uint4*>(p + e + u * 256 * VE);
+#pragma unroll
+      for (int u = 0; u < U; ++u) put(o + e + u * 256 * VE, v[u]);
+    }
+    for (; e < hi; e += 256 * VE) {
+      if (e >= 0 && e + VE <= hi) {
+        put(o + e, *reinterpret_cast<const uint4*>(p + e));
+      } else {
+        for (int i = 0; i < VE; ++i)
+          if (e + i >= 0 && e + i < hi) o[e + i] = from_f32<O>(to_f32(p[e + i]) * f);
+      }
+    }
+  });
+}
+
+// Tables of the spans of one dtype pair; go(table, workgroups) per launch.
+template <class Go>
+static hipError_t for_tables(const GradSpan* g, int64_t n, int in_dtype, int out_dtype, int place, int64_t chunk, int max_groups, const Go& go) {
+  const int es = in_dtype == DT_F32 ? 4 : 2, ve = 16 / es;
+  SpanTable S;
+  S.count = S.chunks = 0;
+  S.chunk = (int)chunk;
+  S.pad = 0;
+  auto flush = [&]() -> hipError_t {
+    if (S.count == 0) return hipSuccess;
+    const hipError_t e = go(S, S.chunks < max_groups ? S.chunks : max_groups);
+    S.count = S.chunks = 0;
+    return e;
+  };
+  for (int64_t i = 0; i < n; ++i) {
+    const GradSpan& x = g[i];
+    if (x.in_dtype != in_dtype || (out_dtype >= 0 && x.out_dtype != out_dtype)) continue;
+    if (place >= 0 && (x.out == x.p) != (place != 0)) continue;
+    // a tensor of more chunks than a launch counts is cut into rows that fit
+    int64_t r0 = 0, c0 = 0;
+    const int64_t most = 1ll << 29;  // chunks of one entry
+    while (r0 < x.rows) {
+      const int64_t cols = x.rows == 1 ? std::min<int64_t>(x.cols - c0, most * chunk / 2) : x.cols;
+      const int64_t per = (cols + ve - 1 + chunk - 1) / chunk;
+      const int64_t rows = std::min<int64_t>(x.rows - r0, std::max<int64_t>(1, most / per));
+      if (S.count == kSpanRows || S.chunks + per * rows > (1ll << 30)) {
+        const hipError_t e = flush();
+        if (e != hipSuccess) return e;
+      }
+      SpanTable::Row& t = S.t[S.count++];
+      const int64_t oe = x.out_dtype == DT_F32 ? 4 : 2;
+      t.p = static_cast<const char*>(x.p) + (r0 * x.ld + c0) * es;
+      t.out = static_cast<char*>(x.out) + (r0 * x.ld_out + c0) * oe;
+      t.cols = cols;
+      t.ld = x.ld;
+      t.ld_out = x.ld_out;
+      t.per_row = (int)per;
+      t.first = S.chunks;
+      S.chunks += (int)(per * rows);
+      if (x.rows == 1) {
+        c0 += cols;
+        if (c0 >= x.cols) ++r0;
+      } else {
+        r0 += rows;
+      }
+    }
+  }
+  return flush();
+}
+
+// 2048 elements (one 16-byte access per thread) where that already fills the
+// chip, longer ones for large sets.
+static int64_t chunk_of(const GradSpan* g, int64_t n) {
+  int64_t total = 0;
+  for (int64_t i = 0; i < n; ++i) total += g[i].rows * g[i].cols;
+  return total < (64ll << 20) ? 2048 : 16384;
+}
+
+template <class T, int KIND>
+static hipError_t norm_go(const SpanTable& S, double* partials, int groups, int first, hipStream_t s) {
+  hipLaunchKernelGGL((k_grad_norm<T, KIND>), dim3(groups), dim3(256), 0, s, S, partials, first);
+  return hipGetLastError();
+}
+template <int KIND>
+static hipError_t norm_kind(const GradSpan* g, int64_t n, double* partials, int max_partials, float* total, hipStream_t s) {
+  // every launch has the same number of workgroups, the first one writes all partials
+  const int64_t chunk = chunk_of(g, n);
+  int64_t elements = 0;
+  for (int64_t i = 0; i < n; ++i) elements += g[i].rows * g[i].cols;
+  int groups = (int)std::min<int64_t>(max_partials, std::max<int64_t>(1, (elements + chunk - 1) / chunk));
+  int first = 1;
+  for (int dt = 0; dt < 3; ++dt) {
+    const hipError_t e = for_tables(g, n, dt, -1, -1, chunk, groups, [&](const SpanTable& S, int) {
+      const int f = first;
+      first = 0;
+      switch (dt) {
+        case DT_BF16: return norm_go<bf16, KIND>(S, partials, groups, f, s);
+        case DT_F16: return norm_go<f16, KIND>(S, partials, groups, f, s);
+        default: return norm_go<float, KIND>(S, partials, groups, f, s);
+      }
+    });
+    if (e != hipSuccess) return e;
+  }
+  if (first) groups = 0;
+  hipLaunchKernelGGL((k_grad_total<KIND>), dim3(1), dim3(256), 0, s, partials, groups, total);
+  return hipGetLastError();
+}
+
+hipError_t launch_grad_norm(const GradSpan* g, int64_t n, int kind, double* partials, int max_partials, float* total, hipStream_t s) {
+  switch (kind) {
+    case 2: return norm_kind<2>(g, n, partials, max_partials, total, s);
+    case 1: return norm_kind<1>(g, n, partials, max_partials, total, s);
+    default: return norm_kind<0>(g, n, partials, max_partials, total, s);
+  }
+}
+
+template <class T, class O>
+static hipError_t clip_go(const SpanTable& S, int groups, const float* total, float max_norm, int in_place, hipStream_t s) {
+  hipLaunchKernelGGL((k_clip<T, O>), dim3(groups), dim3(256), 0, s, S, total, max_norm, in_place);
+  return hipGetLastError();
+}
+template <class T>
+static hipError_t clip_out(const SpanTable& S, int groups, int out, const float* total, float max_norm, int in_place, hipStream_t s) {
+  switch (out) {
+    case DT_BF16: return clip_go<T, bf16>(S, groups, total, max_norm, in_place, s);
+    case DT_F16: return clip_go<T, f16>(S, groups, total, max_norm, in_place, s);
+    default: return clip_go<T, float>(S, groups, total, max_norm, in_place, s);
+  }
+}
+
+hipError_t launch_clip_grads(const GradSpan* g, int64_t n, const float* total, float max_norm, hipStream_t s) {
+  const int64_t chunk = chunk_of(g, n);
+  for (int in = 0; in < 3; ++in)
+    for (int out = 0; out < 3; ++out)
+      for (int place = 0; place < 2; ++place) {
+        if (place && in != out) continue;
+        const hipError_t e = for_tables(g, n, in, out, place, chunk, 8192, [&](const SpanTable& S, int groups) {
+          switch (in) {
+            case DT_BF16: return clip_out<bf16>(S, groups, out, total, max_norm, place, s);
+            case DT_F16: return clip_out<f16>(S, groups, out, total, max_norm, place, s);
+            default: return clip_out<float>(S, groups, out, total, max_norm, place, s);
+          }
+        });
+        if (e != hipSuccess) return e;
+      }
+  return hipSuccess;
+}
+
+}  // namespace orda

@@ -1,0 +1,130 @@
+// op_kernels.hpp -- launchers of the projection's and the feed-forward block's
+// kernels, instantiated per dtype by k_op_*.hip.
+#pragma once
+#include "op_launch.hpp"
+
+namespace orda {
+
+// Column sums and the activation's derivative of the projection's backward
+// pass, one pass over dy and z.  A wave takes 1 KiB (64 lanes x 16 bytes) of a
+// row, the four waves of a workgroup alternate rows; bias gradients are summed
+// per workgroup and added up by k_colsum, in a fixed order.  Bound by memory.
+template <class T>
+__global__ __launch_bounds__(256) void k_dz(DzParams P) {
+  constexpr int W = 16 / (int)sizeof(T);
+  __shared__ float red[3][64][W];
+  const int w = wave_id(), lane = threadIdx.x & 63;
+  const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * W;
+  const int64_t r0 = (int64_t)blockIdx.y * P.rows_per_block, r1 = lmin(P.rows, r0 + P.rows_per_block);
+  const int64_t left = P.cols - c;
+  const int cnt = left <= 0 ? 0 : (left >= W ? W : (int)left);
+  const bool wide = P.wide && cnt == W;
+  const T* dy = static_cast<const T*>(P.dy);
+  const T* z = static_cast<const T*>(P.z);
+  T* dz = static_cast<T*>(P.dz);
+  float sum[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) sum[e] = 0.f;
+  if (c < P.ldz) {
+    for (int64_t r = r0 + w; r < r1; r += 4) {
+      float g[W], x[W], f[W], df[W];
+      ld_row<T, W>(dy + r * P.ldy + c, g, wide, cnt);
+      if (z) {
+        ld_row<T, W>(z + r * P.ldz + c, x, true, W);  // (rows padded to ldz, a multiple of W)
+        act_eval<T, true, W>(P.act, x, f, df);
+#pragma unroll
+        for (int e = 0; e < W; ++e) g[e] = e < cnt ? g[e] * df[e] : 0.f;
+      }
+      if (dz) st_row<T, W>(dz + r * P.ldz + c, g, true, W);
+#pragma unroll
+      for (int e = 0; e < W; ++e) sum[e] += g[e];
+    }
+  }
+  if (!P.partial) return;
+  if (w > 0)
+#pragma unroll
+    for (int e = 0; e < W; ++e) red[w - 1][lane][e] = sum[e];
+  __syncthreads();
+  if (w > 0) return;
+#pragma unroll
+  for (int e = 0; e < W; ++e)
+    if (e < cnt) P.partial[(int64_t)blockIdx.y * P.cols + c + e] = ((sum[e] + red[0][lane][e]) + red[1][lane][e]) + red[2][lane][e];
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void k_colsum(const float* __restrict__ partial, int64_t blocks, int64_t cols, T* out) {
+  __shared__ float red[3][64];
+  const int w = wave_id(), lane = threadIdx.x & 63;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (c < cols)
+    for (int64_t b = w; b < blocks; b += 4) s += partial[b * cols + c];
+  if (w > 0) red[w - 1][lane] = s;
+  __syncthreads();
+  if (w == 0 && c < cols) out[c] = from_f32<T>(((s + red[0][lane]) + red[1][lane]) + red[2][lane]);
+}
+
+template <class T> hipError_t dz_go(const DzParams& P, hipStream_t s) {
+  constexpr int64_t per = 64 * (16 / (int64_t)sizeof(T));
+  const dim3 grid((unsigned)((P.ldz + per - 1) / per), (unsigned)((P.rows + P.rows_per_block - 1) / P.rows_per_block));
+  hipLaunchKernelGGL((k_dz<T>), grid, dim3(256), 0, s, P);
+  return hipGetLastError();
+}
+template <class T> hipError_t colsum_go(const float* partial, int64_t blocks, int64_t cols, void* out, hipStream_t s) {
+  hipLaunchKernelGGL((k_colsum<T>), dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, s, partial, blocks, cols, static_cast<T*>(out));
+  return hipGetLastError();
+}
+
+template <class T, class Epi>
+hipError_t skinny_go(const TileParams& P, const Epi& E, hipStream_t s) {
+  SkinnyParams S{P.A, P.B, P.B1, P.M, P.N, P.K, P.lda, P.ldb};
+  hipLaunchKernelGGL((k_skinny<T, Epi>), dim3((unsigned)((E.cols + 15) / 16)), dim3(kSkinnyWaves * 64), 0, s, S, E);
+  return hipGetLastError();
+}
+
+template <class T, int LA, int LB, class Epi>
+hipError_t tile_go(const OpPlan& pl, TileParams P, const Epi& E, hipStream_t s) {
+  const int64_t bn = Epi::kDual ? pl.tile / 2 : pl.tile;
+  P.tiles_m = (int)((P.M + pl.tile - 1) / pl.tile);
+  P.tiles_n = (int)((E.cols + bn - 1) / bn);
+  P.splits = pl.splits;
+  P.kps = pl.kps;
+  const unsigned grid = (unsigned)((int64_t)P.tiles_m * P.tiles_n * P.splits);
+  if (pl.tile == 128) hipLaunchKernelGGL((k_tile<T, LA, LB, 128, 128, 2, Epi>), dim3(grid), dim3(256), 0, s, P, E);
+  else hipLaunchKernelGGL((k_tile<T, LA, LB, 64, 64, 3, Epi>), dim3(grid), dim3(256), 0, s, P, E);
+  return hipGetLastError();
+}
+
+// The product on tiles, or its K ranges into `part` and their sum.
+template <class Epi, class Go>
+hipError_t with_splits(const OpPlan& pl, const TileParams& P, const Epi& E, float* part, hipStream_t s, const Go& go) {
+  if (pl.splits == 1) return go(E);
+  const int64_t cols = (E.cols + 3) / 4 * 4, ld = Epi::kDual ? 2 * cols : cols;
+  EpiPart<Epi::kDual> Q{part, P.M * ld, ld, cols};
+  const hipError_t e = go(Q);
+  if (e != hipSuccess) return e;
+  const int64_t n = P.M * (cols / 4);
+  hipLaunchKernelGGL((k_part_reduce<Epi>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, part, pl.splits, P.M * ld, ld, P.M, cols, E);
+  return hipGetLastError();
+}
+
+}  // namespace orda
+
+#define ORDA_INSTANTIATE_OPS16(T)                                                                                  \
+  template <> hipError_t launch_op_linear<T>(const OpPlan& pl, int la, int lb, TileParams P, const EpiLinear<T>& E, float* part, hipStream_t s) { \
+    if (pl.engine == OP_SKINNY) return la == KMAJ && lb == KMAJ ? skinny_go<T>(P, E, s) : hipErrorInvalidValue;    \
+    return with_splits(pl, P, E, part, s, [&](const auto& e) {                                                     \
+      if (la == MNMAJ) return tile_go<T, MNMAJ, MNMAJ>(pl, P, e, s);                                               \
+      if (lb == MNMAJ) return tile_go<T, KMAJ, MNMAJ>(pl, P, e, s);                                                \
+      return tile_go<T, KMAJ, KMAJ>(pl, P, e, s);                                                                  \
+    });                                                                                                            \
+  }                                                                                                                \
+  template <> hipError_t launch_op_gate<T>(const OpPlan& pl, TileParams P, const EpiGate<T>& E, float* part, hipStream_t s) { \
+    if (pl.engine == OP_SKINNY) return skinny_go<T>(P, E, s);                                                      \
+    return with_splits(pl, P, E, part, s, [&](const auto& e) { return tile_go<T, KMAJ, KMAJ>(pl, P, e, s); });     \
+  }                                                                                                                \
+  template <> hipError_t launch_op_gate_grad<T>(const OpPlan& pl, TileParams P, const EpiGateGrad<T>& E, float* part, hipStream_t s) { \
+    return with_splits(pl, P, E, part, s, [&](const auto& e) { return tile_go<T, KMAJ, MNMAJ>(pl, P, e, s); });    \
+  }                                                                                                                \
+  template <> hipError_t launch_dz<T>(const DzParams& P, hipStream_t s) { return dz_go<T>(P, s); }                 \
+  template <> hipError_t launch_colsum<T>(const float* p, int64_t b, int64_t c, void* o, hipStream_t s) { return colsum_go<T>(p, b, c, o, s); }

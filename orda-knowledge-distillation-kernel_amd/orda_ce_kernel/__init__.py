@@ -21,11 +21,16 @@ from .api import (
 )
 
 
+from .ops.feed_forward import gated_feed_forward  # noqa: E402
+from .ops.grad_norm import clip_grad_norm_, grad_norm  # noqa: E402
+from .ops.linear import fused_linear  # noqa: E402
 from . import compiled  # noqa: E402,F401  (torch.compile-friendly entry; not in __all__)
 
 # TopKTeacher (a top-k precomputed teacher) and StudentRMSNorm (the student's
 # final RMSNorm fused in front of the loss) are importable from here but kept
-# out of __all__, which stays the reference's public surface.
+# out of __all__, which stays the reference's public surface; so are the
+# operators around the loss: fused_linear, gated_feed_forward (a student's
+# layers), grad_norm and clip_grad_norm_ (what follows the backward pass).
 
 
 def is_available() -> bool:

@@ -18,6 +18,8 @@ __all__ = [
     "ABI_VERSION", "PlanInfo", "Problem", "Tensors", "library", "plan_info", "library_path", "forward", "forward_static", "backward",
     "saved_bytes", "forward_workspace_bytes", "backward_workspace_bytes", "gemm_abt", "gemm",
     "MODE", "DTYPE", "FLAG", "KERNEL_CLASSES", "timing_enable", "timing_collect",
+    "ACTIVATION", "Linear", "FeedForward", "linear_forward", "linear_backward", "ffn_forward", "ffn_backward",
+    "grad_norm", "clip_grads",
 ]
 
 ABI_VERSION = 4
@@ -121,6 +123,29 @@ class Tensors(ctypes.Structure):
     ]
 
 
+ACTIVATION = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigmoid": 5}
+
+
+class Linear(ctypes.Structure):
+    """orda_linear_t"""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "dtype", "activation", "reserved")] + [
+        (n, ctypes.c_int64) for n in ("tokens", "in_features", "out_features", "ldx", "ldw", "ldr", "ldgx", "ldgw")
+    ]
+
+
+class FeedForward(ctypes.Structure):
+    """orda_ffn_t"""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "dtype", "activation", "reserved")] + [
+        (n, ctypes.c_int64) for n in ("tokens", "hidden", "inner", "out_features", "ldx", "ldw", "ldd", "ldr", "ldg",
+                                      "ldgx", "ldgw", "ldgd")
+    ]
+
+
+# orda_grad_t as int64 words: data, out, rows, cols, ld, ld_out, dtype | out_dtype << 32
+GRAD_WORDS = 7
+
 _LOCK = threading.Lock()
 _LIB = None
 
@@ -176,6 +201,22 @@ def library() -> ctypes.CDLL:
         lib.orda_scale_gradient.restype = ctypes.c_int
         lib.orda_scale_gradient.argtypes = [ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                                             ctypes.c_void_p]
+        L, F, vp, sz = ctypes.POINTER(Linear), ctypes.POINTER(FeedForward), ctypes.c_void_p, ctypes.c_size_t
+        for name, arg in (("orda_linear", L), ("orda_ffn", F)):
+            fn = getattr(lib, name + "_workspace_bytes")
+            fn.restype, fn.argtypes = sz, [arg, ctypes.c_int32]
+        for name, arg in (("orda_linear_saved_pitch", L), ("orda_ffn_inner_pitch", F)):
+            fn = getattr(lib, name)
+            fn.restype, fn.argtypes = ctypes.c_int64, [arg]
+        for name, arg, tensors in (("orda_linear_forward", L, 6), ("orda_linear_backward", L, 7),
+                                   ("orda_ffn_forward", F, 9), ("orda_ffn_backward", F, 12)):
+            fn = getattr(lib, name)
+            fn.restype, fn.argtypes = ctypes.c_int, [arg] + [vp] * (tensors + 1) + [sz, vp]
+        lib.orda_grad_norm_workspace_bytes.restype, lib.orda_grad_norm_workspace_bytes.argtypes = sz, []
+        lib.orda_grad_norm.restype = ctypes.c_int
+        lib.orda_grad_norm.argtypes = [vp, ctypes.c_int64, ctypes.c_double, vp, vp, sz, vp]
+        lib.orda_clip_grads.restype = ctypes.c_int
+        lib.orda_clip_grads.argtypes = [vp, ctypes.c_int64, vp, ctypes.c_double, vp]
         lib.orda_timing_enable.restype = ctypes.c_int
         lib.orda_timing_enable.argtypes = [ctypes.c_int]
         lib.orda_timing_collect.restype = ctypes.c_int
@@ -304,6 +345,84 @@ def gemm(a: torch.Tensor, b: torch.Tensor, *, a_mn: bool = False, b_mn: bool = F
     )
     _check(rc, "orda_gemm")
     return c
+
+
+def _address(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _run_op(name: str, problem, backward: int, tensors, device: torch.device) -> None:
+    """One orda_linear_* / orda_ffn_* call on the device's current stream, with its workspace from torch."""
+    lib = library()
+    query = lib.orda_linear_workspace_bytes if isinstance(problem, Linear) else lib.orda_ffn_workspace_bytes
+    p = ctypes.byref(problem)
+    with _on(device):
+        n = query(p, backward)
+        if n == 0:
+            _check(-1, name)
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
+        rc = getattr(lib, name)(p, *[_address(t) for t in tensors], ws.data_ptr(), n, _stream(device))
+    _check(rc, name)
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on(device: torch.device):
+    """`device` as the current one for the launches (nothing to do where it is)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def linear_saved_pitch(problem: Linear) -> int:
+    return int(library().orda_linear_saved_pitch(ctypes.byref(problem)))
+
+
+def ffn_inner_pitch(problem: FeedForward) -> int:
+    return int(library().orda_ffn_inner_pitch(ctypes.byref(problem)))
+
+
+def linear_forward(problem: Linear, x, weight, bias, residual, y, z) -> None:
+    _run_op("orda_linear_forward", problem, 0, (x, weight, bias, residual, y, z), x.device)
+
+
+def linear_backward(problem: Linear, x, weight, z, grad_output, grad_x, grad_weight, grad_bias) -> None:
+    _run_op("orda_linear_backward", problem, 1, (x, weight, z, grad_output, grad_x, grad_weight, grad_bias),
+            grad_output.device)
+
+
+def ffn_forward(problem: FeedForward, x, w_gate, w_up, w_down, residual, y, h, a, b) -> None:
+    _run_op("orda_ffn_forward", problem, 0, (x, w_gate, w_up, w_down, residual, y, h, a, b), x.device)
+
+
+def ffn_backward(problem: FeedForward, x, w_gate, w_up, w_down, h, a, b, grad_output, grad_x, grad_gate, grad_up,
+                 grad_down) -> None:
+    _run_op("orda_ffn_backward", problem, 1,
+            (x, w_gate, w_up, w_down, h, a, b, grad_output, grad_x, grad_gate, grad_up, grad_down), x.device)
+
+
+def grad_norm(table, n: int, norm_type: float, total: torch.Tensor) -> None:
+    """orda_grad_norm of a table of n orda_grad_t (an ``array('q')`` of GRAD_WORDS words each)."""
+    lib, dev = library(), total.device
+    with _on(dev):
+        nb = lib.orda_grad_norm_workspace_bytes()
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+        rc = lib.orda_grad_norm(table.buffer_info()[0], n, norm_type, total.data_ptr(), ws.data_ptr(), nb, _stream(dev))
+    _check(rc, "orda_grad_norm")
+
+
+def clip_grads(table, n: int, total: torch.Tensor, max_norm: float) -> None:
+    """orda_clip_grads of a table as :func:`grad_norm` takes it."""
+    with _on(total.device):
+        rc = library().orda_clip_grads(table.buffer_info()[0], n, total.data_ptr(), max_norm, _stream(total.device))
+    _check(rc, "orda_clip_grads")
 
 
 def timing_enable(enable: bool = True) -> None:
