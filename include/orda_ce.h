@@ -359,9 +359,9 @@ typedef struct orda_linear {
   int64_t ldgx, ldgw;    /* of grad_x and grad_weight (backward only)        */
 } orda_linear_t;
 
-/* Elements between the rows of the pre-activations that orda_linear_forward
- * keeps for the backward pass ([tokens x this], in dtype). */
-int64_t orda_linear_saved_pitch(const orda_linear_t* p);
+/* Bytes of the pre-activations that orda_linear_forward keeps for the backward
+ * pass (fp32; for 16-bit tensors the upper 24 bits of the fp32 values). */
+size_t orda_linear_saved_bytes(const orda_linear_t* p);
 
 /* Scratch bytes of the forward (backward = 0) or the backward call (1). */
 size_t orda_linear_workspace_bytes(const orda_linear_t* p, int32_t backward);
@@ -404,8 +404,11 @@ typedef struct orda_ffn {
   int64_t ldgd;          /* backward: of grad_down                           */
 } orda_ffn_t;
 
-/* Elements between the rows of h, a and b ([tokens x this] each, in dtype). */
+/* Elements between the rows of h ([tokens x this], in dtype). */
 int64_t orda_ffn_inner_pitch(const orda_ffn_t* p);
+/* Bytes of a, and of b, as the forward call keeps them (fp32; for 16-bit tensors
+ * the upper 24 bits of the fp32 values). */
+size_t orda_ffn_saved_bytes(const orda_ffn_t* p);
 size_t orda_ffn_workspace_bytes(const orda_ffn_t* p, int32_t backward);
 
 /* Writes y [tokens x out_features], dense, and h; a and b too when not NULL

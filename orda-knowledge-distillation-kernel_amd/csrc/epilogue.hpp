@@ -125,23 +125,90 @@ __device__ __forceinline__ void st_row(T* p, const float (&v)[W], bool wide, int
   }
 }
 
+// Pre-activations that the backward pass reads again.  For 16-bit tensors they
+// are kept as the upper 24 bits of the fp32 value (15 bits after the leading
+// one, fp32's range), in a plane of 16-bit halves and a plane of bytes behind
+// it (`lo` bytes on): rounded to bf16 they made the gradients of the
+// feed-forward block 1.8 times as far off float64 as one rounding at the end,
+// with 24 bits 1.4 times (da and db are rounded as operands).  fp32: as is.
+// i: index of the first of W values, a multiple of W.
+template <class T>
+constexpr int kKeptBytes = sizeof(T) == 4 ? 4 : 3;
+template <class T, int W>
+__device__ __forceinline__ void keep(void* base, int64_t lo, int64_t i, const float (&v)[W]) {
+  if constexpr (sizeof(T) == 4) {
+    st_row<float, W>(static_cast<float*>(base) + i, v, true, W);
+  } else {
+    uint32_t h[W / 2], l[W / 4];
+#pragma unroll
+    for (int e = 0; e < W / 2; ++e)
+      h[e] = __builtin_amdgcn_perm(__float_as_uint(v[2 * e + 1]), __float_as_uint(v[2 * e]), 0x07060302u);
+#pragma unroll
+    for (int e = 0; e < W / 4; ++e) {
+      const uint32_t a = __builtin_amdgcn_perm(__float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e]), 0x0c0c0501u);
+      const uint32_t b = __builtin_amdgcn_perm(__float_as_uint(v[4 * e + 3]), __float_as_uint(v[4 * e + 2]), 0x0c0c0501u);
+      l[e] = a | (b << 16);
+    }
+    char* p = static_cast<char*>(base);
+    if constexpr (W == 4) {
+      *reinterpret_cast<uint2*>(p + i * 2) = make_uint2(h[0], h[1]);
+      *reinterpret_cast<uint32_t*>(p + lo + i) = l[0];
+    } else {
+      *reinterpret_cast<uint4*>(p + i * 2) = make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint2*>(p + lo + i) = make_uint2(l[0], l[1]);
+    }
+  }
+}
+template <class T, int W>
+__device__ __forceinline__ void kept(const void* base, int64_t lo, int64_t i, float (&v)[W]) {
+  if constexpr (sizeof(T) == 4) {
+    ld_row<float, W>(static_cast<const float*>(base) + i, v, true, W);
+  } else {
+    const char* p = static_cast<const char*>(base);
+    uint32_t h[W / 2], l[W / 4];
+    if constexpr (W == 4) {
+      const uint2 a = *reinterpret_cast<const uint2*>(p + i * 2);
+      h[0] = a.x; h[1] = a.y;
+      l[0] = *reinterpret_cast<const uint32_t*>(p + lo + i);
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(p + i * 2);
+      const uint2 b = *reinterpret_cast<const uint2*>(p + lo + i);
+      h[0] = a.x; h[1] = a.y; h[2] = a.z; h[3] = a.w;
+      l[0] = b.x; l[1] = b.y;
+    }
+    // value e: halves (h[e / 2] >> 16 (e % 2)) and byte e of l, as bytes h1 h0 l 0
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      constexpr uint32_t kSel[8] = {0x0504000cu, 0x0706010cu, 0x0504020cu, 0x0706030cu, 0x0504000cu, 0x0706010cu, 0x0504020cu, 0x0706030cu};
+      v[e] = __uint_as_float(__builtin_amdgcn_perm(h[e / 2], l[e / 4], kSel[e]));
+    }
+  }
+}
+
 // Epilogues: E(m, n, v[, u], cnt, wide) with cnt <= W valid columns; `cols` is
 // the number of columns written; kDual: v and u are the two products of the
 // same columns.  at(split): the epilogue of one K range (partials only).
 
 // y = act(v + bias) + residual; z, when given, keeps v + bias for the backward
-// pass (rounded to T as y is).
+// pass, in rows of ldz (a multiple of 8, at least cols; the columns past cols
+// are written too and hold nothing).
 template <class T>
 struct EpiLinear {
   static constexpr bool kDual = false;
   T* y;
-  T* z;
+  T* y1;  // the output of a pair's second product
+  void* z;
   const T* bias;
   const T* res;
-  int64_t ldy, ldz, ldr, cols;
+  int64_t ldy, ldz, zlo, ldr, cols;
   int act;
   int wide;  // every row of every tensor is 16-byte aligned
-  __device__ __forceinline__ const EpiLinear& at(int) const { return *this; }
+  __device__ __forceinline__ EpiLinear at(int) const { return *this; }
+  __device__ __forceinline__ EpiLinear second() const {
+    EpiLinear e = *this;
+    e.y = y1;
+    return e;
+  }
   template <int W>
   __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt) const {
     const bool full = wide && cnt == W;
@@ -151,7 +218,7 @@ struct EpiLinear {
 #pragma unroll
       for (int e = 0; e < W; ++e) v[e] += t[e];
     }
-    if (z) st_row<T, W>(z + m * ldz + n, v, full, cnt);
+    if (z) keep<T, W>(z, zlo, m * ldz + n, v);
     if (act != ACT_NONE) {
       float f[W];
       act_eval<T, false, W>(act, v, f, t);
@@ -167,63 +234,58 @@ struct EpiLinear {
   }
 };
 
-// h = act(a) b; a and b are kept for the backward pass when asked for (all
-// three [M x ld], rounded to T: h is the next product's operand, which the
-// matrix cores take in T, and a, b are held as activations are between the
-// passes).
+// h = act(a) b, rounded to T as the next product's operand; a and b are kept
+// for the backward pass when asked for.  All [M x ld], cols = ld a multiple of
+// 64, so that every access is whole and aligned.
 template <class T>
 struct EpiGate {
   static constexpr bool kDual = true;
   T* h;
-  T* a;
-  T* b;
-  int64_t ld, cols;
+  void* a;
+  void* b;
+  int64_t ld, cols, lo;
   int act;
-  int wide;
-  __device__ __forceinline__ const EpiGate& at(int) const { return *this; }
+  __device__ __forceinline__ EpiGate at(int) const { return *this; }
   template <int W>
   __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&g)[W], float (&u)[W], int cnt) const {
-    const bool full = wide && cnt == W;
     const int64_t o = m * ld + n;
     if (a) {
-      st_row<T, W>(a + o, g, full, cnt);
-      st_row<T, W>(b + o, u, full, cnt);
+      keep<T, W>(a, lo, o, g);
+      keep<T, W>(b, lo, o, u);
     }
     float f[W], t[W];
     act_eval<T, false, W>(act, g, f, t);
 #pragma unroll
     for (int e = 0; e < W; ++e) f[e] *= u[e];
-    st_row<T, W>(h + o, f, full, cnt);
+    st_row<T, W>(h + o, f, true, cnt);
   }
 };
 
 // From dh (fp32, never rounded): da = dh b act'(a), db = dh act(a), rounded to
 // T as the operands of the next products.  d is [M x 2 ld']: da in the first
-// `cols` columns of a row, db in the next.
+// `cols` columns of a row, db in the next; cols = ld a multiple of 64.
 template <class T>
 struct EpiGateGrad {
   static constexpr bool kDual = false;
   T* d;
-  const T* a;
-  const T* b;
-  int64_t ldd, ld, cols;
+  const void* a;
+  const void* b;
+  int64_t ldd, ld, cols, lo;
   int act;
-  int wide;
-  __device__ __forceinline__ const EpiGateGrad& at(int) const { return *this; }
+  __device__ __forceinline__ EpiGateGrad at(int) const { return *this; }
   template <int W>
   __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt) const {
-    const bool full = wide && cnt == W;
     float av[W], bv[W], f[W], df[W];
-    ld_row<T, W>(a + m * ld + n, av, full, cnt);
-    ld_row<T, W>(b + m * ld + n, bv, full, cnt);
+    kept<T, W>(a, lo, m * ld + n, av);
+    kept<T, W>(b, lo, m * ld + n, bv);
     act_eval<T, true, W>(act, av, f, df);
 #pragma unroll
     for (int e = 0; e < W; ++e) {
       bv[e] *= v[e] * df[e];
       f[e] *= v[e];
     }
-    st_row<T, W>(d + m * ldd + n, bv, full, cnt);
-    st_row<T, W>(d + m * ldd + cols + n, f, full, cnt);
+    st_row<T, W>(d + m * ldd + n, bv, true, cnt);
+    st_row<T, W>(d + m * ldd + cols + n, f, true, cnt);
   }
 };
 

@@ -2,6 +2,7 @@
 // kernels, instantiated per dtype by k_op_*.hip.
 #pragma once
 #include "op_launch.hpp"
+#include "ring_op.hpp"
 
 namespace orda {
 
@@ -20,7 +21,6 @@ __global__ __launch_bounds__(256) void k_dz(DzParams P) {
   const int cnt = left <= 0 ? 0 : (left >= W ? W : (int)left);
   const bool wide = P.wide && cnt == W;
   const T* dy = static_cast<const T*>(P.dy);
-  const T* z = static_cast<const T*>(P.z);
   T* dz = static_cast<T*>(P.dz);
   float sum[W];
 #pragma unroll
@@ -29,8 +29,8 @@ __global__ __launch_bounds__(256) void k_dz(DzParams P) {
     for (int64_t r = r0 + w; r < r1; r += 4) {
       float g[W], x[W], f[W], df[W];
       ld_row<T, W>(dy + r * P.ldy + c, g, wide, cnt);
-      if (z) {
-        ld_row<T, W>(z + r * P.ldz + c, x, true, W);  // (rows padded to ldz, a multiple of W)
+      if (P.z) {
+        kept<T, W>(P.z, P.zlo, r * P.ldz + c, x);  // (rows padded to ldz, a multiple of W)
         act_eval<T, true, W>(P.act, x, f, df);
 #pragma unroll
         for (int e = 0; e < W; ++e) g[e] = e < cnt ? g[e] * df[e] : 0.f;
@@ -95,6 +95,32 @@ hipError_t tile_go(const OpPlan& pl, TileParams P, const Epi& E, hipStream_t s) 
   return hipGetLastError();
 }
 
+// One workgroup per CU of the current device (160 KiB of LDS each).
+inline int ring_groups() {
+  static const int cus = [] {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) == hipSuccess && hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && n > 0) return n;
+    return 256;
+  }();
+  return cus;
+}
+template <class T, int LA, int LB, class Epi>
+hipError_t ring_go(const OpPlan& pl, TileParams P, const Epi& E, hipStream_t s) {
+  const int64_t bn = Epi::kDual ? 128 : 256;
+  P.tiles_m = (int)((P.M + 255) / 256) * (P.pair > 0 ? 2 : 1);
+  P.tiles_n = (int)((E.cols + bn - 1) / bn);
+  P.splits = pl.splits;
+  P.kps = pl.kps;
+  const int64_t total = (int64_t)P.tiles_m * P.tiles_n * P.splits;
+  const unsigned grid = (unsigned)(total < ring_groups() ? total : ring_groups());
+  hipLaunchKernelGGL((k_ring<T, LA, LB, Epi>), dim3(grid), dim3(kThreads4), 0, s, P, E);
+  return hipGetLastError();
+}
+template <class T, int LA, int LB, class Epi>
+hipError_t any_go(const OpPlan& pl, const TileParams& P, const Epi& E, hipStream_t s) {
+  return pl.engine == OP_RING ? ring_go<T, LA, LB>(pl, P, E, s) : tile_go<T, LA, LB>(pl, P, E, s);
+}
+
 // The product on tiles, or its K ranges into `part` and their sum.
 template <class Epi, class Go>
 hipError_t with_splits(const OpPlan& pl, const TileParams& P, const Epi& E, float* part, hipStream_t s, const Go& go) {
@@ -114,17 +140,17 @@ hipError_t with_splits(const OpPlan& pl, const TileParams& P, const Epi& E, floa
   template <> hipError_t launch_op_linear<T>(const OpPlan& pl, int la, int lb, TileParams P, const EpiLinear<T>& E, float* part, hipStream_t s) { \
     if (pl.engine == OP_SKINNY) return la == KMAJ && lb == KMAJ ? skinny_go<T>(P, E, s) : hipErrorInvalidValue;    \
     return with_splits(pl, P, E, part, s, [&](const auto& e) {                                                     \
-      if (la == MNMAJ) return tile_go<T, MNMAJ, MNMAJ>(pl, P, e, s);                                               \
-      if (lb == MNMAJ) return tile_go<T, KMAJ, MNMAJ>(pl, P, e, s);                                                \
-      return tile_go<T, KMAJ, KMAJ>(pl, P, e, s);                                                                  \
+      if (la == MNMAJ) return any_go<T, MNMAJ, MNMAJ>(pl, P, e, s);                                               \
+      if (lb == MNMAJ) return any_go<T, KMAJ, MNMAJ>(pl, P, e, s);                                                \
+      return any_go<T, KMAJ, KMAJ>(pl, P, e, s);                                                                  \
     });                                                                                                            \
   }                                                                                                                \
   template <> hipError_t launch_op_gate<T>(const OpPlan& pl, TileParams P, const EpiGate<T>& E, float* part, hipStream_t s) { \
     if (pl.engine == OP_SKINNY) return skinny_go<T>(P, E, s);                                                      \
-    return with_splits(pl, P, E, part, s, [&](const auto& e) { return tile_go<T, KMAJ, KMAJ>(pl, P, e, s); });     \
+    return with_splits(pl, P, E, part, s, [&](const auto& e) { return any_go<T, KMAJ, KMAJ>(pl, P, e, s); });     \
   }                                                                                                                \
   template <> hipError_t launch_op_gate_grad<T>(const OpPlan& pl, TileParams P, const EpiGateGrad<T>& E, float* part, hipStream_t s) { \
-    return with_splits(pl, P, E, part, s, [&](const auto& e) { return tile_go<T, KMAJ, MNMAJ>(pl, P, e, s); });    \
+    return with_splits(pl, P, E, part, s, [&](const auto& e) { return any_go<T, KMAJ, MNMAJ>(pl, P, e, s); });    \
   }                                                                                                                \
   template <> hipError_t launch_dz<T>(const DzParams& P, hipStream_t s) { return dz_go<T>(P, s); }                 \
   template <> hipError_t launch_colsum<T>(const float* p, int64_t b, int64_t c, void* o, hipStream_t s) { return colsum_go<T>(p, b, c, o, s); }

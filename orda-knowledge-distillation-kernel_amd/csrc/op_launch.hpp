@@ -30,7 +30,8 @@ template <class T> hipError_t launch_op_gate_grad(const OpPlan& pl, TileParams P
 // cols) and, with partial, its column sums per block of rows.
 struct DzParams {
   const void* dy;
-  const void* z;   // null: dz = dy
+  const void* z;   // as keep() wrote it (zlo: its second plane); null: dz = dy
+  int64_t zlo;
   void* dz;        // null: only the sums
   float* partial;  // [row blocks][cols], or null
   int64_t rows, cols, ldy, ldz;

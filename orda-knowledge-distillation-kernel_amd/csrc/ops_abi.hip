@@ -32,11 +32,13 @@ int fail(int code, const char* fmt, ...) {
 inline int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t esize(int dtype) { return dtype == ORDA_F32 ? 4 : 2; }
+inline int64_t kept_bytes(int dtype) { return dtype == ORDA_F32 ? kKeptBytes<float> : kKeptBytes<bf16>; }
 inline int64_t granule(int dtype) { return dtype == ORDA_F32 ? 4 : 8; }  // elements of 16 bytes
 inline bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 inline char* base256(void* ws) { return reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(ws) + 255) / 256 * 256); }
 
-constexpr int64_t kMaxTokens = 1ll << 30, kMaxWidth = 1ll << 22;
+constexpr int64_t kMaxTokens = 1ll << 30;
+constexpr int64_t kMaxWidth = 1ll << 21, kMaxPitch = 1ll << 22;  // (128 rows of a K-major operand in one buffer resource)
 
 // ------------------------------------------------------------- the engine
 // One product C[M x cols] = A B^T over K; dual: two weights.
@@ -44,7 +46,17 @@ struct Shape {
   int dtype, la, lb;
   bool dual;
   int64_t M, cols, K;
+  int64_t lda, ldb;   // pitches of MN-major operands
+  bool pair;          // two products side by side (A's columns)
 };
+
+// The ring engine's limits: more than one K step, MN-major operands within a
+// buffer resource (2^31 bytes of K rows).
+bool ring_fits(const Shape& q) {
+  const int64_t lim = 0x7fffffffll / 2;
+  return q.dtype != ORDA_F32 && q.K > 64 && (q.la == KMAJ || q.K * q.lda < lim) && (q.lb == KMAJ || q.K * q.ldb < lim);
+}
+int64_t ring_items(const Shape& q) { return cdiv(q.M, 256) * (q.pair ? 2 : 1) * cdiv(q.cols, q.dual ? 128 : 256); }
 
 OpPlan plan_of(const Shape& q) {
   OpPlan pl{};
@@ -70,6 +82,11 @@ OpPlan plan_of(const Shape& q) {
         }
       }
     want = pl.splits;
+  } else if (ring_fits(q) && ring_items(q) >= 200) {
+    pl.engine = OP_RING;
+    pl.tile = 256;
+    pl.kps = q.K;
+    return pl;
   } else {
     pl.engine = OP_TILE;
     auto items = [&](int64_t t) { return cdiv(q.M, t) * cdiv(q.cols, q.dual ? t / 2 : t); };
@@ -110,13 +127,13 @@ int check_common(const char* what, int32_t abi, int32_t dtype, int32_t act, int3
   return ORDA_OK;
 }
 int check_width(const char* what, const char* name, int64_t v) {
-  if (v <= 0 || v > kMaxWidth) return fail(ORDA_EINVAL, "%s: %s must be in [1, 2^22], got %lld", what, name, (long long)v);
+  if (v <= 0 || v > kMaxWidth) return fail(ORDA_EINVAL, "%s: %s must be in [1, 2^21], got %lld", what, name, (long long)v);
   return ORDA_OK;
 }
 int check_pitch(const char* what, const char* name, int64_t ld, int64_t width, int dtype) {
   const int64_t g = granule(dtype);
-  if (ld < up(width, g) || ld % g != 0 || ld > 2 * kMaxWidth)
-    return fail(ORDA_EINVAL, "%s: %s must be a multiple of %lld and at least %lld, got %lld", what, name, (long long)g,
+  if (ld < up(width, g) || ld % g != 0 || ld > kMaxPitch)
+    return fail(ORDA_EINVAL, "%s: %s must be a multiple of %lld in [%lld, 2^22], got %lld", what, name, (long long)g,
                 (long long)up(width, g), (long long)ld);
   return ORDA_OK;
 }
@@ -149,9 +166,9 @@ int linear_shapes(const orda_linear_t* p, LinearShapes& s) {
   OP_TRY(check_pitch(what, "ldw", p->ldw, p->in_features, p->dtype));
   const int64_t g = granule(p->dtype), kp = up(p->in_features, g);
   s.op = up(p->out_features, g);
-  s.fwd = {p->dtype, KMAJ, KMAJ, false, p->tokens, p->out_features, kp};
-  s.dx = {p->dtype, KMAJ, MNMAJ, false, p->tokens, kp, s.op};
-  s.dw = {p->dtype, MNMAJ, MNMAJ, false, p->out_features, kp, p->tokens};
+  s.fwd = {p->dtype, KMAJ, KMAJ, false, p->tokens, p->out_features, kp, 0, 0, false};
+  s.dx = {p->dtype, KMAJ, MNMAJ, false, p->tokens, kp, s.op, 0, p->ldw, false};
+  s.dw = {p->dtype, MNMAJ, MNMAJ, false, p->out_features, kp, p->tokens, s.op, p->ldx, false};
   // about 1024 workgroups, at least 16 rows each
   const int64_t per = 64 * g, cb = cdiv(s.op, per);
   s.rows_per_block = std::max<int64_t>(16, up(cdiv(p->tokens * cb, 1024), 4));
@@ -204,12 +221,12 @@ int ffn_shapes(const orda_ffn_t* p, FfnShapes& s) {
   OP_TRY(check_pitch(what, "ldd", p->ldd, p->inner, p->dtype));
   const int64_t g = granule(p->dtype), hp = up(p->hidden, g), ip = up(p->inner, g);
   s.fp = up(p->inner, 64);
-  s.gate = {p->dtype, KMAJ, KMAJ, true, p->tokens, s.fp, hp};
-  s.down = {p->dtype, KMAJ, KMAJ, false, p->tokens, p->out_features, ip};
-  s.dh = {p->dtype, KMAJ, MNMAJ, false, p->tokens, s.fp, up(p->out_features, g)};
-  s.dx = {p->dtype, KMAJ, MNMAJ, false, p->tokens, hp, 2 * s.fp};
-  s.dw = {p->dtype, MNMAJ, MNMAJ, false, p->inner, hp, p->tokens};
-  s.dd = {p->dtype, MNMAJ, MNMAJ, false, p->out_features, ip, p->tokens};
+  s.gate = {p->dtype, KMAJ, KMAJ, true, p->tokens, s.fp, hp, 0, 0, false};
+  s.down = {p->dtype, KMAJ, KMAJ, false, p->tokens, p->out_features, ip, 0, 0, false};
+  s.dh = {p->dtype, KMAJ, MNMAJ, false, p->tokens, s.fp, up(p->out_features, g), 0, p->ldd, false};
+  s.dx = {p->dtype, KMAJ, MNMAJ, false, p->tokens, hp, 2 * s.fp, 0, p->ldw, false};
+  s.dw = {p->dtype, MNMAJ, MNMAJ, false, p->inner, hp, p->tokens, 2 * s.fp, p->ldx, false};
+  s.dd = {p->dtype, MNMAJ, MNMAJ, false, p->out_features, ip, p->tokens, p->ldg, s.fp, false};
   return ORDA_OK;
 }
 size_t ffn_part(const FfnShapes& s, bool backward) {
@@ -225,10 +242,10 @@ size_t ffn_ws(const orda_ffn_t* p, const FfnShapes& s, bool backward) {
 
 extern "C" {
 
-int64_t orda_linear_saved_pitch(const orda_linear_t* p) {
+size_t orda_linear_saved_bytes(const orda_linear_t* p) {
   set_last_error(0, nullptr);
   LinearShapes s;
-  return linear_shapes(p, s) == ORDA_OK ? s.op : 0;
+  return linear_shapes(p, s) == ORDA_OK ? (size_t)(p->tokens * s.op * kept_bytes(p->dtype)) : 0;
 }
 
 size_t orda_linear_workspace_bytes(const orda_linear_t* p, int32_t backward) {
@@ -250,7 +267,8 @@ int orda_linear_forward(const orda_linear_t* p, const void* x, const void* weigh
   return by_dtype(p->dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     EpiLinear<T> e = store_to<T>(y, p->out_features, p->out_features, p->dtype);
-    e.z = static_cast<T*>(z);
+    e.z = z;
+    e.zlo = 2 * p->tokens * s.op;
     e.bias = static_cast<const T*>(bias);
     e.res = static_cast<const T*>(residual);
     e.ldz = s.op;
@@ -295,6 +313,7 @@ int orda_linear_backward(const orda_linear_t* p, const void* x, const void* weig
       DzParams d{};
       d.dy = grad_output;
       d.z = act ? z : nullptr;
+      d.zlo = 2 * p->tokens * s.op;
       d.dz = products && !direct ? own_dz : nullptr;
       d.partial = grad_bias ? sums : nullptr;
       d.rows = p->tokens;
@@ -326,6 +345,12 @@ int64_t orda_ffn_inner_pitch(const orda_ffn_t* p) {
   return ffn_shapes(p, s) == ORDA_OK ? s.fp : 0;
 }
 
+size_t orda_ffn_saved_bytes(const orda_ffn_t* p) {
+  set_last_error(0, nullptr);
+  FfnShapes s;
+  return ffn_shapes(p, s) == ORDA_OK ? (size_t)(p->tokens * s.fp * kept_bytes(p->dtype)) : 0;
+}
+
 size_t orda_ffn_workspace_bytes(const orda_ffn_t* p, int32_t backward) {
   set_last_error(0, nullptr);
   FfnShapes s;
@@ -348,7 +373,7 @@ int orda_ffn_forward(const orda_ffn_t* p, const void* x, const void* w_gate, con
   float* part = reinterpret_cast<float*>(base256(workspace));
   return by_dtype(p->dtype, [&](auto tag) -> int {
     using T = decltype(tag);
-    EpiGate<T> g{static_cast<T*>(h), static_cast<T*>(a), static_cast<T*>(b), s.fp, s.fp, p->activation, 1};
+    EpiGate<T> g{static_cast<T*>(h), a, b, s.fp, s.fp, 2 * p->tokens * s.fp, p->activation};
     TileParams t = product<T>(x, p->ldx, w_gate, p->ldw, p->tokens, p->inner, s.gate.K);
     t.B1 = w_up;
     OP_LAUNCH(launch_op_gate<T>(plan_of(s.gate), t, g, part, st));
@@ -384,7 +409,7 @@ int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, co
   return by_dtype(p->dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     if (grad_x || grad_gate || grad_up) {
-      const EpiGateGrad<T> e{reinterpret_cast<T*>(d), static_cast<const T*>(a), static_cast<const T*>(b), 2 * s.fp, s.fp, s.fp, p->activation, 1};
+      const EpiGateGrad<T> e{reinterpret_cast<T*>(d), a, b, 2 * s.fp, s.fp, s.fp, 2 * p->tokens * s.fp, p->activation};
       TileParams t = product<T>(grad_output, p->ldg, w_down, p->ldd, p->tokens, p->inner, s.dh.K);
       t.kval = p->out_features;
       OP_LAUNCH(launch_op_gate_grad<T>(plan_of(s.dh), t, e, part, st));
@@ -396,7 +421,17 @@ int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, co
       t.kval = p->inner;
       OP_LAUNCH(launch_op_linear<T>(plan_of(s.dx), KMAJ, MNMAJ, t, store_to<T>(grad_x, p->ldgx, s.dx.cols, p->dtype), part, st));
     }
-    for (int i = 0; i < 2; ++i) {
+    Shape both = s.dw;
+    both.pair = true;
+    const bool pair = grad_gate && grad_up && plan_of(both).engine == OP_RING;
+    if (pair) {  // one launch: its tiles fill the chip's last round better than two launches' do
+      TileParams t = product<T>(d, 2 * s.fp, x, p->ldx, p->inner, s.dw.cols, p->tokens);
+      t.pair = s.fp;
+      EpiLinear<T> e = store_to<T>(grad_gate, p->ldgw, s.dw.cols, p->dtype);
+      e.y1 = static_cast<T*>(grad_up);
+      OP_LAUNCH(launch_op_linear<T>(plan_of(both), MNMAJ, MNMAJ, t, e, part, st));
+    }
+    for (int i = 0; i < 2 && !pair; ++i) {
       void* out = i ? grad_up : grad_gate;
       if (!out) continue;
       const TileParams t = product<T>(d + i * s.fp * (int64_t)sizeof(T), 2 * s.fp, x, p->ldx, p->inner, s.dw.cols, p->tokens);

@@ -107,6 +107,11 @@ __device__ __forceinline__ void pipeline16(Acc16& acc, char* lds, int ntiles, in
   if (ntiles <= 0 || nk < 2) return;
   auto mod5 = [](int j) { return j >= kRing ? j - kRing : j; };
   auto slot = [&](int j) { return lds + j * kTileBytes; };
+  // an opnd that also takes the K step serves operands of two K segments
+  auto opnd_of = [&](const auto& ti, int op, int kd) {
+    if constexpr (std::is_invocable_v<Opnd, decltype(ti), int, int>) return opnd(ti, op, kd);
+    else return opnd(ti, op);
+  };
   auto live_b = [](int nb) { return nb < 4 ? H0 : H1; };
   auto live_dma = [](int op, int q) { return op == 0 || LB == MNMAJ || (q < 4 ? H0 : H1); };
 
@@ -256,7 +261,7 @@ __device__ __forceinline__ void pipeline16(Acc16& acc, char* lds, int ntiles, in
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int op = 0; op < 2; ++op) {
-        const Step st = prep(opnd(cur, op), op, g, true);
+        const Step st = prep(opnd_of(cur, op, g), op, g, true);
         char* sb = slot(2 * g + op);
 #pragma unroll
         for (int q = 0; q < 8; ++q)
@@ -282,11 +287,11 @@ __device__ __forceinline__ void pipeline16(Acc16& acc, char* lds, int ntiles, in
       const int kd = in_cur ? kt + 2 : kt + 2 - nk;
       const bool dlive = in_cur || nxt_live;
       const int j1 = mod5(j0 + 1), j2 = mod5(j0 + 2), j3 = mod5(j0 + 3), j4 = mod5(j0 + 4);
-      half_step(0, 1, j0, j1, 1, prep(in_cur ? opnd(cur, 0) : opnd(nxt, 0), 0, kd, dlive), 0, j4);
+      half_step(0, 1, j0, j1, 1, prep(in_cur ? opnd_of(cur, 0, kd) : opnd_of(nxt, 0, kd), 0, kd, dlive), 0, j4);
       end_half(1);
       wait_vmem<8>();
       bar4();
-      half_step(1, 0, j2, j3, 0, prep(in_cur ? opnd(cur, 1) : opnd(nxt, 1), 1, kd, dlive), 1, j0);
+      half_step(1, 0, j2, j3, 0, prep(in_cur ? opnd_of(cur, 1, kd) : opnd_of(nxt, 1, kd), 1, kd, dlive), 1, j0);
       end_half(0);
       j0 = j2;
     }

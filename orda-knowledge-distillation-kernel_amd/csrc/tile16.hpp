@@ -34,6 +34,7 @@ struct TileParams {
   int64_t kval;          // valid K rows of an MN-major B (of each segment)
   int tiles_m, tiles_n, splits;
   int64_t kps;           // K of one split (a multiple of 64)
+  int64_t pair;          // > 0: two products side by side, the second with A's columns from here on (MN/MN, one split)
 };
 
 template <int R>

@@ -205,9 +205,10 @@ def library() -> ctypes.CDLL:
         for name, arg in (("orda_linear", L), ("orda_ffn", F)):
             fn = getattr(lib, name + "_workspace_bytes")
             fn.restype, fn.argtypes = sz, [arg, ctypes.c_int32]
-        for name, arg in (("orda_linear_saved_pitch", L), ("orda_ffn_inner_pitch", F)):
+        for name, arg, res in (("orda_linear_saved_bytes", L, sz), ("orda_ffn_saved_bytes", F, sz),
+                               ("orda_ffn_inner_pitch", F, ctypes.c_int64)):
             fn = getattr(lib, name)
-            fn.restype, fn.argtypes = ctypes.c_int64, [arg]
+            fn.restype, fn.argtypes = res, [arg]
         for name, arg, tensors in (("orda_linear_forward", L, 6), ("orda_linear_backward", L, 7),
                                    ("orda_ffn_forward", F, 9), ("orda_ffn_backward", F, 12)):
             fn = getattr(lib, name)
@@ -381,12 +382,16 @@ def _on(device: torch.device):
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def linear_saved_pitch(problem: Linear) -> int:
-    return int(library().orda_linear_saved_pitch(ctypes.byref(problem)))
+def linear_saved_bytes(problem: Linear) -> int:
+    return int(library().orda_linear_saved_bytes(ctypes.byref(problem)))
 
 
 def ffn_inner_pitch(problem: FeedForward) -> int:
     return int(library().orda_ffn_inner_pitch(ctypes.byref(problem)))
+
+
+def ffn_saved_bytes(problem: FeedForward) -> int:
+    return int(library().orda_ffn_saved_bytes(ctypes.byref(problem)))
 
 
 def linear_forward(problem: Linear, x, weight, bias, residual, y, z) -> None:

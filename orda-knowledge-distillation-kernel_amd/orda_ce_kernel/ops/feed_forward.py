@@ -10,8 +10,8 @@ Backward, with dh = dy Wd never leaving the accumulators:
     dx = da Wg + db Wu   (one product over both weights)
     dWg = da^T x    dWu = db^T x    dWd = dy^T h
 
-h, da and db are rounded to the compute dtype as operands of the next product, a and b as activations kept between the
-passes; products accumulate in fp32.  No counterpart in the reference, whose models use torch.
+h, da and db are rounded to the compute dtype as operands of the next product; a and b are kept in fp32, for 16-bit tensors
+in its upper 24 bits; products accumulate in fp32.  No counterpart in the reference, whose models use torch.
 """
 from __future__ import annotations
 
@@ -39,8 +39,10 @@ def _forward(x2, w_gate, w_up, w_down, res2, act: str, dtype, keep: bool):
     fp = _native.ffn_inner_pitch(p)
     y = torch.empty((N, O), dtype=dtype, device=x2.device)
     h = torch.empty((N, fp), dtype=dtype, device=x2.device)
-    a = torch.empty_like(h) if keep else None
-    b = torch.empty_like(h) if keep else None
+    a = b = None
+    if keep:
+        n = _native.ffn_saved_bytes(p)
+        a, b = (torch.empty(n, dtype=torch.uint8, device=x2.device) for _ in range(2))
     _native.ffn_forward(p, xo, ga, up, dn, res2, y, h, a, b)
     return y, (xo, ga, up, dn, h, a, b), p
 
@@ -85,7 +87,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     ``x`` is ``(..., hidden)``, ``w_gate`` and ``w_up`` ``(inner, hidden)`` (two halves of one tensor serve), ``w_down``
     ``(out_features, inner)``, ``residual`` ``(..., out_features)``; ``activation`` one of ``none``, ``relu``, ``gelu``,
     ``gelu_tanh``, ``silu``, ``sigmoid``.  Dtypes, strides, alignment and ``backend`` as :func:`fused_linear`.  A training
-    call keeps three ``[tokens, inner]`` tensors for its backward pass."""
+    call keeps h, a and b for its backward pass: 8 bytes (fp32: 12) per token and inner column."""
     check_tensors("gated_feed_forward", activation, x, w_gate=w_gate, w_up=w_up, w_down=w_down, residual=residual)
     if w_gate.ndim != 2 or w_gate.shape[1] != x.shape[-1] or w_gate.shape[0] == 0:
         raise ValueError(f"gated_feed_forward: w_gate must have shape (inner, {x.shape[-1]}), got {tuple(w_gate.shape)}")

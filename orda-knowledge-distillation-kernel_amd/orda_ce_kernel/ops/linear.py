@@ -3,8 +3,8 @@
     y = act(x W^T + bias) + residual
 
 One kernel computes it (few rows: one that streams W; more: tiles of the matrix cores, with K split over workgroups where
-there are few tiles); for the backward pass it also keeps z = x W^T + bias where an activation needs it, rounded to the
-compute dtype.  Backward: dz = dy act'(z) and the bias gradient in one pass over dy and z, then dx = dz W and dW = dz^T x;
+there are few tiles); for the backward pass it also keeps z = x W^T + bias where an activation needs it (fp32; for 16-bit
+tensors the upper 24 bits of the fp32 values).  Backward: dz = dy act'(z) and the bias gradient in one pass over dy and z, then dx = dz W and dW = dz^T x;
 the residual's gradient is dy.  Products accumulate in fp32, every output is rounded once.  No counterpart in the
 reference, whose models use torch.
 """
@@ -35,7 +35,7 @@ def _forward(x2, weight, bias, res2, act: str, dtype, keep: bool):
     y = torch.empty((x2.shape[0], O), dtype=dtype, device=x2.device)
     z = None
     if keep and act != "none":
-        z = torch.empty((x2.shape[0], _native.linear_saved_pitch(p)), dtype=dtype, device=x2.device)
+        z = torch.empty(_native.linear_saved_bytes(p), dtype=torch.uint8, device=x2.device)
     _native.linear_forward(p, xo, wo, bias, res2, y, z)
     return y, xo, wo, z, p
 
