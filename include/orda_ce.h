@@ -359,25 +359,24 @@ typedef struct orda_linear {
   int64_t ldgx, ldgw;    /* of grad_x and grad_weight (backward only)        */
 } orda_linear_t;
 
-/* Bytes of the pre-activations that orda_linear_forward keeps for the backward
- * pass (fp32; for 16-bit tensors the upper 24 bits of the fp32 values). */
+/* Bytes of d = act'(x W^T + bias) as orda_linear_forward keeps it for the
+ * backward pass (fp32; for 16-bit tensors the upper 24 bits of fp32 values). */
 size_t orda_linear_saved_bytes(const orda_linear_t* p);
 
 /* Scratch bytes of the forward (backward = 0) or the backward call (1). */
 size_t orda_linear_workspace_bytes(const orda_linear_t* p, int32_t backward);
 
 /* Writes y [tokens x out_features], dense.  bias [out_features] and residual
- * may be NULL; z (saved pre-activations, 16-byte aligned) is written when not
- * NULL. */
+ * may be NULL; d (16-byte aligned) is written when not NULL. */
 int orda_linear_forward(const orda_linear_t* p, const void* x, const void* weight, const void* bias,
-                        const void* residual, void* y, void* z, void* workspace, size_t workspace_bytes,
+                        const void* residual, void* y, void* d, void* workspace, size_t workspace_bytes,
                         void* stream);
 
-/* dz = grad_output * act'(z) (grad_output [tokens x out_features], dense);
+/* dz = grad_output * d (grad_output [tokens x out_features], dense);
  * grad_x = dz W [tokens x ldgx], grad_weight = dz^T x [out_features x ldgw] and
- * grad_bias = sum of dz over the tokens; each may be NULL.  z may be NULL for
+ * grad_bias = sum of dz over the tokens; each may be NULL.  d may be NULL for
  * ORDA_ACT_NONE.  The residual's gradient is grad_output itself. */
-int orda_linear_backward(const orda_linear_t* p, const void* x, const void* weight, const void* z,
+int orda_linear_backward(const orda_linear_t* p, const void* x, const void* weight, const void* d,
                          const void* grad_output, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
                          size_t workspace_bytes, void* stream);
 
@@ -406,22 +405,23 @@ typedef struct orda_ffn {
 
 /* Elements between the rows of h ([tokens x this], in dtype). */
 int64_t orda_ffn_inner_pitch(const orda_ffn_t* p);
-/* Bytes of a, and of b, as the forward call keeps them (fp32; for 16-bit tensors
- * the upper 24 bits of the fp32 values). */
+/* Bytes of each factor that the forward call keeps for the backward pass (fp32;
+ * for 16-bit tensors the upper 24 bits of fp32 values). */
 size_t orda_ffn_saved_bytes(const orda_ffn_t* p);
 size_t orda_ffn_workspace_bytes(const orda_ffn_t* p, int32_t backward);
 
-/* Writes y [tokens x out_features], dense, and h; a and b too when not NULL
- * (the three are what the backward call reads). */
+/* Writes y [tokens x out_features], dense, and h; when not NULL also the factors
+ * da_factor = b act'(a) and db_factor = act(a) (what the backward call reads
+ * beside h). */
 int orda_ffn_forward(const orda_ffn_t* p, const void* x, const void* w_gate, const void* w_up, const void* w_down,
-                     const void* residual, void* y, void* h, void* a, void* b, void* workspace,
+                     const void* residual, void* y, void* h, void* da_factor, void* db_factor, void* workspace,
                      size_t workspace_bytes, void* stream);
 
-/* With dh = grad_output Wd: da = dh b act'(a), db = dh act(a), grad_x = da Wg +
+/* With dh = grad_output Wd: da = dh da_factor, db = dh db_factor, grad_x = da Wg +
  * db Wu, grad_gate = da^T x, grad_up = db^T x, grad_down = grad_output^T h; each
  * gradient may be NULL. */
 int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, const void* w_up, const void* w_down,
-                      const void* h, const void* a, const void* b, const void* grad_output, void* grad_x,
+                      const void* h, const void* da_factor, const void* db_factor, const void* grad_output, void* grad_x,
                       void* grad_gate, void* grad_up, void* grad_down, void* workspace, size_t workspace_bytes,
                       void* stream);
 

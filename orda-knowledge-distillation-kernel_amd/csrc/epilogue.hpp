@@ -21,9 +21,34 @@ __device__ __forceinline__ float sigmoid_of(float x) {
   else return __builtin_amdgcn_rcpf(1.0f + fexp(-x));
 }
 
+// Phi(x) = erfc(-x / sqrt 2) / 2, which keeps its relative accuracy where
+// 1 + erf cancels, and e = exp(-x^2 / 2).  For 16-bit outputs erfc(u) exp(u^2),
+// u = |x| / sqrt 2, is t P(t) with t = 1 / (1 + u / 2) and P of degree 6 fitted
+// to least relative error on u in [0, 9.5] (iterated reweighted least squares;
+// 1.4e-6 in fp32 arithmetic): a dozen instructions, where the library's erfc
+// made the epilogue of an 8192 x 2048 x 4096 product 80 us of its 186.
+template <class T>
+__device__ __forceinline__ float normal_cdf(float x, float& e) {
+  if constexpr (sizeof(T) == 4) {
+    e = expf(-0.5f * x * x);
+    return 0.5f * erfcf(x * -0.70710678118654752f);
+  } else {
+    e = __builtin_amdgcn_exp2f(-0.72134752f * x * x);
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(x), 0.35355339f, 1.0f));
+    float p = 0.08912547f;
+    p = fmaf(p, t, -0.35998616f);
+    p = fmaf(p, t, 0.39377975f);
+    p = fmaf(p, t, 0.03465823f);
+    p = fmaf(p, t, 0.28271983f);
+    p = fmaf(p, t, 0.27735361f);
+    p = fmaf(p, t, 0.28234809f);
+    const float q = 0.5f * p * t * e;
+    return x < 0.0f ? q : 1.0f - q;
+  }
+}
+
 // f = act(x), and with GRAD also df = act'(x).
-//   relu: a NaN stays one.  gelu: x Phi(x), Phi(x) = erfc(-x / sqrt 2) / 2,
-//   which keeps its relative accuracy where 1 + erf cancels.  gelu_tanh:
+//   relu: a NaN stays one.  gelu: x Phi(x).  gelu_tanh:
 //   (1 + tanh u) / 2 = sigmoid(2 u), u = sqrt(2 / pi) (x + 0.044715 x^3).
 // `kind` is uniform over the grid (a scalar branch).
 template <class T, bool GRAD, int W>
@@ -39,13 +64,10 @@ __device__ __forceinline__ void act_eval(int kind, const float (&x)[W], float (&
     case ACT_GELU:
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        const float phi = 0.5f * erfcf(x[e] * -0.70710678118654752f);
+        float g;
+        const float phi = normal_cdf<T>(x[e], g);
         f[e] = x[e] * phi;
-        if constexpr (GRAD) {
-          const float g = -0.5f * x[e] * x[e];
-          const float d = 0.3989422804014327f * (sizeof(T) == 4 ? expf(g) : fexp(g));
-          df[e] = d == 0.0f ? phi : phi + x[e] * d;
-        }
+        if constexpr (GRAD) df[e] = g == 0.0f ? phi : phi + x[e] * (0.3989422804014327f * g);
       }
       break;
     case ACT_GELU_TANH:
@@ -125,12 +147,28 @@ __device__ __forceinline__ void st_row(T* p, const float (&v)[W], bool wide, int
   }
 }
 
-// Pre-activations that the backward pass reads again.  For 16-bit tensors they
-// are kept as the upper 24 bits of the fp32 value (15 bits after the leading
-// one, fp32's range), in a plane of 16-bit halves and a plane of bytes behind
-// it (`lo` bytes on): rounded to bf16 they made the gradients of the
-// feed-forward block 1.8 times as far off float64 as one rounding at the end,
-// with 24 bits 1.4 times (da and db are rounded as operands).  fp32: as is.
+// W consecutive values as they lie in memory: loaded early, unpacked later.
+template <class T, int W>
+struct RawRow {
+  typedef T vec __attribute__((ext_vector_type(W)));
+  vec v;
+  __device__ __forceinline__ void load(const T* p, bool wide, int cnt) {
+    if (wide) {
+      v = *reinterpret_cast<const vec*>(p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] = e < cnt ? p[e] : (T)0.0f;
+    }
+  }
+  __device__ __forceinline__ float operator[](int e) const { return to_f32(v[e]); }
+};
+
+// Factors that the backward pass multiplies by.  For 16-bit tensors they are
+// kept as the upper 24 bits of the fp32 value (15 bits after the leading one,
+// fp32's range), in a plane of 16-bit halves and a plane of bytes `lo` bytes
+// behind it: rounded to bf16 they made the gradients of the feed-forward block
+// 1.8 times as far off float64 as one rounding at the end, with 24 bits 1.4
+// times (da and db are rounded as operands).  fp32: as is.
 // i: index of the first of W values, a multiple of W.
 template <class T>
 constexpr int kKeptBytes = sizeof(T) == 4 ? 4 : 3;
@@ -160,47 +198,48 @@ __device__ __forceinline__ void keep(void* base, int64_t lo, int64_t i, const fl
   }
 }
 template <class T, int W>
-__device__ __forceinline__ void kept(const void* base, int64_t lo, int64_t i, float (&v)[W]) {
-  if constexpr (sizeof(T) == 4) {
-    ld_row<float, W>(static_cast<const float*>(base) + i, v, true, W);
-  } else {
+struct Kept {
+  typedef uint32_t hv __attribute__((ext_vector_type(sizeof(T) == 4 ? W : W / 2)));
+  typedef uint32_t lv __attribute__((ext_vector_type(W / 4)));
+  hv h;
+  lv l;
+  __device__ __forceinline__ void load(const void* base, int64_t lo, int64_t i) {
     const char* p = static_cast<const char*>(base);
-    uint32_t h[W / 2], l[W / 4];
-    if constexpr (W == 4) {
-      const uint2 a = *reinterpret_cast<const uint2*>(p + i * 2);
-      h[0] = a.x; h[1] = a.y;
-      l[0] = *reinterpret_cast<const uint32_t*>(p + lo + i);
+    if constexpr (sizeof(T) == 4) {
+      h = *reinterpret_cast<const hv*>(p + i * 4);
     } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(p + i * 2);
-      const uint2 b = *reinterpret_cast<const uint2*>(p + lo + i);
-      h[0] = a.x; h[1] = a.y; h[2] = a.z; h[3] = a.w;
-      l[0] = b.x; l[1] = b.y;
-    }
-    // value e: halves (h[e / 2] >> 16 (e % 2)) and byte e of l, as bytes h1 h0 l 0
-#pragma unroll
-    for (int e = 0; e < W; ++e) {
-      constexpr uint32_t kSel[8] = {0x0504000cu, 0x0706010cu, 0x0504020cu, 0x0706030cu, 0x0504000cu, 0x0706010cu, 0x0504020cu, 0x0706030cu};
-      v[e] = __uint_as_float(__builtin_amdgcn_perm(h[e / 2], l[e / 4], kSel[e]));
+      h = *reinterpret_cast<const hv*>(p + i * 2);
+      l = *reinterpret_cast<const lv*>(p + lo + i);
     }
   }
-}
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(h[e]);
+    // value e: half e % 2 of h[e / 2] above byte e % 4 of l[e / 4], as bytes h1 h0 l 0
+    constexpr uint32_t kSel[4] = {0x0504000cu, 0x0706010cu, 0x0504020cu, 0x0706030cu};
+    if constexpr (W == 4) return __uint_as_float(__builtin_amdgcn_perm(h[e / 2], ((const uint32_t&)l), kSel[e % 4]));
+    else return __uint_as_float(__builtin_amdgcn_perm(h[e / 2], l[e / 4], kSel[e % 4]));
+  }
+};
 
-// Epilogues: E(m, n, v[, u], cnt, wide) with cnt <= W valid columns; `cols` is
-// the number of columns written; kDual: v and u are the two products of the
-// same columns.  at(split): the epilogue of one K range (partials only).
+// Epilogues.  E(m, n, v[, u], cnt, pre, col) takes W <= 8 columns n .. of row m,
+// of which cnt are valid; pre<W>(m, n, cnt) and, for what depends on the
+// columns alone, col<W>(n, cnt) load what it reads.  epi_apply() is all three.  `cols` is the number of columns written; kDual: v and u are
+// the two products of the same columns.  at(split): the epilogue of one K range
+// (partials only).
+struct NoPre {};
 
-// y = act(v + bias) + residual; z, when given, keeps v + bias for the backward
-// pass, in rows of ldz (a multiple of 8, at least cols; the columns past cols
-// are written too and hold nothing).
+// y = act(v + bias) + residual; d, when given, keeps act'(v + bias) for the
+// backward pass, in rows of ldd (a multiple of 8, at least cols; the columns
+// past cols are written too and hold nothing).
 template <class T>
 struct EpiLinear {
-  static constexpr bool kDual = false;
+  static constexpr bool kDual = false, kLight = false;
   T* y;
   T* y1;  // the output of a pair's second product
-  void* z;
+  void* d;
   const T* bias;
   const T* res;
-  int64_t ldy, ldz, zlo, ldr, cols;
+  int64_t ldy, ldd, dlo, ldr, cols;
   int act;
   int wide;  // every row of every tensor is 16-byte aligned
   __device__ __forceinline__ EpiLinear at(int) const { return *this; }
@@ -210,82 +249,125 @@ struct EpiLinear {
     return e;
   }
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt) const {
+  struct Pre {
+    RawRow<T, W> r;
+  };
+  template <int W>
+  struct Col {
+    RawRow<T, W> b;
+  };
+  template <int W>
+  __device__ __forceinline__ Col<W> col(int64_t n, int cnt) const {
+    Col<W> c;
+    if (bias) c.b.load(bias + n, wide && cnt == W, cnt);
+    return c;
+  }
+  template <int W>
+  __device__ __forceinline__ Pre<W> pre(int64_t m, int64_t n, int cnt) const {
+    Pre<W> p;
+    if (res) p.r.load(res + m * ldr + n, wide && cnt == W, cnt);
+    return p;
+  }
+  template <int W>
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt, const Pre<W>& p,
+                                             const Col<W>& c) const {
     const bool full = wide && cnt == W;
-    float t[W];
     if (bias) {
-      ld_row<T, W>(bias + n, t, full, cnt);
 #pragma unroll
-      for (int e = 0; e < W; ++e) v[e] += t[e];
+      for (int e = 0; e < W; ++e) v[e] += c.b[e];
     }
-    if (z) keep<T, W>(z, zlo, m * ldz + n, v);
     if (act != ACT_NONE) {
-      float f[W];
-      act_eval<T, false, W>(act, v, f, t);
+      float f[W], df[W];
+      if (d) {
+        act_eval<T, true, W>(act, v, f, df);
+        keep<T, W>(d, dlo, m * ldd + n, df);
+      } else {
+        act_eval<T, false, W>(act, v, f, df);
+      }
 #pragma unroll
       for (int e = 0; e < W; ++e) v[e] = f[e];
     }
     if (res) {
-      ld_row<T, W>(res + m * ldr + n, t, full, cnt);
 #pragma unroll
-      for (int e = 0; e < W; ++e) v[e] += t[e];
+      for (int e = 0; e < W; ++e) v[e] += p.r[e];
     }
     st_row<T, W>(y + m * ldy + n, v, full, cnt);
   }
 };
 
-// h = act(a) b, rounded to T as the next product's operand; a and b are kept
-// for the backward pass when asked for.  All [M x ld], cols = ld a multiple of
-// 64, so that every access is whole and aligned.
+// h = act(a) b, rounded to T as the next product's operand; for the backward
+// pass, when asked for, the factors p = b act'(a) of da and q = act(a) of db are
+// kept: the activation is not evaluated again.  All [M x ld], cols = ld a
+// multiple of 64, so that every access is whole and aligned.
 template <class T>
 struct EpiGate {
-  static constexpr bool kDual = true;
+  static constexpr bool kDual = true, kLight = false;
   T* h;
-  void* a;
-  void* b;
+  void* p;
+  void* q;
   int64_t ld, cols, lo;
   int act;
   __device__ __forceinline__ EpiGate at(int) const { return *this; }
+  template <int W> using Pre = NoPre;
+  template <int W> using Col = NoPre;
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&g)[W], float (&u)[W], int cnt) const {
+  __device__ __forceinline__ NoPre pre(int64_t, int64_t, int) const { return {}; }
+  template <int W>
+  __device__ __forceinline__ NoPre col(int64_t, int) const { return {}; }
+  template <int W>
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&g)[W], float (&u)[W], int cnt, NoPre, NoPre) const {
     const int64_t o = m * ld + n;
-    if (a) {
-      keep<T, W>(a, lo, o, g);
-      keep<T, W>(b, lo, o, u);
+    float f[W], df[W];
+    if (p) {
+      act_eval<T, true, W>(act, g, f, df);
+#pragma unroll
+      for (int e = 0; e < W; ++e) df[e] *= u[e];
+      keep<T, W>(p, lo, o, df);
+      keep<T, W>(q, lo, o, f);
+    } else {
+      act_eval<T, false, W>(act, g, f, df);
     }
-    float f[W], t[W];
-    act_eval<T, false, W>(act, g, f, t);
 #pragma unroll
     for (int e = 0; e < W; ++e) f[e] *= u[e];
     st_row<T, W>(h + o, f, true, cnt);
   }
 };
 
-// From dh (fp32, never rounded): da = dh b act'(a), db = dh act(a), rounded to
-// T as the operands of the next products.  d is [M x 2 ld']: da in the first
-// `cols` columns of a row, db in the next; cols = ld a multiple of 64.
+// From dh (fp32, never rounded): da = dh p, db = dh q, rounded to T as the
+// operands of the next products.  d is [M x ldd]: da in the first `cols`
+// columns of a row, db in the next; cols = ld a multiple of 64.
 template <class T>
 struct EpiGateGrad {
-  static constexpr bool kDual = false;
+  static constexpr bool kDual = false, kLight = true;
   T* d;
-  const void* a;
-  const void* b;
+  const void* p;
+  const void* q;
   int64_t ldd, ld, cols, lo;
-  int act;
   __device__ __forceinline__ EpiGateGrad at(int) const { return *this; }
+  template <int W> using Col = NoPre;
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt) const {
-    float av[W], bv[W], f[W], df[W];
-    kept<T, W>(a, lo, m * ld + n, av);
-    kept<T, W>(b, lo, m * ld + n, bv);
-    act_eval<T, true, W>(act, av, f, df);
+  __device__ __forceinline__ NoPre col(int64_t, int) const { return {}; }
+  template <int W>
+  struct Pre {
+    Kept<T, W> p, q;
+  };
+  template <int W>
+  __device__ __forceinline__ Pre<W> pre(int64_t m, int64_t n, int) const {
+    Pre<W> x;
+    x.p.load(p, lo, m * ld + n);
+    x.q.load(q, lo, m * ld + n);
+    return x;
+  }
+  template <int W>
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt, const Pre<W>& x, NoPre) const {
+    float da[W], db[W];
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-      bv[e] *= v[e] * df[e];
-      f[e] *= v[e];
+      da[e] = v[e] * x.p[e];
+      db[e] = v[e] * x.q[e];
     }
-    st_row<T, W>(d + m * ldd + n, bv, true, cnt);
-    st_row<T, W>(d + m * ldd + cols + n, f, true, cnt);
+    st_row<T, W>(d + m * ldd + n, da, true, cnt);
+    st_row<T, W>(d + m * ldd + cols + n, db, true, cnt);
   }
 };
 
@@ -293,20 +375,35 @@ struct EpiGateGrad {
 // in columns cols .. of a row.  (ld a multiple of 4.)
 template <bool DUAL>
 struct EpiPart {
-  static constexpr bool kDual = DUAL;
+  static constexpr bool kDual = DUAL, kLight = false;
   float* p;
   int64_t stride, ld, cols;
   __device__ __forceinline__ EpiPart at(int split) const { return EpiPart{p + split * stride, stride, ld, cols}; }
+  template <int W> using Pre = NoPre;
+  template <int W> using Col = NoPre;
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt) const {
+  __device__ __forceinline__ NoPre pre(int64_t, int64_t, int) const { return {}; }
+  template <int W>
+  __device__ __forceinline__ NoPre col(int64_t, int) const { return {}; }
+  template <int W>
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt, NoPre, NoPre) const {
     st_row<float, W>(p + m * ld + n, v, cnt == W, cnt);
   }
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], float (&u)[W], int cnt) const {
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], float (&u)[W], int cnt, NoPre, NoPre) const {
     st_row<float, W>(p + m * ld + n, v, cnt == W, cnt);
     st_row<float, W>(p + m * ld + cols + n, u, cnt == W, cnt);
   }
 };
+
+template <class Epi, int W>
+__device__ __forceinline__ void epi_apply(const Epi& E, int64_t m, int64_t n, float (&v)[W], int cnt) {
+  E(m, n, v, cnt, E.template pre<W>(m, n, cnt), E.template col<W>(n, cnt));
+}
+template <class Epi, int W>
+__device__ __forceinline__ void epi_apply(const Epi& E, int64_t m, int64_t n, float (&v)[W], float (&u)[W], int cnt) {
+  E(m, n, v, u, cnt, E.template pre<W>(m, n, cnt), E.template col<W>(n, cnt));
+}
 
 // Sum of the partials in split order, then the epilogue; a thread takes 4
 // columns of a row.  cols a multiple of 4.
@@ -331,8 +428,8 @@ __global__ __launch_bounds__(256) void k_part_reduce(const float* __restrict__ p
   const int64_t rem = E.cols - n;
   const int cnt = rem >= 4 ? 4 : (int)rem;
   if (cnt <= 0) return;
-  if constexpr (Epi::kDual) E(m, n, v, u, cnt);
-  else E(m, n, v, cnt);
+  if constexpr (Epi::kDual) epi_apply(E, m, n, v, u, cnt);
+  else epi_apply(E, m, n, v, cnt);
 }
 
 }  // namespace orda

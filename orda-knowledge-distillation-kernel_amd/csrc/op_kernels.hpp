@@ -6,8 +6,8 @@
 
 namespace orda {
 
-// Column sums and the activation's derivative of the projection's backward
-// pass, one pass over dy and z.  A wave takes 1 KiB (64 lanes x 16 bytes) of a
+// The projection's backward pass in front of its products: dz = dy act'(z) and
+// the column sums of dz, one pass over dy and the kept derivative.  A wave takes 1 KiB (64 lanes x 16 bytes) of a
 // row, the four waves of a workgroup alternate rows; bias gradients are summed
 // per workgroup and added up by k_colsum, in a fixed order.  Bound by memory.
 template <class T>
@@ -27,13 +27,13 @@ __global__ __launch_bounds__(256) void k_dz(DzParams P) {
   for (int e = 0; e < W; ++e) sum[e] = 0.f;
   if (c < P.ldz) {
     for (int64_t r = r0 + w; r < r1; r += 4) {
-      float g[W], x[W], f[W], df[W];
+      float g[W];
       ld_row<T, W>(dy + r * P.ldy + c, g, wide, cnt);
-      if (P.z) {
-        kept<T, W>(P.z, P.zlo, r * P.ldz + c, x);  // (rows padded to ldz, a multiple of W)
-        act_eval<T, true, W>(P.act, x, f, df);
+      if (P.d) {
+        Kept<T, W> k;
+        k.load(P.d, P.dlo, r * P.ldz + c);  // (rows padded to ldz, a multiple of W)
 #pragma unroll
-        for (int e = 0; e < W; ++e) g[e] = e < cnt ? g[e] * df[e] : 0.f;
+        for (int e = 0; e < W; ++e) g[e] = e < cnt ? g[e] * k[e] : 0.f;
       }
       if (dz) st_row<T, W>(dz + r * P.ldz + c, g, true, W);
 #pragma unroll
@@ -84,14 +84,16 @@ hipError_t skinny_go(const TileParams& P, const Epi& E, hipStream_t s) {
 
 template <class T, int LA, int LB, class Epi>
 hipError_t tile_go(const OpPlan& pl, TileParams P, const Epi& E, hipStream_t s) {
-  const int64_t bn = Epi::kDual ? pl.tile / 2 : pl.tile;
-  P.tiles_m = (int)((P.M + pl.tile - 1) / pl.tile);
+  const int64_t bm = pl.tile / 1000, bn = pl.tile % 1000 / (Epi::kDual ? 2 : 1);
+  P.tiles_m = (int)((P.M + bm - 1) / bm);
   P.tiles_n = (int)((E.cols + bn - 1) / bn);
   P.splits = pl.splits;
   P.kps = pl.kps;
   const unsigned grid = (unsigned)((int64_t)P.tiles_m * P.tiles_n * P.splits);
-  if (pl.tile == 128) hipLaunchKernelGGL((k_tile<T, LA, LB, 128, 128, 2, Epi>), dim3(grid), dim3(256), 0, s, P, E);
-  else hipLaunchKernelGGL((k_tile<T, LA, LB, 64, 64, 3, Epi>), dim3(grid), dim3(256), 0, s, P, E);
+  if (pl.tile == 128128) hipLaunchKernelGGL((k_tile<T, LA, LB, 128, 128, 2, Epi>), dim3(grid), dim3(256), 0, s, P, E);
+  else if (pl.tile == 64128) hipLaunchKernelGGL((k_tile<T, LA, LB, 64, 128, 3, Epi>), dim3(grid), dim3(256), 0, s, P, E);
+  else if (pl.tile == 64064) hipLaunchKernelGGL((k_tile<T, LA, LB, 64, 64, 3, Epi>), dim3(grid), dim3(256), 0, s, P, E);
+  else return hipErrorInvalidValue;
   return hipGetLastError();
 }
 

@@ -16,7 +16,7 @@ enum OpEngine { OP_SKINNY = 0, OP_TILE = 1, OP_RING = 2, OP_SPLIT3 = 3 };
 // How one product runs: the engine, its tile, and K in `splits` ranges of kps.
 struct OpPlan {
   int engine;
-  int tile;  // OP_TILE: 64 or 128; OP_SPLIT3: 64 (small) or 256 (large)
+  int tile;  // OP_TILE: 1000 rows + columns; OP_SPLIT3: 64 (small) or 256 (large)
   int splits;
   int64_t kps;
 };
@@ -26,17 +26,17 @@ template <class T> hipError_t launch_op_linear(const OpPlan& pl, int la, int lb,
 template <class T> hipError_t launch_op_gate(const OpPlan& pl, TileParams P, const EpiGate<T>& E, float* part, hipStream_t s);
 template <class T> hipError_t launch_op_gate_grad(const OpPlan& pl, TileParams P, const EpiGateGrad<T>& E, float* part, hipStream_t s);
 
-// dz = dy act'(z) into dz ([rows x ldz], columns up to ldz written, zeros past
-// cols) and, with partial, its column sums per block of rows.
+// dz = dy d (d: the kept act'(z)) into dz ([rows x ldz], columns up to ldz
+// written, zeros past cols) and, with partial, its column sums per block of
+// rows.
 struct DzParams {
   const void* dy;
-  const void* z;   // as keep() wrote it (zlo: its second plane); null: dz = dy
-  int64_t zlo;
+  const void* d;   // as keep() wrote it, in rows of ldz (dlo: its second plane); null: dz = dy
+  int64_t dlo;
   void* dz;        // null: only the sums
   float* partial;  // [row blocks][cols], or null
   int64_t rows, cols, ldy, ldz;
   int64_t rows_per_block;
-  int act;
   int wide;        // every row of dy is 16-byte aligned
 };
 template <class T> hipError_t launch_dz(const DzParams& P, hipStream_t s);

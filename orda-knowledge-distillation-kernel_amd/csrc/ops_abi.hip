@@ -50,13 +50,50 @@ struct Shape {
   bool pair;          // two products side by side (A's columns)
 };
 
-// The ring engine's limits: more than one K step, MN-major operands within a
-// buffer resource (2^31 bytes of K rows).
-bool ring_fits(const Shape& q) {
-  const int64_t lim = 0x7fffffffll / 2;
-  return q.dtype != ORDA_F32 && q.K > 64 && (q.la == KMAJ || q.K * q.lda < lim) && (q.lb == KMAJ || q.K * q.ldb < lim);
+// Splits without which a split's MN-major K rows would pass a buffer resource
+// (2^31 bytes).
+int64_t splits_needed(const Shape& q) {
+  const int64_t row = std::max<int64_t>(q.la == MNMAJ ? q.lda : 0, q.lb == MNMAJ ? q.ldb : 0) * 2;
+  const int64_t rows = std::max<int64_t>(64, row ? (0x7fffffffll / row) / 64 * 64 : up(q.K, 64));
+  return cdiv(q.K, rows);
+}
+
+// Estimated microseconds of a 16-bit product, from a sweep of 18 shapes (20 x
+// 1024 x 1024 to 8192 x 4096 x 2048) in the three layouts over tiles and
+// splits.  A K step of 64 takes the CU `step` per workgroup on it, and at least
+// `alone`; the ring engine 1.45 us per step of its 256 x 256 tiles (one
+// workgroup per CU) and 8 per tile for the epilogue.  Partials go out and back
+// at 8 TB/s (they stay in the caches), their sum is one more launch.
+//   1024^3: 64 x 64 8.2 us (model 8.1), 64 x 128 10.2, 128 x 128 14.5
+//   2048 x 4096 x 1024: 128 x 128 23.6 us (22), 64 x 64 30.8 (27), ring 37 (39)
+//   8192 x 4096 x 2048: ring 118 us (116), 128 x 128 135 (132)
+//   512 x 1024 x 2736: 64 x 64 in 2 ranges 13.1 us (13.9), in one 14.9 (15.7)
+struct TileCost {
+  int bm, bn;
+  double fixed, step, alone;
+};
+constexpr TileCost kTileCosts[] = {{64, 64, 3.8, 0.19, 0.27}, {64, 128, 4.8, 0.33, 0.33}, {128, 128, 6.0, 0.49, 0.58}};
+constexpr double kCus = 256.0;
+
+double split_cost(const Shape& q, int64_t sp) {
+  return sp == 1 ? 0.0 : 3.0 + (double)sp * q.M * q.cols * (q.dual ? 2 : 1) * 8.0 / 8e6;
+}
+double tile_cost(const Shape& q, const TileCost& t, int64_t sp) {
+  const double items = (double)(cdiv(q.M, t.bm) * cdiv(q.cols, q.dual ? t.bn / 2 : t.bn) * sp);
+  const double per_cu = std::ceil(items / kCus), steps = (double)cdiv(cdiv(q.K, sp), 64);
+  return t.fixed + steps * (per_cu <= 1 ? std::max(t.alone, t.step) : per_cu * t.step) + split_cost(q, sp);
 }
 int64_t ring_items(const Shape& q) { return cdiv(q.M, 256) * (q.pair ? 2 : 1) * cdiv(q.cols, q.dual ? 128 : 256); }
+double ring_cost(const Shape& q, int64_t sp) {
+  const double rounds = std::ceil((double)(ring_items(q) * sp) / kCus);
+  return 8.0 + rounds * ((double)cdiv(cdiv(q.K, sp), 64) * 1.45 + 8.0) + split_cost(q, sp);
+}
+// The ring engine takes more than one K step, and of a K-major operand whole
+// K ranges only.
+bool ring_fits(const Shape& q, int64_t sp) {
+  if (q.K <= 64 * sp || sp < splits_needed(q)) return false;
+  return sp == 1 || (q.la == MNMAJ && !q.pair) || q.K % (64 * sp) == 0;
+}
 
 OpPlan plan_of(const Shape& q) {
   OpPlan pl{};
@@ -67,35 +104,44 @@ OpPlan plan_of(const Shape& q) {
     return pl;
   }
   const int64_t steps = cdiv(q.K, 64);
-  int64_t want;
+  int64_t splits = 1;
+  double best = 1e300;
   if (q.dtype == ORDA_F32) {
     pl.engine = OP_SPLIT3;
     const double n = (double)q.cols * (q.dual ? 2 : 1);
-    double best = 0;
     for (int large = 0; large < 2; ++large)
       for (int64_t sp = 1; sp <= 16 && sp * 2 <= steps + 1; ++sp) {
         const double c = s3_cost((double)q.M, n, (double)q.K, (int)sp, large != 0);
-        if (pl.tile == 0 || c < best) {
+        if (c < best) {
           best = c;
           pl.tile = large ? 256 : 64;
-          pl.splits = (int)sp;
+          splits = sp;
         }
       }
-    want = pl.splits;
-  } else if (ring_fits(q) && ring_items(q) >= 200) {
-    pl.engine = OP_RING;
-    pl.tile = 256;
-    pl.kps = q.K;
-    return pl;
   } else {
-    pl.engine = OP_TILE;
-    auto items = [&](int64_t t) { return cdiv(q.M, t) * cdiv(q.cols, q.dual ? t / 2 : t); };
-    pl.tile = items(128) >= 256 ? 128 : 64;
-    const int64_t have = items(pl.tile), room = pl.tile == 128 ? 512 : 768;
-    want = std::max<int64_t>(1, std::min<int64_t>({room / have, steps / 8, 16}));
+    const int64_t need = splits_needed(q), most = std::max<int64_t>(need, std::min<int64_t>(16, std::max<int64_t>(1, steps / 2)));
+    for (int64_t sp = need; sp <= (q.pair ? need : most); ++sp) {
+      for (const TileCost& t : kTileCosts) {
+        if (q.pair) break;  // (the ring engine alone has pairs)
+        const double c = tile_cost(q, t, sp);
+        if (c < best) {
+          best = c;
+          pl.engine = OP_TILE;
+          pl.tile = t.bm * 1000 + t.bn;
+          splits = sp;
+        }
+      }
+      if (ring_fits(q, sp) && ring_cost(q, sp) < best) {
+        best = ring_cost(q, sp);
+        pl.engine = OP_RING;
+        pl.tile = 256;
+        splits = sp;
+      }
+    }
   }
-  if (want > 1) {
-    pl.kps = up(cdiv(q.K, want), 64);
+  if (pl.engine == OP_RING && splits == 1) pl.kps = q.K;
+  if (splits > 1) {
+    pl.kps = up(cdiv(q.K, splits), 64);
     pl.splits = (int)cdiv(q.K, pl.kps);
   }
   return pl;
@@ -255,23 +301,23 @@ size_t orda_linear_workspace_bytes(const orda_linear_t* p, int32_t backward) {
 }
 
 int orda_linear_forward(const orda_linear_t* p, const void* x, const void* weight, const void* bias, const void* residual,
-                        void* y, void* z, void* workspace, size_t workspace_bytes, void* stream) {
+                        void* y, void* d, void* workspace, size_t workspace_bytes, void* stream) {
   set_last_error(0, nullptr);
   LinearShapes s;
   OP_TRY(linear_shapes(p, s));
   if (!x || !weight || !y) return fail(ORDA_EINVAL, "orda_linear_forward: x, weight and y are required");
-  if (!aligned16(x) || !aligned16(weight) || !aligned16(z)) return fail(ORDA_EINVAL, "orda_linear_forward: x, weight and z must be 16-byte aligned");
+  if (!aligned16(x) || !aligned16(weight) || !aligned16(d)) return fail(ORDA_EINVAL, "orda_linear_forward: x, weight and d must be 16-byte aligned");
   if (residual && p->ldr < p->out_features) return fail(ORDA_EINVAL, "orda_linear_forward: ldr must be at least out_features");
   OP_TRY(check_workspace("orda_linear_forward", workspace, workspace_bytes, linear_ws(p, s, false)));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return by_dtype(p->dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     EpiLinear<T> e = store_to<T>(y, p->out_features, p->out_features, p->dtype);
-    e.z = z;
-    e.zlo = 2 * p->tokens * s.op;
+    e.d = d;
+    e.dlo = 2 * p->tokens * s.op;
     e.bias = static_cast<const T*>(bias);
     e.res = static_cast<const T*>(residual);
-    e.ldz = s.op;
+    e.ldd = s.op;
     e.ldr = p->ldr;
     e.act = p->activation;
     e.wide = e.wide && rows_aligned(residual, p->ldr, p->dtype) && aligned16(bias);
@@ -281,17 +327,17 @@ int orda_linear_forward(const orda_linear_t* p, const void* x, const void* weigh
   });
 }
 
-int orda_linear_backward(const orda_linear_t* p, const void* x, const void* weight, const void* z, const void* grad_output,
+int orda_linear_backward(const orda_linear_t* p, const void* x, const void* weight, const void* d, const void* grad_output,
                          void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
                          void* stream) {
   set_last_error(0, nullptr);
   LinearShapes s;
   OP_TRY(linear_shapes(p, s));
   if (!grad_output) return fail(ORDA_EINVAL, "orda_linear_backward: grad_output is required");
-  if (p->activation != ORDA_ACT_NONE && !z) return fail(ORDA_EINVAL, "orda_linear_backward: z is required with an activation");
+  if (p->activation != ORDA_ACT_NONE && !d) return fail(ORDA_EINVAL, "orda_linear_backward: d is required with an activation");
   if ((grad_x && !weight) || (grad_weight && !x)) return fail(ORDA_EINVAL, "orda_linear_backward: grad_x needs weight, grad_weight needs x");
-  if (!aligned16(x) || !aligned16(weight) || !aligned16(z) || !aligned16(grad_x) || !aligned16(grad_weight))
-    return fail(ORDA_EINVAL, "orda_linear_backward: x, weight, z, grad_x and grad_weight must be 16-byte aligned");
+  if (!aligned16(x) || !aligned16(weight) || !aligned16(d) || !aligned16(grad_x) || !aligned16(grad_weight))
+    return fail(ORDA_EINVAL, "orda_linear_backward: x, weight, d, grad_x and grad_weight must be 16-byte aligned");
   if (grad_x) OP_TRY(check_pitch("orda_linear_backward", "ldgx", p->ldgx, p->in_features, p->dtype));
   if (grad_weight) OP_TRY(check_pitch("orda_linear_backward", "ldgw", p->ldgw, p->in_features, p->dtype));
   OP_TRY(check_workspace("orda_linear_backward", workspace, workspace_bytes, linear_ws(p, s, true)));
@@ -310,20 +356,19 @@ int orda_linear_backward(const orda_linear_t* p, const void* x, const void* weig
     const bool products = grad_x || grad_weight;
     const void* dz = direct ? grad_output : own_dz;
     if (grad_bias || (products && !direct)) {
-      DzParams d{};
-      d.dy = grad_output;
-      d.z = act ? z : nullptr;
-      d.zlo = 2 * p->tokens * s.op;
-      d.dz = products && !direct ? own_dz : nullptr;
-      d.partial = grad_bias ? sums : nullptr;
-      d.rows = p->tokens;
-      d.cols = p->out_features;
-      d.ldy = p->out_features;
-      d.ldz = s.op;
-      d.rows_per_block = s.rows_per_block;
-      d.act = p->activation;
-      d.wide = aligned;
-      OP_LAUNCH(launch_dz<T>(d, st));
+      DzParams z{};
+      z.dy = grad_output;
+      z.d = act ? d : nullptr;
+      z.dlo = 2 * p->tokens * s.op;
+      z.dz = products && !direct ? own_dz : nullptr;
+      z.partial = grad_bias ? sums : nullptr;
+      z.rows = p->tokens;
+      z.cols = p->out_features;
+      z.ldy = p->out_features;
+      z.ldz = s.op;
+      z.rows_per_block = s.rows_per_block;
+      z.wide = aligned;
+      OP_LAUNCH(launch_dz<T>(z, st));
       if (grad_bias) OP_LAUNCH(launch_colsum<T>(sums, s.blocks, p->out_features, grad_bias, st));
     }
     if (grad_x) {
@@ -358,22 +403,22 @@ size_t orda_ffn_workspace_bytes(const orda_ffn_t* p, int32_t backward) {
 }
 
 int orda_ffn_forward(const orda_ffn_t* p, const void* x, const void* w_gate, const void* w_up, const void* w_down,
-                     const void* residual, void* y, void* h, void* a, void* b, void* workspace, size_t workspace_bytes,
+                     const void* residual, void* y, void* h, void* da_factor, void* db_factor, void* workspace, size_t workspace_bytes,
                      void* stream) {
   set_last_error(0, nullptr);
   FfnShapes s;
   OP_TRY(ffn_shapes(p, s));
   if (!x || !w_gate || !w_up || !w_down || !y || !h) return fail(ORDA_EINVAL, "orda_ffn_forward: x, the three weights, y and h are required");
-  if ((a == nullptr) != (b == nullptr)) return fail(ORDA_EINVAL, "orda_ffn_forward: a and b are kept together");
-  for (const void* q : {x, w_gate, w_up, w_down, (const void*)h, (const void*)a, (const void*)b})
-    if (!aligned16(q)) return fail(ORDA_EINVAL, "orda_ffn_forward: x, the weights, h, a and b must be 16-byte aligned");
+  if ((da_factor == nullptr) != (db_factor == nullptr)) return fail(ORDA_EINVAL, "orda_ffn_forward: the two factors are kept together");
+  for (const void* q : {x, w_gate, w_up, w_down, (const void*)h, (const void*)da_factor, (const void*)db_factor})
+    if (!aligned16(q)) return fail(ORDA_EINVAL, "orda_ffn_forward: x, the weights, h and the factors must be 16-byte aligned");
   if (residual && p->ldr < p->out_features) return fail(ORDA_EINVAL, "orda_ffn_forward: ldr must be at least out_features");
   OP_TRY(check_workspace("orda_ffn_forward", workspace, workspace_bytes, ffn_ws(p, s, false)));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   float* part = reinterpret_cast<float*>(base256(workspace));
   return by_dtype(p->dtype, [&](auto tag) -> int {
     using T = decltype(tag);
-    EpiGate<T> g{static_cast<T*>(h), a, b, s.fp, s.fp, 2 * p->tokens * s.fp, p->activation};
+    EpiGate<T> g{static_cast<T*>(h), da_factor, db_factor, s.fp, s.fp, 2 * p->tokens * s.fp, p->activation};
     TileParams t = product<T>(x, p->ldx, w_gate, p->ldw, p->tokens, p->inner, s.gate.K);
     t.B1 = w_up;
     OP_LAUNCH(launch_op_gate<T>(plan_of(s.gate), t, g, part, st));
@@ -388,18 +433,18 @@ int orda_ffn_forward(const orda_ffn_t* p, const void* x, const void* w_gate, con
 }
 
 int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, const void* w_up, const void* w_down,
-                      const void* h, const void* a, const void* b, const void* grad_output, void* grad_x, void* grad_gate,
+                      const void* h, const void* da_factor, const void* db_factor, const void* grad_output, void* grad_x, void* grad_gate,
                       void* grad_up, void* grad_down, void* workspace, size_t workspace_bytes, void* stream) {
   set_last_error(0, nullptr);
   FfnShapes s;
   OP_TRY(ffn_shapes(p, s));
-  if (!x || !w_gate || !w_up || !w_down || !h || !a || !b || !grad_output)
-    return fail(ORDA_EINVAL, "orda_ffn_backward: x, the three weights, h, a, b and grad_output are required");
+  if (!x || !w_gate || !w_up || !w_down || !h || !da_factor || !db_factor || !grad_output)
+    return fail(ORDA_EINVAL, "orda_ffn_backward: x, the three weights, h, the two factors and grad_output are required");
   OP_TRY(check_pitch("orda_ffn_backward", "ldg", p->ldg, p->out_features, p->dtype));
   if (grad_x) OP_TRY(check_pitch("orda_ffn_backward", "ldgx", p->ldgx, p->hidden, p->dtype));
   if (grad_gate || grad_up) OP_TRY(check_pitch("orda_ffn_backward", "ldgw", p->ldgw, p->hidden, p->dtype));
   if (grad_down) OP_TRY(check_pitch("orda_ffn_backward", "ldgd", p->ldgd, p->inner, p->dtype));
-  for (const void* q : {x, w_gate, w_up, w_down, h, a, b, grad_output, (const void*)grad_x, (const void*)grad_gate, (const void*)grad_up, (const void*)grad_down})
+  for (const void* q : {x, w_gate, w_up, w_down, h, da_factor, db_factor, grad_output, (const void*)grad_x, (const void*)grad_gate, (const void*)grad_up, (const void*)grad_down})
     if (!aligned16(q)) return fail(ORDA_EINVAL, "orda_ffn_backward: every tensor must be 16-byte aligned");
   OP_TRY(check_workspace("orda_ffn_backward", workspace, workspace_bytes, ffn_ws(p, s, true)));
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -409,7 +454,7 @@ int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, co
   return by_dtype(p->dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     if (grad_x || grad_gate || grad_up) {
-      const EpiGateGrad<T> e{reinterpret_cast<T*>(d), a, b, 2 * s.fp, s.fp, s.fp, 2 * p->tokens * s.fp, p->activation};
+      const EpiGateGrad<T> e{reinterpret_cast<T*>(d), da_factor, db_factor, 2 * s.fp, s.fp, s.fp, 2 * p->tokens * s.fp};
       TileParams t = product<T>(grad_output, p->ldg, w_down, p->ldd, p->tokens, p->inner, s.dh.K);
       t.kval = p->out_features;
       OP_LAUNCH(launch_op_gate_grad<T>(plan_of(s.dh), t, e, part, st));
@@ -423,7 +468,7 @@ int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, co
     }
     Shape both = s.dw;
     both.pair = true;
-    const bool pair = grad_gate && grad_up && plan_of(both).engine == OP_RING;
+    const bool pair = grad_gate && grad_up && p->dtype != ORDA_F32 && plan_of(s.dw).engine == OP_RING && plan_of(s.dw).splits == 1;
     if (pair) {  // one launch: its tiles fill the chip's last round better than two launches' do
       TileParams t = product<T>(d, 2 * s.fp, x, p->ldx, p->inner, s.dw.cols, p->tokens);
       t.pair = s.fp;

@@ -20,7 +20,7 @@ template <class T, int LA, int LB, class Epi>
 __global__ __launch_bounds__(kThreads4, 1) void k_ring(TileParams P, Epi E0) {
   constexpr bool DUAL = Epi::kDual;
   static_assert(LA == LB || (LA == KMAJ && LB == MNMAJ), "K/K, K/MN or MN/MN");
-  static_assert(!DUAL || LB == KMAJ, "two weights are K-major");
+  static_assert(!DUAL || (LB == KMAJ && !Epi::kLight), "two weights are K-major, and nothing is loaded for them");
   __shared__ __attribute__((aligned(16))) char lds[kLds4Bytes];
   Acc16 acc;
   zero_acc16(acc);
@@ -93,8 +93,25 @@ __global__ __launch_bounds__(kThreads4, 1) void k_ring(TileParams P, Epi E0) {
     char* buf = slot + wave_id() * 8192;
     const int64_t nlim = E.cols - x.n0;  // columns left from the tile's first one
     const int64_t mw = x.m0 + wm * 128;
-#pragma unroll
-    for (int mb = 0; mb < 8; ++mb) {
+    constexpr int kIt = DUAL ? 2 : 4;
+    struct Item {
+      int64_t m;
+      int row, g, col, cnt;
+      bool live;
+    };
+    auto item = [&](int mb, int it) __attribute__((always_inline)) {
+      const int i = it * 64 + lane;
+      Item q;
+      q.row = DUAL ? i >> 3 : i >> 4;
+      q.g = DUAL ? i & 7 : i & 15;
+      q.col = (q.g >> 3) * 128 + wn * 64 + (q.g & 7) * 8;
+      q.m = mw + mb * 16 + q.row;
+      const int64_t left = nlim - q.col;
+      q.cnt = left >= 8 ? 8 : (int)left;
+      q.live = q.m < P.M && q.cnt > 0;
+      return q;
+    };
+    auto dump = [&](int mb) __attribute__((always_inline)) {
       const int r = lane & 15;
 #pragma unroll
       for (int nb = 0; nb < 8; ++nb) {
@@ -106,28 +123,74 @@ __global__ __launch_bounds__(kThreads4, 1) void k_ring(TileParams P, Epi E0) {
         v.w = acc16_get(c[mb][nb], 3);
         *reinterpret_cast<float4*>(buf + r * 512 + ((ch ^ r) << 4)) = v;
       }
-      auto take = [&](int row, int g, float (&v)[8]) __attribute__((always_inline)) {
-        const float4 a = *reinterpret_cast<const float4*>(buf + row * 512 + (((2 * g) ^ row) << 4));
-        const float4 d = *reinterpret_cast<const float4*>(buf + row * 512 + (((2 * g + 1) ^ row) << 4));
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = d.x; v[5] = d.y; v[6] = d.z; v[7] = d.w;
+    };
+    auto take = [&](int row, int g, float (&v)[8]) __attribute__((always_inline)) {
+      const float4 a = *reinterpret_cast<const float4*>(buf + row * 512 + (((2 * g) ^ row) << 4));
+      const float4 d = *reinterpret_cast<const float4*>(buf + row * 512 + (((2 * g + 1) ^ row) << 4));
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = d.x; v[5] = d.y; v[6] = d.z; v[7] = d.w;
+    };
+    typedef typename Epi::template Pre<8> Pre;
+    if constexpr (Epi::kLight) {
+      // little code per element: all unrolled, each item's loads one row block
+      // (four items) ahead of their use.  With the loads where they are used,
+      // dh's epilogue (8192 tokens, 4096 x 14336) took 1070 us in all.
+      Pre p[kIt];
+#pragma unroll
+      for (int it = 0; it < kIt; ++it) {
+        const Item q = item(0, it);
+        if (q.live) p[it] = E.template pre<8>(q.m, x.n0 + q.col, q.cnt);
+      }
+#pragma unroll
+      for (int mb = 0; mb < 8; ++mb) {
+        dump(mb);
+#pragma unroll
+        for (int it = 0; it < kIt; ++it) {
+          const Item q = item(mb, it);
+          float v[8];
+          take(q.row, q.g, v);
+          const Pre now = p[it];
+          if (mb < 7) {
+            const Item f = item(mb + 1, it);
+            if (f.live) p[it] = E.template pre<8>(f.m, x.n0 + f.col, f.cnt);
+          }
+          if (q.live) E(q.m, x.n0 + q.col, v, q.cnt, now, {});
+        }
+      }
+    } else {
+      // much code per element: a loop over a row block's items, with the loads
+      // of the next block's items in flight; a lane has the same columns in all
+      Pre p[2][kIt];
+      auto fetch = [&](int mb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int it = 0; it < kIt; ++it) {
+          const Item q = item(mb, it);
+          if (q.live) p[mb & 1][it] = E.template pre<8>(q.m, x.n0 + q.col, q.cnt);
+        }
       };
+      const Item first = item(0, 0);
+      const auto col = E.template col<8>(x.n0 + first.col, first.cnt);
+      fetch(0);
+#pragma unroll
+      for (int mb = 0; mb < 8; ++mb) {
+        if (mb < 7) fetch(mb + 1);
+        dump(mb);
 #pragma unroll 1
-      for (int it = 0; it < (DUAL ? 2 : 4); ++it) {
-        const int i = it * 64 + lane;
-        const int row = DUAL ? i >> 3 : i >> 4, g = DUAL ? i & 7 : i & 15;
-        const int col = (g >> 3) * 128 + wn * 64 + (g & 7) * 8;
-        const int64_t m = mw + mb * 16 + row;
-        const int64_t left = nlim - col;
-        const int cnt = left >= 8 ? 8 : (int)left;
-        float v[8];
-        take(row, g, v);
-        if constexpr (DUAL) {
-          float u[8];
-          take(row, g + 8, u);
-          if (m < P.M && cnt > 0) E(m, x.n0 + col, v, u, cnt);
-        } else {
-          if (m < P.M && cnt > 0) E(m, x.n0 + col, v, cnt);
+        for (int it = 0; it < kIt; ++it) {
+          const Item q = item(mb, it);
+          float v[8];
+          take(q.row, q.g, v);
+          if constexpr (DUAL) {
+            float u[8];
+            take(q.row, q.g + 8, u);
+            if (q.live) E(q.m, x.n0 + q.col, v, u, q.cnt, p[mb & 1][0], col);
+          } else {
+            Pre now = p[mb & 1][0];
+            if (it == 1) now = p[mb & 1][1];
+            if (it == 2) now = p[mb & 1][2];
+            if (it == 3) now = p[mb & 1][3];
+            if (q.live) E(q.m, x.n0 + q.col, v, q.cnt, now, col);
+          }
         }
       }
     }

@@ -114,9 +114,9 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void k_skinny(SkinnyParams P, Ep
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (n + e >= P.N) v[e] = u[e] = 0.f;
-    E(r, n, v, u, cnt);
+    epi_apply(E, r, n, v, u, cnt);
   } else {
-    E(r, n, v, cnt);
+    epi_apply(E, r, n, v, cnt);
   }
 }
 

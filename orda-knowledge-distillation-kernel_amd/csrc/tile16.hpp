@@ -39,28 +39,77 @@ struct TileParams {
 
 template <int R>
 __device__ __forceinline__ int mn_f(int k) {
-  return R == 128 ? (k & 3) | (((k >> 3) & 1) << 2) : ((k >> 1) & 1) | (((k >> 3) & 1) << 1);
+  return R >= 128 ? (k & 3) | (((k >> 3) & 1) << 2) : ((k >> 1) & 1) | (((k >> 3) & 1) << 1);
 }
 
-// Fragment (8 K values of row row0 + lane % 16, K 32 hf + 8 (lane / 16) ..).
-template <class T, int L, int R>
-__device__ __forceinline__ typename Traits<T>::Frag tile_frag(const char* t, int row0, int hf, int lane) {
-  if constexpr (L == KMAJ) {
-    const int r = row0 + (lane & 15);
-    return *reinterpret_cast<const typename Traits<T>::Frag*>(t + r * 128 + (((hf * 4 + (lane >> 4)) ^ kswz(r)) << 4));
-  } else {
-    typedef short s4 __attribute__((ext_vector_type(4)));
-    const int k = hf * 32 + 8 * (lane >> 4) + ((lane & 15) >> 2);
-    const int m = row0 + 4 * (lane & 3);
-    const char* p = t + k * (2 * R) + (((m >> 3) ^ (mn_f<R>(k) << 1)) << 4) + (m & 7) * 2;
-    auto rd = [](const char* q) {
-      return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)q);
-    };
-    const s4 lo = rd(p), hi = rd(p + 4 * (2 * R));  // (f(k + 4) = f(k))
-    typedef short s8 __attribute__((ext_vector_type(8)));
-    const s8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    return __builtin_bit_cast(typename Traits<T>::Frag, both);
+// Where a lane reads its fragments of one operand: 8 K values of row
+// row0 + lane % 16 at K 32 hf + 8 (lane / 16).., for blocks of 16 rows row0 =
+// r0, r0 + 16, .. .  K-major: one address per half, the block's offset an
+// immediate.  MN-major: two transposed reads four K rows apart; the block
+// enters an exclusive or with the lane's swizzle, so one address per block,
+// the half an immediate.
+template <class T, int L, int R, int NBLK>
+struct TileFrags {
+  static constexpr int kHalf = 32 * 2 * R, kFour = 4 * 2 * R;  // MN-major: 32 and 4 K rows on
+  uint32_t at[L == KMAJ ? 2 : NBLK];
+  template <class Row>
+  __device__ __forceinline__ void init(const Row& row0) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (L == KMAJ) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = lane & 15;
+        at[h] = (uint32_t)((row0(0) + r) * 128 + (((h * 4 + (lane >> 4)) ^ kswz(r)) << 4));
+      }
+    } else {
+      const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
+#pragma unroll
+      for (int i = 0; i < NBLK; ++i) {
+        const int m = row0(i) + 4 * (lane & 3);
+        at[i] = (uint32_t)(k * (2 * R) + (((m >> 3) ^ (mn_f<R>(k) << 1)) << 4) + (m & 7) * 2);
+      }
+    }
   }
+  // K-major; off: the block's rows past row0(0)
+  __device__ __forceinline__ typename Traits<T>::Frag read(const char* tile, int off, int hf) const {
+    static_assert(L == KMAJ, "transposed reads go through tr_read");
+    return *reinterpret_cast<const typename Traits<T>::Frag*>(tile + at[hf] + off * 128);
+  }
+};
+
+// Transposed reads of NB blocks (2 or 4) at LDS addresses a[] + OFF and a[] +
+// OFF + FOUR, waited for in the same block.  Assembly, because the compiler
+// waits for every DMA in flight before its own transposed read (it cannot tell
+// the stages apart): 4096 x 1024 x 4096, K-major x MN-major, took 103 us so.
+typedef short tr_s4 __attribute__((ext_vector_type(4)));
+typedef short tr_s8 __attribute__((ext_vector_type(8)));
+template <int OFF, int FOUR, int NB>
+__device__ __forceinline__ void tr_read(const uint32_t (&a)[NB], uint32_t tile, tr_s8 (&o)[NB]) {
+  static_assert(NB == 2 || NB == 4, "blocks");
+  static_assert(OFF + FOUR < 65536, "ds offset field");
+  tr_s4 x[NB][2];
+  if constexpr (NB == 2) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+        "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1])
+        : "v"(a[0] + tile), "v"(a[1] + tile), "n"(OFF), "n"(OFF + FOUR)
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1]), "=&v"(x[2][0]), "=&v"(x[2][1]),
+          "=&v"(x[3][0]), "=&v"(x[3][1])
+        : "v"(a[0] + tile), "v"(a[1] + tile), "v"(a[2] + tile), "v"(a[3] + tile), "n"(OFF), "n"(OFF + FOUR)
+        : "memory");
+  }
+#pragma unroll
+  for (int i = 0; i < NB; ++i) o[i] = __builtin_shufflevector(x[i][0], x[i][1], 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 typedef float f4v __attribute__((ext_vector_type(4)));
@@ -82,30 +131,25 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* p, int64
 template <class T, int L, int R>
 struct TileDma {
   static constexpr int NQ = R / 32;
+  static constexpr int kPer = L == KMAJ ? 8 : R / 8;  // 16-byte chunks of a tile row
   uint32_t row, chunk;  // K-major: row of chunk 0; MN-major: K row.  Logical 16-byte chunk
   __device__ __forceinline__ TileDma() {
-    const int w = wave_id(), lane = threadIdx.x & 63;
-    if constexpr (L == KMAJ) {
-      row = (uint32_t)(w * 8 + (lane >> 3));
-      chunk = (uint32_t)((lane & 7) ^ kswz((int)row));
-    } else if constexpr (R == 128) {
-      row = (uint32_t)(w * 4 + (lane >> 4));
-      chunk = (uint32_t)((lane & 15) ^ (mn_f<R>((int)row) << 1));
-    } else {
-      row = (uint32_t)(w * 8 + (lane >> 3));
-      chunk = (uint32_t)((lane & 7) ^ (mn_f<R>((int)row) << 1));
-    }
+    const int i = wave_id() * 64 + (threadIdx.x & 63);
+    row = (uint32_t)(i / kPer);
+    chunk = (uint32_t)((i % kPer) ^ (L == KMAJ ? kswz((int)row) : mn_f<R>((int)row) << 1));
   }
-  static constexpr int kRowStep = L == KMAJ ? 32 : (R == 128 ? 16 : 32);
-  // chunk q of the step at byte k0b of K (K-major; kb the K extent in bytes)
-  // or at the resource's first K row (MN-major; cols valid columns)
-  __device__ __forceinline__ void issue(__amdgpu_buffer_rsrc_t r, uint32_t ldb, uint32_t k0b, uint32_t kb, int64_t cols,
-                                        int q, char* tile) const {
-    uint32_t off;
-    if constexpr (L == KMAJ) off = k0b + chunk * 16 < kb ? row * ldb + chunk * 16 + k0b : kOob;
-    else off = (int64_t)chunk * 8 < cols ? row * ldb + chunk * 16 : kOob;
+  static constexpr int kRowStep = 256 / kPer;
+  // The thread's offset for chunk q (added by the caller: q kRowStep rows), or
+  // past every resource.  K-major: left = bytes of K from the step on;
+  // MN-major: left = valid columns.
+  __device__ __forceinline__ uint32_t off(uint32_t ldb, int left, int q) const {
+    // (MN-major rows of 512 bytes: K rows 8 apart differ in f's third bit)
+    const uint32_t c = L == MNMAJ && R == 256 && (q & 1) ? chunk ^ 8u : chunk;
+    return (int)(c * (L == KMAJ ? 16 : 8)) < left ? row * ldb + c * 16 : kOob;
+  }
+  static __device__ __forceinline__ void go(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t soff, int q, char* tile) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(tile + (q * 4 + wave_id()) * 1024),
-                                             16, off, (uint32_t)q * kRowStep * ldb, 0, 0);
+                                             16, off, soff, 0, 0);
   }
 };
 
@@ -134,49 +178,66 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
   const TileDma<T, LA, BM> da;
   const TileDma<T, LB, BN> db;
 
-  // K-major resources are fixed: rows from the tile's first one at K = 0
-  // (a K extent below 2^30 bytes, checked on the host)
-  __amdgpu_buffer_rsrc_t ra = tile_rsrc(A, 0), rb0 = ra, rb1 = ra;
-  if constexpr (LA == KMAJ) ra = tile_rsrc(A + m0 * ldab, lmin(P.M - m0, BM) * ldab);
-  if constexpr (LB == KMAJ) {
-    if constexpr (DUAL) {
-      rb0 = tile_rsrc(B + n0 * ldbb, lmin(P.N - n0, BN / 2) * ldbb);
-      // (rows BN / 2 .. of the tile are B1's first ones: the base is moved back)
-      rb1 = tile_rsrc(B1 + n0 * ldbb, lmin(P.N - n0, BN / 2) * ldbb);
-    } else {
-      rb0 = tile_rsrc(B + n0 * ldbb, lmin(P.N - n0, BN) * ldbb);
-    }
+  // Resources of the tile's rows (K-major) or of the split's K rows from the
+  // tile's first column on (MN-major), ending where the data does; a step adds
+  // a scalar offset.  A split's MN-major K rows span less than 2^31 bytes and
+  // a K-major row less than 2^23 (host).
+  const int64_t klen = ke - kb0;
+  __amdgpu_buffer_rsrc_t ra, rb0, rb1;
+  if constexpr (LA == KMAJ) ra = tile_rsrc(A + m0 * ldab + kb0 * 2, lmin(P.M - m0, BM) * ldab);
+  else ra = tile_rsrc(A + kb0 * ldab + m0 * 2, klen * ldab - m0 * 2);
+  rb1 = ra;
+  if constexpr (DUAL) {
+    rb0 = tile_rsrc(B + n0 * ldbb + kb0 * 2, lmin(P.N - n0, BN / 2) * ldbb);
+    rb1 = tile_rsrc(B1 + n0 * ldbb + kb0 * 2, lmin(P.N - n0, BN / 2) * ldbb);
+  } else if constexpr (LB == KMAJ) {
+    rb0 = tile_rsrc(B + n0 * ldbb + kb0 * 2, lmin(P.N - n0, BN) * ldbb);
+  } else {
+    // (B1's base lies kseg rows before it: both are addressed by the K row
+    // within the split)
+    rb0 = tile_rsrc(B + kb0 * ldbb + n0 * 2, (P.kval - kb0) * ldbb - n0 * 2);
+    if (B1) rb1 = tile_rsrc(B1 + (kb0 - P.kseg) * (int64_t)ldbb + n0 * 2, (P.kseg + P.kval - kb0) * ldbb - n0 * 2);
   }
-  auto issue = [&](int kt) __attribute__((always_inline)) {
-    char* st = lds + (kt % NS) * kStage;
-    const bool live = kt < nk;
-    const int64_t k0 = kb0 + (int64_t)kt * 64;
-    const uint32_t kend = live ? (uint32_t)(ke * 2) : 0u;
-    if constexpr (LA == MNMAJ) ra = tile_rsrc(A + k0 * ldab + m0 * 2, live ? lmin(ke - k0, 64) * ldab - m0 * 2 : 0);
-    if constexpr (LB == MNMAJ) {
-      const bool second = k0 >= P.kseg;
-      const int64_t kk = second ? k0 - P.kseg : k0;
-      rb0 = tile_rsrc((second ? B1 : B) + kk * ldbb + n0 * 2, live ? lmin(P.kval - kk, 64) * ldbb - n0 * 2 : 0);
+  const int seg = (int)lmin((P.kseg - kb0 + 63) / 64, 0x7fffffff);  // B1's first step
+  const int kbytes = (int)(klen * 2);
+  const int mleft = (int)lmin(P.M - m0, BM), nleft = (int)lmin(P.N - n0, BN);
+  uint32_t offa[TileDma<T, LA, BM>::NQ], offb[TileDma<T, LB, BN>::NQ];
+  if constexpr (LA == MNMAJ) {
+#pragma unroll
+    for (int q = 0; q < TileDma<T, LA, BM>::NQ; ++q) offa[q] = da.off(ldab, mleft, q);
+  }
+  if constexpr (LB == MNMAJ) {
+#pragma unroll
+    for (int q = 0; q < TileDma<T, LB, BN>::NQ; ++q) offb[q] = db.off(ldbb, nleft, q);
+  }
+  auto issue = [&](int kt, char* st) __attribute__((always_inline)) {
+    const int left = kbytes - kt * 128;  // (past the end: <= 0, zeros; the count of DMAs stays the same)
+    {
+      const uint32_t o = LA == KMAJ ? da.off(ldab, left, 0) : 0u;
+      const uint32_t so = LA == KMAJ ? (uint32_t)kt * 128u : (uint32_t)kt * 64u * ldab;
+#pragma unroll
+      for (int q = 0; q < TileDma<T, LA, BM>::NQ; ++q)
+        da.go(ra, LA == KMAJ ? o : (left > 0 ? offa[q] : kOob), so + (uint32_t)(q * TileDma<T, LA, BM>::kRowStep) * ldab, q, st);
     }
+    {
+      const uint32_t o = LB == KMAJ ? db.off(ldbb, left, 0) : 0u;
+      const uint32_t so = LB == KMAJ ? (uint32_t)kt * 128u : (uint32_t)kt * 64u * ldbb;
+      constexpr int H = TileDma<T, LB, BN>::NQ / 2;
 #pragma unroll
-    for (int q = 0; q < TileDma<T, LA, BM>::NQ; ++q) da.issue(ra, ldab, (uint32_t)(k0 * 2), kend, P.M - m0, q, st);
-#pragma unroll
-    for (int q = 0; q < TileDma<T, LB, BN>::NQ; ++q) {
-      if constexpr (DUAL) {
-        constexpr int H = TileDma<T, LB, BN>::NQ / 2;
-        const auto r = q < H ? rb0 : rb1;
-        uint32_t off = (uint32_t)(k0 * 2) + db.chunk * 16 < kend ? db.row * ldbb + db.chunk * 16 + (uint32_t)(k0 * 2) : kOob;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            r, (__attribute__((address_space(3))) void*)(st + kA + (q * 4 + wave_id()) * 1024), 16, off,
-            (uint32_t)(q < H ? q : q - H) * 32u * ldbb, 0, 0);
-      } else {
-        db.issue(rb0, ldbb, (uint32_t)(k0 * 2), kend, P.N - n0, q, st + kA);
+      for (int q = 0; q < TileDma<T, LB, BN>::NQ; ++q) {
+        const bool two = DUAL ? q >= H : (LB == MNMAJ && LA == KMAJ && kt >= seg);
+        db.go(two ? rb1 : rb0, LB == KMAJ ? o : (left > 0 ? offb[q] : kOob),
+              so + (uint32_t)((DUAL && q >= H ? q - H : q) * TileDma<T, LB, BN>::kRowStep) * ldbb, q, st + kA);
       }
     }
   };
   const int w = wave_id(), wm = w >> 1, wn = w & 1;
   const int lane = threadIdx.x & 63;
   auto brow = [&](int nb) { return (nb / (NB / 2)) * (BN / 2) + wn * (BN / 4) + (nb % (NB / 2)) * 16; };
+  TileFrags<T, LA, BM, MB> fa;
+  TileFrags<T, LB, BN, NB> fb;
+  fa.init([&](int i) { return wm * (BM / 2) + i * 16; });
+  fb.init(brow);
   f4v acc[MB][NB];
 #pragma unroll
   for (int i = 0; i < MB; ++i)
@@ -184,26 +245,49 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
     for (int j = 0; j < NB; ++j) acc[i][j] = f4v{0.f, 0.f, 0.f, 0.f};
 
 #pragma unroll
-  for (int s = 0; s < NS - 1; ++s) issue(s);
+  for (int s = 0; s < NS - 1; ++s) issue(s, lds + s * kStage);
   constexpr int kDma = BM / 32 + BN / 32;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds;
+  int rd = 0, wr = (NS - 1) * kStage;  // the stages of step kt and of step kt + NS - 1
+#pragma unroll 1
   for (int kt = 0; kt < nk; ++kt) {
     wait_vmem<(NS - 2) * kDma>();  // step kt has landed
     tile_barrier();
-    issue(kt + NS - 1);  // (the slot of step kt - 1; past the end: zeros, so that the count above holds)
-    const char* sa = lds + (kt % NS) * kStage;
+    issue(kt + NS - 1, lds + wr);  // (the stage of step kt - 1)
+    const char* sa = lds + rd;
     const char* sb = sa + kA;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       Frag a[MB], b[NB];
+      if constexpr (LA == KMAJ) {
 #pragma unroll
-      for (int i = 0; i < MB; ++i) a[i] = tile_frag<T, LA, BM>(sa, wm * (BM / 2) + i * 16, hf, lane);
+        for (int i = 0; i < MB; ++i) a[i] = fa.read(sa, i * 16, hf);
+      }
+      if constexpr (LB == KMAJ) {
 #pragma unroll
-      for (int j = 0; j < NB; ++j) b[j] = tile_frag<T, LB, BN>(sb, brow(j), hf, lane);
+        for (int j = 0; j < NB; ++j) b[j] = fb.read(sb, (j / (NB / 2)) * (BN / 2) + (j % (NB / 2)) * 16, hf);
+      }
+      auto transposed = [&](const auto& f, uint32_t tile, auto& frags, auto half) __attribute__((always_inline)) {
+        using FR = std::remove_reference_t<decltype(f)>;
+        constexpr int N = sizeof(frags) / sizeof(frags[0]);
+        tr_s8 o[N];
+        tr_read<decltype(half)::value * FR::kHalf, FR::kFour, N>(f.at, tile, o);
+#pragma unroll
+        for (int i = 0; i < N; ++i) frags[i] = __builtin_bit_cast(Frag, o[i]);
+      };
+      auto both = [&](auto half) __attribute__((always_inline)) {
+        if constexpr (LB == MNMAJ) transposed(fb, lds0 + rd + kA, b, half);
+        if constexpr (LA == MNMAJ) transposed(fa, lds0 + rd, a, half);
+      };
+      if (hf == 0) both(std::integral_constant<int, 0>{});
+      else both(std::integral_constant<int, 1>{});
 #pragma unroll
       for (int i = 0; i < MB; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = mma16(b[j], a[i], acc[i][j]);
     }
+    wr = rd;
+    rd = rd + kStage == NS * kStage ? 0 : rd + kStage;
   }
   wait_vmem<0>();  // nothing may land after the waves end
 
@@ -221,9 +305,9 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
         if constexpr (DUAL) {
           const f4v c = acc[i][j + NB / 2];
           float u[4] = {c[0], c[1], c[2], c[3]};
-          E(m, n, v, u, cnt);
+          epi_apply(E, m, n, v, u, cnt);
         } else {
-          E(m, n, v, cnt);
+          epi_apply(E, m, n, v, cnt);
         }
       }
     }

@@ -135,9 +135,9 @@ __global__ __launch_bounds__(C::kThreads, C::MB == 4 ? 2 : 3) void k_tile_s3(Til
           float v[4] = {acc[mb][nb][0], acc[mb][nb][1], acc[mb][nb][2], acc[mb][nb][3]};
           if constexpr (DUAL) {
             float u[4] = {acc[mb][nb + MB / 2][0], acc[mb][nb + MB / 2][1], acc[mb][nb + MB / 2][2], acc[mb][nb + MB / 2][3]};
-            E(m, n, v, u, cnt);
+            epi_apply(E, m, n, v, u, cnt);
           } else {
-            E(m, n, v, cnt);
+            epi_apply(E, m, n, v, cnt);
           }
         }
       }

@@ -4,13 +4,13 @@
 
 Two launches forward: both projections, the activation and the product in one kernel (a tile holds the same columns of Wg
 and Wu, so a lane has a's and b's element side by side), then the down projection with the residual in its epilogue.
-Backward, with dh = dy Wd never leaving the accumulators:
+A training call also keeps the factors p = b act'(a) and q = act(a).  Backward, with dh = dy Wd never leaving the accumulators:
 
-    da = dh b act'(a)    db = dh act(a)                        (epilogue of dh's product)
+    da = dh p    db = dh q                                     (epilogue of dh's product)
     dx = da Wg + db Wu   (one product over both weights)
     dWg = da^T x    dWu = db^T x    dWd = dy^T h
 
-h, da and db are rounded to the compute dtype as operands of the next product; a and b are kept in fp32, for 16-bit tensors
+h, da and db are rounded to the compute dtype as operands of the next product; p and q are kept in fp32, for 16-bit tensors
 in its upper 24 bits; products accumulate in fp32.  No counterpart in the reference, whose models use torch.
 """
 from __future__ import annotations
@@ -39,12 +39,12 @@ def _forward(x2, w_gate, w_up, w_down, res2, act: str, dtype, keep: bool):
     fp = _native.ffn_inner_pitch(p)
     y = torch.empty((N, O), dtype=dtype, device=x2.device)
     h = torch.empty((N, fp), dtype=dtype, device=x2.device)
-    a = b = None
+    fa = fb = None
     if keep:
         n = _native.ffn_saved_bytes(p)
-        a, b = (torch.empty(n, dtype=torch.uint8, device=x2.device) for _ in range(2))
-    _native.ffn_forward(p, xo, ga, up, dn, res2, y, h, a, b)
-    return y, (xo, ga, up, dn, h, a, b), p
+        fa, fb = (torch.empty(n, dtype=torch.uint8, device=x2.device) for _ in range(2))
+    _native.ffn_forward(p, xo, ga, up, dn, res2, y, h, fa, fb)
+    return y, (xo, ga, up, dn, h, fa, fb), p
 
 
 class GatedFeedForwardFunction(torch.autograd.Function):
@@ -62,7 +62,7 @@ class GatedFeedForwardFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        xo, ga, up, dn, h, a, b = ctx.saved_tensors
+        xo, ga, up, dn, h, fa, fb = ctx.saved_tensors
         given, need = ctx.given, ctx.needs_input_grad
         g_r = grad_y.to(given[4][1]) if given[4] is not None and need[4] else None
         grads = [None] * 4
@@ -74,7 +74,7 @@ class GatedFeedForwardFunction(torch.autograd.Function):
             mult = 4 if ctx.dtype == torch.float32 else 8
             p.ldgx = p.ldgw = p.hidden + (-p.hidden) % mult
             p.ldgd = p.inner + (-p.inner) % mult
-            _native.ffn_backward(p, xo, ga, up, dn, h, a, b, dy, *grads)
+            _native.ffn_backward(p, xo, ga, up, dn, h, fa, fb, dy, *grads)
         return (*[trim(v, g[0][1], g[0], g[1]) for v, g in zip(grads, given)], g_r, None)
 
 
@@ -87,7 +87,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     ``x`` is ``(..., hidden)``, ``w_gate`` and ``w_up`` ``(inner, hidden)`` (two halves of one tensor serve), ``w_down``
     ``(out_features, inner)``, ``residual`` ``(..., out_features)``; ``activation`` one of ``none``, ``relu``, ``gelu``,
     ``gelu_tanh``, ``silu``, ``sigmoid``.  Dtypes, strides, alignment and ``backend`` as :func:`fused_linear`.  A training
-    call keeps h, a and b for its backward pass: 8 bytes (fp32: 12) per token and inner column."""
+    call keeps h and two factors for its backward pass: 8 bytes (fp32: 12) per token and inner column."""
     check_tensors("gated_feed_forward", activation, x, w_gate=w_gate, w_up=w_up, w_down=w_down, residual=residual)
     if w_gate.ndim != 2 or w_gate.shape[1] != x.shape[-1] or w_gate.shape[0] == 0:
         raise ValueError(f"gated_feed_forward: w_gate must have shape (inner, {x.shape[-1]}), got {tuple(w_gate.shape)}")

@@ -22,7 +22,7 @@ __all__ = ["FusedLinearFunction", "fused_linear"]
 
 
 def _forward(x2, weight, bias, res2, act: str, dtype, keep: bool):
-    """(y, operands, z, problem); z None where it is not needed."""
+    """(y, operands, d, problem); d None where it is not needed."""
     xo, wo = operand(x2, dtype), operand(weight, dtype)
     if bias is not None:
         bias = bias.to(dtype).contiguous()
@@ -33,11 +33,11 @@ def _forward(x2, weight, bias, res2, act: str, dtype, keep: bool):
                        tokens=x2.shape[0], in_features=x2.shape[1], out_features=O, ldx=pitch(xo), ldw=pitch(wo),
                        ldr=pitch(res2) if res2 is not None else 0)
     y = torch.empty((x2.shape[0], O), dtype=dtype, device=x2.device)
-    z = None
+    d = None
     if keep and act != "none":
-        z = torch.empty(_native.linear_saved_bytes(p), dtype=torch.uint8, device=x2.device)
-    _native.linear_forward(p, xo, wo, bias, res2, y, z)
-    return y, xo, wo, z, p
+        d = torch.empty(_native.linear_saved_bytes(p), dtype=torch.uint8, device=x2.device)
+    _native.linear_forward(p, xo, wo, bias, res2, y, d)
+    return y, xo, wo, d, p
 
 
 class FusedLinearFunction(torch.autograd.Function):
@@ -46,8 +46,8 @@ class FusedLinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation: str):
         dtype = default_compute_dtype(*[t for t in (x, weight) if t is not None])
-        y, xo, wo, z, p = _forward(x, weight, bias, residual, activation, dtype, True)
-        ctx.save_for_backward(xo, wo, z)
+        y, xo, wo, d, p = _forward(x, weight, bias, residual, activation, dtype, True)
+        ctx.save_for_backward(xo, wo, d)
         ctx.problem, ctx.dtype = p, dtype
         ctx.given = tuple(None if t is None else (t.shape, t.dtype) for t in (x, weight, bias, residual))
         return y
@@ -55,7 +55,7 @@ class FusedLinearFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        xo, wo, z = ctx.saved_tensors
+        xo, wo, d = ctx.saved_tensors
         (xs, xd), (ws, wd), b, r = ctx.given
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         g_r = grad_y.to(r[1]) if r is not None and need_r else None
@@ -68,7 +68,7 @@ class FusedLinearFunction(torch.autograd.Function):
             g_b = torch.empty(ws[0], dtype=ctx.dtype, device=dy.device) if need_b else None
             p = _native.Linear.from_buffer_copy(ctx.problem)
             p.ldgx = p.ldgw = new_pitch(xs[1], ctx.dtype)
-            _native.linear_backward(p, xo, wo, z, dy, g_x, g_w, g_b)
+            _native.linear_backward(p, xo, wo, d, dy, g_x, g_w, g_b)
         return (trim(g_x, xs[1], xs, xd), trim(g_w, ws[1], ws, wd), g_b.to(b[1]) if need_b else None, g_r, None)
 
 

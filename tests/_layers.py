@@ -4,7 +4,8 @@ u is half a step of the dtype relative to the value (eps / 2); `sub` half its sm
 fp32: gamma(K) = (K + 16) 2^-24 of the sum of magnitudes bounds any order of K additions, the exact products included (fp32
 operands: each product loses 2^-23 more).  Activations: |act'| <= 1.13, |act''| <= 1; the 16-bit kernels evaluate them with
 the hardware's exp2 and reciprocal, within 2^-19 (1 + |z|), fp32 with the library's functions, within 2^-20 (1 + |z|); their
-derivatives within 2^-18.  A value that is rounded to the dtype and used again carries u of its magnitude on.
+derivatives within 2^-18.  A value that is rounded to the dtype and used again carries u of its magnitude on; a factor kept
+for the backward pass is cut to 24 bits in 16-bit calls (2^-15 of it), exact in fp32.
 """
 from __future__ import annotations
 
@@ -20,6 +21,7 @@ class Unit:
         self.sub = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
         self.act = 2.0 ** (-20 if dtype == torch.float32 else -19)
         self.single = dtype == torch.float32
+        self.cut = 0.0 if self.single else 2.0 ** -15
 
     def gamma(self, n):
         return (n + 16) * 2.0 ** -24 + (2.0 ** -23 if self.single else 0.0)
@@ -60,10 +62,11 @@ def linear64(act, dtype, x, w, bias=None, residual=None, dy=None):
     if dy is None:
         return out
     dz = dy * df
-    if act in ("none", "relu"):
+    if act == "none":
         sums, edz = torch.zeros_like(dz), torch.zeros_like(dz)
     else:
-        sums = dy.abs() * (CURVE * (q.rounded(z) + ez) + 2.0 ** -18)
+        sums = torch.zeros_like(dz) if act == "relu" else dy.abs() * (CURVE * ez + 2.0 ** -18)
+        sums = sums + q.cut * dz.abs() + 2.0 ** -24 * dz.abs()
         edz = sums + q.rounded(dz)
     out["x"] = _product(q, dz, edz, w, 0.0, w.shape[0])
     out["w"] = _product(q, dz.t(), edz.t(), x, 0.0, x.shape[0])
@@ -103,12 +106,12 @@ def ffn64(act, dtype, x, wg, wu, wd, residual=None, dy=None):
         return out
     dh = dy @ wd
     edh = q.gamma(wd.shape[0]) * (dy.abs() @ wd.abs())
-    ka, kb = q.rounded(a) + ea, q.rounded(b) + eb  # of the kept a and b
     own1 = 0.0 if act in ("none", "relu") else 2.0 ** -18
     curve = 0.0 if act in ("none", "relu") else CURVE
     da, db = dh * b * df, dh * f
-    eda = (b * df).abs() * edh + (dh * df).abs() * kb + (dh * b).abs() * (curve * ka + own1)
-    edb = f.abs() * edh + dh.abs() * (SLOPE * ka + own * (1 + a.abs()))
+    keep = q.cut + 2.0 ** -23
+    eda = (b * df).abs() * edh + (dh * df).abs() * eb + (dh * b).abs() * (curve * ea + own1) + keep * da.abs()
+    edb = f.abs() * edh + dh.abs() * (SLOPE * ea + own * (1 + a.abs())) + keep * db.abs()
     eda, edb = 1.02 * eda + q.rounded(da), 1.02 * edb + q.rounded(db)  # (2%: products of errors)
     ga, gea = _product(q, da, eda, wg, 0.0, 2 * F)
     gb, geb = _product(q, db, edb, wu, 0.0, 2 * F)
