@@ -341,6 +341,17 @@ enum orda_activation {
   ORDA_ACT_SIGMOID = 5
 };
 
+/* Copies of operands with their rows padded: dst[r][c] = src[r][c] for c < cols,
+ * 0 up to ld_dst, r < rows; rows of src ld_src elements apart, of any
+ * alignment; those of dst 16-byte aligned, ld_dst a multiple of 8 (fp32: 4).
+ * n at most 4, one launch. */
+typedef struct orda_rows {
+  const void* src;
+  void* dst;
+  int64_t rows, cols, ld_src, ld_dst;
+} orda_rows_t;
+int orda_pad_rows(int32_t dtype, const orda_rows_t* t, int64_t n, void* stream);
+
 /* y = act(x W^T + bias) + residual.  Rows of x, weight and their gradients are
  * ld* elements apart, a multiple of 8 (fp32: 4), and start 16-byte aligned; x
  * and weight are zero from in_features up to the next such multiple, and their

@@ -1,4 +1,5 @@
-// norms.hip -- the norm over all elements of many tensors, and their clipping.
+// norms.hip -- the norm over all elements of many tensors, their clipping, and
+// copies of operands with padded rows.
 //
 // A launch takes a table of tensors in its arguments (no copy to the device,
 // so it can be captured) and splits their rows into chunks; workgroup b of G
@@ -178,6 +179,39 @@ __global__ __launch_bounds__(256) void k_clip(SpanTable S, const float* total, f
       }
     }
   });
+}
+
+// A thread writes 16 bytes of a destination row: a source piece that lies
+// inside its row as one load at the elements' own alignment, a row's last one
+// element by element, zeros behind.
+template <int ES>
+__global__ __launch_bounds__(256) void k_pad_rows(PadParams P) {
+  constexpr int VE = 16 / ES;
+  typedef typename std::conditional<ES == 2, uint16_t, uint32_t>::type E;
+  typedef E vec __attribute__((ext_vector_type(VE), aligned(ES)));
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < P.pieces; i += (int64_t)gridDim.x * 256) {
+    int k = 0;
+    while (k + 1 < P.n && i >= P.t[k + 1].first) ++k;
+    const PadParams::Item& t = P.t[k];
+    const int64_t per = t.ld_dst / VE, j = i - t.first, row = j / per, c = (j - row * per) * VE;
+    const E* s = reinterpret_cast<const E*>(t.src) + row * t.ld_src + c;
+    vec v;
+    if (c + VE <= t.cols) {
+      v = *reinterpret_cast<const vec*>(s);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[e] = c + e < t.cols ? s[e] : (E)0;
+    }
+    *reinterpret_cast<uint4*>(t.dst + (row * t.ld_dst + c) * ES) = __builtin_bit_cast(uint4, v);
+  }
+}
+
+hipError_t launch_pad_rows(const PadParams& P, int esize, hipStream_t s) {
+  const int64_t g = (P.pieces + 255) / 256;
+  const dim3 grid((unsigned)(g < 4096 ? g : 4096));
+  if (esize == 2) hipLaunchKernelGGL((k_pad_rows<2>), grid, dim3(256), 0, s, P);
+  else hipLaunchKernelGGL((k_pad_rows<4>), grid, dim3(256), 0, s, P);
+  return hipGetLastError();
 }
 
 // Tables of the spans of one dtype pair; go(table, workgroups) per launch.

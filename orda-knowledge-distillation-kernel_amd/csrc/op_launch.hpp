@@ -43,6 +43,20 @@ template <class T> hipError_t launch_dz(const DzParams& P, hipStream_t s);
 // out[c] = sum over b of partial[b][c], in order
 template <class T> hipError_t launch_colsum(const float* partial, int64_t blocks, int64_t cols, void* out, hipStream_t s);
 
+// Rows copied and zero-padded, up to kPadMax tensors of one element size.
+constexpr int kPadMax = 4;
+struct PadParams {
+  struct Item {
+    const char* src;
+    char* dst;
+    int64_t rows, cols, ld_src, ld_dst;  // elements
+    int64_t first;                       // its first 16-byte piece of dst
+  } t[kPadMax];
+  int n;
+  int64_t pieces;
+};
+hipError_t launch_pad_rows(const PadParams& P, int esize, hipStream_t s);
+
 // Norm and clipping of many tensors (norms.hip).
 struct GradSpan {  // rows x cols elements, ld apart; dense: one row
   void* p;

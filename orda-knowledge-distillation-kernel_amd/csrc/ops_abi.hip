@@ -288,6 +288,26 @@ size_t ffn_ws(const orda_ffn_t* p, const FfnShapes& s, bool backward) {
 
 extern "C" {
 
+int orda_pad_rows(int32_t dtype, const orda_rows_t* t, int64_t n, void* stream) {
+  set_last_error(0, nullptr);
+  if (dtype < ORDA_BF16 || dtype > ORDA_F32) return fail(ORDA_EINVAL, "orda_pad_rows: unknown dtype %d", dtype);
+  if (n < 0 || n > kPadMax || (n > 0 && !t)) return fail(ORDA_EINVAL, "orda_pad_rows: n must be in [0, %d]", kPadMax);
+  const int64_t es = esize(dtype), g = granule(dtype);
+  PadParams P{};
+  for (int64_t i = 0; i < n; ++i) {
+    const orda_rows_t& x = t[i];
+    if (x.rows < 0 || x.cols <= 0 || x.cols > kMaxPitch || x.rows > kMaxTokens) return fail(ORDA_EINVAL, "orda_pad_rows: tensor %lld has a size out of range", (long long)i);
+    if (x.rows == 0) continue;
+    if (!x.src || !x.dst || !aligned16(x.dst) || reinterpret_cast<uintptr_t>(x.src) % es) return fail(ORDA_EINVAL, "orda_pad_rows: tensor %lld is not aligned", (long long)i);
+    if (x.ld_dst < x.cols || x.ld_dst % g || x.ld_dst > kMaxPitch || (x.rows > 1 && x.ld_src < x.cols)) return fail(ORDA_EINVAL, "orda_pad_rows: tensor %lld has a pitch out of range", (long long)i);
+    P.t[P.n++] = {static_cast<const char*>(x.src), static_cast<char*>(x.dst), x.rows, x.cols, x.ld_src, x.ld_dst, P.pieces};
+    P.pieces += x.rows * (x.ld_dst / g);
+  }
+  if (P.n == 0) return ORDA_OK;
+  OP_LAUNCH(launch_pad_rows(P, (int)es, static_cast<hipStream_t>(stream)));
+  return ORDA_OK;
+}
+
 size_t orda_linear_saved_bytes(const orda_linear_t* p) {
   set_last_error(0, nullptr);
   LinearShapes s;

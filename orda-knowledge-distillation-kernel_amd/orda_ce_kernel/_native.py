@@ -8,6 +8,8 @@ the HIP path reports it.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 from pathlib import Path
@@ -18,8 +20,7 @@ __all__ = [
     "ABI_VERSION", "PlanInfo", "Problem", "Tensors", "library", "plan_info", "library_path", "forward", "forward_static", "backward",
     "saved_bytes", "forward_workspace_bytes", "backward_workspace_bytes", "gemm_abt", "gemm",
     "MODE", "DTYPE", "FLAG", "KERNEL_CLASSES", "timing_enable", "timing_collect",
-    "ACTIVATION", "Linear", "FeedForward", "linear_forward", "linear_backward", "ffn_forward", "ffn_backward",
-    "grad_norm", "clip_grads",
+    "ACTIVATION", "Linear", "FeedForward", "torch_ops",
 ]
 
 ABI_VERSION = 4
@@ -146,6 +147,15 @@ class FeedForward(ctypes.Structure):
 # orda_grad_t as int64 words: data, out, rows, cols, ld, ld_out, dtype | out_dtype << 32
 GRAD_WORDS = 7
 
+
+class Rows(ctypes.Structure):
+    """orda_rows_t"""
+
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p)] + [
+        (n, ctypes.c_int64) for n in ("rows", "cols", "ld_src", "ld_dst")
+    ]
+
+
 _LOCK = threading.Lock()
 _LIB = None
 
@@ -213,6 +223,8 @@ def library() -> ctypes.CDLL:
                                    ("orda_ffn_forward", F, 9), ("orda_ffn_backward", F, 12)):
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = ctypes.c_int, [arg] + [vp] * (tensors + 1) + [sz, vp]
+        lib.orda_pad_rows.restype = ctypes.c_int
+        lib.orda_pad_rows.argtypes = [ctypes.c_int32, ctypes.POINTER(Rows), ctypes.c_int64, vp]
         lib.orda_grad_norm_workspace_bytes.restype, lib.orda_grad_norm_workspace_bytes.argtypes = sz, []
         lib.orda_grad_norm.restype = ctypes.c_int
         lib.orda_grad_norm.argtypes = [vp, ctypes.c_int64, ctypes.c_double, vp, vp, sz, vp]
@@ -348,86 +360,37 @@ def gemm(a: torch.Tensor, b: torch.Tensor, *, a_mn: bool = False, b_mn: bool = F
     return c
 
 
-def _address(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
+_TORCH_OPS = None
+_TORCH_API = (
+    "orda_last_error", "orda_pad_rows", "orda_linear_saved_bytes", "orda_linear_workspace_bytes", "orda_linear_forward",
+    "orda_linear_backward", "orda_ffn_inner_pitch", "orda_ffn_saved_bytes", "orda_ffn_workspace_bytes",
+    "orda_ffn_forward", "orda_ffn_backward", "orda_grad_norm_workspace_bytes", "orda_grad_norm", "orda_clip_grads",
+)
 
 
-def _run_op(name: str, problem, backward: int, tensors, device: torch.device) -> None:
-    """One orda_linear_* / orda_ffn_* call on the device's current stream, with its workspace from torch."""
+def torch_ops():
+    """The native binding of the layers and the gradient norm (``_lib/orda_torch.so``, built from ``csrc/torch_ops.cpp``),
+    loaded once and given the loaded library's entry points; RuntimeError if it cannot be loaded."""
+    global _TORCH_OPS
+    if _TORCH_OPS is not None:
+        return _TORCH_OPS
     lib = library()
-    query = lib.orda_linear_workspace_bytes if isinstance(problem, Linear) else lib.orda_ffn_workspace_bytes
-    p = ctypes.byref(problem)
-    with _on(device):
-        n = query(p, backward)
-        if n == 0:
-            _check(-1, name)
-        ws = torch.empty(n, dtype=torch.uint8, device=device)
-        rc = getattr(lib, name)(p, *[_address(t) for t in tensors], ws.data_ptr(), n, _stream(device))
-    _check(rc, name)
-
-
-class _Here:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
-def _on(device: torch.device):
-    """`device` as the current one for the launches (nothing to do where it is)."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def linear_saved_bytes(problem: Linear) -> int:
-    return int(library().orda_linear_saved_bytes(ctypes.byref(problem)))
-
-
-def ffn_inner_pitch(problem: FeedForward) -> int:
-    return int(library().orda_ffn_inner_pitch(ctypes.byref(problem)))
-
-
-def ffn_saved_bytes(problem: FeedForward) -> int:
-    return int(library().orda_ffn_saved_bytes(ctypes.byref(problem)))
-
-
-def linear_forward(problem: Linear, x, weight, bias, residual, y, z) -> None:
-    _run_op("orda_linear_forward", problem, 0, (x, weight, bias, residual, y, z), x.device)
-
-
-def linear_backward(problem: Linear, x, weight, z, grad_output, grad_x, grad_weight, grad_bias) -> None:
-    _run_op("orda_linear_backward", problem, 1, (x, weight, z, grad_output, grad_x, grad_weight, grad_bias),
-            grad_output.device)
-
-
-def ffn_forward(problem: FeedForward, x, w_gate, w_up, w_down, residual, y, h, a, b) -> None:
-    _run_op("orda_ffn_forward", problem, 0, (x, w_gate, w_up, w_down, residual, y, h, a, b), x.device)
-
-
-def ffn_backward(problem: FeedForward, x, w_gate, w_up, w_down, h, a, b, grad_output, grad_x, grad_gate, grad_up,
-                 grad_down) -> None:
-    _run_op("orda_ffn_backward", problem, 1,
-            (x, w_gate, w_up, w_down, h, a, b, grad_output, grad_x, grad_gate, grad_up, grad_down), x.device)
-
-
-def grad_norm(table, n: int, norm_type: float, total: torch.Tensor) -> None:
-    """orda_grad_norm of a table of n orda_grad_t (an ``array('q')`` of GRAD_WORDS words each)."""
-    lib, dev = library(), total.device
-    with _on(dev):
-        nb = lib.orda_grad_norm_workspace_bytes()
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-        rc = lib.orda_grad_norm(table.buffer_info()[0], n, norm_type, total.data_ptr(), ws.data_ptr(), nb, _stream(dev))
-    _check(rc, "orda_grad_norm")
-
-
-def clip_grads(table, n: int, total: torch.Tensor, max_norm: float) -> None:
-    """orda_clip_grads of a table as :func:`grad_norm` takes it."""
-    with _on(total.device):
-        rc = library().orda_clip_grads(table.buffer_info()[0], n, total.data_ptr(), max_norm, _stream(total.device))
-    _check(rc, "orda_clip_grads")
+    with _LOCK:
+        if _TORCH_OPS is None:
+            path = Path(__file__).resolve().parent / "_lib" / "orda_torch.so"
+            if not path.exists():
+                raise RuntimeError(f"orda_torch.so not found at {path}; build it with `make -C csrc` "
+                                   "(or __graft_entry__.build())")
+            try:
+                spec = importlib.util.spec_from_loader(
+                    "orda_torch", importlib.machinery.ExtensionFileLoader("orda_torch", str(path)))
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+            except ImportError as exc:
+                raise RuntimeError(f"orda_torch.so could not be loaded: {exc}") from exc
+            module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _TORCH_API})
+            _TORCH_OPS = module
+    return _TORCH_OPS
 
 
 def timing_enable(enable: bool = True) -> None:

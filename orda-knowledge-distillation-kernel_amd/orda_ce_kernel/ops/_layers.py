@@ -1,5 +1,5 @@
-"""What the projection and the feed-forward block share: argument checks, the compute dtype, operands as the kernels
-read them."""
+"""What the projection and the feed-forward block share: argument checks, the choice between the kernels and torch, and when
+autograd has to see a call."""
 from __future__ import annotations
 
 import torch
@@ -9,8 +9,7 @@ from torch.autograd import forward_ad
 from .. import _native
 from .._runtime import HAS_NATIVE, native_error
 
-__all__ = ["ACTIVATIONS", "activation_torch", "check_tensors", "needs_function", "operand", "same_pitch", "use_kernels",
-           "new_grad", "trim"]
+__all__ = ["ACTIVATIONS", "activation_torch", "check_shape", "check_tensors", "needs_function", "use_kernels"]
 
 ACTIVATIONS = tuple(_native.ACTIVATION)
 
@@ -27,7 +26,7 @@ def use_kernels(backend: str, x: torch.Tensor, entry: str) -> bool:
     """Whether the call runs on the HIP kernels (the loss's rule: never a silent fallback on a HIP device)."""
     if backend not in ("auto", "triton", "hip", "torch"):
         raise ValueError(f"backend must be 'auto', 'triton', 'hip', or 'torch', got {backend!r}")
-    on_device = x.device.type == "cuda"
+    on_device = x.is_cuda
     if backend == "torch" or (backend == "auto" and not on_device):
         return False
     if not (HAS_NATIVE and on_device):
@@ -61,62 +60,8 @@ def check_shape(entry: str, name: str, t: torch.Tensor | None, shape: tuple) -> 
 
 
 def needs_function(*tensors) -> bool:
-    """Whether autograd has to see the call: a gradient is wanted, or a forward-mode level is open (the Functions have no
-    jvp, and autograd then refuses the call instead of dropping a tangent)."""
+    """Whether autograd has to see the call: a gradient is wanted, or a forward-mode level is open (the nodes have no jvp,
+    and autograd then refuses the call instead of dropping a tangent)."""
     if forward_ad._current_level >= 0:
         return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def operand(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """A 2-D operand as the kernels read it: rows in memory order, 16-byte aligned and zero-padded to 16 bytes.  Row-strided
-    tensors that already are so stay where they are."""
-    if t.dtype != dtype:
-        t = t.to(dtype)
-    mult = 4 if dtype == torch.float32 else 8
-    rows, cols = t.shape
-    if cols % mult:
-        return F.pad(t, (0, -cols % mult))
-    if t.stride(1) != 1 or (rows > 1 and (t.stride(0) % mult or t.stride(0) < cols)):
-        t = t.contiguous()
-    if t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def pitch(t: torch.Tensor) -> int:
-    """Elements between the rows of an operand (one row: its length)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def same_pitch(a: torch.Tensor, b: torch.Tensor):
-    """Both operands with the same row pitch."""
-    if pitch(a) != pitch(b):
-        a, b = a.contiguous(), b.contiguous()
-    return a, b
-
-
-def rows_of(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """A 2-D tensor with contiguous rows in `dtype` (any row pitch, any alignment)."""
-    if t.dtype != dtype:
-        t = t.to(dtype)
-    if t.stride(1) != 1 and t.shape[1] > 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t
-
-
-def new_grad(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
-    """A gradient's buffer, its rows padded to 16 bytes."""
-    mult = 4 if dtype == torch.float32 else 8
-    return torch.empty((rows, cols + (-cols) % mult), dtype=dtype, device=device)
-
-
-def trim(grad: torch.Tensor | None, cols: int, shape, dtype: torch.dtype):
-    """The gradient in its tensor's shape and dtype, without the padding."""
-    if grad is None:
-        return None
-    if grad.shape[1] != cols:
-        grad = grad[:, :cols]
-    if grad.dtype != dtype:
-        grad = grad.to(dtype)
-    return grad if grad.shape == shape else grad.reshape(shape)

@@ -11,71 +11,18 @@ A training call also keeps the factors p = b act'(a) and q = act(a).  Backward, 
     dWg = da^T x    dWu = db^T x    dWd = dy^T h
 
 h, da and db are rounded to the compute dtype as operands of the next product; p and q are kept in fp32, for 16-bit tensors
-in its upper 24 bits; products accumulate in fp32.  No counterpart in the reference, whose models use torch.
+in its upper 24 bits; products accumulate in fp32.  The operands, workspaces and the autograd node are in
+csrc/torch_ops.cpp.  No counterpart in the reference, whose models use torch.
 """
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _native
 from .._runtime import default_compute_dtype
-from ._layers import (activation_torch, check_shape, check_tensors, needs_function, new_grad, operand, pitch, rows_of,
-                      same_pitch, trim, use_kernels)
+from ._layers import activation_torch, check_shape, check_tensors, needs_function, use_kernels
 
-__all__ = ["GatedFeedForwardFunction", "gated_feed_forward"]
-
-
-def _forward(x2, w_gate, w_up, w_down, res2, act: str, dtype, keep: bool):
-    xo, dn = operand(x2, dtype), operand(w_down, dtype)
-    ga, up = same_pitch(operand(w_gate, dtype), operand(w_up, dtype))
-    if res2 is not None:
-        res2 = rows_of(res2, dtype)
-    N, O = x2.shape[0], w_down.shape[0]
-    p = _native.FeedForward(abi_version=_native.ABI_VERSION, dtype=_native.DTYPE[dtype],
-                            activation=_native.ACTIVATION[act], tokens=N, hidden=x2.shape[1], inner=w_gate.shape[0],
-                            out_features=O, ldx=pitch(xo), ldw=pitch(ga), ldd=pitch(dn),
-                            ldr=pitch(res2) if res2 is not None else 0)
-    fp = _native.ffn_inner_pitch(p)
-    y = torch.empty((N, O), dtype=dtype, device=x2.device)
-    h = torch.empty((N, fp), dtype=dtype, device=x2.device)
-    fa = fb = None
-    if keep:
-        n = _native.ffn_saved_bytes(p)
-        fa, fb = (torch.empty(n, dtype=torch.uint8, device=x2.device) for _ in range(2))
-    _native.ffn_forward(p, xo, ga, up, dn, res2, y, h, fa, fb)
-    return y, (xo, ga, up, dn, h, fa, fb), p
-
-
-class GatedFeedForwardFunction(torch.autograd.Function):
-    """``(x [N, H], w_gate [F, H], w_up [F, H], w_down [O, F], residual [N, O], activation)`` -> ``y [N, O]``."""
-
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, residual, activation: str):
-        dtype = default_compute_dtype(x, w_gate, w_up, w_down)
-        y, saved, p = _forward(x, w_gate, w_up, w_down, residual, activation, dtype, True)
-        ctx.save_for_backward(*saved)
-        ctx.problem, ctx.dtype = p, dtype
-        ctx.given = tuple(None if t is None else (t.shape, t.dtype) for t in (x, w_gate, w_up, w_down, residual))
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y):
-        xo, ga, up, dn, h, fa, fb = ctx.saved_tensors
-        given, need = ctx.given, ctx.needs_input_grad
-        g_r = grad_y.to(given[4][1]) if given[4] is not None and need[4] else None
-        grads = [None] * 4
-        if any(need[:4]):
-            dy = operand(grad_y, ctx.dtype)
-            grads = [new_grad(*g[0], ctx.dtype, dy.device) if n else None for g, n in zip(given, need[:4])]
-            p = _native.FeedForward.from_buffer_copy(ctx.problem)
-            p.ldg = pitch(dy)
-            mult = 4 if ctx.dtype == torch.float32 else 8
-            p.ldgx = p.ldgw = p.hidden + (-p.hidden) % mult
-            p.ldgd = p.inner + (-p.inner) % mult
-            _native.ffn_backward(p, xo, ga, up, dn, h, fa, fb, dy, *grads)
-        return (*[trim(v, g[0][1], g[0], g[1]) for v, g in zip(grads, given)], g_r, None)
+__all__ = ["gated_feed_forward"]
 
 
 @torch._dynamo.disable
@@ -104,10 +51,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
         lin = torch.nn.functional.linear
         y = lin(activation_torch(activation, lin(xc, w_gate.to(dtype))) * lin(xc, w_up.to(dtype)), w_down.to(dtype))
         return y if residual is None else y + residual.to(dtype)
-    x2 = x.reshape(-1, x.shape[-1])
-    res2 = None if residual is None else residual.reshape(-1, w_down.shape[0])
-    if needs_function(x, w_gate, w_up, w_down, residual):
-        y = GatedFeedForwardFunction.apply(x2, w_gate, w_up, w_down, res2, activation)
-    else:
-        y = _forward(x2, w_gate, w_up, w_down, res2, activation, dtype, False)[0]
+    x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
+    res2 = residual if residual is None or residual.ndim == 2 else residual.reshape(-1, w_down.shape[0])
+    y = _native.torch_ops().feed_forward(x2, w_gate, w_up, w_down, res2, _native.ACTIVATION[activation], dtype,
+                                         needs_function(x, w_gate, w_up, w_down, residual))
     return y if x.ndim == 2 else y.reshape(out_shape)

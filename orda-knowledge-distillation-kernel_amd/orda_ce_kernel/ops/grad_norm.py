@@ -3,13 +3,12 @@
     total = (sum |g|^p)^(1/p), p = 1, 2 or infinity        g *= min(1, max_norm / (total + 1e-6))
 
 Two kernels over a table of tensors (one launch each per 80 tensors and dtype) and one that adds up the norm's partial sums;
-sums are fp64 in a fixed order and the factor is formed on the device, so nothing synchronises the host.  No counterpart in
-the reference, whose training loop calls torch.
+sums are fp64 in a fixed order and the factor is formed on the device, so nothing synchronises the host.  The tables are
+built in csrc/torch_ops.cpp.  No counterpart in the reference, whose training loop calls torch.
 """
 from __future__ import annotations
 
 import math
-from array import array
 
 import torch
 
@@ -17,8 +16,6 @@ from .. import _native
 from ._layers import use_kernels
 
 __all__ = ["clip_grad_norm_", "grad_norm"]
-
-_CODE = _native.DTYPE
 
 
 def _listed(tensors) -> list:
@@ -37,40 +34,8 @@ def _check_grad(entry: str, g: torch.Tensor, device) -> None:
         raise ValueError(f"{entry}: gradients must be dense, got layout {g.layout}")
     if g.device != device:
         raise ValueError(f"{entry}: gradients must be on one device, got {device} and {g.device}")
-    if g.dtype not in _CODE:
+    if g.dtype not in _native.DTYPE:
         raise ValueError(f"{entry}: gradients must be bfloat16, float16 or float32, got {g.dtype}")
-
-
-def _rows(g: torch.Tensor):
-    """``(rows, cols, ld)`` of a tensor whose elements the kernels reach in place, row-major; None for other strides."""
-    if g.is_contiguous():
-        n = g.numel()
-        return 1, n, n
-    if g.ndim == 2 and g.stride(1) == 1 and g.stride(0) >= g.shape[1]:
-        return g.shape[0], g.shape[1], g.stride(0)
-    return None
-
-
-def _table(entry: str, grads, outs=None) -> array:
-    device = grads[0].device
-    words = []
-    for i, g in enumerate(grads):
-        code = _CODE.get(g.dtype)
-        if code is None or g.device != device or g.layout is not torch.strided:
-            _check_grad(entry, g, device)
-        if outs is None or outs[i] is g:
-            rows, cols, ld = _rows(g)
-            words += (g.data_ptr(), 0, rows, cols, ld, ld, code | code << 32)
-        else:
-            o = outs[i]
-            r, ro = _rows(g), _rows(o)
-            if r != ro and (r[0] == 1) != (ro[0] == 1):  # a dense side beside a row-strided one: as rows both
-                r = ro = None
-                rows, cols = g.shape
-                words += (g.data_ptr(), o.data_ptr(), rows, cols, g.stride(0), o.stride(0), code | _CODE[o.dtype] << 32)
-                continue
-            words += (g.data_ptr(), o.data_ptr(), r[0], r[1], r[2], ro[2], code | _CODE[o.dtype] << 32)
-    return array("q", words)
 
 
 def _norm_torch(grads, norm_type: float) -> torch.Tensor:
@@ -79,11 +44,34 @@ def _norm_torch(grads, norm_type: float) -> torch.Tensor:
     ).float()
 
 
-def _norm(entry: str, grads, norm_type: float) -> torch.Tensor:
-    """The norm of device tensors (at least one)."""
-    grads = [g if _rows(g) is not None else g.contiguous() for g in grads]
-    total = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    _native.grad_norm(_table(entry, grads), len(grads), norm_type, total)
+def _clip_torch(entry, params, outs, max_norm, norm_type, error_if_nonfinite, total_norm):
+    grads, dests, seen = [], [], set()
+    for i, p in enumerate(params):
+        g = p.grad
+        if g is None or id(p) in seen:
+            continue
+        seen.add(id(p))
+        _check_grad(entry, g, grads[0].device if grads else g.device)
+        if outs is not None:
+            o = outs[i]
+            if o.shape != g.shape or o.device != g.device or o.dtype not in _native.DTYPE:
+                raise ValueError(f"{entry}: out[{i}] must be a bfloat16, float16 or float32 tensor of shape "
+                                 f"{tuple(g.shape)} on {g.device}")
+            dests.append(o)
+        grads.append(g)
+    if total_norm is None:
+        total = _norm_torch(grads, norm_type)
+    elif total_norm.numel() != 1 or total_norm.device != grads[0].device:
+        raise ValueError(f"{entry}: total_norm must be a one-element tensor on {grads[0].device}")
+    else:
+        total = total_norm.detach().float().reshape(())
+    if error_if_nonfinite and not bool(torch.isfinite(total)):
+        raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot "
+                           "be clipped. To disable this error and scale the gradients by the non-finite norm anyway, set "
+                           "`error_if_nonfinite=False`")
+    factor = (max_norm / (total + 1e-6)).clamp(max=1.0)
+    for g, o in zip(grads, dests or grads):
+        o.copy_(g.float() * factor)
     return total
 
 
@@ -98,16 +86,16 @@ def grad_norm(tensors, norm_type: float = 2.0, *, backend: str = "auto") -> torc
     for g in grads:
         if not isinstance(g, torch.Tensor):
             raise TypeError(f"grad_norm: expected tensors, got {type(g).__name__}")
-        _check_grad("grad_norm", g, grads[0].device)
     if not grads:
         return torch.zeros(())
-    if not use_kernels(backend, grads[0], "grad_norm"):
-        return _norm_torch(grads, norm_type)
-    return _norm("grad_norm", grads, norm_type)
+    if use_kernels(backend, grads[0], "grad_norm"):
+        return _native.torch_ops().grad_norm(grads, norm_type)
+    for g in grads:
+        _check_grad("grad_norm", g, grads[0].device)
+    return _norm_torch(grads, norm_type)
 
 
 @torch._dynamo.disable
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False, *,
                     total_norm: torch.Tensor | None = None, out=None, backend: str = "auto") -> torch.Tensor:
     """Scale the parameters' gradients by ``min(1, max_norm / (total + 1e-6))`` in place and return their total norm, as
@@ -125,48 +113,12 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     outs = None if out is None else _listed(out)
     if outs is not None and len(outs) != len(params):
         raise ValueError(f"{entry}: out must have one tensor per parameter ({len(params)}), got {len(outs)}")
-    grads, dests, seen = [], [], set()
-    for i, p in enumerate(params):
-        g = p.grad
-        if g is None or id(p) in seen:
-            continue
-        seen.add(id(p))
-        grads.append(g)
-        if outs is not None:
-            o = outs[i]
-            if not isinstance(o, torch.Tensor) or o.shape != g.shape or o.device != g.device or o.dtype not in _CODE:
-                raise ValueError(f"{entry}: out[{i}] must be a bfloat16, float16 or float32 tensor of shape "
-                                 f"{tuple(g.shape)} on {g.device}")
-            dests.append(o)
-    if not grads:
+    if total_norm is not None and not isinstance(total_norm, torch.Tensor):
+        raise ValueError(f"{entry}: total_norm must be a one-element tensor, got {type(total_norm).__name__}")
+    first = next((p.grad for p in params if p.grad is not None), None)
+    if first is None:
         return torch.zeros(()) if total_norm is None else total_norm
-    for g in grads:
-        _check_grad(entry, g, grads[0].device)
-    kernels = use_kernels(backend, grads[0], entry)
-    if total_norm is not None:
-        if not isinstance(total_norm, torch.Tensor) or total_norm.numel() != 1 or total_norm.device != grads[0].device:
-            raise ValueError(f"{entry}: total_norm must be a one-element tensor on {grads[0].device}")
-        total = total_norm.detach().to(torch.float32).reshape(())
-    else:
-        total = _norm(entry, grads, norm_type) if kernels else _norm_torch(grads, norm_type)
-    if error_if_nonfinite and not bool(torch.isfinite(total)):
-        raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot "
-                           "be clipped. To disable this error and scale the gradients by the non-finite norm anyway, set "
-                           "`error_if_nonfinite=False`")
-    if not kernels:
-        factor = (max_norm / (total + 1e-6)).clamp(max=1.0)
-        for g, o in zip(grads, dests or grads):
-            o.copy_(g.float() * factor)
-        return total
-    # tensors whose strides the kernels do not walk go through a dense copy
-    src = [g if _rows(g) is not None else g.contiguous() for g in grads]
-    dst = None
-    if outs is not None:
-        dst = [o if _rows(o) is not None else torch.empty(o.shape, dtype=o.dtype, device=o.device) for o in dests]
-    _native.clip_grads(_table(entry, src, dst), len(src), total, max_norm)
-    final = grads if outs is None else dests
-    for made, want in zip(src if dst is None else dst, final):
-        if made is not want:
-            want.copy_(made)
-    torch.autograd.graph.increment_version(final)
-    return total
+    if use_kernels(backend, first, entry):
+        return _native.torch_ops().clip(params, max_norm, norm_type, bool(error_if_nonfinite), total_norm, outs)
+    with torch.no_grad():
+        return _clip_torch(entry, params, outs, max_norm, norm_type, error_if_nonfinite, total_norm)
