@@ -456,6 +456,11 @@ size_t orda_grad_norm_workspace_bytes(void);
 int orda_grad_norm(const orda_grad_t* grads, int64_t n, double norm_type, float* total, void* workspace,
                    size_t workspace_bytes, void* stream);
 
+/* orda_grad_norm and orda_clip_grads in one call (fewer launches for small
+ * sets). */
+int orda_clip_grad_norm(const orda_grad_t* grads, int64_t n, double norm_type, double max_norm, float* total,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
 /* out = g * min(1, max_norm / (*total + 1e-6)), *total read on the device; a
  * factor of 1 leaves gradients in place untouched.  Gradients written by one
  * call must not overlap (ORDA_EINVAL). */

@@ -3,12 +3,15 @@
 //
 // A launch takes a table of tensors in its arguments (no copy to the device,
 // so it can be captured) and splits their rows into chunks; workgroup b of G
-// takes the b-th G-th of the chunks.  Both kernels are bound by memory: the
-// norm reads every element once, clipping reads and writes it once, in 16-byte
-// accesses from the first aligned address of a row on.  Squares and sums are
-// fp64, so neither tiny nor huge gradients lose anything, and every sum has a
-// fixed order: a thread's elements, the lanes of a wave, the waves, the
-// workgroups.
+// takes chunks b, b + G, ... .  Both kernels are bound by memory: the norm reads
+// every element once, clipping reads and writes it once, from the first 16-byte
+// aligned address of a row on.  600 M elements, MI355X: the norm 5.8 TB/s in
+// fp32 (torch's sum 4.0), 5.1 in bf16 behind a kernel that wrote 2.4 GB; clipping
+// bf16 into fp32 6.5 TB/s, fp32 6.0.  Clipping takes one workgroup per 2048
+// elements: with 8192 workgroups of many chunks it ran at 5.0 and 5.4 TB/s, and
+// with nontemporal stores at 3.8 and 5.3.  Squares and sums are fp64, so
+// neither tiny nor huge gradients lose anything, and every sum has a fixed
+// order: a thread's elements, the lanes of a wave, the waves, the workgroups.
 #include <algorithm>
 
 #include "epilogue.hpp"
@@ -34,27 +37,28 @@ struct SpanTable {
 constexpr int kSpanRows = kSpanMax - 16;
 static_assert(sizeof(SpanTable) <= 4000, "kernel arguments");
 
-// The chunks of workgroup b: f(tensor, first element of the row, elements
+// The chunks of workgroup b (b, b + G, ...: the workgroups that run together
+// walk memory side by side): f(tensor, row, the row's first element, elements
 // [lo, hi) of the row).  A row's chunks are cut at 16-byte aligned addresses.
 template <class T, class F>
 __device__ __forceinline__ void for_chunks(const SpanTable& S, const F& f) {
-  constexpr int VE = 16 / (int)sizeof(T);
-  const int c0 = (int)((int64_t)S.chunks * blockIdx.x / gridDim.x), c1 = (int)((int64_t)S.chunks * (blockIdx.x + 1) / gridDim.x);
-  if (c0 >= c1) return;
-  int i = 0, n = S.count;  // the last tensor that starts at or before c0
-  while (n - i > 1) {
-    const int m = (i + n) / 2;
-    if (S.t[m].first <= c0) i = m;
-    else n = m;
-  }
-  for (int c = c0; c < c1; ++c) {
-    while (i + 1 < S.count && S.t[i + 1].first <= c) ++i;
-    const int k = c - S.t[i].first, row = k / S.t[i].per_row, part = k - row * S.t[i].per_row;
+  int i = 0;
+  for (int c = blockIdx.x; c < S.chunks; c += gridDim.x) {
+    int n = S.count;  // i: the last tensor that starts at or before c
+    while (n - i > 1) {
+      const int m = (i + n) / 2;
+      if (S.t[m].first <= c) i = m;
+      else n = m;
+    }
+    int k = c - S.t[i].first, row = 0;
+    if (S.t[i].per_row <= k) {
+      row = k / S.t[i].per_row;
+      k -= row * S.t[i].per_row;
+    }
     const T* p = static_cast<const T*>(S.t[i].p) + row * S.t[i].ld;
     const int skew = (int)((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));  // elements past an aligned address
-    const int64_t lo = (int64_t)part * S.chunk - skew, hi = lmin(lo + S.chunk, S.t[i].cols);
+    const int64_t lo = (int64_t)k * S.chunk - skew, hi = lmin(lo + S.chunk, S.t[i].cols);
     f(i, row, p, lo, hi);
-    (void)VE;
   }
 }
 
@@ -126,53 +130,74 @@ __global__ __launch_bounds__(256) void k_grad_norm(SpanTable S, double* partials
   partials[blockIdx.x] = first ? s : norm_join<KIND>(partials[blockIdx.x], s);
 }
 
+// The norm from n partials, by all 256 threads of a workgroup (valid in all).
 template <int KIND>
-__global__ __launch_bounds__(256) void k_grad_total(const double* partials, int n, float* total) {
+__device__ __forceinline__ float norm_total(const double* partials, int n) {
   __shared__ double red[4];
   double s = 0.0;
+#pragma unroll 4
   for (int i = threadIdx.x; i < n; i += 256) s = norm_join<KIND>(s, partials[i]);
   for (int m = 1; m < 64; m <<= 1) s = norm_join<KIND>(s, __shfl_xor(s, m));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x != 0) return;
+  s = red[0];
   for (int i = 1; i < 4; ++i) s = norm_join<KIND>(s, red[i]);
-  *total = (float)(KIND == 2 ? sqrt(s) : s);
+  return (float)(KIND == 2 ? sqrt(s) : s);
+}
+template <int KIND>
+__global__ __launch_bounds__(256) void k_grad_total(const double* partials, int n, float* total) {
+  const float t = norm_total<KIND>(partials, n);
+  if (threadIdx.x == 0) *total = t;
 }
 
-// min(1, max_norm / (total + 1e-6)); a NaN norm gives a NaN factor.
-__device__ __forceinline__ float clip_factor(const float* total, float max_norm) {
-  const float f = max_norm / (*total + 1e-6f);
-  return f > 1.0f ? 1.0f : f;
-}
-
-template <class T, class O>
-__global__ __launch_bounds__(256) void k_clip(SpanTable S, const float* total, float max_norm, int in_place) {
-  constexpr int VE = 16 / (int)sizeof(T), U = 2;
-  const float f = clip_factor(total, max_norm);
-  if (in_place && f == 1.0f) return;
+// g * min(1, max_norm / (total + 1e-6)); a NaN norm gives a NaN factor.  KIND >=
+// 0: every workgroup adds up the norm's partials itself and the first writes
+// it, which saves small sets a launch; else *total is there.
+struct ClipParams {
+  const double* partials;
+  int n_partials;
+  float* total;
+  float max_norm;
+  int in_place;
+};
+template <class T, class O, int KIND>
+__global__ __launch_bounds__(256) void k_clip(SpanTable S, ClipParams P) {
+  // 16 bytes a lane and access on the wider side: 16 in and 2 x 16 out leave
+  // half of each line to another store (bf16 into fp32: 5.1 TB/s, 6.5 so)
+  constexpr int VE = sizeof(O) == 4 ? 4 : 16 / (int)sizeof(T), U = 4;
+  typedef T in_vec __attribute__((ext_vector_type(VE)));
   // (outputs at any element: the hardware's unaligned stores)
-  typedef O vec __attribute__((ext_vector_type(VE), aligned(sizeof(O))));
-  auto put = [&](O* o, const uint4& u) {
-    float x[VE];
-    unpack16<T>(u, x);
-    vec y;
+  typedef O out_vec __attribute__((ext_vector_type(VE), aligned(sizeof(O))));
+  float total;
+  if constexpr (KIND >= 0) {
+    total = norm_total<KIND>(P.partials, P.n_partials);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *P.total = total;
+  } else {
+    total = *P.total;
+  }
+  float f = P.max_norm / (total + 1e-6f);
+  f = f > 1.0f ? 1.0f : f;
+  if (P.in_place && f == 1.0f) return;
+  auto put = [&](O* o, const in_vec& x) {
+    out_vec y;
 #pragma unroll
-    for (int i = 0; i < VE; ++i) y[i] = from_f32<O>(x[i] * f);
-    *reinterpret_cast<vec*>(o) = y;
+    for (int i = 0; i < VE; ++i) y[i] = from_f32<O>(to_f32(x[i]) * f);
+    *reinterpret_cast<out_vec*>(o) = y;
   };
   for_chunks<T>(S, [&](int t, int row, const T* p, int64_t lo, int64_t hi) {
     O* o = static_cast<O*>(S.t[t].out) + row * S.t[t].ld_out;
     int64_t e = lo + (int64_t)threadIdx.x * VE;
     for (; e + (U - 1) * 256 * VE + VE <= hi && lo >= 0; e += U * 256 * VE) {
-      uint4 v[U];
+      in_vec v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const uint4*>(p + e + u * 256 * VE);
+      for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const in_vec*>(p + e + u * 256 * VE);
 #pragma unroll
       for (int u = 0; u < U; ++u) put(o + e + u * 256 * VE, v[u]);
     }
+#pragma unroll 2
     for (; e < hi; e += 256 * VE) {
       if (e >= 0 && e + VE <= hi) {
-        put(o + e, *reinterpret_cast<const uint4*>(p + e));
+        put(o + e, *reinterpret_cast<const in_vec*>(p + e));
       } else {
         for (int i = 0; i < VE; ++i)
           if (e + i >= 0 && e + i < hi) o[e + i] = from_f32<O>(to_f32(p[e + i]) * f);
@@ -264,40 +289,48 @@ static hipError_t for_tables(const GradSpan* g, int64_t n, int in_dtype, int out
   return flush();
 }
 
-// 2048 elements (one 16-byte access per thread) where that already fills the
-// chip, longer ones for large sets.
-static int64_t chunk_of(const GradSpan* g, int64_t n) {
+static int64_t elements_of(const GradSpan* g, int64_t n) {
   int64_t total = 0;
   for (int64_t i = 0; i < n; ++i) total += g[i].rows * g[i].cols;
-  return total < (64ll << 20) ? 2048 : 16384;
+  return total;
 }
+// Elements of a chunk of the norm: one 16-byte access per thread of bf16 where
+// that fills the chip, longer ones for large sets.  Of clipping: 2048.
+constexpr int64_t kClipChunk = 2048, kNormLarge = 64ll << 20;
+static int64_t norm_chunk(int64_t elements) { return elements < kNormLarge ? 2048 : 16384; }
 
 template <class T, int KIND>
 static hipError_t norm_go(const SpanTable& S, double* partials, int groups, int first, hipStream_t s) {
   hipLaunchKernelGGL((k_grad_norm<T, KIND>), dim3(groups), dim3(256), 0, s, S, partials, first);
   return hipGetLastError();
 }
+// The partials of all tensors: every launch has the same workgroups, the first
+// one writes all partials.  Returns their number (0: no elements) in *groups.
 template <int KIND>
-static hipError_t norm_kind(const GradSpan* g, int64_t n, double* partials, int max_partials, float* total, hipStream_t s) {
-  // every launch has the same number of workgroups, the first one writes all partials
-  const int64_t chunk = chunk_of(g, n);
-  int64_t elements = 0;
-  for (int64_t i = 0; i < n; ++i) elements += g[i].rows * g[i].cols;
-  int groups = (int)std::min<int64_t>(max_partials, std::max<int64_t>(1, (elements + chunk - 1) / chunk));
+static hipError_t norm_partials(const GradSpan* g, int64_t n, double* partials, int max_partials, int* groups, hipStream_t s) {
+  const int64_t elements = elements_of(g, n), chunk = norm_chunk(elements);
+  const int count = (int)std::min<int64_t>(max_partials, std::max<int64_t>(1, (elements + chunk - 1) / chunk));
   int first = 1;
   for (int dt = 0; dt < 3; ++dt) {
-    const hipError_t e = for_tables(g, n, dt, -1, -1, chunk, groups, [&](const SpanTable& S, int) {
+    const hipError_t e = for_tables(g, n, dt, -1, -1, chunk, count, [&](const SpanTable& S, int) {
       const int f = first;
       first = 0;
       switch (dt) {
-        case DT_BF16: return norm_go<bf16, KIND>(S, partials, groups, f, s);
-        case DT_F16: return norm_go<f16, KIND>(S, partials, groups, f, s);
-        default: return norm_go<float, KIND>(S, partials, groups, f, s);
+        case DT_BF16: return norm_go<bf16, KIND>(S, partials, count, f, s);
+        case DT_F16: return norm_go<f16, KIND>(S, partials, count, f, s);
+        default: return norm_go<float, KIND>(S, partials, count, f, s);
       }
     });
     if (e != hipSuccess) return e;
   }
-  if (first) groups = 0;
+  *groups = first ? 0 : count;
+  return hipSuccess;
+}
+template <int KIND>
+static hipError_t norm_kind(const GradSpan* g, int64_t n, double* partials, int max_partials, float* total, hipStream_t s) {
+  int groups = 0;
+  const hipError_t e = norm_partials<KIND>(g, n, partials, max_partials, &groups, s);
+  if (e != hipSuccess) return e;
   hipLaunchKernelGGL((k_grad_total<KIND>), dim3(1), dim3(256), 0, s, partials, groups, total);
   return hipGetLastError();
 }
@@ -310,36 +343,63 @@ hipError_t launch_grad_norm(const GradSpan* g, int64_t n, int kind, double* part
   }
 }
 
-template <class T, class O>
-static hipError_t clip_go(const SpanTable& S, int groups, const float* total, float max_norm, int in_place, hipStream_t s) {
-  hipLaunchKernelGGL((k_clip<T, O>), dim3(groups), dim3(256), 0, s, S, total, max_norm, in_place);
+template <class T, class O, int KIND>
+static hipError_t clip_go(const SpanTable& S, int groups, const ClipParams& P, hipStream_t s) {
+  hipLaunchKernelGGL((k_clip<T, O, KIND>), dim3(groups), dim3(256), 0, s, S, P);
   return hipGetLastError();
 }
-template <class T>
-static hipError_t clip_out(const SpanTable& S, int groups, int out, const float* total, float max_norm, int in_place, hipStream_t s) {
+template <class T, int KIND>
+static hipError_t clip_out(const SpanTable& S, int groups, int out, const ClipParams& P, hipStream_t s) {
   switch (out) {
-    case DT_BF16: return clip_go<T, bf16>(S, groups, total, max_norm, in_place, s);
-    case DT_F16: return clip_go<T, f16>(S, groups, total, max_norm, in_place, s);
-    default: return clip_go<T, float>(S, groups, total, max_norm, in_place, s);
+    case DT_BF16: return clip_go<T, bf16, KIND>(S, groups, P, s);
+    case DT_F16: return clip_go<T, f16, KIND>(S, groups, P, s);
+    default: return clip_go<T, float, KIND>(S, groups, P, s);
   }
 }
-
-hipError_t launch_clip_grads(const GradSpan* g, int64_t n, const float* total, float max_norm, hipStream_t s) {
-  const int64_t chunk = chunk_of(g, n);
+template <int KIND>
+static hipError_t clip_kind(const GradSpan* g, int64_t n, ClipParams P, hipStream_t s) {
   for (int in = 0; in < 3; ++in)
     for (int out = 0; out < 3; ++out)
       for (int place = 0; place < 2; ++place) {
         if (place && in != out) continue;
-        const hipError_t e = for_tables(g, n, in, out, place, chunk, 8192, [&](const SpanTable& S, int groups) {
+        P.in_place = place;
+        const hipError_t e = for_tables(g, n, in, out, place, kClipChunk, 1 << 30, [&](const SpanTable& S, int groups) {
           switch (in) {
-            case DT_BF16: return clip_out<bf16>(S, groups, out, total, max_norm, place, s);
-            case DT_F16: return clip_out<f16>(S, groups, out, total, max_norm, place, s);
-            default: return clip_out<float>(S, groups, out, total, max_norm, place, s);
+            case DT_BF16: return clip_out<bf16, KIND>(S, groups, out, P, s);
+            case DT_F16: return clip_out<f16, KIND>(S, groups, out, P, s);
+            default: return clip_out<float, KIND>(S, groups, out, P, s);
           }
         });
         if (e != hipSuccess) return e;
       }
   return hipSuccess;
+}
+
+hipError_t launch_clip_grads(const GradSpan* g, int64_t n, const float* total, float max_norm, hipStream_t s) {
+  return clip_kind<-1>(g, n, ClipParams{nullptr, 0, const_cast<float*>(total), max_norm, 0}, s);
+}
+
+// Norm, then clipping.  In sets below kFuseTotal elements the clipping kernels
+// add up the partials (40 tensors, 12 M elements: 27.4 -> 25.7 us a pass; 201
+// tensors, 60 M elements: 167 -> 182 us of kernels, so not there).
+constexpr int64_t kFuseTotal = 16ll << 20;
+template <int KIND>
+static hipError_t clip_norm_kind(const GradSpan* g, int64_t n, double* partials, int max_partials, float* total, float max_norm, hipStream_t s) {
+  const int64_t elements = elements_of(g, n);
+  if (elements == 0 || elements >= kFuseTotal) {
+    const hipError_t e = norm_kind<KIND>(g, n, partials, max_partials, total, s);
+    return e != hipSuccess ? e : launch_clip_grads(g, n, total, max_norm, s);
+  }
+  int groups = 0;
+  const hipError_t e = norm_partials<KIND>(g, n, partials, max_partials, &groups, s);
+  return e != hipSuccess ? e : clip_kind<KIND>(g, n, ClipParams{partials, groups, total, max_norm, 0}, s);
+}
+hipError_t launch_clip_grad_norm(const GradSpan* g, int64_t n, int kind, double* partials, int max_partials, float* total, float max_norm, hipStream_t s) {
+  switch (kind) {
+    case 2: return clip_norm_kind<2>(g, n, partials, max_partials, total, max_norm, s);
+    case 1: return clip_norm_kind<1>(g, n, partials, max_partials, total, max_norm, s);
+    default: return clip_norm_kind<0>(g, n, partials, max_partials, total, max_norm, s);
+  }
 }
 
 }  // namespace orda

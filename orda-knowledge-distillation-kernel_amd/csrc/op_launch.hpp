@@ -66,6 +66,7 @@ struct GradSpan {  // rows x cols elements, ld apart; dense: one row
 };
 constexpr int kNormPartials = 2048;  // fp64 partials of one kernel, added up by the next
 hipError_t launch_grad_norm(const GradSpan* g, int64_t n, int kind, double* partials, int max_partials, float* total, hipStream_t s);
+hipError_t launch_clip_grad_norm(const GradSpan* g, int64_t n, int kind, double* partials, int max_partials, float* total, float max_norm, hipStream_t s);
 hipError_t launch_clip_grads(const GradSpan* g, int64_t n, const float* total, float max_norm, hipStream_t s);
 
 }  // namespace orda

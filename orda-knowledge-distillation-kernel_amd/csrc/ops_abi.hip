@@ -548,6 +548,8 @@ int spans_of(const char* what, const orda_grad_t* g, int64_t n, bool outputs, st
   return ORDA_OK;
 }
 
+int norm_kind_of(double p) { return p == 2.0 ? 2 : p == 1.0 ? 1 : (std::isinf(p) && p > 0) ? 0 : -1; }
+
 // Whether the bytes of two row sets meet, a.lo <= b.lo < a's end.  Sets of the
 // same pitch whose columns lie beside each other (two halves of one buffer)
 // do not; anything else that is interleaved counts as meeting.
@@ -595,7 +597,7 @@ int orda_grad_norm(const orda_grad_t* grads, int64_t n, double norm_type, float*
   set_last_error(0, nullptr);
   try {
     if (!total) return fail(ORDA_EINVAL, "orda_grad_norm: total is required");
-    const int kind = norm_type == 2.0 ? 2 : norm_type == 1.0 ? 1 : (std::isinf(norm_type) && norm_type > 0) ? 0 : -1;
+    const int kind = norm_kind_of(norm_type);
     if (kind < 0) return fail(ORDA_EINVAL, "orda_grad_norm: norm_type must be 1, 2 or infinity, got %g", norm_type);
     OP_TRY(check_workspace("orda_grad_norm", workspace, workspace_bytes, orda_grad_norm_workspace_bytes()));
     std::vector<GradSpan> v;
@@ -604,6 +606,26 @@ int orda_grad_norm(const orda_grad_t* grads, int64_t n, double norm_type, float*
     return ORDA_OK;
   } catch (const std::exception& e) {
     return fail(ORDA_EINVAL, "orda_grad_norm: %s", e.what());
+  }
+}
+
+int orda_clip_grad_norm(const orda_grad_t* grads, int64_t n, double norm_type, double max_norm, float* total, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  set_last_error(0, nullptr);
+  try {
+    if (!total) return fail(ORDA_EINVAL, "orda_clip_grad_norm: total is required");
+    const int kind = norm_kind_of(norm_type);
+    if (kind < 0) return fail(ORDA_EINVAL, "orda_clip_grad_norm: norm_type must be 1, 2 or infinity, got %g", norm_type);
+    if (!(max_norm >= 0.0)) return fail(ORDA_EINVAL, "orda_clip_grad_norm: max_norm must be >= 0, got %g", max_norm);
+    OP_TRY(check_workspace("orda_clip_grad_norm", workspace, workspace_bytes, orda_grad_norm_workspace_bytes()));
+    std::vector<GradSpan> v;
+    OP_TRY(spans_of("orda_clip_grad_norm", grads, n, true, v));
+    OP_TRY(check_overlap("orda_clip_grad_norm", v));
+    OP_LAUNCH(launch_clip_grad_norm(v.data(), (int64_t)v.size(), kind, reinterpret_cast<double*>(base256(workspace)), kNormPartials, total,
+                                    (float)max_norm, static_cast<hipStream_t>(stream)));
+    return ORDA_OK;
+  } catch (const std::exception& e) {
+    return fail(ORDA_EINVAL, "orda_clip_grad_norm: %s", e.what());
   }
 }
 

@@ -47,6 +47,7 @@ struct Api {
   decltype(&orda_grad_norm_workspace_bytes) grad_norm_workspace_bytes;
   decltype(&orda_grad_norm) grad_norm;
   decltype(&orda_clip_grads) clip_grads;
+  decltype(&orda_clip_grad_norm) clip_grad_norm;
 } api;
 
 void bind(const std::map<std::string, uintptr_t>& at) {
@@ -65,6 +66,7 @@ void bind(const std::map<std::string, uintptr_t>& at) {
   ORDA_BIND(grad_norm_workspace_bytes);
   ORDA_BIND(grad_norm);
   ORDA_BIND(clip_grads);
+  ORDA_BIND(clip_grad_norm);
 #undef ORDA_BIND
 }
 
@@ -447,19 +449,27 @@ Tensor clip(const std::vector<Tensor>& params, double max_norm, double norm_type
     if (g.unsafeGetTensorImpl() != grads[i].unsafeGetTensorImpl()) grads[i] = g;  // (kept alive)
   }
   Tensor total;
-  if (given_total) {
-    TORCH_CHECK_VALUE(given_total->numel() == 1 && given_total->device() == grads[0].device(), entry,
-                      ": total_norm must be a one-element tensor on ", grads[0].device());
-    total = given_total->detach().to(at::kFloat).reshape({});
+  if (!given_total && !raise) {
+    total = at::empty({}, grads[0].options().dtype(at::kFloat));
+    const size_t n = api.grad_norm_workspace_bytes();
+    const Tensor ws = bytes(n, grads[0]);
+    check(api.clip_grad_norm(table.data(), (int64_t)table.size(), norm_type, max_norm, static_cast<float*>(total.data_ptr()), out(ws), n, s),
+          "orda_clip_grad_norm");
   } else {
-    total = norm_of(table, norm_type, grads[0], s);
+    if (given_total) {
+      TORCH_CHECK_VALUE(given_total->numel() == 1 && given_total->device() == grads[0].device(), entry,
+                        ": total_norm must be a one-element tensor on ", grads[0].device());
+      total = given_total->detach().to(at::kFloat).reshape({});
+    } else {
+      total = norm_of(table, norm_type, grads[0], s);
+    }
+    if (raise) {
+      TORCH_CHECK(std::isfinite(total.item<float>()), "The total norm of order ", norm_type,
+                  " for gradients from `parameters` is non-finite, so it cannot be clipped. To disable this error and scale the "
+                  "gradients by the non-finite norm anyway, set `error_if_nonfinite=False`");
+    }
+    check(api.clip_grads(table.data(), (int64_t)table.size(), static_cast<const float*>(total.const_data_ptr()), max_norm, s), "orda_clip_grads");
   }
-  if (raise) {
-    TORCH_CHECK(std::isfinite(total.item<float>()), "The total norm of order ", norm_type,
-                " for gradients from `parameters` is non-finite, so it cannot be clipped. To disable this error and scale the "
-                "gradients by the non-finite norm anyway, set `error_if_nonfinite=False`");
-  }
-  check(api.clip_grads(table.data(), (int64_t)table.size(), static_cast<const float*>(total.const_data_ptr()), max_norm, s), "orda_clip_grads");
   for (auto& [made, want] : back) want.copy_(made);
   for (size_t i = 0; i < params.size(); ++i)
     if (params[i].grad().defined()) {

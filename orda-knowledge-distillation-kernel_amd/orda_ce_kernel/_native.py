@@ -228,6 +228,8 @@ def library() -> ctypes.CDLL:
         lib.orda_grad_norm_workspace_bytes.restype, lib.orda_grad_norm_workspace_bytes.argtypes = sz, []
         lib.orda_grad_norm.restype = ctypes.c_int
         lib.orda_grad_norm.argtypes = [vp, ctypes.c_int64, ctypes.c_double, vp, vp, sz, vp]
+        lib.orda_clip_grad_norm.restype = ctypes.c_int
+        lib.orda_clip_grad_norm.argtypes = [vp, ctypes.c_int64, ctypes.c_double, ctypes.c_double, vp, vp, sz, vp]
         lib.orda_clip_grads.restype = ctypes.c_int
         lib.orda_clip_grads.argtypes = [vp, ctypes.c_int64, vp, ctypes.c_double, vp]
         lib.orda_timing_enable.restype = ctypes.c_int
@@ -365,6 +367,7 @@ _TORCH_API = (
     "orda_last_error", "orda_pad_rows", "orda_linear_saved_bytes", "orda_linear_workspace_bytes", "orda_linear_forward",
     "orda_linear_backward", "orda_ffn_inner_pitch", "orda_ffn_saved_bytes", "orda_ffn_workspace_bytes",
     "orda_ffn_forward", "orda_ffn_backward", "orda_grad_norm_workspace_bytes", "orda_grad_norm", "orda_clip_grads",
+    "orda_clip_grad_norm",
 )
 
 
