@@ -308,6 +308,7 @@ struct EpiGate {
   int64_t ld, cols, lo;
   int act;
   __device__ __forceinline__ EpiGate at(int) const { return *this; }
+  __device__ __forceinline__ EpiGate second() const { return *this; }  // (no pairs)
   template <int W> using Pre = NoPre;
   template <int W> using Col = NoPre;
   template <int W>
@@ -344,6 +345,7 @@ struct EpiGateGrad {
   const void* q;
   int64_t ldd, ld, cols, lo;
   __device__ __forceinline__ EpiGateGrad at(int) const { return *this; }
+  __device__ __forceinline__ EpiGateGrad second() const { return *this; }  // (no pairs)
   template <int W> using Col = NoPre;
   template <int W>
   __device__ __forceinline__ NoPre col(int64_t, int) const { return {}; }
@@ -378,7 +380,9 @@ struct EpiPart {
   static constexpr bool kDual = DUAL, kLight = false;
   float* p;
   int64_t stride, ld, cols;
-  __device__ __forceinline__ EpiPart at(int split) const { return EpiPart{p + split * stride, stride, ld, cols}; }
+  int64_t half;  // elements of a pair's first product in each split
+  __device__ __forceinline__ EpiPart at(int split) const { return EpiPart{p + split * stride, stride, ld, cols, half}; }
+  __device__ __forceinline__ EpiPart second() const { return EpiPart{p + half, stride, ld, cols, half}; }
   template <int W> using Pre = NoPre;
   template <int W> using Col = NoPre;
   template <int W>
@@ -406,14 +410,16 @@ __device__ __forceinline__ void epi_apply(const Epi& E, int64_t m, int64_t n, fl
 }
 
 // Sum of the partials in split order, then the epilogue; a thread takes 4
-// columns of a row.  cols a multiple of 4.
+// columns of a row.  cols a multiple of 4.  rows: M, or 2 M of a pair (the
+// second product's behind the first's).
 template <class Epi>
 __global__ __launch_bounds__(256) void k_part_reduce(const float* __restrict__ part, int splits, int64_t stride,
-                                                     int64_t ld, int64_t M, int64_t cols, Epi E) {
+                                                     int64_t ld, int64_t M, int64_t rows, int64_t cols, Epi E) {
   const int64_t nq = cols / 4;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= M * nq) return;
-  const int64_t m = i / nq, n = (i - m * nq) * 4;
+  if (i >= rows * nq) return;
+  int64_t m = i / nq;
+  const int64_t n = (i - m * nq) * 4;
   float v[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
   const float* p = part + m * ld + n;
 #pragma unroll 4
@@ -428,6 +434,10 @@ __global__ __launch_bounds__(256) void k_part_reduce(const float* __restrict__ p
   const int64_t rem = E.cols - n;
   const int cnt = rem >= 4 ? 4 : (int)rem;
   if (cnt <= 0) return;
+  if (m >= M) {
+    m -= M;
+    E = E.second();
+  }
   if constexpr (Epi::kDual) epi_apply(E, m, n, v, u, cnt);
   else epi_apply(E, m, n, v, cnt);
 }

@@ -8,7 +8,7 @@ namespace orda {
 template <class C, int LA, int LB, class Epi>
 static hipError_t s3_go(const OpPlan& pl, TileParams P, const Epi& E, hipStream_t s) {
   const int64_t bn = Epi::kDual ? C::kRowsB / 2 : C::kRowsB;
-  P.tiles_m = (int)((P.M + C::kRowsA - 1) / C::kRowsA);
+  P.tiles_m = (int)((P.M + C::kRowsA - 1) / C::kRowsA) * (P.pair > 0 ? 2 : 1);
   P.tiles_n = (int)((E.cols + bn - 1) / bn);
   P.splits = pl.splits;
   P.kps = pl.kps;

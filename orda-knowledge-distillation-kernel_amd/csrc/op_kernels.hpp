@@ -94,7 +94,7 @@ hipError_t skinny_go(const TileParams& P, const Epi& E, hipStream_t s) {
 template <class T, int LA, int LB, class Epi>
 hipError_t tile_go(const OpPlan& pl, TileParams P, const Epi& E, hipStream_t s) {
   const int64_t bm = pl.tile / 1000, bn = pl.tile % 1000 / (Epi::kDual ? 2 : 1);
-  P.tiles_m = (int)((P.M + bm - 1) / bm);
+  P.tiles_m = (int)((P.M + bm - 1) / bm) * (P.pair > 0 ? 2 : 1);
   P.tiles_n = (int)((E.cols + bn - 1) / bn);
   P.splits = pl.splits;
   P.kps = pl.kps;
@@ -136,12 +136,12 @@ hipError_t any_go(const OpPlan& pl, const TileParams& P, const Epi& E, hipStream
 template <class Epi, class Go>
 hipError_t with_splits(const OpPlan& pl, const TileParams& P, const Epi& E, float* part, hipStream_t s, const Go& go) {
   if (pl.splits == 1) return go(E);
-  const int64_t cols = (E.cols + 3) / 4 * 4, ld = Epi::kDual ? 2 * cols : cols;
-  EpiPart<Epi::kDual> Q{part, P.M * ld, ld, cols};
+  const int64_t cols = (E.cols + 3) / 4 * 4, ld = Epi::kDual ? 2 * cols : cols, rows = P.M * (P.pair > 0 ? 2 : 1);
+  EpiPart<Epi::kDual> Q{part, rows * ld, ld, cols, P.M * ld};
   const hipError_t e = go(Q);
   if (e != hipSuccess) return e;
-  const int64_t n = P.M * (cols / 4);
-  hipLaunchKernelGGL((k_part_reduce<Epi>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, part, pl.splits, P.M * ld, ld, P.M, cols, E);
+  const int64_t n = rows * (cols / 4);
+  hipLaunchKernelGGL((k_part_reduce<Epi>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, part, pl.splits, rows * ld, ld, P.M, rows, cols, E);
   return hipGetLastError();
 }
 

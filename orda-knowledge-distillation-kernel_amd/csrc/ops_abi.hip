@@ -75,24 +75,43 @@ struct TileCost {
 constexpr TileCost kTileCosts[] = {{64, 64, 3.8, 0.19, 0.27}, {64, 128, 4.8, 0.33, 0.33}, {128, 128, 6.0, 0.49, 0.58}};
 constexpr double kCus = 256.0;
 
+int64_t products(const Shape& q) { return q.pair ? 2 : 1; }
 double split_cost(const Shape& q, int64_t sp) {
-  return sp == 1 ? 0.0 : 3.0 + (double)sp * q.M * q.cols * (q.dual ? 2 : 1) * 8.0 / 8e6;
+  return sp == 1 ? 0.0 : 3.0 + (double)sp * q.M * products(q) * q.cols * (q.dual ? 2 : 1) * 8.0 / 8e6;
+}
+// Tiles of bm x bn (dual: half of them of each weight) times splits.
+double items_of(const Shape& q, int64_t bm, int64_t bn, int64_t sp) {
+  return (double)(cdiv(q.M, bm) * products(q) * cdiv(q.cols, q.dual ? bn / 2 : bn) * sp);
 }
 double tile_cost(const Shape& q, const TileCost& t, int64_t sp) {
-  const double items = (double)(cdiv(q.M, t.bm) * cdiv(q.cols, q.dual ? t.bn / 2 : t.bn) * sp);
-  const double per_cu = std::ceil(items / kCus), steps = (double)cdiv(cdiv(q.K, sp), 64);
+  const double per_cu = std::ceil(items_of(q, t.bm, t.bn, sp) / kCus), steps = (double)cdiv(cdiv(q.K, sp), 64);
   return t.fixed + steps * (per_cu <= 1 ? std::max(t.alone, t.step) : per_cu * t.step) + split_cost(q, sp);
 }
-int64_t ring_items(const Shape& q) { return cdiv(q.M, 256) * (q.pair ? 2 : 1) * cdiv(q.cols, q.dual ? 128 : 256); }
 double ring_cost(const Shape& q, int64_t sp) {
-  const double rounds = std::ceil((double)(ring_items(q) * sp) / kCus);
+  const double rounds = std::ceil(items_of(q, 256, 256, sp) / kCus);
   return 8.0 + rounds * ((double)cdiv(cdiv(q.K, sp), 64) * 1.45 + 8.0) + split_cost(q, sp);
 }
 // The ring engine takes more than one K step, and of a K-major operand whole
 // K ranges only.
 bool ring_fits(const Shape& q, int64_t sp) {
   if (q.K <= 64 * sp || sp < splits_needed(q)) return false;
-  return sp == 1 || (q.la == MNMAJ && !q.pair) || q.K % (64 * sp) == 0;
+  return sp == 1 || q.la == MNMAJ || q.K % (64 * sp) == 0;
+}
+// fp32, K steps of 32 on the split-operand engine: 1.9 to 2.4 us per step of a
+// 256 x 128 tile (one to a CU; the clock falls with the load) and 8 per tile; 64 x 64 tiles, up to three to a CU, by
+// how many there are and whether an operand is MN-major (a sweep of 13 shapes;
+// 2048^3 in 2 ranges 92 us, model 96; 1000 x 2668 x 777 in 3 ranges of large
+// tiles 41 us, 44; 300 x 300 x 4096 in 16 of small ones 17.6 us, 17.6).
+double s3_op_cost(const Shape& q, int64_t sp, bool large) {
+  const double steps = (double)cdiv(cdiv(q.K, sp), 32), part = split_cost(q, sp);
+  if (large) {
+    const double fill = items_of(q, 256, 128, sp) / kCus;
+    return std::ceil(fill) * (steps * (1.9 + 0.5 * std::min(1.0, fill)) + 8.0) + part;
+  }
+  const double items = items_of(q, 64, 64, sp), rounds = std::ceil(items / (3 * kCus));
+  constexpr double kStep[2][3] = {{0.75, 1.0, 1.45}, {1.15, 1.55, 2.0}};
+  const int load = rounds > 1 ? 2 : (int)std::ceil(items / kCus) - 1;
+  return 5.0 + rounds * steps * kStep[q.la == MNMAJ || q.lb == MNMAJ][load] + part;
 }
 
 OpPlan plan_of(const Shape& q) {
@@ -104,40 +123,25 @@ OpPlan plan_of(const Shape& q) {
     return pl;
   }
   const int64_t steps = cdiv(q.K, 64);
+  const int64_t need = q.dtype == ORDA_F32 ? 1 : splits_needed(q);
+  const int64_t most = std::max<int64_t>(need, std::min<int64_t>(16, std::max<int64_t>(1, steps / 2)));
   int64_t splits = 1;
   double best = 1e300;
-  if (q.dtype == ORDA_F32) {
-    pl.engine = OP_SPLIT3;
-    const double n = (double)q.cols * (q.dual ? 2 : 1);
-    for (int large = 0; large < 2; ++large)
-      for (int64_t sp = 1; sp <= 16 && sp * 2 <= steps + 1; ++sp) {
-        const double c = s3_cost((double)q.M, n, (double)q.K, (int)sp, large != 0);
-        if (c < best) {
-          best = c;
-          pl.tile = large ? 256 : 64;
-          splits = sp;
-        }
-      }
-  } else {
-    const int64_t need = splits_needed(q), most = std::max<int64_t>(need, std::min<int64_t>(16, std::max<int64_t>(1, steps / 2)));
-    for (int64_t sp = need; sp <= (q.pair ? need : most); ++sp) {
-      for (const TileCost& t : kTileCosts) {
-        if (q.pair) break;  // (the ring engine alone has pairs)
-        const double c = tile_cost(q, t, sp);
-        if (c < best) {
-          best = c;
-          pl.engine = OP_TILE;
-          pl.tile = t.bm * 1000 + t.bn;
-          splits = sp;
-        }
-      }
-      if (ring_fits(q, sp) && ring_cost(q, sp) < best) {
-        best = ring_cost(q, sp);
-        pl.engine = OP_RING;
-        pl.tile = 256;
-        splits = sp;
-      }
+  auto take = [&](double cost, int engine, int tile, int64_t sp) {
+    if (cost >= best) return;
+    best = cost;
+    pl.engine = engine;
+    pl.tile = tile;
+    splits = sp;
+  };
+  for (int64_t sp = need; sp <= most; ++sp) {
+    if (q.dtype == ORDA_F32) {
+      take(s3_op_cost(q, sp, true), OP_SPLIT3, 256, sp);
+      take(s3_op_cost(q, sp, false), OP_SPLIT3, 64, sp);
+      continue;
     }
+    for (const TileCost& t : kTileCosts) take(tile_cost(q, t, sp), OP_TILE, t.bm * 1000 + t.bn, sp);
+    if (ring_fits(q, sp)) take(ring_cost(q, sp), OP_RING, 256, sp);
   }
   if (pl.engine == OP_RING && splits == 1) pl.kps = q.K;
   if (splits > 1) {
@@ -150,7 +154,7 @@ OpPlan plan_of(const Shape& q) {
 // fp32 partials of a product in K ranges
 size_t part_bytes(const Shape& q) {
   const OpPlan pl = plan_of(q);
-  return pl.splits > 1 ? (size_t)pl.splits * q.M * up(q.cols, 4) * (q.dual ? 2 : 1) * 4 : 0;
+  return pl.splits > 1 ? (size_t)pl.splits * q.M * products(q) * up(q.cols, 4) * (q.dual ? 2 : 1) * 4 : 0;
 }
 
 bool rows_aligned(const void* p, int64_t ld, int dtype) { return !p || (aligned16(p) && ld % granule(dtype) == 0); }
@@ -251,7 +255,7 @@ EpiLinear<T> store_to(void* y, int64_t ldy, int64_t cols, int dtype) {
 
 // ------------------------------------------------------------ feed-forward
 struct FfnShapes {
-  Shape gate, down, dh, dx, dw, dd;
+  Shape gate, down, dh, dx, dw, dw2, dd;
   int64_t fp;  // pitch of h, a, b: inner rounded to 64 (the K step of dx, whose K has two segments of it)
 };
 int ffn_shapes(const orda_ffn_t* p, FfnShapes& s) {
@@ -272,11 +276,13 @@ int ffn_shapes(const orda_ffn_t* p, FfnShapes& s) {
   s.dh = {p->dtype, KMAJ, MNMAJ, false, p->tokens, s.fp, up(p->out_features, g), 0, p->ldd, false};
   s.dx = {p->dtype, KMAJ, MNMAJ, false, p->tokens, hp, 2 * s.fp, 0, p->ldw, false};
   s.dw = {p->dtype, MNMAJ, MNMAJ, false, p->inner, hp, p->tokens, 2 * s.fp, p->ldx, false};
+  s.dw2 = s.dw;
+  s.dw2.pair = true;
   s.dd = {p->dtype, MNMAJ, MNMAJ, false, p->out_features, ip, p->tokens, p->ldg, s.fp, false};
   return ORDA_OK;
 }
 size_t ffn_part(const FfnShapes& s, bool backward) {
-  return backward ? std::max(std::max(part_bytes(s.dh), part_bytes(s.dx)), std::max(part_bytes(s.dw), part_bytes(s.dd)))
+  return backward ? std::max(std::max(part_bytes(s.dh), part_bytes(s.dx)), std::max(part_bytes(s.dw), std::max(part_bytes(s.dw2), part_bytes(s.dd))))
                   : std::max(part_bytes(s.gate), part_bytes(s.down));
 }
 size_t ffn_ws(const orda_ffn_t* p, const FfnShapes& s, bool backward) {
@@ -486,21 +492,15 @@ int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, co
       t.kval = p->inner;
       OP_LAUNCH(launch_op_linear<T>(plan_of(s.dx), KMAJ, MNMAJ, t, store_to<T>(grad_x, p->ldgx, s.dx.cols, p->dtype), part, st));
     }
-    Shape both = s.dw;
-    both.pair = true;
-    const bool pair = grad_gate && grad_up && p->dtype != ORDA_F32 && plan_of(s.dw).engine == OP_RING && plan_of(s.dw).splits == 1;
-    if (pair) {  // one launch: its tiles fill the chip's last round better than two launches' do
-      TileParams t = product<T>(d, 2 * s.fp, x, p->ldx, p->inner, s.dw.cols, p->tokens);
+    if (grad_gate && grad_up) {  // one launch: its tiles fill the chip's last round better than two launches' do
+      TileParams t = product<T>(d, 2 * s.fp, x, p->ldx, p->inner, s.dw2.cols, p->tokens);
       t.pair = s.fp;
-      EpiLinear<T> e = store_to<T>(grad_gate, p->ldgw, s.dw.cols, p->dtype);
+      EpiLinear<T> e = store_to<T>(grad_gate, p->ldgw, s.dw2.cols, p->dtype);
       e.y1 = static_cast<T*>(grad_up);
-      OP_LAUNCH(launch_op_linear<T>(plan_of(both), MNMAJ, MNMAJ, t, e, part, st));
-    }
-    for (int i = 0; i < 2 && !pair; ++i) {
-      void* out = i ? grad_up : grad_gate;
-      if (!out) continue;
-      const TileParams t = product<T>(d + i * s.fp * (int64_t)sizeof(T), 2 * s.fp, x, p->ldx, p->inner, s.dw.cols, p->tokens);
-      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw), MNMAJ, MNMAJ, t, store_to<T>(out, p->ldgw, s.dw.cols, p->dtype), part, st));
+      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw2), MNMAJ, MNMAJ, t, e, part, st));
+    } else if (grad_gate || grad_up) {
+      const TileParams t = product<T>(d + (grad_up ? s.fp * (int64_t)sizeof(T) : 0), 2 * s.fp, x, p->ldx, p->inner, s.dw.cols, p->tokens);
+      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw), MNMAJ, MNMAJ, t, store_to<T>(grad_up ? grad_up : grad_gate, p->ldgw, s.dw.cols, p->dtype), part, st));
     }
     if (grad_down) {
       const TileParams t = product<T>(grad_output, p->ldg, h, s.fp, p->out_features, s.dd.cols, p->tokens);

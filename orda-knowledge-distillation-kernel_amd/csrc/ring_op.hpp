@@ -87,8 +87,8 @@ __global__ __launch_bounds__(kThreads4, 1) void k_ring(TileParams P, Epi E0) {
     const int lane = opaque_lane();
     const int wm = w4_m(), wn = w4_n();
     Epi E = E0.at(x.split);
-    if constexpr (LA == MNMAJ && !std::is_same_v<Epi, EpiPart<false>>) {
-      if (x.second) E = E0.second();
+    if constexpr (LA == MNMAJ) {
+      if (x.second) E = E.second();
     }
     char* buf = slot + wave_id() * 8192;
     const int64_t nlim = E.cols - x.n0;  // columns left from the tile's first one

@@ -6,7 +6,8 @@
 // Workgroup: 16 rows of W (of both weights when dual), K split over its waves
 // in blocks of 128 bytes a row, the waves' sums added through LDS in wave
 // order.  A lane holds row l % 16 of W and of x (rows past M are zero) and the
-// same 32 bytes of K in both: any order of K serves when both operands use it.
+// same two 16-byte pieces of K in both (any order of K serves when both
+// operands use it), so that 4 lanes read 64 contiguous bytes at a time.
 // The result has row (token) l % 16 and columns 4 (l / 16) .. + 3 per lane.
 #pragma once
 #include "tile16.hpp"
@@ -22,22 +23,22 @@ struct SkinnyParams {
 
 constexpr int kSkinnyWaves = 8;
 
-// 32 bytes of K of one row: K elements [k, k + 32 / sizeof(T)), those past K
-// (a multiple of 16 bytes) zero.
+// A lane's two pieces of a block, 64 bytes apart; those past K (`left` bytes
+// from the first on, a multiple of 16) are zero.
 struct Raw32 {
   uint4 v[2];
 };
 __device__ __forceinline__ Raw32 skinny_load(const char* p) {
   Raw32 r;
-  r.v[0] = reinterpret_cast<const uint4*>(p)[0];
-  r.v[1] = reinterpret_cast<const uint4*>(p)[1];
+  r.v[0] = *reinterpret_cast<const uint4*>(p);
+  r.v[1] = *reinterpret_cast<const uint4*>(p + 64);
   return r;
 }
 __device__ __forceinline__ Raw32 skinny_load(const char* p, int64_t left) {
   Raw32 r;
   r.v[0] = r.v[1] = make_uint4(0, 0, 0, 0);
-  if (left > 0) r.v[0] = reinterpret_cast<const uint4*>(p)[0];
-  if (left > 16) r.v[1] = reinterpret_cast<const uint4*>(p)[1];
+  if (left > 0) r.v[0] = *reinterpret_cast<const uint4*>(p);
+  if (left > 64) r.v[1] = *reinterpret_cast<const uint4*>(p + 64);
   return r;
 }
 template <class T>
@@ -66,10 +67,10 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void k_skinny(SkinnyParams P, Ep
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int64_t row = n0 + r < P.N ? n0 + r : P.N - 1;  // (a row past N repeats the last one and is not written)
   const int64_t kb = P.K * (int64_t)sizeof(T);          // bytes of a row
-  const char* pw = static_cast<const char*>(P.w) + row * P.ldw * (int64_t)sizeof(T) + g * 32;
-  const char* pw1 = DUAL ? static_cast<const char*>(P.w1) + row * P.ldw * (int64_t)sizeof(T) + g * 32 : nullptr;
+  const char* pw = static_cast<const char*>(P.w) + row * P.ldw * (int64_t)sizeof(T) + g * 16;
+  const char* pw1 = DUAL ? static_cast<const char*>(P.w1) + row * P.ldw * (int64_t)sizeof(T) + g * 16 : nullptr;
   const bool live = r < P.M;
-  const char* px = static_cast<const char*>(P.x) + (live ? r : 0) * P.ldx * (int64_t)sizeof(T) + g * 32;
+  const char* px = static_cast<const char*>(P.x) + (live ? r : 0) * P.ldx * (int64_t)sizeof(T) + g * 16;
   f4v c = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
   const int64_t full = kb / 128;  // whole blocks
   int64_t b = w;
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void k_skinny(SkinnyParams P, Ep
       const int64_t o = (b + u * kSkinnyWaves) * 128;
       a[u] = skinny_load(pw + o);
       if constexpr (DUAL) a1[u] = skinny_load(pw1 + o);
-      x[u] = skinny_load(px + o, live ? 32 : 0);
+      x[u] = skinny_load(px + o, live ? 128 : 0);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -89,7 +90,7 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void k_skinny(SkinnyParams P, Ep
     }
   }
   for (; b * 128 < kb; b += kSkinnyWaves) {  // the rest, and the last block's part inside K
-    const int64_t o = b * 128, left = kb - o - g * 32;
+    const int64_t o = b * 128, left = kb - o - g * 16;
     const Raw32 x = skinny_load(px + o, live ? left : 0);
     skinny_mma<T>(c, skinny_load(pw + o, left), x);
     if constexpr (DUAL) skinny_mma<T>(c1, skinny_load(pw1 + o, left), x);

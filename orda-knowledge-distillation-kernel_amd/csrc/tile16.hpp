@@ -34,7 +34,7 @@ struct TileParams {
   int64_t kval;          // valid K rows of an MN-major B (of each segment)
   int tiles_m, tiles_n, splits;
   int64_t kps;           // K of one split (a multiple of 64)
-  int64_t pair;          // > 0: two products side by side, the second with A's columns from here on (MN/MN, one split)
+  int64_t pair;          // > 0: two products side by side, the second with A's columns from here on (MN-major A; tiles_m counts both)
 };
 
 template <int R>
@@ -167,12 +167,15 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
   constexpr int G = 8;
   const int band = t / (G * P.tiles_n), first_m = band * G;
   const int gm = min(P.tiles_m - first_m, G), rem = t % (G * P.tiles_n);
-  const int64_t m0 = (int64_t)(first_m + rem % gm) * BM;
+  int tm = first_m + rem % gm;
+  const bool second = LA == MNMAJ && P.pair > 0 && tm >= P.tiles_m / 2;
+  if (second) tm -= P.tiles_m / 2;
+  const int64_t m0 = (int64_t)tm * BM;
   const int64_t n0 = (int64_t)(rem / gm) * (DUAL ? BN / 2 : BN);
   const int64_t kb0 = (int64_t)split * P.kps, ke = lmin(P.K, kb0 + P.kps);
   const int nk = (int)((ke - kb0 + 63) / 64);
   const uint32_t ldab = (uint32_t)(P.lda * 2), ldbb = (uint32_t)(P.ldb * 2);
-  const char* A = static_cast<const char*>(P.A);
+  const char* A = static_cast<const char*>(P.A) + (second ? P.pair * 2 : 0);
   const char* B = static_cast<const char*>(P.B);
   const char* B1 = static_cast<const char*>(P.B1);
   const TileDma<T, LA, BM> da;
@@ -291,7 +294,10 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
   }
   wait_vmem<0>();  // nothing may land after the waves end
 
-  const Epi E = E0.at(split);
+  Epi E = E0.at(split);
+  if constexpr (LA == MNMAJ) {
+    if (second) E = E.second();
+  }
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
     const int64_t m = m0 + wm * (BM / 2) + i * 16 + (lane & 15);

@@ -28,6 +28,7 @@ __global__ __launch_bounds__(C::kThreads, C::MB == 4 ? 2 : 3) void k_tile_s3(Til
   const int nt = b0 < total ? (total - 1 - b0) / grid + 1 : 0;
   struct Tile {
     int split;
+    bool second;  // a pair's second product
     int64_t m0, n0;
   };
   auto tile_of = [&](int i) {
@@ -38,7 +39,10 @@ __global__ __launch_bounds__(C::kThreads, C::MB == 4 ? 2 : 3) void k_tile_s3(Til
     constexpr int G = 8;
     const int band = t / (G * P.tiles_n), first_m = band * G;
     const int gm = min(P.tiles_m - first_m, G), rem = t % (G * P.tiles_n);
-    x.m0 = (int64_t)(first_m + rem % gm) * RA;
+    int tm = first_m + rem % gm;
+    x.second = LA == MNMAJ && P.pair > 0 && tm >= P.tiles_m / 2;
+    if (x.second) tm -= P.tiles_m / 2;
+    x.m0 = (int64_t)tm * RA;
     x.n0 = (int64_t)(rem / gm) * NC;
     return x;
   };
@@ -55,7 +59,7 @@ __global__ __launch_bounds__(C::kThreads, C::MB == 4 ? 2 : 3) void k_tile_s3(Til
     const int64_t kb = (int64_t)f.split * P.kps, k0 = kb + (int64_t)fs * kS3Step;
     const int64_t left = lmin(P.K, kb + P.kps) - k0;
     if constexpr (LA == KMAJ) la.template load<0, RA * 8 / C::kThreads>(A + f.m0 * P.lda + k0, P.lda, P.M - f.m0, left);
-    else la.load(A + k0 * P.lda + f.m0, P.lda, P.M - f.m0, left);
+    else la.load(A + (f.second ? P.pair : 0) + k0 * P.lda + f.m0, P.lda, P.M - f.m0, left);
     if constexpr (DUAL) {
       lb.template load<0, 1>(B + f.n0 * P.ldb + k0, P.ldb, P.N - f.n0, left);
       lb.template load<1, 2>(B1 + f.n0 * P.ldb + k0, P.ldb, P.N - f.n0, left);
@@ -98,7 +102,7 @@ __global__ __launch_bounds__(C::kThreads, C::MB == 4 ? 2 : 3) void k_tile_s3(Til
     if (P.K <= kS3Short || marks.met(mi - 1)) {
       s3_zero<MB>(acc);
       const auto* q = s3_args<TileParams>();
-      const float* a = static_cast<const float*>(q->A);
+      const float* a = static_cast<const float*>(q->A) + (x.second ? q->pair : 0);
       const float* b = static_cast<const float*>(q->B);
       const float* b1 = static_cast<const float*>(q->B1);
       const int64_t kb = (int64_t)x.split * q->kps;
@@ -122,7 +126,10 @@ __global__ __launch_bounds__(C::kThreads, C::MB == 4 ? 2 : 3) void k_tile_s3(Til
       };
       s3_native<C, 0, MB, true>(acc, kb, lmin(q->K, kb + q->kps), av, bv);
     }
-    const Epi E = E0.at(x.split);
+    Epi E = E0.at(x.split);
+    if constexpr (LA == MNMAJ) {
+      if (x.second) E = E.second();
+    }
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
       const int64_t m = ml + mb * 16;
