@@ -105,14 +105,18 @@ __device__ __forceinline__ void act_eval(int kind, const float (&x)[W], float (&
   }
 }
 
-// W consecutive values; `wide`: the address is aligned to min(16, W sizeof(T))
-// bytes and all W are there.  Otherwise the first cnt, one by one (the rest
-// read as zero).
+// W consecutive values at any address that is aligned to one of them (the
+// hardware's unaligned vector accesses; rows of odd lengths), or the first cnt
+// of them.
+template <class T, int N>
+struct AnyVec {
+  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
 template <class T, int W>
-__device__ __forceinline__ void ld_row(const T* p, float (&v)[W], bool wide, int cnt) {
-  constexpr int kB = W * (int)sizeof(T), kV = kB < 16 ? kB : 16, kE = kV / (int)sizeof(T);
-  typedef T vec __attribute__((ext_vector_type(kE)));
-  if (wide) {
+__device__ __forceinline__ void ld_row(const T* p, float (&v)[W], int cnt) {
+  constexpr int kE = W * (int)sizeof(T) <= 16 ? W : 16 / (int)sizeof(T);
+  typedef typename AnyVec<T, kE>::type vec;
+  if (cnt == W) {
 #pragma unroll
     for (int i = 0; i < W / kE; ++i) {
       const vec x = *reinterpret_cast<const vec*>(p + i * kE);
@@ -125,19 +129,24 @@ __device__ __forceinline__ void ld_row(const T* p, float (&v)[W], bool wide, int
   }
 }
 template <class T, int W>
-__device__ __forceinline__ void st_row(T* p, const float (&v)[W], bool wide, int cnt) {
-  constexpr int kB = W * (int)sizeof(T), kV = kB < 16 ? kB : 16, kE = kV / (int)sizeof(T);
-  if (wide) {
+__device__ __forceinline__ void st_row(T* p, const float (&v)[W], int cnt) {
+  constexpr int kE = W * (int)sizeof(T) <= 16 ? W : 16 / (int)sizeof(T);
+  typedef typename AnyVec<T, kE>::type vec;
+  if (cnt == W) {
 #pragma unroll
     for (int i = 0; i < W / kE; ++i) {
       if constexpr (sizeof(T) == 2) {
-        uint32_t u[kE / 2];
+        typedef uint32_t words __attribute__((ext_vector_type(kE / 2)));
+        words u;
 #pragma unroll
         for (int e = 0; e < kE / 2; ++e) u[e] = pack2<T>(v[i * kE + 2 * e], v[i * kE + 2 * e + 1]);
-        if constexpr (kE == 4) *reinterpret_cast<uint2*>(p + i * kE) = make_uint2(u[0], u[1]);
-        else *reinterpret_cast<uint4*>(p + i * kE) = make_uint4(u[0], u[1], u[2], u[3]);
+        typedef typename AnyVec<uint16_t, kE>::type half_words;
+        *reinterpret_cast<half_words*>(p + i * kE) = __builtin_bit_cast(half_words, u);
       } else {
-        *reinterpret_cast<float4*>(p + i * kE) = make_float4(v[i * 4], v[i * 4 + 1], v[i * 4 + 2], v[i * 4 + 3]);
+        vec x;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) x[e] = v[i * kE + e];
+        *reinterpret_cast<vec*>(p + i * kE) = x;
       }
     }
   } else {
@@ -152,9 +161,9 @@ template <class T, int W>
 struct RawRow {
   typedef T vec __attribute__((ext_vector_type(W)));
   vec v;
-  __device__ __forceinline__ void load(const T* p, bool wide, int cnt) {
-    if (wide) {
-      v = *reinterpret_cast<const vec*>(p);
+  __device__ __forceinline__ void load(const T* p, int cnt) {
+    if (cnt == W) {
+      v = *reinterpret_cast<const typename AnyVec<T, W>::type*>(p);
     } else {
 #pragma unroll
       for (int e = 0; e < W; ++e) v[e] = e < cnt ? p[e] : (T)0.0f;
@@ -175,7 +184,7 @@ constexpr int kKeptBytes = sizeof(T) == 4 ? 4 : 3;
 template <class T, int W>
 __device__ __forceinline__ void keep(void* base, int64_t lo, int64_t i, const float (&v)[W]) {
   if constexpr (sizeof(T) == 4) {
-    st_row<float, W>(static_cast<float*>(base) + i, v, true, W);
+    st_row<float, W>(static_cast<float*>(base) + i, v, W);
   } else {
     uint32_t h[W / 2], l[W / 4];
 #pragma unroll
@@ -241,7 +250,6 @@ struct EpiLinear {
   const T* res;
   int64_t ldy, ldd, dlo, ldr, cols;
   int act;
-  int wide;  // every row of every tensor is 16-byte aligned
   __device__ __forceinline__ EpiLinear at(int) const { return *this; }
   __device__ __forceinline__ EpiLinear second() const {
     EpiLinear e = *this;
@@ -259,19 +267,18 @@ struct EpiLinear {
   template <int W>
   __device__ __forceinline__ Col<W> col(int64_t n, int cnt) const {
     Col<W> c;
-    if (bias) c.b.load(bias + n, wide && cnt == W, cnt);
+    if (bias) c.b.load(bias + n, cnt);
     return c;
   }
   template <int W>
   __device__ __forceinline__ Pre<W> pre(int64_t m, int64_t n, int cnt) const {
     Pre<W> p;
-    if (res) p.r.load(res + m * ldr + n, wide && cnt == W, cnt);
+    if (res) p.r.load(res + m * ldr + n, cnt);
     return p;
   }
   template <int W>
   __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt, const Pre<W>& p,
                                              const Col<W>& c) const {
-    const bool full = wide && cnt == W;
     if (bias) {
 #pragma unroll
       for (int e = 0; e < W; ++e) v[e] += c.b[e];
@@ -291,7 +298,7 @@ struct EpiLinear {
 #pragma unroll
       for (int e = 0; e < W; ++e) v[e] += p.r[e];
     }
-    st_row<T, W>(y + m * ldy + n, v, full, cnt);
+    st_row<T, W>(y + m * ldy + n, v, cnt);
   }
 };
 
@@ -330,7 +337,7 @@ struct EpiGate {
     }
 #pragma unroll
     for (int e = 0; e < W; ++e) f[e] *= u[e];
-    st_row<T, W>(h + o, f, true, cnt);
+    st_row<T, W>(h + o, f, cnt);
   }
 };
 
@@ -368,8 +375,8 @@ struct EpiGateGrad {
       da[e] = v[e] * x.p[e];
       db[e] = v[e] * x.q[e];
     }
-    st_row<T, W>(d + m * ldd + n, da, true, cnt);
-    st_row<T, W>(d + m * ldd + cols + n, db, true, cnt);
+    st_row<T, W>(d + m * ldd + n, da, cnt);
+    st_row<T, W>(d + m * ldd + cols + n, db, cnt);
   }
 };
 
@@ -391,12 +398,12 @@ struct EpiPart {
   __device__ __forceinline__ NoPre col(int64_t, int) const { return {}; }
   template <int W>
   __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt, NoPre, NoPre) const {
-    st_row<float, W>(p + m * ld + n, v, cnt == W, cnt);
+    st_row<float, W>(p + m * ld + n, v, cnt);
   }
   template <int W>
   __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], float (&u)[W], int cnt, NoPre, NoPre) const {
-    st_row<float, W>(p + m * ld + n, v, cnt == W, cnt);
-    st_row<float, W>(p + m * ld + cols + n, u, cnt == W, cnt);
+    st_row<float, W>(p + m * ld + n, v, cnt);
+    st_row<float, W>(p + m * ld + cols + n, u, cnt);
   }
 };
 

@@ -19,23 +19,23 @@ __global__ __launch_bounds__(256) void k_dz(DzParams P) {
   const int64_t r0 = (int64_t)blockIdx.y * P.rows_per_block, r1 = lmin(P.rows, r0 + P.rows_per_block);
   const int64_t left = P.cols - c;
   const int cnt = left <= 0 ? 0 : (left >= W ? W : (int)left);
-  const bool wide = P.wide && cnt == W;
   const T* dy = static_cast<const T*>(P.dy);
   T* dz = static_cast<T*>(P.dz);
   float sum[W];
 #pragma unroll
   for (int e = 0; e < W; ++e) sum[e] = 0.f;
   if (c < P.ldz) {
-    for (int64_t r = r0 + w; r < r1; r += 4) {
+#pragma unroll 4
+    for (int64_t r = r0 + w; r < r1; r += 4) {  // (four rows' loads in flight)
       float g[W];
-      ld_row<T, W>(dy + r * P.ldy + c, g, wide, cnt);
+      ld_row<T, W>(dy + r * P.ldy + c, g, cnt);
       if (P.d) {
         Kept<T, W> k;
         k.load(P.d, P.dlo, r * P.ldz + c);  // (rows padded to ldz, a multiple of W)
 #pragma unroll
         for (int e = 0; e < W; ++e) g[e] = e < cnt ? g[e] * k[e] : 0.f;
       }
-      if (dz) st_row<T, W>(dz + r * P.ldz + c, g, true, W);
+      if (dz) st_row<T, W>(dz + r * P.ldz + c, g, W);
 #pragma unroll
       for (int e = 0; e < W; ++e) sum[e] += g[e];
     }

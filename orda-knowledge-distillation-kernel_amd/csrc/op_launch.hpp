@@ -37,7 +37,6 @@ struct DzParams {
   float* partial;  // [row blocks][cols], or null
   int64_t rows, cols, ldy, ldz;
   int64_t rows_per_block;
-  int wide;        // every row of dy is 16-byte aligned
 };
 template <class T> hipError_t launch_dz(const DzParams& P, hipStream_t s);
 // out[c] = sum over b of partial[b][c], in order

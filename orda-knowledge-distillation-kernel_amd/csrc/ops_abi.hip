@@ -243,13 +243,12 @@ TileParams product(const void* A, int64_t lda, const void* B, int64_t ldb, int64
   return t;
 }
 template <class T>
-EpiLinear<T> store_to(void* y, int64_t ldy, int64_t cols, int dtype) {
+EpiLinear<T> store_to(void* y, int64_t ldy, int64_t cols) {
   EpiLinear<T> e{};
   e.y = static_cast<T*>(y);
   e.ldy = ldy;
   e.cols = cols;
   e.act = ACT_NONE;
-  e.wide = rows_aligned(y, ldy, dtype);
   return e;
 }
 
@@ -338,7 +337,7 @@ int orda_linear_forward(const orda_linear_t* p, const void* x, const void* weigh
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return by_dtype(p->dtype, [&](auto tag) -> int {
     using T = decltype(tag);
-    EpiLinear<T> e = store_to<T>(y, p->out_features, p->out_features, p->dtype);
+    EpiLinear<T> e = store_to<T>(y, p->out_features, p->out_features);
     e.d = d;
     e.dlo = 2 * p->tokens * s.op;
     e.bias = static_cast<const T*>(bias);
@@ -346,7 +345,6 @@ int orda_linear_forward(const orda_linear_t* p, const void* x, const void* weigh
     e.ldd = s.op;
     e.ldr = p->ldr;
     e.act = p->activation;
-    e.wide = e.wide && rows_aligned(residual, p->ldr, p->dtype) && aligned16(bias);
     const TileParams t = product<T>(x, p->ldx, weight, p->ldw, p->tokens, p->out_features, s.fwd.K);
     OP_LAUNCH(launch_op_linear<T>(plan_of(s.fwd), KMAJ, KMAJ, t, e, reinterpret_cast<float*>(base256(workspace)), st));
     return ORDA_OK;
@@ -393,18 +391,17 @@ int orda_linear_backward(const orda_linear_t* p, const void* x, const void* weig
       z.ldy = p->out_features;
       z.ldz = s.op;
       z.rows_per_block = s.rows_per_block;
-      z.wide = aligned;
       OP_LAUNCH(launch_dz<T>(z, st));
       if (grad_bias) OP_LAUNCH(launch_colsum<T>(sums, s.blocks, p->out_features, grad_bias, st));
     }
     if (grad_x) {
       TileParams t = product<T>(dz, s.op, weight, p->ldw, p->tokens, s.dx.cols, s.dx.K);
       t.kval = p->out_features;
-      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dx), KMAJ, MNMAJ, t, store_to<T>(grad_x, p->ldgx, s.dx.cols, p->dtype), part, st));
+      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dx), KMAJ, MNMAJ, t, store_to<T>(grad_x, p->ldgx, s.dx.cols), part, st));
     }
     if (grad_weight) {
       const TileParams t = product<T>(dz, s.op, x, p->ldx, p->out_features, s.dw.cols, p->tokens);
-      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw), MNMAJ, MNMAJ, t, store_to<T>(grad_weight, p->ldgw, s.dw.cols, p->dtype), part, st));
+      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw), MNMAJ, MNMAJ, t, store_to<T>(grad_weight, p->ldgw, s.dw.cols), part, st));
     }
     return ORDA_OK;
   });
@@ -448,10 +445,9 @@ int orda_ffn_forward(const orda_ffn_t* p, const void* x, const void* w_gate, con
     TileParams t = product<T>(x, p->ldx, w_gate, p->ldw, p->tokens, p->inner, s.gate.K);
     t.B1 = w_up;
     OP_LAUNCH(launch_op_gate<T>(plan_of(s.gate), t, g, part, st));
-    EpiLinear<T> e = store_to<T>(y, p->out_features, p->out_features, p->dtype);
+    EpiLinear<T> e = store_to<T>(y, p->out_features, p->out_features);
     e.res = static_cast<const T*>(residual);
     e.ldr = p->ldr;
-    e.wide = e.wide && rows_aligned(residual, p->ldr, p->dtype);
     t = product<T>(h, s.fp, w_down, p->ldd, p->tokens, p->out_features, s.down.K);
     OP_LAUNCH(launch_op_linear<T>(plan_of(s.down), KMAJ, KMAJ, t, e, part, st));
     return ORDA_OK;
@@ -490,21 +486,21 @@ int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, co
       t.B1 = w_up;
       t.kseg = s.fp;
       t.kval = p->inner;
-      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dx), KMAJ, MNMAJ, t, store_to<T>(grad_x, p->ldgx, s.dx.cols, p->dtype), part, st));
+      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dx), KMAJ, MNMAJ, t, store_to<T>(grad_x, p->ldgx, s.dx.cols), part, st));
     }
     if (grad_gate && grad_up) {  // one launch: its tiles fill the chip's last round better than two launches' do
       TileParams t = product<T>(d, 2 * s.fp, x, p->ldx, p->inner, s.dw2.cols, p->tokens);
       t.pair = s.fp;
-      EpiLinear<T> e = store_to<T>(grad_gate, p->ldgw, s.dw2.cols, p->dtype);
+      EpiLinear<T> e = store_to<T>(grad_gate, p->ldgw, s.dw2.cols);
       e.y1 = static_cast<T*>(grad_up);
       OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw2), MNMAJ, MNMAJ, t, e, part, st));
     } else if (grad_gate || grad_up) {
       const TileParams t = product<T>(d + (grad_up ? s.fp * (int64_t)sizeof(T) : 0), 2 * s.fp, x, p->ldx, p->inner, s.dw.cols, p->tokens);
-      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw), MNMAJ, MNMAJ, t, store_to<T>(grad_up ? grad_up : grad_gate, p->ldgw, s.dw.cols, p->dtype), part, st));
+      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw), MNMAJ, MNMAJ, t, store_to<T>(grad_up ? grad_up : grad_gate, p->ldgw, s.dw.cols), part, st));
     }
     if (grad_down) {
       const TileParams t = product<T>(grad_output, p->ldg, h, s.fp, p->out_features, s.dd.cols, p->tokens);
-      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dd), MNMAJ, MNMAJ, t, store_to<T>(grad_down, p->ldgd, s.dd.cols, p->dtype), part, st));
+      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dd), MNMAJ, MNMAJ, t, store_to<T>(grad_down, p->ldgd, s.dd.cols), part, st));
     }
     return ORDA_OK;
   });
