@@ -18,7 +18,7 @@
 // different banks.
 //
 // The MFMAs run swapped (B x A^T): lane l holds row l % 16 of a block and
-// columns 4 (l / 16) .. + 3.
+// columns 4 (l / 16) .. + 3, until the epilogue.
 #pragma once
 #include "epilogue.hpp"
 
@@ -236,7 +236,11 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
   };
   const int w = wave_id(), wm = w >> 1, wn = w & 1;
   const int lane = threadIdx.x & 63;
-  auto brow = [&](int nb) { return (nb / (NB / 2)) * (BN / 2) + wn * (BN / 4) + (nb % (NB / 2)) * 16; };
+  // B rows (output columns) of a wave's block nb: BN / 2 in a row, dual the same
+  // BN / 4 of each half
+  auto bofs = [](int nb) { return DUAL ? (nb / (NB / 2)) * (BN / 2) + (nb % (NB / 2)) * 16 : nb * 16; };
+  const int wcol = wn * (DUAL ? BN / 4 : BN / 2);
+  auto brow = [&](int nb) { return wcol + bofs(nb); };
   TileFrags<T, LA, BM, MB> fa;
   TileFrags<T, LB, BN, NB> fb;
   fa.init([&](int i) { return wm * (BM / 2) + i * 16; });
@@ -268,7 +272,7 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
       }
       if constexpr (LB == KMAJ) {
 #pragma unroll
-        for (int j = 0; j < NB; ++j) b[j] = fb.read(sb, (j / (NB / 2)) * (BN / 2) + (j % (NB / 2)) * 16, hf);
+        for (int j = 0; j < NB; ++j) b[j] = fb.read(sb, bofs(j), hf);
       }
       auto transposed = [&](const auto& f, uint32_t tile, auto& frags, auto half) __attribute__((always_inline)) {
         using FR = std::remove_reference_t<decltype(f)>;
@@ -298,24 +302,53 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
   if constexpr (LA == MNMAJ) {
     if (second) E = E.second();
   }
+  // The accumulators through LDS (each wave its own part of the stages), so that
+  // a lane takes 8 consecutive columns of a row and 8 or 4 lanes a row's
+  // contiguous bytes, and the epilogue's code is there once: 8192 x 2048 x 4096
+  // with gelu and its kept derivative takes 174 us, from the accumulators' own
+  // layout (4 columns of 16 rows) it took 219; 48 x 4096 x 11008 gated 32.
+  __syncthreads();
+  constexpr int kC = BN / 8;  // 16-byte chunks of a wave's row
+  char* buf = lds + w * (BM / 2) * (BN / 2) * 4;
+  static_assert(4 * (BM / 2) * (BN / 2) * 4 <= NS * kStage, "the accumulators fit the stages");
+  auto at = [](int row, int c) {
+    return kC == 16 ? row * 256 + ((c ^ (row & 15)) << 4) : row * 128 + ((c ^ ((row >> 1) & 7)) << 4);
+  };
 #pragma unroll
-  for (int i = 0; i < MB; ++i) {
-    const int64_t m = m0 + wm * (BM / 2) + i * 16 + (lane & 15);
+  for (int i = 0; i < MB; ++i)
 #pragma unroll
-    for (int j = 0; j < (DUAL ? NB / 2 : NB); ++j) {
-      const int64_t n = n0 + brow(j) + 4 * (lane >> 4);
-      const int64_t left = E.cols - n;
-      const int cnt = left >= 4 ? 4 : (int)left;
-      if (m < P.M && cnt > 0) {
-        float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        if constexpr (DUAL) {
-          const f4v c = acc[i][j + NB / 2];
-          float u[4] = {c[0], c[1], c[2], c[3]};
-          epi_apply(E, m, n, v, u, cnt);
-        } else {
-          epi_apply(E, m, n, v, cnt);
-        }
-      }
+    for (int j = 0; j < NB; ++j)
+      *reinterpret_cast<f4v*>(buf + at(i * 16 + (lane & 15), j * 4 + (lane >> 4))) = acc[i][j];
+  // (the same wave reads them: LDS serves a wave in order)
+  constexpr int kG = (DUAL ? kC / 2 : kC) / 2;  // groups of 8 columns in a row (of one half)
+  const int g = lane % kG;
+  const int64_t n = n0 + wcol + g * 8;
+  const int64_t left = E.cols - n;
+  const int cnt = left >= 8 ? 8 : (int)left;
+  if (cnt <= 0) return;
+  const auto col = E.template col<8>(n, cnt);
+  auto take = [&](int row, int c, float (&v)[8]) __attribute__((always_inline)) {
+    const f4v x = *reinterpret_cast<const f4v*>(buf + at(row, c)), y = *reinterpret_cast<const f4v*>(buf + at(row, c + 1));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = x[e];
+      v[4 + e] = y[e];
+    }
+  };
+  const int64_t mw = m0 + wm * (BM / 2);
+#pragma unroll 2
+  for (int row = lane / kG; row < BM / 2; row += 64 / kG) {
+    const int64_t m = mw + row;
+    if (m >= P.M) break;
+    const auto pre = E.template pre<8>(m, n, cnt);
+    float v[8];
+    take(row, 2 * g, v);
+    if constexpr (DUAL) {
+      float u[8];
+      take(row, kC / 2 + 2 * g, u);
+      E(m, n, v, u, cnt, pre, col);
+    } else {
+      E(m, n, v, cnt, pre, col);
     }
   }
 }
