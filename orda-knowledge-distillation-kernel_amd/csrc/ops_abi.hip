@@ -37,6 +37,7 @@ inline int64_t granule(int dtype) { return dtype == ORDA_F32 ? 4 : 8; }  // elem
 inline bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 inline char* base256(void* ws) { return reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(ws) + 255) / 256 * 256); }
 
+// (Outputs are dense, so memory bounds the grids: 288 GB are 7e7 tiles of 64 x 32.)
 constexpr int64_t kMaxTokens = 1ll << 30;
 constexpr int64_t kMaxWidth = 1ll << 21, kMaxPitch = 1ll << 22;  // (128 rows of a K-major operand in one buffer resource)
 
@@ -50,11 +51,12 @@ struct Shape {
   bool pair;          // two products side by side (A's columns)
 };
 
-// Splits without which a split's MN-major K rows would pass a buffer resource
-// (2^31 bytes).
+// Splits without which a split's MN-major K rows would pass 2^30 bytes: the
+// offset of a step and the one that marks a chunk as out of range (2^31) add up
+// in 32 bits.
 int64_t splits_needed(const Shape& q) {
   const int64_t row = std::max<int64_t>(q.la == MNMAJ ? q.lda : 0, q.lb == MNMAJ ? q.ldb : 0) * 2;
-  const int64_t rows = std::max<int64_t>(64, row ? (0x7fffffffll / row) / 64 * 64 : up(q.K, 64));
+  const int64_t rows = std::max<int64_t>(64, row ? (0x3fffffffll / row) / 64 * 64 : up(q.K, 64));
   return cdiv(q.K, rows);
 }
 

@@ -73,9 +73,10 @@ __global__ __launch_bounds__(kThreads4, 1) void k_ring(TileParams P, Epi E0) {
     } else if constexpr (LA == KMAJ) {
       // K rows [0, kseg) from B and the rest from B1, both addressed by the K
       // row within the split (the second base lies kseg rows before B1)
-      x.b = kop4_mn(B + kb * P.ldb + x.n0, P.ldb, P.kval - kb, P.N - x.n0);
+      const int64_t klen = lmin(P.K - kb, P.kps);
+      x.b = kop4_mn(B + kb * P.ldb + x.n0, P.ldb, lmin(P.kval - kb, klen), P.N - x.n0);
       x.b1 = x.b;
-      if (B1) x.b1 = kop4_mn(B1 + (kb - P.kseg) * P.ldb + x.n0, P.ldb, P.kseg + P.kval - kb, P.N - x.n0);
+      if (B1) x.b1 = kop4_mn(B1 + (kb - P.kseg) * P.ldb + x.n0, P.ldb, lmin(P.kseg + P.kval - kb, klen), P.N - x.n0);
     }
     return x;
   };

@@ -183,8 +183,9 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
 
   // Resources of the tile's rows (K-major) or of the split's K rows from the
   // tile's first column on (MN-major), ending where the data does; a step adds
-  // a scalar offset.  A split's MN-major K rows span less than 2^31 bytes and
-  // a K-major row less than 2^23 (host).
+  // a scalar offset.  A split's MN-major K rows span less than 2^30 bytes and
+  // a K-major row at most 2^23 (host), so that kOob and a step's offset together
+  // stay below 2^32.
   const int64_t klen = ke - kb0;
   __amdgpu_buffer_rsrc_t ra, rb0, rb1;
   if constexpr (LA == KMAJ) ra = tile_rsrc(A + m0 * ldab + kb0 * 2, lmin(P.M - m0, BM) * ldab);
@@ -198,8 +199,8 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
   } else {
     // (B1's base lies kseg rows before it: both are addressed by the K row
     // within the split)
-    rb0 = tile_rsrc(B + kb0 * ldbb + n0 * 2, (P.kval - kb0) * ldbb - n0 * 2);
-    if (B1) rb1 = tile_rsrc(B1 + (kb0 - P.kseg) * (int64_t)ldbb + n0 * 2, (P.kseg + P.kval - kb0) * ldbb - n0 * 2);
+    rb0 = tile_rsrc(B + kb0 * ldbb + n0 * 2, lmin(P.kval - kb0, klen) * ldbb - n0 * 2);
+    if (B1) rb1 = tile_rsrc(B1 + (kb0 - P.kseg) * (int64_t)ldbb + n0 * 2, lmin(P.kseg + P.kval - kb0, klen) * ldbb - n0 * 2);
   }
   const int seg = (int)lmin((P.kseg - kb0 + 63) / 64, 0x7fffffff);  // B1's first step
   const int kbytes = (int)(klen * 2);
@@ -217,14 +218,14 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
     const int left = kbytes - kt * 128;  // (past the end: <= 0, zeros; the count of DMAs stays the same)
     {
       const uint32_t o = LA == KMAJ ? da.off(ldab, left, 0) : 0u;
-      const uint32_t so = LA == KMAJ ? (uint32_t)kt * 128u : (uint32_t)kt * 64u * ldab;
+      const uint32_t so = LA == KMAJ ? (uint32_t)kt * 128u : left > 0 ? (uint32_t)kt * 64u * ldab : 0u;
 #pragma unroll
       for (int q = 0; q < TileDma<T, LA, BM>::NQ; ++q)
         da.go(ra, LA == KMAJ ? o : (left > 0 ? offa[q] : kOob), so + (uint32_t)(q * TileDma<T, LA, BM>::kRowStep) * ldab, q, st);
     }
     {
       const uint32_t o = LB == KMAJ ? db.off(ldbb, left, 0) : 0u;
-      const uint32_t so = LB == KMAJ ? (uint32_t)kt * 128u : (uint32_t)kt * 64u * ldbb;
+      const uint32_t so = LB == KMAJ ? (uint32_t)kt * 128u : left > 0 ? (uint32_t)kt * 64u * ldbb : 0u;
       constexpr int H = TileDma<T, LB, BN>::NQ / 2;
 #pragma unroll
       for (int q = 0; q < TileDma<T, LB, BN>::NQ; ++q) {

@@ -14,7 +14,7 @@ import torch
 
 import orda_ce_kernel as orda
 from orda_ce_kernel import _native
-from tests._layers import ACTS, act64
+from tests._layers import ACTS, act64, ffn64, linear64
 
 ROOT = Path(__file__).resolve().parents[1]
 
@@ -227,11 +227,103 @@ def test_memory_that_meets_is_refused(rows, ok):
     assert "meet in memory" in message()
 
 
+def test_clip_grad_norm_and_pad_rows_are_checked():
+    lib, t = _native.library(), grads((256, 0, 1, 4, 4, 4, 0))
+    a = t.buffer_info()[0]
+    call = lib.orda_clip_grad_norm
+    assert call(a, 1, 3.0, 1.0, 256, 256, 1 << 20, None) == -1 and "norm_type" in message()
+    assert call(a, 1, 2.0, -1.0, 256, 256, 1 << 20, None) == -1 and "max_norm" in message()
+    assert call(a, 1, 2.0, 1.0, None, 256, 1 << 20, None) == -1 and "total" in message()
+    assert call(a, 1, 2.0, 1.0, 256, 256, 16, None) == -2 and "workspace" in message()
+    assert call(None, 1, 2.0, 1.0, 256, 256, 1 << 20, None) == -1 and "table" in message()
+    twice = grads((1024, 0, 1, 64, 64, 64, 0), (1024, 0, 1, 64, 64, 64, 0))
+    assert call(twice.buffer_info()[0], 2, 2.0, 1.0, 256, 256, 1 << 20, None) == -1 and "meet in memory" in message()
+
+    def rows(*r):
+        return (_native.Rows * len(r))(*(_native.Rows(*v) for v in r))
+
+    good = (256, 512, 2, 5, 5, 8)
+    for dtype, table, n, text in (
+            (3, rows(good), 1, "dtype"), (0, rows(good), 5, "n must be"), (0, None, 1, "n must be"), (0, rows(good), -1, "n must be"),
+            (0, rows((256, 520, 2, 5, 5, 8)), 1, "aligned"), (0, rows((257, 512, 2, 5, 5, 8)), 1, "aligned"),
+            (0, rows((None, 512, 2, 5, 5, 8)), 1, "aligned"), (0, rows((256, 512, 2, 9, 9, 8)), 1, "pitch"),
+            (0, rows((256, 512, 2, 5, 4, 8)), 1, "pitch"), (2, rows((256, 512, 2, 5, 5, 6)), 1, "pitch"),
+            (0, rows((256, 512, -1, 5, 5, 8)), 1, "size"), (0, rows((256, 512, 2, 0, 5, 8)), 1, "size")):
+        assert lib.orda_pad_rows(dtype, table, n, None) == -1 and text in message(), text
+    assert lib.orda_pad_rows(0, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("tokens,ldx", [(1 << 20, 4096), (1 << 22, 16), (1000, 1 << 22), (1 << 30, 1 << 12)])
+def test_long_operands_are_read_in_ranges_of_at_most_2_to_30_bytes(tokens, ldx):
+    """The weight gradient's operands have tokens as K: as many ranges of it, each with its fp32 partials in the workspace."""
+    p = linear(tokens=tokens, activation=0, ldx=ldx)
+    n = _native.library().orda_linear_workspace_bytes(ctypes.byref(p), 1)
+    dz = tokens * 16 * 2
+    ranges = -(-tokens * ldx * 2 // (1 << 30))
+    assert n >= dz + (ranges if ranges > 1 else 0) * 12 * 16 * 4
+
+
+def test_gradients_of_the_definitions_against_differences():
+    """linear64 and ffn64 (what the GPU tests compare with): the gradients' products with random directions against central
+    differences of y . dy; the truncation is below h^2 times the third derivative along the direction (below 1e4 here)."""
+    g = torch.Generator().manual_seed(3)
+
+    def compare(value, grads, tensors):
+        h = 1e-5
+        for name, t in tensors.items():
+            d = torch.randn(t.shape, generator=g, dtype=torch.float64)
+            hi, lo = value({**tensors, name: t + h * d}), value({**tensors, name: t - h * d})
+            assert abs(float(hi - lo) / (2 * h) - float((grads[name][0] * d).sum())) < 1e4 * h * h + 1e-7, name
+
+    def tensors(**shapes):
+        return {n: torch.randn(*s, generator=g, dtype=torch.float64) * 0.5 for n, s in shapes.items()}
+
+    for act in ("none", "gelu", "gelu_tanh", "silu", "sigmoid"):
+        t = tensors(x=(5, 7), w=(4, 7), bias=(4,), residual=(5, 4))
+        dy = torch.randn(5, 4, generator=g, dtype=torch.float64)
+        compare(lambda a: (linear64(act, torch.float32, **a)["y"][0] * dy).sum(), linear64(act, torch.float32, **t, dy=dy), t)
+        f = tensors(x=(5, 7), w_gate=(6, 7), w_up=(6, 7), w_down=(4, 6), residual=(5, 4))
+
+        def ffn_of(a, dy=None):
+            return ffn64(act, torch.float32, a["x"], a["w_gate"], a["w_up"], a["w_down"], a["residual"], dy)
+
+        compare(lambda a: (ffn_of(a)["y"][0] * dy).sum(), ffn_of(f, dy), f)
+
+
+def _sharded_clip(rank, path, results):
+    torch.distributed.init_process_group("gloo", init_method=f"file://{path}", rank=rank, world_size=2)
+    g = torch.Generator().manual_seed(rank)
+    p = torch.nn.Parameter(torch.zeros(1000))
+    p.grad = torch.randn(1000, generator=g)
+    total = orda.grad_norm([p.grad]) ** 2
+    torch.distributed.all_reduce(total)
+    got = orda.clip_grad_norm_([p], 0.5, total_norm=total.sqrt())
+    torch.save((got, p.grad), f"{results}/{rank}")
+    torch.distributed.destroy_process_group()
+
+
+def test_norm_of_gradients_sharded_over_two_ranks(tmp_path):
+    torch.multiprocessing.spawn(_sharded_clip, (str(tmp_path / "rendezvous"), str(tmp_path)), nprocs=2)
+    shards = [torch.randn(1000, generator=torch.Generator().manual_seed(r)) for r in range(2)]
+    norm = torch.cat(shards).double().norm()
+    for r, s in enumerate(shards):
+        got, grad = torch.load(tmp_path / str(r), weights_only=True)
+        assert float(got) == pytest.approx(float(norm), rel=1e-6)
+        assert torch.allclose(grad.double(), s.double() * 0.5 / norm, rtol=1e-6, atol=0)
+
+
+def test_a_missing_binding_is_an_error(monkeypatch, tmp_path):
+    monkeypatch.setattr(_native, "_TORCH_OPS", None)
+    monkeypatch.setattr(_native, "__file__", str(tmp_path / "_native.py"))
+    with pytest.raises(RuntimeError, match="orda_torch.so not found"):
+        _native.torch_ops()
+
+
 def test_struct_layouts_match_the_header(tmp_path):
     gcc = shutil.which("gcc")
     if not gcc:
         pytest.skip("no gcc")
-    names = {"orda_linear_t": _native.Linear, "orda_ffn_t": _native.FeedForward}
+    names = {"orda_linear_t": _native.Linear, "orda_ffn_t": _native.FeedForward, "orda_rows_t": _native.Rows}
     lines = [f'printf("{t}.{f} %zu\\n", offsetof({t}, {f}));' for t, c in names.items() for f, _ in c._fields_]
     lines += [f'printf("{t} %zu\\n", sizeof({t}));' for t in names]
     lines += [f'printf("orda_grad_t.{f} %zu\\n", offsetof(orda_grad_t, {f}));'
