@@ -3,10 +3,11 @@
     y = act(x W^T + bias) + residual
 
 One kernel computes it (few rows: one that streams W; more: tiles of the matrix cores, with K split over workgroups where
-there are few tiles); for the backward pass it also keeps z = x W^T + bias where an activation needs it (fp32; for 16-bit
-tensors the upper 24 bits of the fp32 values).  Backward: dz = dy act'(z) and the bias gradient in one pass over dy and z, then dx = dz W and dW = dz^T x;
-the residual's gradient is dy.  Products accumulate in fp32, every output is rounded once.  The operands, workspaces and the
-autograd node are in csrc/torch_ops.cpp.  No counterpart in the reference, whose models use torch.
+there are few tiles); for the backward pass it also keeps d = act'(x W^T + bias) where there is an activation (fp32; for
+16-bit tensors the upper 24 bits of the fp32 values).  Backward: dz = dy d and the bias gradient in one pass over dy and d,
+then dx = dz W and dW = dz^T x; the residual's gradient is dy.  Products accumulate in fp32, every output is rounded once.
+The operands, workspaces and the autograd node are in csrc/torch_ops.cpp.  No counterpart in the reference, whose models use
+torch.
 """
 from __future__ import annotations
 
@@ -29,7 +30,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     ``gelu_tanh``, ``silu``, ``sigmoid``.  The result has the compute dtype of ``x`` and ``weight`` (the loss's rule: an
     active autocast dtype, else bf16 if either is, fp16, fp32).  Rows that are a multiple of 16 bytes apart are read where
     they are; odd feature counts, unaligned or transposed tensors are copied first.  Gradients for every tensor; once
-    differentiable.  ``backend`` as :func:`distillation_loss` has it."""
+    differentiable.  A training call with an activation keeps 3 bytes (fp32: 4) per output element.  ``backend`` as :func:`distillation_loss` has it."""
     check_tensors("fused_linear", activation, x, weight=weight, bias=bias, residual=residual)
     if weight.ndim != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] == 0:
         raise ValueError(f"fused_linear: weight must have shape (out_features, {x.shape[-1]}), got {tuple(weight.shape)}")
