@@ -297,6 +297,7 @@ static int64_t elements_of(const GradSpan* g, int64_t n) {
 // Elements of a chunk of the norm: one 16-byte access per thread of bf16 where
 // that fills the chip, longer ones for large sets.  Of clipping: 2048.
 constexpr int64_t kClipChunk = 2048, kNormLarge = 64ll << 20;
+constexpr int kClipGroups = 1 << 23;  // (a launch has fewer than 2^32 threads; past them workgroups take several chunks)
 static int64_t norm_chunk(int64_t elements) { return elements < kNormLarge ? 2048 : 16384; }
 
 template <class T, int KIND>
@@ -363,7 +364,7 @@ static hipError_t clip_kind(const GradSpan* g, int64_t n, ClipParams P, hipStrea
       for (int place = 0; place < 2; ++place) {
         if (place && in != out) continue;
         P.in_place = place;
-        const hipError_t e = for_tables(g, n, in, out, place, kClipChunk, 1 << 30, [&](const SpanTable& S, int groups) {
+        const hipError_t e = for_tables(g, n, in, out, place, kClipChunk, kClipGroups, [&](const SpanTable& S, int groups) {
           switch (in) {
             case DT_BF16: return clip_out<bf16, KIND>(S, groups, out, P, s);
             case DT_F16: return clip_out<f16, KIND>(S, groups, out, P, s);

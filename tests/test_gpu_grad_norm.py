@@ -169,3 +169,17 @@ def test_captured_norm_and_clipping():
         check_clipped(outs, grads, float(total), 1.0)
         orda.grad_norm(grads)
         torch.cuda.synchronize()
+
+
+def test_more_than_2_to_31_elements():
+    """One gradient past 32-bit indexes, beside a small one: 0.5 and, at its end, -3; every square and sum is exact."""
+    n = (1 << 31) + 77
+    big, small = torch.nn.Parameter(torch.empty(n, dtype=torch.bfloat16, device="cuda")), torch.nn.Parameter(torch.zeros(5, device="cuda"))
+    big.grad, small.grad = torch.full_like(big.data, 0.5), torch.ones(5, device="cuda")
+    big.grad[-3:] = -3.0
+    want = math.sqrt((n - 3) * 0.25 + 27 + 5)
+    assert float(orda.grad_norm([big.grad, small.grad])) == pytest.approx(want, rel=2.0 ** -23)
+    total = orda.clip_grad_norm_([big, small], want / 2)
+    assert float(total) == pytest.approx(want, rel=2.0 ** -23)
+    assert bool((big.grad[:-3] == 0.25).all()) and big.grad[-3:].tolist() == [-1.5] * 3
+    assert torch.allclose(small.grad, torch.full_like(small.grad, 0.5), rtol=1e-5)
