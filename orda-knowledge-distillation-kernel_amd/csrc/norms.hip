@@ -62,16 +62,20 @@ __device__ __forceinline__ void for_chunks(const SpanTable& S, const F& f) {
   }
 }
 
-template <class T, int KIND>
-__device__ __forceinline__ void norm_add(double& s, float x) {
+// What a thread adds up in: fp64, and the largest magnitude, which is one of the
+// values, in fp32.
+template <int KIND>
+using NormSum = typename std::conditional<KIND == 0, float, double>::type;
+template <int KIND>
+__device__ __forceinline__ void norm_add(NormSum<KIND>& s, float x) {
   if constexpr (KIND == 2) s = fma((double)x, (double)x, s);
   else if constexpr (KIND == 1) s += (double)fabsf(x);
-  else s = (fabsf(x) > s || x != x) ? (double)fabsf(x) : s;  // (a NaN stays: nothing compares above it)
+  else s = !(fabsf(x) <= s) && s == s ? fabsf(x) : s;  // (a NaN takes its place and stays)
 }
-template <int KIND>
-__device__ __forceinline__ double norm_join(double a, double b) {
+template <int KIND, class S>
+__device__ __forceinline__ S norm_join(S a, S b) {
   if constexpr (KIND != 0) return a + b;
-  else return (b > a || b != b) ? b : a;
+  else return !(b <= a) && a == a ? b : a;
 }
 
 // A 16-byte vector of T as floats.
@@ -93,8 +97,8 @@ __device__ __forceinline__ void unpack16(const uint4& u, float (&v)[16 / sizeof(
 template <class T, int KIND>
 __global__ __launch_bounds__(256) void k_grad_norm(SpanTable S, double* partials, int first) {
   constexpr int VE = 16 / (int)sizeof(T), U = 4;
-  __shared__ double red[4];
-  double s = 0.0;
+  __shared__ NormSum<KIND> red[4];
+  NormSum<KIND> s = 0;
   for_chunks<T>(S, [&](int, int, const T* p, int64_t lo, int64_t hi) {
     int64_t e = lo + (int64_t)threadIdx.x * VE;
     for (; e + (U - 1) * 256 * VE + VE <= hi && lo >= 0; e += U * 256 * VE) {
@@ -106,7 +110,7 @@ __global__ __launch_bounds__(256) void k_grad_norm(SpanTable S, double* partials
         float x[VE];
         unpack16<T>(v[u], x);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) norm_add<T, KIND>(s, x[i]);
+        for (int i = 0; i < VE; ++i) norm_add<KIND>(s, x[i]);
       }
     }
     for (; e < hi; e += 256 * VE) {
@@ -114,11 +118,11 @@ __global__ __launch_bounds__(256) void k_grad_norm(SpanTable S, double* partials
       if (e >= 0 && e + VE <= hi) {
         unpack16<T>(*reinterpret_cast<const uint4*>(p + e), x);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) norm_add<T, KIND>(s, x[i]);
+        for (int i = 0; i < VE; ++i) norm_add<KIND>(s, x[i]);
       } else {
 #pragma unroll
         for (int i = 0; i < VE; ++i)
-          if (e + i >= 0 && e + i < hi) norm_add<T, KIND>(s, to_f32(p[e + i]));
+          if (e + i >= 0 && e + i < hi) norm_add<KIND>(s, to_f32(p[e + i]));
       }
     }
   });
@@ -127,7 +131,7 @@ __global__ __launch_bounds__(256) void k_grad_norm(SpanTable S, double* partials
   __syncthreads();
   if (threadIdx.x != 0) return;
   for (int i = 1; i < 4; ++i) s = norm_join<KIND>(s, red[i]);
-  partials[blockIdx.x] = first ? s : norm_join<KIND>(partials[blockIdx.x], s);
+  partials[blockIdx.x] = first ? (double)s : norm_join<KIND>(partials[blockIdx.x], (double)s);
 }
 
 // The norm from n partials, by all 256 threads of a workgroup (valid in all).
