@@ -366,7 +366,7 @@ typedef struct orda_linear {
   int64_t in_features;   /* columns of x                                     */
   int64_t out_features;  /* rows of weight                                   */
   int64_t ldx, ldw;      /* row pitches of x and weight in elements          */
-  int64_t ldr;           /* of residual                                      */
+  int64_t ldr;           /* of residual, at most 2^22                        */
   int64_t ldgx, ldgw;    /* of grad_x and grad_weight (backward only)        */
 } orda_linear_t;
 
@@ -406,7 +406,7 @@ typedef struct orda_ffn {
   int64_t ldx;           /* pitch of x                                       */
   int64_t ldw;           /* of w_gate and w_up                               */
   int64_t ldd;           /* of w_down                                        */
-  int64_t ldr;           /* of residual                                      */
+  int64_t ldr;           /* of residual, at most 2^22                        */
   int64_t ldg;           /* backward: of grad_output, a multiple of 8 (fp32:
                             4), rows 16-byte aligned and zero-padded         */
   int64_t ldgx;          /* backward: of grad_x                              */

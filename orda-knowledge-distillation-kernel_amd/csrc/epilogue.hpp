@@ -4,6 +4,8 @@
 // activation's derivative on the way back.  Every engine hands an epilogue W
 // consecutive columns of one row, in fp32; each output is rounded once.
 #pragma once
+#include <type_traits>
+
 #include "orda_core.hpp"
 
 namespace orda {
@@ -174,17 +176,31 @@ struct RawRow {
 
 // Factors that the backward pass multiplies by.  For 16-bit tensors they are
 // kept as the upper 24 bits of the fp32 value (15 bits after the leading one,
-// fp32's range), in a plane of 16-bit halves and a plane of bytes `lo` bytes
-// behind it: rounded to bf16 they made the gradients of the feed-forward block
-// 1.8 times as far off float64 as one rounding at the end, with 24 bits 1.4
-// times (da and db are rounded as operands).  fp32: as is.
+// fp32's range), in a plane of 16-bit halves and a plane of bytes: rounded to
+// bf16 they made the gradients of the feed-forward block 1.8 times as far off
+// float64 as one rounding at the end, with 24 bits 1.4 times (da and db are
+// rounded as operands).  fp32: as is, in the first plane.
 // i: index of the first of W values, a multiple of W.
 template <class T>
 constexpr int kKeptBytes = sizeof(T) == 4 ? 4 : 3;
+struct Planes {
+  char* hi;
+  char* lo;
+  // the planes from value i on
+  template <class T>
+  __device__ __forceinline__ Planes from(int64_t i) const {
+    return {hi + i * (sizeof(T) == 4 ? 4 : 2), lo + i};
+  }
+};
+template <class T>
+__host__ inline Planes planes(const void* base, int64_t values) {
+  char* p = static_cast<char*>(const_cast<void*>(base));
+  return {p, p ? p + 2 * values : nullptr};
+}
 template <class T, int W>
-__device__ __forceinline__ void keep(void* base, int64_t lo, int64_t i, const float (&v)[W]) {
+__device__ __forceinline__ void keep(const Planes& p, uint32_t i, const float (&v)[W]) {
   if constexpr (sizeof(T) == 4) {
-    st_row<float, W>(static_cast<float*>(base) + i, v, W);
+    st_row<float, W>(reinterpret_cast<float*>(p.hi + i * 4), v, W);
   } else {
     uint32_t h[W / 2], l[W / 4];
 #pragma unroll
@@ -196,13 +212,12 @@ __device__ __forceinline__ void keep(void* base, int64_t lo, int64_t i, const fl
       const uint32_t b = __builtin_amdgcn_perm(__float_as_uint(v[4 * e + 3]), __float_as_uint(v[4 * e + 2]), 0x0c0c0501u);
       l[e] = a | (b << 16);
     }
-    char* p = static_cast<char*>(base);
     if constexpr (W == 4) {
-      *reinterpret_cast<uint2*>(p + i * 2) = make_uint2(h[0], h[1]);
-      *reinterpret_cast<uint32_t*>(p + lo + i) = l[0];
+      *reinterpret_cast<uint2*>(p.hi + i * 2) = make_uint2(h[0], h[1]);
+      *reinterpret_cast<uint32_t*>(p.lo + i) = l[0];
     } else {
-      *reinterpret_cast<uint4*>(p + i * 2) = make_uint4(h[0], h[1], h[2], h[3]);
-      *reinterpret_cast<uint2*>(p + lo + i) = make_uint2(l[0], l[1]);
+      *reinterpret_cast<uint4*>(p.hi + i * 2) = make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint2*>(p.lo + i) = make_uint2(l[0], l[1]);
     }
   }
 }
@@ -212,13 +227,12 @@ struct Kept {
   typedef uint32_t lv __attribute__((ext_vector_type(W / 4)));
   hv h;
   lv l;
-  __device__ __forceinline__ void load(const void* base, int64_t lo, int64_t i) {
-    const char* p = static_cast<const char*>(base);
+  __device__ __forceinline__ void load(const Planes& p, uint32_t i) {
     if constexpr (sizeof(T) == 4) {
-      h = *reinterpret_cast<const hv*>(p + i * 4);
+      h = *reinterpret_cast<const hv*>(p.hi + i * 4);
     } else {
-      h = *reinterpret_cast<const hv*>(p + i * 2);
-      l = *reinterpret_cast<const lv*>(p + lo + i);
+      h = *reinterpret_cast<const hv*>(p.hi + i * 2);
+      l = *reinterpret_cast<const lv*>(p.lo + i);
     }
   }
   __device__ __forceinline__ float operator[](int e) const {
@@ -230,12 +244,23 @@ struct Kept {
   }
 };
 
-// Epilogues.  E(m, n, v[, u], cnt, pre, col) takes W <= 8 columns n .. of row m,
-// of which cnt are valid; pre<W>(m, n, cnt) and, for what depends on the
-// columns alone, col<W>(n, cnt) load what it reads.  epi_apply() is all three.  `cols` is the number of columns written; kDual: v and u are
-// the two products of the same columns.  at(split): the epilogue of one K range
-// (partials only).
+// Epilogues.  E.tile(m0, n0) is the epilogue of a tile: its rows and columns
+// count from there, so that an element is a uniform pointer and 32 bits of
+// lane offset (at most 256 rows of at most 2^24 bytes): with 64-bit offsets from
+// the tensors' own bases 8192 x 2048 x 4096 with gelu took 177 us instead of 174,
+// and two row blocks of loads ahead (ring_op.hpp) did not fit the registers.  E(m, n, v[, u], cnt, pre, col) takes W <= 8
+// columns n .. of row m, of which cnt are valid; pre<W>(m, n, cnt) and, for what
+// depends on the columns alone, col<W>(n, cnt) load what it reads.  epi_apply()
+// is all three.  `cols`: columns left from the tile's first one.  kDual: v and u
+// are the two products of the same columns.  at(split): the epilogue of one K
+// range (partials only); second(): of a pair's second product.
 struct NoPre {};
+
+// The element `i` elements on (32 bits of byte offset).
+template <class T>
+__device__ __forceinline__ T* on(T* p, uint32_t i) {
+  return reinterpret_cast<T*>(reinterpret_cast<char*>(const_cast<typename std::remove_const<T>::type*>(p)) + i * (uint32_t)sizeof(T));
+}
 
 // y = act(v + bias) + residual; d, when given, keeps act'(v + bias) for the
 // backward pass, in rows of ldd (a multiple of 8, at least cols; the columns
@@ -245,15 +270,24 @@ struct EpiLinear {
   static constexpr bool kDual = false, kLight = false;
   T* y;
   T* y1;  // the output of a pair's second product
-  void* d;
+  Planes d;
   const T* bias;
   const T* res;
-  int64_t ldy, ldd, dlo, ldr, cols;
+  int64_t ldy, ldd, ldr, cols;
   int act;
   __device__ __forceinline__ EpiLinear at(int) const { return *this; }
   __device__ __forceinline__ EpiLinear second() const {
     EpiLinear e = *this;
     e.y = y1;
+    return e;
+  }
+  __device__ __forceinline__ EpiLinear tile(int64_t m0, int64_t n0) const {
+    EpiLinear e = *this;
+    e.y += m0 * ldy + n0;
+    if (d.hi) e.d = d.template from<T>(m0 * ldd + n0);
+    if (bias) e.bias += n0;
+    if (res) e.res += m0 * ldr + n0;
+    e.cols -= n0;
     return e;
   }
   template <int W>
@@ -265,19 +299,19 @@ struct EpiLinear {
     RawRow<T, W> b;
   };
   template <int W>
-  __device__ __forceinline__ Col<W> col(int64_t n, int cnt) const {
+  __device__ __forceinline__ Col<W> col(uint32_t n, int cnt) const {
     Col<W> c;
-    if (bias) c.b.load(bias + n, cnt);
+    if (bias) c.b.load(on(bias, n), cnt);
     return c;
   }
   template <int W>
-  __device__ __forceinline__ Pre<W> pre(int64_t m, int64_t n, int cnt) const {
+  __device__ __forceinline__ Pre<W> pre(uint32_t m, uint32_t n, int cnt) const {
     Pre<W> p;
-    if (res) p.r.load(res + m * ldr + n, cnt);
+    if (res) p.r.load(on(res, m * (uint32_t)ldr + n), cnt);
     return p;
   }
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt, const Pre<W>& p,
+  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, float (&v)[W], int cnt, const Pre<W>& p,
                                              const Col<W>& c) const {
     if (bias) {
 #pragma unroll
@@ -285,9 +319,9 @@ struct EpiLinear {
     }
     if (act != ACT_NONE) {
       float f[W], df[W];
-      if (d) {
+      if (d.hi) {
         act_eval<T, true, W>(act, v, f, df);
-        keep<T, W>(d, dlo, m * ldd + n, df);
+        keep<T, W>(d, m * (uint32_t)ldd + n, df);
       } else {
         act_eval<T, false, W>(act, v, f, df);
       }
@@ -298,7 +332,7 @@ struct EpiLinear {
 #pragma unroll
       for (int e = 0; e < W; ++e) v[e] += p.r[e];
     }
-    st_row<T, W>(y + m * ldy + n, v, cnt);
+    st_row<T, W>(on(y, m * (uint32_t)ldy + n), v, cnt);
   }
 };
 
@@ -310,109 +344,136 @@ template <class T>
 struct EpiGate {
   static constexpr bool kDual = true, kLight = false;
   T* h;
-  void* p;
-  void* q;
-  int64_t ld, cols, lo;
+  Planes p, q;
+  int64_t ld, cols;
   int act;
   __device__ __forceinline__ EpiGate at(int) const { return *this; }
   __device__ __forceinline__ EpiGate second() const { return *this; }  // (no pairs)
+  __device__ __forceinline__ EpiGate tile(int64_t m0, int64_t n0) const {
+    EpiGate e = *this;
+    const int64_t i = m0 * ld + n0;
+    e.h += i;
+    if (p.hi) {
+      e.p = p.template from<T>(i);
+      e.q = q.template from<T>(i);
+    }
+    e.cols -= n0;
+    return e;
+  }
   template <int W> using Pre = NoPre;
   template <int W> using Col = NoPre;
   template <int W>
-  __device__ __forceinline__ NoPre pre(int64_t, int64_t, int) const { return {}; }
+  __device__ __forceinline__ NoPre pre(uint32_t, uint32_t, int) const { return {}; }
   template <int W>
-  __device__ __forceinline__ NoPre col(int64_t, int) const { return {}; }
+  __device__ __forceinline__ NoPre col(uint32_t, int) const { return {}; }
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&g)[W], float (&u)[W], int cnt, NoPre, NoPre) const {
-    const int64_t o = m * ld + n;
+  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, float (&g)[W], float (&u)[W], int, NoPre, NoPre) const {
+    const uint32_t o = m * (uint32_t)ld + n;
     float f[W], df[W];
-    if (p) {
+    if (p.hi) {
       act_eval<T, true, W>(act, g, f, df);
 #pragma unroll
       for (int e = 0; e < W; ++e) df[e] *= u[e];
-      keep<T, W>(p, lo, o, df);
-      keep<T, W>(q, lo, o, f);
+      keep<T, W>(p, o, df);
+      keep<T, W>(q, o, f);
     } else {
       act_eval<T, false, W>(act, g, f, df);
     }
 #pragma unroll
     for (int e = 0; e < W; ++e) f[e] *= u[e];
-    st_row<T, W>(h + o, f, cnt);
+    st_row<T, W>(on(h, o), f, W);
   }
 };
 
 // From dh (fp32, never rounded): da = dh p, db = dh q, rounded to T as the
-// operands of the next products.  d is [M x ldd]: da in the first `cols`
-// columns of a row, db in the next; cols = ld a multiple of 64.
+// operands of the next products.  da and db are the two halves of rows of ldd;
+// cols = ld a multiple of 64.
 template <class T>
 struct EpiGateGrad {
   static constexpr bool kDual = false, kLight = true;
-  T* d;
-  const void* p;
-  const void* q;
-  int64_t ldd, ld, cols, lo;
+  T* da;
+  T* db;
+  Planes p, q;
+  int64_t ldd, ld, cols;
   __device__ __forceinline__ EpiGateGrad at(int) const { return *this; }
   __device__ __forceinline__ EpiGateGrad second() const { return *this; }  // (no pairs)
+  __device__ __forceinline__ EpiGateGrad tile(int64_t m0, int64_t n0) const {
+    EpiGateGrad e = *this;
+    e.da += m0 * ldd + n0;
+    e.db += m0 * ldd + n0;
+    e.p = p.template from<T>(m0 * ld + n0);
+    e.q = q.template from<T>(m0 * ld + n0);
+    e.cols -= n0;
+    return e;
+  }
   template <int W> using Col = NoPre;
   template <int W>
-  __device__ __forceinline__ NoPre col(int64_t, int) const { return {}; }
+  __device__ __forceinline__ NoPre col(uint32_t, int) const { return {}; }
   template <int W>
   struct Pre {
     Kept<T, W> p, q;
   };
   template <int W>
-  __device__ __forceinline__ Pre<W> pre(int64_t m, int64_t n, int) const {
+  __device__ __forceinline__ Pre<W> pre(uint32_t m, uint32_t n, int) const {
     Pre<W> x;
-    x.p.load(p, lo, m * ld + n);
-    x.q.load(q, lo, m * ld + n);
+    x.p.load(p, m * (uint32_t)ld + n);
+    x.q.load(q, m * (uint32_t)ld + n);
     return x;
   }
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt, const Pre<W>& x, NoPre) const {
-    float da[W], db[W];
+  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, float (&v)[W], int, const Pre<W>& x, NoPre) const {
+    float a[W], b[W];
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-      da[e] = v[e] * x.p[e];
-      db[e] = v[e] * x.q[e];
+      a[e] = v[e] * x.p[e];
+      b[e] = v[e] * x.q[e];
     }
-    st_row<T, W>(d + m * ldd + n, da, cnt);
-    st_row<T, W>(d + m * ldd + cols + n, db, cnt);
+    const uint32_t o = m * (uint32_t)ldd + n;
+    st_row<T, W>(on(da, o), a, W);
+    st_row<T, W>(on(db, o), b, W);
   }
 };
 
 // fp32 partial of one K range: [splits][M][ld], a dual product's second half
-// in columns cols .. of a row.  (ld a multiple of 4.)
+// `cols` columns behind its first (p1).  (ld a multiple of 4.)
 template <bool DUAL>
 struct EpiPart {
   static constexpr bool kDual = DUAL, kLight = false;
   float* p;
+  float* p1;
   int64_t stride, ld, cols;
   int64_t half;  // elements of a pair's first product in each split
-  __device__ __forceinline__ EpiPart at(int split) const { return EpiPart{p + split * stride, stride, ld, cols, half}; }
-  __device__ __forceinline__ EpiPart second() const { return EpiPart{p + half, stride, ld, cols, half}; }
+  __device__ __forceinline__ EpiPart moved(int64_t by) const { return {p + by, p1 + by, stride, ld, cols, half}; }
+  __device__ __forceinline__ EpiPart at(int split) const { return moved(split * stride); }
+  __device__ __forceinline__ EpiPart second() const { return moved(half); }
+  __device__ __forceinline__ EpiPart tile(int64_t m0, int64_t n0) const {
+    EpiPart e = moved(m0 * ld + n0);
+    e.cols -= n0;
+    return e;
+  }
   template <int W> using Pre = NoPre;
   template <int W> using Col = NoPre;
   template <int W>
-  __device__ __forceinline__ NoPre pre(int64_t, int64_t, int) const { return {}; }
+  __device__ __forceinline__ NoPre pre(uint32_t, uint32_t, int) const { return {}; }
   template <int W>
-  __device__ __forceinline__ NoPre col(int64_t, int) const { return {}; }
+  __device__ __forceinline__ NoPre col(uint32_t, int) const { return {}; }
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], int cnt, NoPre, NoPre) const {
-    st_row<float, W>(p + m * ld + n, v, cnt);
+  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, float (&v)[W], int cnt, NoPre, NoPre) const {
+    st_row<float, W>(on(p, m * (uint32_t)ld + n), v, cnt);
   }
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&v)[W], float (&u)[W], int cnt, NoPre, NoPre) const {
-    st_row<float, W>(p + m * ld + n, v, cnt);
-    st_row<float, W>(p + m * ld + cols + n, u, cnt);
+  __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, float (&v)[W], float (&u)[W], int cnt, NoPre, NoPre) const {
+    st_row<float, W>(on(p, m * (uint32_t)ld + n), v, cnt);
+    st_row<float, W>(on(p1, m * (uint32_t)ld + n), u, cnt);
   }
 };
 
 template <class Epi, int W>
-__device__ __forceinline__ void epi_apply(const Epi& E, int64_t m, int64_t n, float (&v)[W], int cnt) {
+__device__ __forceinline__ void epi_apply(const Epi& E, uint32_t m, uint32_t n, float (&v)[W], int cnt) {
   E(m, n, v, cnt, E.template pre<W>(m, n, cnt), E.template col<W>(n, cnt));
 }
 template <class Epi, int W>
-__device__ __forceinline__ void epi_apply(const Epi& E, int64_t m, int64_t n, float (&v)[W], float (&u)[W], int cnt) {
+__device__ __forceinline__ void epi_apply(const Epi& E, uint32_t m, uint32_t n, float (&v)[W], float (&u)[W], int cnt) {
   E(m, n, v, u, cnt, E.template pre<W>(m, n, cnt), E.template col<W>(n, cnt));
 }
 
@@ -438,15 +499,15 @@ __global__ __launch_bounds__(256) void k_part_reduce(const float* __restrict__ p
       u[0] += y.x; u[1] += y.y; u[2] += y.z; u[3] += y.w;
     }
   }
-  const int64_t rem = E.cols - n;
-  const int cnt = rem >= 4 ? 4 : (int)rem;
-  if (cnt <= 0) return;
   if (m >= M) {
     m -= M;
     E = E.second();
   }
-  if constexpr (Epi::kDual) epi_apply(E, m, n, v, u, cnt);
-  else epi_apply(E, m, n, v, cnt);
+  E = E.tile(m, n);
+  const int cnt = E.cols >= 4 ? 4 : (int)E.cols;
+  if (cnt <= 0) return;
+  if constexpr (Epi::kDual) epi_apply(E, 0, 0, v, u, cnt);
+  else epi_apply(E, 0, 0, v, cnt);
 }
 
 }  // namespace orda

@@ -29,9 +29,9 @@ __global__ __launch_bounds__(256) void k_dz(DzParams P) {
     for (int64_t r = r0 + w; r < r1; r += 4) {  // (four rows' loads in flight)
       float g[W];
       ld_row<T, W>(dy + r * P.ldy + c, g, cnt);
-      if (P.d) {
+      if (P.d.hi) {
         Kept<T, W> k;
-        k.load(P.d, P.dlo, r * P.ldz + c);  // (rows padded to ldz, a multiple of W)
+        k.load(P.d.template from<T>(r * P.ldz + c), 0);  // (rows padded to ldz, a multiple of W)
 #pragma unroll
         for (int e = 0; e < W; ++e) g[e] = e < cnt ? g[e] * k[e] : 0.f;
       }
@@ -137,7 +137,7 @@ template <class Epi, class Go>
 hipError_t with_splits(const OpPlan& pl, const TileParams& P, const Epi& E, float* part, hipStream_t s, const Go& go) {
   if (pl.splits == 1) return go(E);
   const int64_t cols = (E.cols + 3) / 4 * 4, ld = Epi::kDual ? 2 * cols : cols, rows = P.M * (P.pair > 0 ? 2 : 1);
-  EpiPart<Epi::kDual> Q{part, rows * ld, ld, cols, P.M * ld};
+  EpiPart<Epi::kDual> Q{part, part + cols, rows * ld, ld, cols, P.M * ld};
   const hipError_t e = go(Q);
   if (e != hipSuccess) return e;
   const int64_t n = rows * (cols / 4);

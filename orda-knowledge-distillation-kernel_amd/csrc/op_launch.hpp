@@ -31,8 +31,7 @@ template <class T> hipError_t launch_op_gate_grad(const OpPlan& pl, TileParams P
 // rows.
 struct DzParams {
   const void* dy;
-  const void* d;   // as keep() wrote it, in rows of ldz (dlo: its second plane); null: dz = dy
-  int64_t dlo;
+  Planes d;        // as keep() wrote it, in rows of ldz; null: dz = dy
   void* dz;        // null: only the sums
   float* partial;  // [row blocks][cols], or null
   int64_t rows, cols, ldy, ldz;

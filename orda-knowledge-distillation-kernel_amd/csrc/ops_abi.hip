@@ -39,7 +39,9 @@ inline char* base256(void* ws) { return reinterpret_cast<char*>((reinterpret_cas
 
 // (Outputs are dense, so memory bounds the grids: 288 GB are 7e7 tiles of 64 x 32.)
 constexpr int64_t kMaxTokens = 1ll << 30;
-constexpr int64_t kMaxWidth = 1ll << 21, kMaxPitch = 1ll << 22;  // (128 rows of a K-major operand in one buffer resource)
+// (128 rows of a K-major operand in one buffer resource, 256 rows of an output
+// within 2^32 bytes)
+constexpr int64_t kMaxWidth = 1ll << 21, kMaxPitch = 1ll << 22;
 
 // ------------------------------------------------------------- the engine
 // One product C[M x cols] = A B^T over K; dual: two weights.
@@ -189,6 +191,10 @@ int check_pitch(const char* what, const char* name, int64_t ld, int64_t width, i
                 (long long)up(width, g), (long long)ld);
   return ORDA_OK;
 }
+int check_residual(const char* what, int64_t ld, int64_t width) {
+  if (ld < width || ld > kMaxPitch) return fail(ORDA_EINVAL, "%s: ldr must be in [%lld, 2^22], got %lld", what, (long long)width, (long long)ld);
+  return ORDA_OK;
+}
 #define OP_TRY(expr)                 \
   do {                               \
     const int rc_ = (expr);          \
@@ -334,14 +340,13 @@ int orda_linear_forward(const orda_linear_t* p, const void* x, const void* weigh
   OP_TRY(linear_shapes(p, s));
   if (!x || !weight || !y) return fail(ORDA_EINVAL, "orda_linear_forward: x, weight and y are required");
   if (!aligned16(x) || !aligned16(weight) || !aligned16(d)) return fail(ORDA_EINVAL, "orda_linear_forward: x, weight and d must be 16-byte aligned");
-  if (residual && p->ldr < p->out_features) return fail(ORDA_EINVAL, "orda_linear_forward: ldr must be at least out_features");
+  if (residual) OP_TRY(check_residual("orda_linear_forward", p->ldr, p->out_features));
   OP_TRY(check_workspace("orda_linear_forward", workspace, workspace_bytes, linear_ws(p, s, false)));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return by_dtype(p->dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     EpiLinear<T> e = store_to<T>(y, p->out_features, p->out_features);
-    e.d = d;
-    e.dlo = 2 * p->tokens * s.op;
+    e.d = planes<T>(d, p->tokens * s.op);
     e.bias = static_cast<const T*>(bias);
     e.res = static_cast<const T*>(residual);
     e.ldd = s.op;
@@ -384,8 +389,7 @@ int orda_linear_backward(const orda_linear_t* p, const void* x, const void* weig
     if (grad_bias || (products && !direct)) {
       DzParams z{};
       z.dy = grad_output;
-      z.d = act ? d : nullptr;
-      z.dlo = 2 * p->tokens * s.op;
+      z.d = planes<T>(act ? d : nullptr, p->tokens * s.op);
       z.dz = products && !direct ? own_dz : nullptr;
       z.partial = grad_bias ? sums : nullptr;
       z.rows = p->tokens;
@@ -437,13 +441,14 @@ int orda_ffn_forward(const orda_ffn_t* p, const void* x, const void* w_gate, con
   if ((da_factor == nullptr) != (db_factor == nullptr)) return fail(ORDA_EINVAL, "orda_ffn_forward: the two factors are kept together");
   for (const void* q : {x, w_gate, w_up, w_down, (const void*)h, (const void*)da_factor, (const void*)db_factor})
     if (!aligned16(q)) return fail(ORDA_EINVAL, "orda_ffn_forward: x, the weights, h and the factors must be 16-byte aligned");
-  if (residual && p->ldr < p->out_features) return fail(ORDA_EINVAL, "orda_ffn_forward: ldr must be at least out_features");
+  if (residual) OP_TRY(check_residual("orda_ffn_forward", p->ldr, p->out_features));
   OP_TRY(check_workspace("orda_ffn_forward", workspace, workspace_bytes, ffn_ws(p, s, false)));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   float* part = reinterpret_cast<float*>(base256(workspace));
   return by_dtype(p->dtype, [&](auto tag) -> int {
     using T = decltype(tag);
-    EpiGate<T> g{static_cast<T*>(h), da_factor, db_factor, s.fp, s.fp, 2 * p->tokens * s.fp, p->activation};
+    const int64_t kept = p->tokens * s.fp;
+    EpiGate<T> g{static_cast<T*>(h), planes<T>(da_factor, kept), planes<T>(db_factor, kept), s.fp, s.fp, p->activation};
     TileParams t = product<T>(x, p->ldx, w_gate, p->ldw, p->tokens, p->inner, s.gate.K);
     t.B1 = w_up;
     OP_LAUNCH(launch_op_gate<T>(plan_of(s.gate), t, g, part, st));
@@ -478,7 +483,9 @@ int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, co
   return by_dtype(p->dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     if (grad_x || grad_gate || grad_up) {
-      const EpiGateGrad<T> e{reinterpret_cast<T*>(d), da_factor, db_factor, 2 * s.fp, s.fp, s.fp, 2 * p->tokens * s.fp};
+      T* const da = reinterpret_cast<T*>(d);
+      const int64_t kept = p->tokens * s.fp;
+      const EpiGateGrad<T> e{da, da + s.fp, planes<T>(da_factor, kept), planes<T>(db_factor, kept), 2 * s.fp, s.fp, s.fp};
       TileParams t = product<T>(grad_output, p->ldg, w_down, p->ldd, p->tokens, p->inner, s.dh.K);
       t.kval = p->out_features;
       OP_LAUNCH(launch_op_gate_grad<T>(plan_of(s.dh), t, e, part, st));

@@ -91,13 +91,13 @@ __global__ __launch_bounds__(kThreads4, 1) void k_ring(TileParams P, Epi E0) {
     if constexpr (LA == MNMAJ) {
       if (x.second) E = E.second();
     }
+    E = E.tile(x.m0, x.n0);
     char* buf = slot + wave_id() * 8192;
-    const int64_t nlim = E.cols - x.n0;  // columns left from the tile's first one
-    const int64_t mw = x.m0 + wm * 128;
+    const int rows = (int)lmin(P.M - x.m0, 256), cols = (int)lmin(E.cols, 256);
+    const int mw = wm * 128;
     constexpr int kIt = DUAL ? 2 : 4;
     struct Item {
-      int64_t m;
-      int row, g, col, cnt;
+      int m, row, g, col, cnt;
       bool live;
     };
     auto item = [&](int mb, int it) __attribute__((always_inline)) {
@@ -107,9 +107,8 @@ __global__ __launch_bounds__(kThreads4, 1) void k_ring(TileParams P, Epi E0) {
       q.g = DUAL ? i & 7 : i & 15;
       q.col = (q.g >> 3) * 128 + wn * 64 + (q.g & 7) * 8;
       q.m = mw + mb * 16 + q.row;
-      const int64_t left = nlim - q.col;
-      q.cnt = left >= 8 ? 8 : (int)left;
-      q.live = q.m < P.M && q.cnt > 0;
+      q.cnt = min(cols - q.col, 8);
+      q.live = q.m < rows && q.cnt > 0;
       return q;
     };
     auto dump = [&](int mb) __attribute__((always_inline)) {
@@ -133,15 +132,21 @@ __global__ __launch_bounds__(kThreads4, 1) void k_ring(TileParams P, Epi E0) {
     };
     typedef typename Epi::template Pre<8> Pre;
     if constexpr (Epi::kLight) {
-      // little code per element: all unrolled, each item's loads one row block
-      // (four items) ahead of their use.  With the loads where they are used,
-      // dh's epilogue (8192 tokens, 4096 x 14336) took 1070 us in all.
-      Pre p[kIt];
+      // little code per element: all unrolled, each item's loads two row blocks
+      // (eight items) ahead of their use.  dh and its epilogue (8192 tokens,
+      // 4096 x 14336: the product alone 650 us) take 910 us, with the loads one
+      // block ahead 1033, where they are used 1070.
+      constexpr int kAhead = 2;
+      Pre p[kAhead][kIt];
+      // (items outside the tile's valid part load from its last row or columns)
+      auto fetch = [&](int mb, int it) __attribute__((always_inline)) {
+        const Item q = item(mb, it);
+        p[mb % kAhead][it] = E.template pre<8>(min(q.m, rows - 1), min(q.col, cols - 8), 8);
+      };
 #pragma unroll
-      for (int it = 0; it < kIt; ++it) {
-        const Item q = item(0, it);
-        if (q.live) p[it] = E.template pre<8>(q.m, x.n0 + q.col, q.cnt);
-      }
+      for (int mb = 0; mb < kAhead; ++mb)
+#pragma unroll
+        for (int it = 0; it < kIt; ++it) fetch(mb, it);
 #pragma unroll
       for (int mb = 0; mb < 8; ++mb) {
         dump(mb);
@@ -150,12 +155,9 @@ __global__ __launch_bounds__(kThreads4, 1) void k_ring(TileParams P, Epi E0) {
           const Item q = item(mb, it);
           float v[8];
           take(q.row, q.g, v);
-          const Pre now = p[it];
-          if (mb < 7) {
-            const Item f = item(mb + 1, it);
-            if (f.live) p[it] = E.template pre<8>(f.m, x.n0 + f.col, f.cnt);
-          }
-          if (q.live) E(q.m, x.n0 + q.col, v, q.cnt, now, {});
+          const Pre now = p[mb % kAhead][it];
+          if (mb + kAhead < 8) fetch(mb + kAhead, it);
+          if (q.live) E(q.m, q.col, v, q.cnt, now, {});
         }
       }
     } else {
@@ -166,11 +168,11 @@ __global__ __launch_bounds__(kThreads4, 1) void k_ring(TileParams P, Epi E0) {
 #pragma unroll
         for (int it = 0; it < kIt; ++it) {
           const Item q = item(mb, it);
-          if (q.live) p[mb & 1][it] = E.template pre<8>(q.m, x.n0 + q.col, q.cnt);
+          if (q.live) p[mb & 1][it] = E.template pre<8>(q.m, q.col, q.cnt);
         }
       };
       const Item first = item(0, 0);
-      const auto col = E.template col<8>(x.n0 + first.col, first.cnt);
+      const auto col = E.template col<8>(first.col, first.cnt);
       fetch(0);
 #pragma unroll
       for (int mb = 0; mb < 8; ++mb) {
@@ -184,13 +186,13 @@ __global__ __launch_bounds__(kThreads4, 1) void k_ring(TileParams P, Epi E0) {
           if constexpr (DUAL) {
             float u[8];
             take(q.row, q.g + 8, u);
-            if (q.live) E(q.m, x.n0 + q.col, v, u, q.cnt, p[mb & 1][0], col);
+            if (q.live) E(q.m, q.col, v, u, q.cnt, p[mb & 1][0], col);
           } else {
             Pre now = p[mb & 1][0];
             if (it == 1) now = p[mb & 1][1];
             if (it == 2) now = p[mb & 1][2];
             if (it == 3) now = p[mb & 1][3];
-            if (q.live) E(q.m, x.n0 + q.col, v, q.cnt, now, col);
+            if (q.live) E(q.m, q.col, v, q.cnt, now, col);
           }
         }
       }

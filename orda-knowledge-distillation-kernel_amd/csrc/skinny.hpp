@@ -103,21 +103,24 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void k_skinny(SkinnyParams P, Ep
   __syncthreads();
   if (threadIdx.x >= 64 || !live) return;
   float v[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+  constexpr int kSum = DUAL ? 4 : kSkinnyWaves;  // (both products' sums in one go need more registers than the K loop)
+#pragma unroll kSum
   for (int i = 0; i < kSkinnyWaves; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[e] += part[i][0][lane][e];
       if constexpr (DUAL) u[e] += part[i][1][lane][e];
     }
-  const int64_t n = n0 + 4 * g, left = E.cols - n;
+  E = E.tile(0, n0);
+  const int n = 4 * g;
+  const int64_t left = E.cols - n;
   const int cnt = left >= 4 ? 4 : (int)left;
   if (cnt <= 0) return;
   if constexpr (DUAL) {
     // (columns past N up to the padded width are zeros)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (n + e >= P.N) v[e] = u[e] = 0.f;
+      if (n0 + n + e >= P.N) v[e] = u[e] = 0.f;
     epi_apply(E, r, n, v, u, cnt);
   } else {
     epi_apply(E, r, n, v, cnt);

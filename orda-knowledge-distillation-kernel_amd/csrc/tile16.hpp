@@ -303,6 +303,7 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
   if constexpr (LA == MNMAJ) {
     if (second) E = E.second();
   }
+  E = E.tile(m0, n0);
   // The accumulators through LDS (each wave its own part of the stages), so that
   // a lane takes 8 consecutive columns of a row and 8 or 4 lanes a row's
   // contiguous bytes, and the epilogue's code is there once: 8192 x 2048 x 4096
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
   // (the same wave reads them: LDS serves a wave in order)
   constexpr int kG = (DUAL ? kC / 2 : kC) / 2;  // groups of 8 columns in a row (of one half)
   const int g = lane % kG;
-  const int64_t n = n0 + wcol + g * 8;
+  const int n = wcol + g * 8;
   const int64_t left = E.cols - n;
   const int cnt = left >= 8 ? 8 : (int)left;
   if (cnt <= 0) return;
@@ -336,11 +337,11 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
       v[4 + e] = y[e];
     }
   };
-  const int64_t mw = m0 + wm * (BM / 2);
+  const int mw = wm * (BM / 2), rows = (int)lmin(P.M - m0, BM);
 #pragma unroll 2
   for (int row = lane / kG; row < BM / 2; row += 64 / kG) {
-    const int64_t m = mw + row;
-    if (m >= P.M) break;
+    const int m = mw + row;
+    if (m >= rows) break;
     const auto pre = E.template pre<8>(m, n, cnt);
     float v[8];
     take(row, 2 * g, v);

@@ -130,15 +130,17 @@ __global__ __launch_bounds__(C::kThreads, C::MB == 4 ? 2 : 3) void k_tile_s3(Til
     if constexpr (LA == MNMAJ) {
       if (x.second) E = E.second();
     }
+    E = E.tile(x.m0, x.n0);
+    const int rows = (int)lmin(P.M - x.m0, RA);
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
-      const int64_t m = ml + mb * 16;
+      const int m = wm * 16 * MB + mb * 16 + (ol & 15);
 #pragma unroll
       for (int nb = 0; nb < (DUAL ? MB / 2 : MB); ++nb) {
-        const int64_t n = x.n0 + s3_brow<C, DUAL>(nb, wn) + 4 * (ol >> 4);
+        const int n = s3_brow<C, DUAL>(nb, wn) + 4 * (ol >> 4);
         const int64_t left = E.cols - n;
         const int cnt = left >= 4 ? 4 : (int)left;
-        if (m < P.M && cnt > 0) {
+        if (m < rows && cnt > 0) {
           float v[4] = {acc[mb][nb][0], acc[mb][nb][1], acc[mb][nb][2], acc[mb][nb][3]};
           if constexpr (DUAL) {
             float u[4] = {acc[mb][nb + MB / 2][0], acc[mb][nb + MB / 2][1], acc[mb][nb + MB / 2][2], acc[mb][nb + MB / 2][3]};

@@ -134,10 +134,10 @@ struct Operands {
 };
 int64_t pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
-// Contiguous rows of any pitch and alignment.
+// Contiguous rows of any pitch up to 2^22 and any alignment.
 Tensor rows_of(const Tensor& given, ScalarType type) {
   Tensor t = given.scalar_type() == type ? given : given.to(type);
-  if ((t.stride(1) != 1 && t.size(1) > 1) || (t.size(0) > 1 && t.stride(0) < t.size(1))) t = t.contiguous();
+  if ((t.stride(1) != 1 && t.size(1) > 1) || (t.size(0) > 1 && (t.stride(0) < t.size(1) || t.stride(0) > (1 << 22)))) t = t.contiguous();
   return t;
 }
 

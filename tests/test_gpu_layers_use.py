@@ -150,14 +150,43 @@ def test_captured_backward_beside_an_eager_graph_of_the_same_leaves():
 @pytest.mark.parametrize("N", [3, 40])
 def test_rows_very_far_apart(N):
     """A pitch past what the C entry points take: the rows are copied."""
-    t = linear_case(N, 96, 77, BF, "none", False, False, seed=29)
+    t = linear_case(N, 96, 77, BF, "none", False, True, seed=29)
     far = torch.zeros(N, (1 << 22) + 64, dtype=BF, device="cuda")
     far[:, :96] = t["x"].cuda()
-    leaf = far[:, :96].requires_grad_(True)
-    w = t["w"].cuda().requires_grad_(True)
-    y = orda.fused_linear(leaf, w)
-    got = torch.autograd.grad(y, (leaf, w), t["dy"].cuda())
-    check({"y": y, "x": got[0], "w": got[1]}, want_linear(t, "none", BF))
+    far[:, 100:177] = t["residual"].cuda()
+    leaves = [v.requires_grad_(True) for v in (far[:, :96].detach(), t["w"].cuda(), far[:, 100:177].detach())]
+    y = orda.fused_linear(leaves[0], leaves[1], None, leaves[2])
+    got = torch.autograd.grad(y, leaves, t["dy"].cuda())
+    check({"y": y, "x": got[0], "w": got[1], "residual": got[2]}, want_linear(t, "none", BF))
+
+
+@pytest.mark.parametrize("K,O", [(1 << 21, 24), (24, 1 << 21)])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_widest_layers(K, O, dtype):
+    """Rows of 2^21 elements, two tiles of them: 256 rows of an fp32 output span 2^32 bytes.  Small whole numbers, exact
+    sums."""
+    N = 300
+    g = torch.Generator(device="cuda").manual_seed(31)
+
+    def whole(*shape):
+        return torch.randint(-1, 2, shape, generator=g, device="cuda", dtype=torch.int8).to(dtype)
+
+    x, w, r, dy = whole(N, K).requires_grad_(True), whole(O, K).requires_grad_(True), whole(N, O), whole(N, O)
+    y = orda.fused_linear(x, w, None, r, activation="relu")
+    gx, gw = torch.autograd.grad(y, (x, w), dy)
+    q = Unit(dtype)
+    with torch.no_grad():
+        for a in range(0, O, 1 << 18):
+            b = slice(a, min(O, a + (1 << 18)))
+            z = x.float() @ w[b].float().t()  # (whole numbers below 2^24: exact in fp32)
+            want = z.clamp(min=0) + r[:, b].float()
+            assert bool(((y[:, b].float() - want).abs() <= q.rounded(want)).all())
+            dz = dy[:, b].float() * (z > 0)
+            dw = dz.t() @ x.float()
+            assert bool(((gw[b].float() - dw).abs() <= q.rounded(dw)).all())
+            part = dz @ w[b].float()
+            total = part if a == 0 else total + part
+        assert bool(((gx.float() - total).abs() <= q.rounded(total)).all())
 
 
 @pytest.mark.parametrize("dtype", [BF, torch.float32])

@@ -170,6 +170,8 @@ def test_operands_and_workspaces_are_checked_before_any_launch():
     refused(lib.orda_linear_forward(p, None, 256, None, None, 256, None, 256, big, None), -1, "required")
     refused(lib.orda_linear_forward(p, 264, 256, None, None, 256, None, 256, big, None), -1, "aligned")
     refused(lib.orda_linear_forward(ctypes.byref(linear(ldr=8)), 256, 256, None, 256, 256, None, 256, big, None), -1, "ldr")
+    refused(lib.orda_linear_forward(ctypes.byref(linear(ldr=(1 << 22) + 8)), 256, 256, None, 256, 256, None, 256, big, None), -1, "ldr")
+    refused(lib.orda_ffn_forward(ctypes.byref(ffn(ldr=(1 << 22) + 8)), *[256] * 5, 256, 256, None, None, 256, big, None), -1, "ldr")
     refused(lib.orda_linear_forward(p, 256, 256, None, None, 256, None, None, 0, None), -2, "workspace")
     refused(lib.orda_linear_backward(p, 256, 256, None, 256, 256, 256, None, 256, big, None), -1, "d is required")
     refused(lib.orda_linear_backward(p, 256, 256, 256, None, 256, 256, None, 256, big, None), -1, "grad_output")
