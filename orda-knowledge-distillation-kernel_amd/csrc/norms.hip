@@ -19,9 +19,15 @@
 
 namespace orda {
 
-constexpr int kSpanMax = 96;  // tensors of one launch (48 bytes each: the arguments hold 4 KiB)
-
+// The table of one launch, in its arguments: 80 tensors (4 KB), or 320 (15 KB)
+// where there are more.  201 fp32 tensors of 60 M elements in one launch each
+// for norm and clipping instead of three: 162 -> 141 us of kernels; 300 of 600 M
+// bf16 elements 878 -> 849, 197 -> 93 us of host; 40 tensors in the large table
+// 26 -> 32 us a pass (the arguments are copied).
+constexpr int kSpanFew = 80, kSpanMany = 320;
+template <int ROWS>
 struct SpanTable {
+  static constexpr int kRows = ROWS;
   int count;
   int chunk;   // elements of a chunk (a multiple of 2048)
   int chunks;  // in all
@@ -32,16 +38,14 @@ struct SpanTable {
     int64_t cols, ld, ld_out;
     int per_row;  // chunks of a row
     int first;    // the tensor's first chunk
-  } t[kSpanMax - 16];
+  } t[ROWS];
 };
-constexpr int kSpanRows = kSpanMax - 16;
-static_assert(sizeof(SpanTable) <= 4000, "kernel arguments");
 
 // The chunks of workgroup b (b, b + G, ...: the workgroups that run together
 // walk memory side by side): f(tensor, row, the row's first element, elements
 // [lo, hi) of the row).  A row's chunks are cut at 16-byte aligned addresses.
-template <class T, class F>
-__device__ __forceinline__ void for_chunks(const SpanTable& S, const F& f) {
+template <class T, class Table, class F>
+__device__ __forceinline__ void for_chunks(const Table& S, const F& f) {
   int i = 0;
   for (int c = blockIdx.x; c < S.chunks; c += gridDim.x) {
     int n = S.count;  // i: the last tensor that starts at or before c
@@ -94,8 +98,8 @@ __device__ __forceinline__ void unpack16(const uint4& u, float (&v)[16 / sizeof(
 }
 
 // partials[b] (+)= workgroup b's share.
-template <class T, int KIND>
-__global__ __launch_bounds__(256) void k_grad_norm(SpanTable S, double* partials, int first) {
+template <class T, int KIND, int ROWS>
+__global__ __launch_bounds__(256) void k_grad_norm(SpanTable<ROWS> S, double* partials, int first) {
   constexpr int VE = 16 / (int)sizeof(T), U = 4;
   __shared__ NormSum<KIND> red[4];
   NormSum<KIND> s = 0;
@@ -164,8 +168,8 @@ struct ClipParams {
   float max_norm;
   int in_place;
 };
-template <class T, class O, int KIND>
-__global__ __launch_bounds__(256) void k_clip(SpanTable S, ClipParams P) {
+template <class T, class O, int KIND, int ROWS>
+__global__ __launch_bounds__(256) void k_clip(SpanTable<ROWS> S, ClipParams P) {
   // 16 bytes a lane and access on the wider side: 16 in and 2 x 16 out leave
   // half of each line to another store (bf16 into fp32: 5.1 TB/s, 6.5 so)
   constexpr int VE = sizeof(O) == 4 ? 4 : 16 / (int)sizeof(T), U = 4;
@@ -243,11 +247,16 @@ hipError_t launch_pad_rows(const PadParams& P, int esize, hipStream_t s) {
   return hipGetLastError();
 }
 
+// Whether a span belongs to the tables of this dtype pair (-1: any) and place
+// (1: in place, 0: not, -1: either).
+static bool taken(const GradSpan& x, int in_dtype, int out_dtype, int place) {
+  return x.in_dtype == in_dtype && (out_dtype < 0 || x.out_dtype == out_dtype) && (place < 0 || (x.out == x.p) == (place != 0));
+}
 // Tables of the spans of one dtype pair; go(table, workgroups) per launch.
-template <class Go>
-static hipError_t for_tables(const GradSpan* g, int64_t n, int in_dtype, int out_dtype, int place, int64_t chunk, int max_groups, const Go& go) {
+template <int ROWS, class Go>
+static hipError_t tables_of(const GradSpan* g, int64_t n, int in_dtype, int out_dtype, int place, int64_t chunk, int max_groups, const Go& go) {
   const int es = in_dtype == DT_F32 ? 4 : 2, ve = 16 / es;
-  SpanTable S;
+  SpanTable<ROWS> S;
   S.count = S.chunks = 0;
   S.chunk = (int)chunk;
   S.pad = 0;
@@ -259,8 +268,7 @@ static hipError_t for_tables(const GradSpan* g, int64_t n, int in_dtype, int out
   };
   for (int64_t i = 0; i < n; ++i) {
     const GradSpan& x = g[i];
-    if (x.in_dtype != in_dtype || (out_dtype >= 0 && x.out_dtype != out_dtype)) continue;
-    if (place >= 0 && (x.out == x.p) != (place != 0)) continue;
+    if (!taken(x, in_dtype, out_dtype, place)) continue;
     // a tensor of more chunks than a launch counts is cut into rows that fit
     int64_t r0 = 0, c0 = 0;
     const int64_t most = 1ll << 29;  // chunks of one entry
@@ -268,11 +276,11 @@ static hipError_t for_tables(const GradSpan* g, int64_t n, int in_dtype, int out
       const int64_t cols = x.rows == 1 ? std::min<int64_t>(x.cols - c0, most * chunk / 2) : x.cols;
       const int64_t per = (cols + ve - 1 + chunk - 1) / chunk;
       const int64_t rows = std::min<int64_t>(x.rows - r0, std::max<int64_t>(1, most / per));
-      if (S.count == kSpanRows || S.chunks + per * rows > (1ll << 30)) {
+      if (S.count == ROWS || S.chunks + per * rows > (1ll << 30)) {
         const hipError_t e = flush();
         if (e != hipSuccess) return e;
       }
-      SpanTable::Row& t = S.t[S.count++];
+      typename SpanTable<ROWS>::Row& t = S.t[S.count++];
       const int64_t oe = x.out_dtype == DT_F32 ? 4 : 2;
       t.p = static_cast<const char*>(x.p) + (r0 * x.ld + c0) * es;
       t.out = static_cast<char*>(x.out) + (r0 * x.ld_out + c0) * oe;
@@ -293,6 +301,14 @@ static hipError_t for_tables(const GradSpan* g, int64_t n, int in_dtype, int out
   return flush();
 }
 
+template <class Go>
+static hipError_t for_tables(const GradSpan* g, int64_t n, int in_dtype, int out_dtype, int place, int64_t chunk, int max_groups, const Go& go) {
+  int64_t spans = 0;
+  for (int64_t i = 0; i < n; ++i) spans += taken(g[i], in_dtype, out_dtype, place);
+  return spans > kSpanFew ? tables_of<kSpanMany>(g, n, in_dtype, out_dtype, place, chunk, max_groups, go)
+                          : tables_of<kSpanFew>(g, n, in_dtype, out_dtype, place, chunk, max_groups, go);
+}
+
 static int64_t elements_of(const GradSpan* g, int64_t n) {
   int64_t total = 0;
   for (int64_t i = 0; i < n; ++i) total += g[i].rows * g[i].cols;
@@ -304,9 +320,9 @@ constexpr int64_t kClipChunk = 2048, kNormLarge = 64ll << 20;
 constexpr int kClipGroups = 1 << 23;  // (a launch has fewer than 2^32 threads; past them workgroups take several chunks)
 static int64_t norm_chunk(int64_t elements) { return elements < kNormLarge ? 2048 : 16384; }
 
-template <class T, int KIND>
-static hipError_t norm_go(const SpanTable& S, double* partials, int groups, int first, hipStream_t s) {
-  hipLaunchKernelGGL((k_grad_norm<T, KIND>), dim3(groups), dim3(256), 0, s, S, partials, first);
+template <class T, int KIND, int ROWS>
+static hipError_t norm_go(const SpanTable<ROWS>& S, double* partials, int groups, int first, hipStream_t s) {
+  hipLaunchKernelGGL((k_grad_norm<T, KIND, ROWS>), dim3(groups), dim3(256), 0, s, S, partials, first);
   return hipGetLastError();
 }
 // The partials of all tensors: every launch has the same workgroups, the first
@@ -317,7 +333,7 @@ static hipError_t norm_partials(const GradSpan* g, int64_t n, double* partials, 
   const int count = (int)std::min<int64_t>(max_partials, std::max<int64_t>(1, (elements + chunk - 1) / chunk));
   int first = 1;
   for (int dt = 0; dt < 3; ++dt) {
-    const hipError_t e = for_tables(g, n, dt, -1, -1, chunk, count, [&](const SpanTable& S, int) {
+    const hipError_t e = for_tables(g, n, dt, -1, -1, chunk, count, [&](const auto& S, int) {
       const int f = first;
       first = 0;
       switch (dt) {
@@ -348,13 +364,13 @@ hipError_t launch_grad_norm(const GradSpan* g, int64_t n, int kind, double* part
   }
 }
 
-template <class T, class O, int KIND>
-static hipError_t clip_go(const SpanTable& S, int groups, const ClipParams& P, hipStream_t s) {
-  hipLaunchKernelGGL((k_clip<T, O, KIND>), dim3(groups), dim3(256), 0, s, S, P);
+template <class T, class O, int KIND, int ROWS>
+static hipError_t clip_go(const SpanTable<ROWS>& S, int groups, const ClipParams& P, hipStream_t s) {
+  hipLaunchKernelGGL((k_clip<T, O, KIND, ROWS>), dim3(groups), dim3(256), 0, s, S, P);
   return hipGetLastError();
 }
-template <class T, int KIND>
-static hipError_t clip_out(const SpanTable& S, int groups, int out, const ClipParams& P, hipStream_t s) {
+template <class T, int KIND, int ROWS>
+static hipError_t clip_out(const SpanTable<ROWS>& S, int groups, int out, const ClipParams& P, hipStream_t s) {
   switch (out) {
     case DT_BF16: return clip_go<T, bf16, KIND>(S, groups, P, s);
     case DT_F16: return clip_go<T, f16, KIND>(S, groups, P, s);
@@ -368,7 +384,7 @@ static hipError_t clip_kind(const GradSpan* g, int64_t n, ClipParams P, hipStrea
       for (int place = 0; place < 2; ++place) {
         if (place && in != out) continue;
         P.in_place = place;
-        const hipError_t e = for_tables(g, n, in, out, place, kClipChunk, kClipGroups, [&](const SpanTable& S, int groups) {
+        const hipError_t e = for_tables(g, n, in, out, place, kClipChunk, kClipGroups, [&](const auto& S, int groups) {
           switch (in) {
             case DT_BF16: return clip_out<bf16, KIND>(S, groups, out, P, s);
             case DT_F16: return clip_out<f16, KIND>(S, groups, out, P, s);

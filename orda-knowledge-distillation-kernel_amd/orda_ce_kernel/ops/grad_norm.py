@@ -2,7 +2,7 @@
 
     total = (sum |g|^p)^(1/p), p = 1, 2 or infinity        g *= min(1, max_norm / (total + 1e-6))
 
-Two kernels over a table of tensors (one launch each per 80 tensors and dtype) and one that adds up the norm's partial sums;
+Two kernels over a table of tensors (one launch each per dtype and up to 320 tensors) and one that adds up the norm's partial sums;
 sums are fp64 in a fixed order and the factor is formed on the device, so nothing synchronises the host.  The tables are
 built in csrc/torch_ops.cpp.  No counterpart in the reference, whose training loop calls torch.
 """

@@ -183,3 +183,28 @@ def test_more_than_2_to_31_elements():
     assert float(total) == pytest.approx(want, rel=2.0 ** -23)
     assert bool((big.grad[:-3] == 0.25).all()) and big.grad[-3:].tolist() == [-1.5] * 3
     assert torch.allclose(small.grad, torch.full_like(small.grad, 0.5), rtol=1e-5)
+
+
+@pytest.mark.parametrize("n", [79, 80, 81, 320, 321, 700])
+def test_tables_of_many_tensors(n):
+    """As many tensors as one launch takes, one more, several launches; captured and replayed."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    sizes = [1 + (i * 37) % 211 for i in range(n)] + [5000]
+    grads = [torch.randn(k, generator=g, device="cuda").bfloat16() for k in sizes]
+    grads += [torch.randn(3 + k, generator=g, device="cuda") for k in range(0, n, 7)]
+    for p in (1.0, 2.0, math.inf):
+        check_norm(orda.grad_norm(grads, p), grads, p)
+    params, outs = params_of(grads), [torch.empty(x.shape, device="cuda") for x in grads]
+    total = orda.clip_grad_norm_(params, 0.5, out=outs)
+    check_norm(total, grads, 2.0)
+    check_clipped(outs, grads, float(total), 0.5)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        total = orda.clip_grad_norm_(params, 0.5, out=outs)
+    for k in range(2):
+        for x in grads:
+            x.mul_(-0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        check_norm(total, grads, 2.0)
+        check_clipped(outs, grads, float(total), 0.5)
