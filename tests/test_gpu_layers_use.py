@@ -77,6 +77,23 @@ def test_checkpointing_and_changed_operands():
         y.sum().backward()
 
 
+def test_inside_compiled_code_and_inference_mode():
+    """A compiled caller breaks its graph at the call and gives the same bits; inference mode records nothing."""
+    t = linear_case(40, 96, 72, BF, "gelu", True, False, seed=33)
+    x, w, b = (t[n].cuda().requires_grad_(True) for n in ("x", "w", "bias"))
+
+    def f(x, w, b):
+        return orda.fused_linear(x * 2, w, b, activation="gelu") + 1
+
+    y, z = f(x, w, b), torch.compile(f, backend="eager")(x, w, b)
+    assert torch.equal(y, z)
+    for one, two in zip(torch.autograd.grad(y, (x, w, b), t["dy"].cuda()), torch.autograd.grad(z, (x, w, b), t["dy"].cuda())):
+        assert torch.equal(one, two)
+    with torch.inference_mode():
+        v = f(x, w, b)
+    assert torch.equal(v, y) and v.grad_fn is None and v.is_inference()
+
+
 def test_the_same_tensor_in_two_places():
     """One weight as gate and up, x as the residual, a square weight as its own input: gradients add up."""
     t = ffn_case(90, 96, 72, 96, BF, "silu", True, seed=25)
@@ -218,3 +235,40 @@ def test_offsets_past_32_bits(dtype):
         total += dz.t() @ xb
     assert float(total.abs().max()) < 2 ** 24
     same(gw, total)
+
+
+def test_block_offsets_past_32_bits():
+    """h, the kept factors, da and db of more than 2^31 elements each.  Values -1, 0, 1: a, b, h and the factors are whole
+    numbers below 2^8, every sum stays below 2^24, so only outputs round."""
+    H, F, O = 8, 2048, 8
+    N = (1 << 31) // F + 70
+    g = torch.Generator(device="cuda").manual_seed(32)
+
+    def whole(*shape):
+        return torch.randint(-1, 2, shape, generator=g, device="cuda", dtype=torch.int8).to(BF)
+
+    t = [whole(N, H), whole(F, H), whole(F, H), whole(O, F)]
+    leaves = [v.requires_grad_(True) for v in t]
+    dy = whole(N, O)
+    y = orda.gated_feed_forward(*leaves, activation="relu")
+    grads = torch.autograd.grad(y, leaves, dy)
+    q = Unit(BF)
+
+    def same(got, want):
+        assert bool(((got.float() - want).abs() <= q.rounded(want)).all())
+
+    with torch.no_grad():
+        x, wg, wu, wd = (v.detach().float() for v in leaves)
+        sums = [torch.zeros_like(w) for w in (wg, wu, wd)]
+        for k in range(0, N, 1 << 16):
+            b = slice(k, min(N, k + (1 << 16)))
+            a, u, d = x[b] @ wg.t(), x[b] @ wu.t(), dy[b].float() @ wd
+            f = a.clamp(min=0)
+            same(y[b], (f * u) @ wd.t())
+            da, db = d * u * (a > 0), d * f
+            same(grads[0][b], da @ wg + db @ wu)
+            for s, v in zip(sums, (da.t() @ x[b], db.t() @ x[b], dy[b].float().t() @ (f * u))):
+                s += v
+        for got, want in zip(grads[1:], sums):
+            assert float(want.abs().max()) < 2 ** 24
+            same(got, want)
