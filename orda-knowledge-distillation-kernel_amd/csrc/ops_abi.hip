@@ -227,7 +227,8 @@ int linear_shapes(const orda_linear_t* p, LinearShapes& s) {
   s.fwd = {p->dtype, KMAJ, KMAJ, false, p->tokens, p->out_features, kp, 0, 0, false};
   s.dx = {p->dtype, KMAJ, MNMAJ, false, p->tokens, kp, s.op, 0, p->ldw, false};
   s.dw = {p->dtype, MNMAJ, MNMAJ, false, p->out_features, kp, p->tokens, s.op, p->ldx, false};
-  // about 1024 workgroups, at least 16 rows each
+  // about 1024 workgroups, at least 16 rows each (8192 x 4096 in bf16 with 512,
+  // 1024, 2048, 4096: 63, 46, 52, 47 us)
   const int64_t per = 64 * g, cb = cdiv(s.op, per);
   s.rows_per_block = std::max<int64_t>(16, up(cdiv(p->tokens * cb, 1024), 4));
   s.blocks = cdiv(p->tokens, s.rows_per_block);
