@@ -15,12 +15,15 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <map>
 #include <optional>
 #include <string>
+#include <tuple>
 #include <unordered_set>
+#include <utility>
 #include <vector>
 
 #include "../../include/orda_ce.h"
@@ -129,10 +132,39 @@ struct Operands {
     return p;
   }
   void copy(void* stream) {
-    if (!copies.empty()) check(api.pad_rows(code(type), copies.data(), (int64_t)copies.size(), stream), "orda_pad_rows");
+    constexpr size_t kMost = 4;  // of one orda_pad_rows call
+    for (size_t i = 0; i < copies.size(); i += kMost)
+      check(api.pad_rows(code(type), copies.data() + i, (int64_t)std::min(kMost, copies.size() - i), stream), "orda_pad_rows");
   }
 };
 int64_t pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// Two weights of one shape with one pitch (a row-strided one beside another is
+// copied).
+std::pair<Tensor, Tensor> add_pair(Operands& ops, const Tensor& a, const Tensor& b) {
+  const bool same = a.size(0) == 1 || a.strides() == b.strides();
+  std::pair<Tensor, Tensor> p(ops.add(same ? a : a.contiguous()), ops.add(same ? b : b.contiguous()));
+  if (pitch(p.first) != pitch(p.second)) {
+    p.first = p.first.contiguous();
+    p.second = p.second.contiguous();
+  }
+  return p;
+}
+
+// What a node saved, as the backward pass reads it.  Saved-tensor hooks
+// (offloading to the host, for one) may hand back a copy, dense where the saved
+// tensor's rows were apart, so that pitches and alignment are taken from what
+// they hand back; its shape and device have to be the saved one's.
+const Tensor& restored(const Tensor& t, at::IntArrayRef sizes, const c10::Device& device) {
+  TORCH_CHECK(t.defined() && t.sizes() == sizes && t.device() == device, "a saved tensor of shape ", sizes, " on ", device,
+              " came back from its hooks ", t.defined() ? "with another shape or on another device" : "undefined");
+  return t;
+}
+// Kept factors and h: dense and 16-byte aligned.
+Tensor restored_dense(const Tensor& t, at::IntArrayRef sizes, const c10::Device& device) {
+  Tensor d = restored(t, sizes, device).contiguous();
+  return aligned(d) ? d : d.clone();
+}
 
 // Contiguous rows of any pitch up to 2^22 and any alignment.
 Tensor rows_of(const Tensor& given, ScalarType type) {
@@ -231,7 +263,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     const bool graph = at::GradMode::is_enabled();
     const at::AutoGradMode off(false);
     const variable_list saved = ctx->get_saved_variables();
-    const orda_linear_t p = unpacked<orda_linear_t>(ctx->saved_data["p"].toStringRef());
+    orda_linear_t p = unpacked<orda_linear_t>(ctx->saved_data["p"].toStringRef());
     const std::vector<int64_t> types = ctx->saved_data["types"].toIntVector();
     auto type = [&](int i) { return static_cast<ScalarType>(types[i]); };
     const ScalarType t = type(0);
@@ -243,13 +275,21 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
       const c10::DeviceGuard guard(grads[0].device());
       check_capture("fused_linear");
       const Tensor dy = grads[0].to(t).contiguous();
+      void* s = stream_of(dy);
+      const int64_t kp = padded(p.in_features, t);
+      Operands ops(t);
+      Tensor x, w, d;
+      if (nw) p.ldx = pitch(x = ops.add(restored(saved[0], {p.tokens, kp}, dy.device())));
+      if (nx) p.ldw = pitch(w = ops.add(restored(saved[1], {p.out_features, kp}, dy.device())));
+      ops.copy(s);
+      if (p.activation != ORDA_ACT_NONE)
+        d = restored_dense(saved[2], {(int64_t)size_of(api.linear_saved_bytes(&p), "orda_linear_saved_bytes")}, dy.device());
       if (nx) g[0] = gradient(dy, p.tokens, p.in_features, t);
       if (nw) g[1] = gradient(dy, p.out_features, p.in_features, t);
       if (nb) g[2] = at::empty({p.out_features}, dy.options());
       const size_t n = size_of(api.linear_workspace_bytes(&p, 1), "orda_linear_workspace_bytes");
       const Tensor ws = bytes(n, dy);
-      check(api.linear_backward(&p, ptr(saved[0]), ptr(saved[1]), ptr(saved[2]), ptr(dy), out(g[0]), out(g[1]), out(g[2]), out(ws), n,
-                                stream_of(dy)), "orda_linear_backward");
+      check(api.linear_backward(&p, ptr(x), ptr(w), ptr(d), ptr(dy), out(g[0]), out(g[1]), out(g[2]), out(ws), n, s), "orda_linear_backward");
       g[0] = trimmed(g[0], p.in_features, type(1));
       g[1] = trimmed(g[1], p.in_features, type(2));
       if (nb) g[2] = g[2].to(type(3));
@@ -276,14 +316,7 @@ FfnCall ffn_run(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tenso
   FfnCall c;
   Operands ops(type);
   c.x = ops.add(x);
-  // one pitch for both weights (a row-strided one beside another is copied)
-  const bool same = wg.size(0) == 1 || wg.strides() == wu.strides();
-  c.gate = ops.add(same ? wg : wg.contiguous());
-  c.up = ops.add(same ? wu : wu.contiguous());
-  if (pitch(c.gate) != pitch(c.up)) {
-    c.gate = c.gate.contiguous();
-    c.up = c.up.contiguous();
-  }
+  std::tie(c.gate, c.up) = add_pair(ops, wg, wu);
   c.down = ops.add(wd);
   ops.copy(s);
   const Tensor r = res.defined() ? rows_of(res, type) : Tensor();
@@ -327,23 +360,30 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
     bool any = false;
     const int64_t rows[4] = {p.tokens, p.inner, p.inner, p.out_features}, cols[4] = {p.hidden, p.hidden, p.hidden, p.inner};
     if (types[6] != 0 && ctx->needs_input_grad(4)) g[4] = grads[0].to(type(5));
-    for (int i = 0; i < 4; ++i) {
-      if (!ctx->needs_input_grad(i)) continue;
-      g[i] = gradient(v[0], rows[i], cols[i], t);
-      any = true;
-    }
+    const c10::Device device = grads[0].device();
+    for (int i = 0; i < 4; ++i) any = any || ctx->needs_input_grad(i);
     if (any) {
-      const c10::DeviceGuard guard(v[0].device());
+      const c10::DeviceGuard guard(device);
       check_capture("gated_feed_forward");
-      void* s = stream_of(v[0]);
+      void* s = stream_of(grads[0]);
+      const int64_t hp = padded(p.hidden, t), kept = (int64_t)size_of(api.ffn_saved_bytes(&p), "orda_ffn_saved_bytes");
       Operands ops(t);
-      const Tensor dy = ops.add(grads[0]);
+      const Tensor dy = ops.add(grads[0]), x = ops.add(restored(v[0], {p.tokens, hp}, device));
+      const auto [gate, up] = add_pair(ops, restored(v[1], {p.inner, hp}, device), restored(v[2], {p.inner, hp}, device));
+      const Tensor down = ops.add(restored(v[3], {p.out_features, padded(p.inner, t)}, device));
       ops.copy(s);
+      const Tensor h = restored_dense(v[4], {p.tokens, api.ffn_inner_pitch(&p)}, device);
+      const Tensor da = restored_dense(v[5], {kept}, device), db = restored_dense(v[6], {kept}, device);
       p.ldg = pitch(dy);
+      p.ldx = pitch(x);
+      p.ldw = pitch(gate);
+      p.ldd = pitch(down);
+      for (int i = 0; i < 4; ++i)
+        if (ctx->needs_input_grad(i)) g[i] = gradient(dy, rows[i], cols[i], t);
       const size_t n = size_of(api.ffn_workspace_bytes(&p, 1), "orda_ffn_workspace_bytes");
       const Tensor ws = bytes(n, dy);
-      check(api.ffn_backward(&p, ptr(v[0]), ptr(v[1]), ptr(v[2]), ptr(v[3]), ptr(v[4]), ptr(v[5]), ptr(v[6]), ptr(dy), out(g[0]), out(g[1]),
-                             out(g[2]), out(g[3]), out(ws), n, s), "orda_ffn_backward");
+      check(api.ffn_backward(&p, ptr(x), ptr(gate), ptr(up), ptr(down), ptr(h), ptr(da), ptr(db), ptr(dy), out(g[0]), out(g[1]), out(g[2]),
+                             out(g[3]), out(ws), n, s), "orda_ffn_backward");
       for (int i = 0; i < 4; ++i) g[i] = trimmed(g[i], cols[i], type(i + 1));
     }
     return once(std::move(g), graph);
