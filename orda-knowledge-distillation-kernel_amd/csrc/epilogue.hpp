@@ -336,16 +336,27 @@ struct EpiLinear {
   }
 };
 
+// v[e] = 0 from e = left on.
+template <int W>
+__device__ __forceinline__ void zero_from(float (&v)[W], int left) {
+  if (left >= W) return;
+#pragma unroll
+  for (int e = 0; e < W; ++e) v[e] = e < left ? v[e] : 0.0f;
+}
+
 // h = act(a) b, rounded to T as the next product's operand; for the backward
 // pass, when asked for, the factors p = b act'(a) of da and q = act(a) of db are
 // kept: the activation is not evaluated again.  All [M x ld], cols = ld a
-// multiple of 64, so that every access is whole and aligned.
+// multiple of 64, so that every access is whole and aligned.  Columns past
+// `inner` are zeros whatever x holds: 0 * infinity in the product would reach y
+// and grad_x through the padding.
 template <class T>
 struct EpiGate {
   static constexpr bool kDual = true, kLight = false;
   T* h;
   Planes p, q;
   int64_t ld, cols;
+  int inner;
   int act;
   __device__ __forceinline__ EpiGate at(int) const { return *this; }
   __device__ __forceinline__ EpiGate second() const { return *this; }  // (no pairs)
@@ -358,6 +369,7 @@ struct EpiGate {
       e.q = q.template from<T>(i);
     }
     e.cols -= n0;
+    e.inner -= (int)n0;
     return e;
   }
   template <int W> using Pre = NoPre;
@@ -369,6 +381,8 @@ struct EpiGate {
   template <int W>
   __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, float (&g)[W], float (&u)[W], int, NoPre, NoPre) const {
     const uint32_t o = m * (uint32_t)ld + n;
+    zero_from<W>(g, inner - (int)n);
+    zero_from<W>(u, inner - (int)n);
     float f[W], df[W];
     if (p.hi) {
       act_eval<T, true, W>(act, g, f, df);
@@ -387,7 +401,7 @@ struct EpiGate {
 
 // From dh (fp32, never rounded): da = dh p, db = dh q, rounded to T as the
 // operands of the next products.  da and db are the two halves of rows of ldd;
-// cols = ld a multiple of 64.
+// cols = ld a multiple of 64; columns past `inner` are zeros.
 template <class T>
 struct EpiGateGrad {
   static constexpr bool kDual = false, kLight = true;
@@ -395,6 +409,7 @@ struct EpiGateGrad {
   T* db;
   Planes p, q;
   int64_t ldd, ld, cols;
+  int inner;
   __device__ __forceinline__ EpiGateGrad at(int) const { return *this; }
   __device__ __forceinline__ EpiGateGrad second() const { return *this; }  // (no pairs)
   __device__ __forceinline__ EpiGateGrad tile(int64_t m0, int64_t n0) const {
@@ -404,6 +419,7 @@ struct EpiGateGrad {
     e.p = p.template from<T>(m0 * ld + n0);
     e.q = q.template from<T>(m0 * ld + n0);
     e.cols -= n0;
+    e.inner -= (int)n0;
     return e;
   }
   template <int W> using Col = NoPre;
@@ -423,6 +439,7 @@ struct EpiGateGrad {
   template <int W>
   __device__ __forceinline__ void operator()(uint32_t m, uint32_t n, float (&v)[W], int, const Pre<W>& x, NoPre) const {
     float a[W], b[W];
+    zero_from<W>(v, inner - (int)n);
 #pragma unroll
     for (int e = 0; e < W; ++e) {
       a[e] = v[e] * x.p[e];

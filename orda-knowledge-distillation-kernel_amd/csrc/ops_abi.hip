@@ -449,7 +449,7 @@ int orda_ffn_forward(const orda_ffn_t* p, const void* x, const void* w_gate, con
   return by_dtype(p->dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     const int64_t kept = p->tokens * s.fp;
-    EpiGate<T> g{static_cast<T*>(h), planes<T>(da_factor, kept), planes<T>(db_factor, kept), s.fp, s.fp, p->activation};
+    EpiGate<T> g{static_cast<T*>(h), planes<T>(da_factor, kept), planes<T>(db_factor, kept), s.fp, s.fp, (int)p->inner, p->activation};
     TileParams t = product<T>(x, p->ldx, w_gate, p->ldw, p->tokens, p->inner, s.gate.K);
     t.B1 = w_up;
     OP_LAUNCH(launch_op_gate<T>(plan_of(s.gate), t, g, part, st));
@@ -486,7 +486,7 @@ int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, co
     if (grad_x || grad_gate || grad_up) {
       T* const da = reinterpret_cast<T*>(d);
       const int64_t kept = p->tokens * s.fp;
-      const EpiGateGrad<T> e{da, da + s.fp, planes<T>(da_factor, kept), planes<T>(db_factor, kept), 2 * s.fp, s.fp, s.fp};
+      const EpiGateGrad<T> e{da, da + s.fp, planes<T>(da_factor, kept), planes<T>(db_factor, kept), 2 * s.fp, s.fp, s.fp, (int)p->inner};
       TileParams t = product<T>(grad_output, p->ldg, w_down, p->ldd, p->tokens, p->inner, s.dh.K);
       t.kval = p->out_features;
       OP_LAUNCH(launch_op_gate_grad<T>(plan_of(s.dh), t, e, part, st));

@@ -116,15 +116,8 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void k_skinny(SkinnyParams P, Ep
   const int64_t left = E.cols - n;
   const int cnt = left >= 4 ? 4 : (int)left;
   if (cnt <= 0) return;
-  if constexpr (DUAL) {
-    // (columns past N up to the padded width are zeros)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n0 + n + e >= P.N) v[e] = u[e] = 0.f;
-    epi_apply(E, r, n, v, u, cnt);
-  } else {
-    epi_apply(E, r, n, v, cnt);
-  }
+  if constexpr (DUAL) epi_apply(E, r, n, v, u, cnt);
+  else epi_apply(E, r, n, v, cnt);
 }
 
 }  // namespace orda
