@@ -436,6 +436,32 @@ int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, co
                       void* grad_gate, void* grad_up, void* grad_down, void* workspace, size_t workspace_bytes,
                       void* stream);
 
+/* The products of one call, and how each would run (host-side, no device work;
+ * orda_plan_info's counterpart).  A product that the call does not need has a
+ * plan all the same. */
+enum orda_product {
+  ORDA_LINEAR_FORWARD = 0,    /* y                                            */
+  ORDA_LINEAR_GRAD_X = 1,
+  ORDA_LINEAR_GRAD_WEIGHT = 2,
+  ORDA_FFN_GATE = 0,          /* a and b, with h                              */
+  ORDA_FFN_DOWN = 1,          /* y                                            */
+  ORDA_FFN_GRAD_H = 2,        /* dh, with da and db                           */
+  ORDA_FFN_GRAD_X = 3,
+  ORDA_FFN_GRAD_GATE_UP = 4,  /* both in one launch                           */
+  ORDA_FFN_GRAD_GATE = 5,     /* one of the two alone                         */
+  ORDA_FFN_GRAD_DOWN = 6
+};
+typedef struct orda_product_plan {
+  int32_t engine;     /* 0 few rows, 1 tiles, 2 ring (256 x 256 tiles), 3
+                         split-operand tiles (fp32)                           */
+  int32_t tile_rows;
+  int32_t tile_cols;  /* (the gate's: half of them of each weight)            */
+  int32_t splits;     /* ranges of K, summed in fp32                          */
+  int64_t items;      /* tiles times splits                                   */
+} orda_product_plan_t;
+int orda_linear_plan(const orda_linear_t* p, int32_t product, orda_product_plan_t* out);
+int orda_ffn_plan(const orda_ffn_t* p, int32_t product, orda_product_plan_t* out);
+
 /* One gradient: `rows` rows of `cols` elements, `ld` elements apart (a dense
  * tensor is one row).  Any alignment.  The table is host memory, read before
  * the call returns. */

@@ -155,6 +155,28 @@ OpPlan plan_of(const Shape& q) {
   return pl;
 }
 
+// Rows and columns of the output that a workgroup (or one turn of a persistent
+// one) takes.
+void tile_of(const OpPlan& pl, int& rows, int& cols) {
+  rows = cols = 16;
+  if (pl.engine == OP_TILE) {
+    rows = pl.tile / 1000;
+    cols = pl.tile % 1000;
+  } else if (pl.engine == OP_RING) {
+    rows = cols = 256;
+  } else if (pl.engine == OP_SPLIT3) {
+    rows = pl.tile;
+    cols = pl.tile == 256 ? 128 : 64;
+  }
+}
+void fill_plan(const Shape& q, orda_product_plan_t* out) {
+  const OpPlan pl = plan_of(q);
+  int rows, cols;
+  tile_of(pl, rows, cols);
+  *out = {pl.engine, rows, cols, pl.splits,
+          pl.engine == OP_SKINNY ? cdiv(q.cols, cols) : (int64_t)items_of(q, rows, cols, pl.splits)};
+}
+
 // fp32 partials of a product in K ranges
 size_t part_bytes(const Shape& q) {
   const OpPlan pl = plan_of(q);
@@ -412,6 +434,26 @@ int orda_linear_backward(const orda_linear_t* p, const void* x, const void* weig
     }
     return ORDA_OK;
   });
+}
+
+int orda_linear_plan(const orda_linear_t* p, int32_t product, orda_product_plan_t* out) {
+  set_last_error(0, nullptr);
+  LinearShapes s;
+  OP_TRY(linear_shapes(p, s));
+  const Shape* const all[] = {&s.fwd, &s.dx, &s.dw};
+  if (!out || product < 0 || product > ORDA_LINEAR_GRAD_WEIGHT) return fail(ORDA_EINVAL, "orda_linear_plan: out is required and product one of orda_product");
+  fill_plan(*all[product], out);
+  return ORDA_OK;
+}
+
+int orda_ffn_plan(const orda_ffn_t* p, int32_t product, orda_product_plan_t* out) {
+  set_last_error(0, nullptr);
+  FfnShapes s;
+  OP_TRY(ffn_shapes(p, s));
+  const Shape* const all[] = {&s.gate, &s.down, &s.dh, &s.dx, &s.dw2, &s.dw, &s.dd};
+  if (!out || product < 0 || product > ORDA_FFN_GRAD_DOWN) return fail(ORDA_EINVAL, "orda_ffn_plan: out is required and product one of orda_product");
+  fill_plan(*all[product], out);
+  return ORDA_OK;
 }
 
 int64_t orda_ffn_inner_pitch(const orda_ffn_t* p) {

@@ -20,7 +20,8 @@ __all__ = [
     "ABI_VERSION", "PlanInfo", "Problem", "Tensors", "library", "plan_info", "library_path", "forward", "forward_static", "backward",
     "saved_bytes", "forward_workspace_bytes", "backward_workspace_bytes", "gemm_abt", "gemm",
     "MODE", "DTYPE", "FLAG", "KERNEL_CLASSES", "timing_enable", "timing_collect",
-    "ACTIVATION", "Linear", "FeedForward", "torch_ops",
+    "ACTIVATION", "Linear", "FeedForward", "torch_ops", "linear_plan",
+    "feed_forward_plan",
 ]
 
 ABI_VERSION = 4
@@ -144,6 +145,16 @@ class FeedForward(ctypes.Structure):
     ]
 
 
+class ProductPlan(ctypes.Structure):
+    """orda_product_plan_t"""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("engine", "tile_rows", "tile_cols", "splits")] + [("items", ctypes.c_int64)]
+
+
+LINEAR_PRODUCTS = ("forward", "grad_x", "grad_weight")
+FFN_PRODUCTS = ("gate", "down", "grad_h", "grad_x", "grad_gate_up", "grad_gate", "grad_down")
+ENGINES = ("few_rows", "tile", "ring", "split3")
+
 # orda_grad_t as int64 words: data, out, rows, cols, ld, ld_out, dtype | out_dtype << 32
 GRAD_WORDS = 7
 
@@ -215,6 +226,8 @@ def library() -> ctypes.CDLL:
         for name, arg in (("orda_linear", L), ("orda_ffn", F)):
             fn = getattr(lib, name + "_workspace_bytes")
             fn.restype, fn.argtypes = sz, [arg, ctypes.c_int32]
+            fn = getattr(lib, name + "_plan")
+            fn.restype, fn.argtypes = ctypes.c_int, [arg, ctypes.c_int32, ctypes.POINTER(ProductPlan)]
         for name, arg, res in (("orda_linear_saved_bytes", L, sz), ("orda_ffn_saved_bytes", F, sz),
                                ("orda_ffn_inner_pitch", F, ctypes.c_int64)):
             fn = getattr(lib, name)
@@ -360,6 +373,32 @@ def gemm(a: torch.Tensor, b: torch.Tensor, *, a_mn: bool = False, b_mn: bool = F
     )
     _check(rc, "orda_gemm")
     return c
+
+
+def _plans(entry: str, problem: ctypes.Structure, products: tuple) -> dict:
+    plans = {}
+    for i, name in enumerate(products):
+        out = ProductPlan()
+        _check(getattr(library(), entry)(ctypes.byref(problem), i, ctypes.byref(out)), entry)
+        plans[name] = {**{f: getattr(out, f) for f, _ in ProductPlan._fields_}, "engine": ENGINES[out.engine]}
+    return plans
+
+
+def linear_plan(tokens: int, in_features: int, out_features: int, dtype: torch.dtype) -> dict:
+    """How each product of a dense :func:`fused_linear` call would run: {product: {engine, tile_rows, tile_cols, splits,
+    items}}."""
+    g = 4 if dtype == torch.float32 else 8
+    kp = -(-in_features // g) * g
+    return _plans("orda_linear_plan", Linear(ABI_VERSION, DTYPE[dtype], 0, 0, tokens, in_features, out_features, kp, kp, out_features,
+                                             kp, kp), LINEAR_PRODUCTS)
+
+
+def feed_forward_plan(tokens: int, hidden: int, inner: int, out_features: int, dtype: torch.dtype) -> dict:
+    """As :func:`linear_plan`, of :func:`gated_feed_forward`."""
+    g = 4 if dtype == torch.float32 else 8
+    hp, ip, op = (-(-n // g) * g for n in (hidden, inner, out_features))
+    return _plans("orda_ffn_plan", FeedForward(ABI_VERSION, DTYPE[dtype], 0, 0, tokens, hidden, inner, out_features, hp, hp, ip,
+                                               out_features, op, hp, hp, ip), FFN_PRODUCTS)
 
 
 _TORCH_OPS = None
