@@ -496,12 +496,13 @@ __device__ __forceinline__ void epi_apply(const Epi& E, uint32_t m, uint32_t n, 
 
 // Sum of the partials in split order, then the epilogue; a thread takes 4
 // columns of a row.  cols a multiple of 4.  rows: M, or 2 M of a pair (the
-// second product's behind the first's).
+// second product's behind the first's).  The grid has a second dimension past
+// 2^22 workgroups (a launch has fewer than 2^32 threads in each).
 template <class Epi>
 __global__ __launch_bounds__(256) void k_part_reduce(const float* __restrict__ part, int splits, int64_t stride,
                                                      int64_t ld, int64_t M, int64_t rows, int64_t cols, Epi E) {
   const int64_t nq = cols / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
   if (i >= rows * nq) return;
   int64_t m = i / nq;
   const int64_t n = (i - m * nq) * 4;

@@ -140,8 +140,9 @@ hipError_t with_splits(const OpPlan& pl, const TileParams& P, const Epi& E, floa
   EpiPart<Epi::kDual> Q{part, part + cols, rows * ld, ld, cols, P.M * ld};
   const hipError_t e = go(Q);
   if (e != hipSuccess) return e;
-  const int64_t n = rows * (cols / 4);
-  hipLaunchKernelGGL((k_part_reduce<Epi>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, part, pl.splits, rows * ld, ld, P.M, rows, cols, E);
+  const int64_t groups = (rows * (cols / 4) + 255) / 256, across = groups < (1 << 22) ? groups : (1 << 22);
+  const dim3 grid((unsigned)across, (unsigned)((groups + across - 1) / across));
+  hipLaunchKernelGGL((k_part_reduce<Epi>), grid, dim3(256), 0, s, part, pl.splits, rows * ld, ld, P.M, rows, cols, E);
   return hipGetLastError();
 }
 
