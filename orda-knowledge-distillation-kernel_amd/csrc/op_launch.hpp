@@ -11,7 +11,7 @@ namespace orda {
 // orda_last_error()'s message on this thread (abi.hip).
 int set_last_error(int code, const char* msg);
 
-enum OpEngine { OP_SKINNY = 0, OP_TILE = 1, OP_RING = 2, OP_SPLIT3 = 3 };
+enum OpEngine { OP_SKINNY = 0, OP_TILE = 1, OP_RING = 2, OP_SPLIT3 = 3, OP_NONE = -1 };
 
 // How one product runs: the engine, its tile, and K in `splits` ranges of kps.
 struct OpPlan {

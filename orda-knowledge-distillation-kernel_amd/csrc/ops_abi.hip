@@ -37,8 +37,10 @@ inline int64_t granule(int dtype) { return dtype == ORDA_F32 ? 4 : 8; }  // elem
 inline bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 inline char* base256(void* ws) { return reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(ws) + 255) / 256 * 256); }
 
-// (Outputs are dense, so memory bounds the grids: 288 GB are 7e7 tiles of 64 x 32.)
 constexpr int64_t kMaxTokens = 1ll << 30;
+// A launch has fewer than 2^32 threads, a tile 256 of them: 2^30 tokens on 64
+// columns are 2^24 tiles of 64 rows, one too many, and half as many of 128.
+constexpr double kMaxItems = 16777216.0;
 // (128 rows of a K-major operand in one buffer resource, 256 rows of an output
 // within 2^32 bytes)
 constexpr int64_t kMaxWidth = 1ll << 21, kMaxPitch = 1ll << 22;
@@ -120,6 +122,7 @@ double s3_op_cost(const Shape& q, int64_t sp, bool large) {
 
 OpPlan plan_of(const Shape& q) {
   OpPlan pl{};
+  pl.engine = OP_NONE;
   pl.splits = 1;
   pl.kps = up(q.K, 64);
   if (q.M <= 16 && q.la == KMAJ && q.lb == KMAJ) {
@@ -144,7 +147,8 @@ OpPlan plan_of(const Shape& q) {
       take(s3_op_cost(q, sp, false), OP_SPLIT3, 64, sp);
       continue;
     }
-    for (const TileCost& t : kTileCosts) take(tile_cost(q, t, sp), OP_TILE, t.bm * 1000 + t.bn, sp);
+    for (const TileCost& t : kTileCosts)
+      if (items_of(q, t.bm, t.bn, sp) < kMaxItems) take(tile_cost(q, t, sp), OP_TILE, t.bm * 1000 + t.bn, sp);
     if (ring_fits(q, sp)) take(ring_cost(q, sp), OP_RING, 256, sp);
   }
   if (pl.engine == OP_RING && splits == 1) pl.kps = q.K;
@@ -153,6 +157,14 @@ OpPlan plan_of(const Shape& q) {
     pl.splits = (int)cdiv(q.K, pl.kps);
   }
   return pl;
+}
+
+// Whether a launch has the workgroups for a product (looked at where it is
+// near: 2^24 tiles of 128 x 64 are at least 2^36 elements).
+int check_launch(const char* what, const Shape& q) {
+  if ((double)q.M * (double)q.cols >= 34359738368.0 && plan_of(q).engine == OP_NONE)
+    return fail(ORDA_EINVAL, "%s: %lld x %lld outputs are more tiles than a launch has workgroups", what, (long long)q.M, (long long)q.cols);
+  return ORDA_OK;
 }
 
 // Rows and columns of the output that a workgroup (or one turn of a persistent
@@ -249,6 +261,7 @@ int linear_shapes(const orda_linear_t* p, LinearShapes& s) {
   s.fwd = {p->dtype, KMAJ, KMAJ, false, p->tokens, p->out_features, kp, 0, 0, false};
   s.dx = {p->dtype, KMAJ, MNMAJ, false, p->tokens, kp, s.op, 0, p->ldw, false};
   s.dw = {p->dtype, MNMAJ, MNMAJ, false, p->out_features, kp, p->tokens, s.op, p->ldx, false};
+  for (const Shape* q : {&s.fwd, &s.dx}) OP_TRY(check_launch(what, *q));
   // about 1024 workgroups, at least 16 rows each (8192 x 4096 in bf16 with 512,
   // 1024, 2048, 4096: 63, 46, 52, 47 us)
   const int64_t per = 64 * g, cb = cdiv(s.op, per);
@@ -309,6 +322,7 @@ int ffn_shapes(const orda_ffn_t* p, FfnShapes& s) {
   s.dw2 = s.dw;
   s.dw2.pair = true;
   s.dd = {p->dtype, MNMAJ, MNMAJ, false, p->out_features, ip, p->tokens, p->ldg, s.fp, false};
+  for (const Shape* q : {&s.gate, &s.down, &s.dh, &s.dx}) OP_TRY(check_launch(what, *q));
   return ORDA_OK;
 }
 size_t ffn_part(const FfnShapes& s, bool backward) {

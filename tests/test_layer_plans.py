@@ -51,3 +51,22 @@ def test_plan_queries_refuse():
         for product in (-1, n):
             assert fn(ctypes.byref(p), product, ctypes.byref(out)) == -1
         assert fn(ctypes.byref(p), 0, None) == -1 and fn(None, 0, ctypes.byref(out)) == -1
+
+
+@pytest.mark.parametrize("size", [(1 << 30, 8, 8), ((1 << 30) - 63, 8, 8), (1 << 30, 8, 64), (1 << 29, 8, 200), (1 << 30, 72, 129)], ids=str)
+def test_launches_have_fewer_than_2_to_32_threads(size):
+    """A tile is a workgroup of 256 threads; 64-row tiles of 2^30 tokens are 2^24 of them."""
+    for p in _native.linear_plan(*size, torch.bfloat16).values():
+        assert p["engine"] == "ring" or p["items"] * 256 < 1 << 32
+    for p in _native.feed_forward_plan(size[0], 8, 64, 8, torch.bfloat16).values():
+        assert p["items"] * 256 < 1 << 32
+
+
+def test_more_tiles_than_a_launch_takes_are_refused():
+    with pytest.raises(ValueError, match="more tiles"):
+        _native.linear_plan(1 << 30, 64, 129, torch.bfloat16)
+    with pytest.raises(ValueError, match="more tiles"):
+        _native.feed_forward_plan(1 << 30, 8, 128, 8, torch.bfloat16)
+    lin = _native.Linear(_native.ABI_VERSION, 0, 0, 0, 1 << 30, 64, 129, 64, 64, 129, 64, 64)
+    assert _native.library().orda_linear_forward(ctypes.byref(lin), 256, 256, None, None, 256, None, 256, 1 << 50, None) == -1
+    assert _native.library().orda_linear_workspace_bytes(ctypes.byref(lin), 0) == 0
