@@ -22,7 +22,7 @@
 #include <optional>
 #include <string>
 #include <tuple>
-#include <unordered_set>
+#include <unordered_map>
 #include <utility>
 #include <vector>
 
@@ -473,12 +473,22 @@ Tensor clip(const std::vector<Tensor>& params, double max_norm, double norm_type
             const std::optional<std::vector<Tensor>>& outs) {
   static const char* entry = "clip_grad_norm_";
   std::vector<Tensor> grads, dests;
-  std::unordered_set<const void*> seen;
+  std::unordered_map<const void*, size_t> seen;
   grads.reserve(params.size());
   seen.reserve(params.size());
   for (size_t i = 0; i < params.size(); ++i) {
     const Tensor& g = params[i].grad();
-    if (!g.defined() || !seen.insert(params[i].unsafeGetTensorImpl()).second) continue;
+    if (!g.defined()) continue;
+    const auto [at, fresh] = seen.emplace(params[i].unsafeGetTensorImpl(), i);
+    if (!fresh) {
+      if (outs) {
+        const Tensor &a = (*outs)[at->second], &b = (*outs)[i];
+        TORCH_CHECK_VALUE(a.is_same(b) || (a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides() &&
+                                           a.scalar_type() == b.scalar_type() && a.device() == b.device()),
+                          entry, ": parameters ", at->second, " and ", i, " are one, their out tensors are not");
+      }
+      continue;
+    }
     check_grad(entry, g, grads.empty() ? g.device() : grads[0].device());
     if (outs) {
       const Tensor& o = (*outs)[i];

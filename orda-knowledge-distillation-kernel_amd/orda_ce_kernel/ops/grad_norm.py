@@ -44,13 +44,22 @@ def _norm_torch(grads, norm_type: float) -> torch.Tensor:
     ).float()
 
 
+def _same_place(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a is b or (a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
+                      and a.dtype == b.dtype and a.device == b.device)
+
+
 def _clip_torch(entry, params, outs, max_norm, norm_type, error_if_nonfinite, total_norm):
-    grads, dests, seen = [], [], set()
+    grads, dests, seen = [], [], {}
     for i, p in enumerate(params):
         g = p.grad
-        if g is None or id(p) in seen:
+        if g is None:
             continue
-        seen.add(id(p))
+        k = seen.setdefault(id(p), i)
+        if k != i:
+            if outs is not None and not _same_place(outs[k], outs[i]):
+                raise ValueError(f"{entry}: parameters {k} and {i} are one, their out tensors are not")
+            continue
         _check_grad(entry, g, grads[0].device if grads else g.device)
         if outs is not None:
             o = outs[i]
@@ -101,10 +110,11 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     """Scale the parameters' gradients by ``min(1, max_norm / (total + 1e-6))`` in place and return their total norm, as
     ``torch.nn.utils.clip_grad_norm_`` does, without synchronising the host (but for ``error_if_nonfinite``).
 
-    Parameters without a gradient are left out; one that is listed twice counts once.  ``total_norm`` (a one-element
-    tensor): the norm to scale by, instead of these gradients' own.  ``out``: one tensor per parameter (any of the three
-    dtypes, the gradient's shape) that receives the scaled gradient, which itself stays as it is: the fp32 buffers of a
-    mixed-precision optimizer.  Tensors that are written must not share memory with any other of the call."""
+    Parameters without a gradient are left out; one that is listed twice counts once (and has one ``out`` tensor).
+    ``total_norm`` (a one-element tensor): the norm to scale by, instead of these gradients' own.  ``out``: one tensor per
+    parameter (any of the three dtypes, the gradient's shape) that receives the scaled gradient, which itself stays as it
+    is: the fp32 buffers of a mixed-precision optimizer.  Tensors that are written must not share memory with any other of
+    the call."""
     entry = "clip_grad_norm_"
     norm_type, max_norm = _check_norm(entry, norm_type), float(max_norm)
     if not max_norm >= 0.0:
