@@ -352,11 +352,12 @@ typedef struct orda_rows {
 } orda_rows_t;
 int orda_pad_rows(int32_t dtype, const orda_rows_t* t, int64_t n, void* stream);
 
-/* y = act(x W^T + bias) + residual.  Rows of x, weight and their gradients are
- * ld* elements apart, a multiple of 8 (fp32: 4), and start 16-byte aligned; x
- * and weight are zero from in_features up to the next such multiple, and their
- * gradients are written up to it.  bias, residual, y and grad_output may have
- * any alignment. */
+/* y = act(x W^T + bias) + residual.  Rows of x and weight are ld* elements
+ * apart, a multiple of 8 (fp32: 4), and start 16-byte aligned; both are zero
+ * from in_features up to the next such multiple.  Their gradients are 16-byte
+ * aligned, in dense rows (ld* = in_features) or in rows as their operands', then
+ * written up to that multiple.  bias, residual, y and grad_output may have any
+ * alignment. */
 typedef struct orda_linear {
   int32_t abi_version;   /* must equal ORDA_ABI_VERSION                      */
   int32_t dtype;         /* enum orda_dtype, of every tensor                 */

@@ -225,6 +225,12 @@ int check_pitch(const char* what, const char* name, int64_t ld, int64_t width, i
                 (long long)up(width, g), (long long)ld);
   return ORDA_OK;
 }
+// Of a gradient: dense rows, or as an operand's; its columns are written up to
+// grad_cols.
+int check_grad_pitch(const char* what, const char* name, int64_t ld, int64_t width, int dtype) {
+  return ld == width ? ORDA_OK : check_pitch(what, name, ld, width, dtype);
+}
+int64_t grad_cols(int64_t ld, int64_t width, int dtype) { return ld == width ? width : up(width, granule(dtype)); }
 int check_residual(const char* what, int64_t ld, int64_t width) {
   if (ld < width || ld > kMaxPitch) return fail(ORDA_EINVAL, "%s: ldr must be in [%lld, 2^22], got %lld", what, (long long)width, (long long)ld);
   return ORDA_OK;
@@ -406,8 +412,8 @@ int orda_linear_backward(const orda_linear_t* p, const void* x, const void* weig
   if ((grad_x && !weight) || (grad_weight && !x)) return fail(ORDA_EINVAL, "orda_linear_backward: grad_x needs weight, grad_weight needs x");
   if (!aligned16(x) || !aligned16(weight) || !aligned16(d) || !aligned16(grad_x) || !aligned16(grad_weight))
     return fail(ORDA_EINVAL, "orda_linear_backward: x, weight, d, grad_x and grad_weight must be 16-byte aligned");
-  if (grad_x) OP_TRY(check_pitch("orda_linear_backward", "ldgx", p->ldgx, p->in_features, p->dtype));
-  if (grad_weight) OP_TRY(check_pitch("orda_linear_backward", "ldgw", p->ldgw, p->in_features, p->dtype));
+  if (grad_x) OP_TRY(check_grad_pitch("orda_linear_backward", "ldgx", p->ldgx, p->in_features, p->dtype));
+  if (grad_weight) OP_TRY(check_grad_pitch("orda_linear_backward", "ldgw", p->ldgw, p->in_features, p->dtype));
   OP_TRY(check_workspace("orda_linear_backward", workspace, workspace_bytes, linear_ws(p, s, true)));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = base256(workspace);
@@ -440,11 +446,11 @@ int orda_linear_backward(const orda_linear_t* p, const void* x, const void* weig
     if (grad_x) {
       TileParams t = product<T>(dz, s.op, weight, p->ldw, p->tokens, s.dx.cols, s.dx.K);
       t.kval = p->out_features;
-      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dx), KMAJ, MNMAJ, t, store_to<T>(grad_x, p->ldgx, s.dx.cols), part, st));
+      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dx), KMAJ, MNMAJ, t, store_to<T>(grad_x, p->ldgx, grad_cols(p->ldgx, p->in_features, p->dtype)), part, st));
     }
     if (grad_weight) {
       const TileParams t = product<T>(dz, s.op, x, p->ldx, p->out_features, s.dw.cols, p->tokens);
-      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw), MNMAJ, MNMAJ, t, store_to<T>(grad_weight, p->ldgw, s.dw.cols), part, st));
+      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw), MNMAJ, MNMAJ, t, store_to<T>(grad_weight, p->ldgw, grad_cols(p->ldgw, p->in_features, p->dtype)), part, st));
     }
     return ORDA_OK;
   });
@@ -527,9 +533,9 @@ int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, co
   if (!x || !w_gate || !w_up || !w_down || !h || !da_factor || !db_factor || !grad_output)
     return fail(ORDA_EINVAL, "orda_ffn_backward: x, the three weights, h, the two factors and grad_output are required");
   OP_TRY(check_pitch("orda_ffn_backward", "ldg", p->ldg, p->out_features, p->dtype));
-  if (grad_x) OP_TRY(check_pitch("orda_ffn_backward", "ldgx", p->ldgx, p->hidden, p->dtype));
-  if (grad_gate || grad_up) OP_TRY(check_pitch("orda_ffn_backward", "ldgw", p->ldgw, p->hidden, p->dtype));
-  if (grad_down) OP_TRY(check_pitch("orda_ffn_backward", "ldgd", p->ldgd, p->inner, p->dtype));
+  if (grad_x) OP_TRY(check_grad_pitch("orda_ffn_backward", "ldgx", p->ldgx, p->hidden, p->dtype));
+  if (grad_gate || grad_up) OP_TRY(check_grad_pitch("orda_ffn_backward", "ldgw", p->ldgw, p->hidden, p->dtype));
+  if (grad_down) OP_TRY(check_grad_pitch("orda_ffn_backward", "ldgd", p->ldgd, p->inner, p->dtype));
   for (const void* q : {x, w_gate, w_up, w_down, h, da_factor, db_factor, grad_output, (const void*)grad_x, (const void*)grad_gate, (const void*)grad_up, (const void*)grad_down})
     if (!aligned16(q)) return fail(ORDA_EINVAL, "orda_ffn_backward: every tensor must be 16-byte aligned");
   OP_TRY(check_workspace("orda_ffn_backward", workspace, workspace_bytes, ffn_ws(p, s, true)));
@@ -552,21 +558,21 @@ int orda_ffn_backward(const orda_ffn_t* p, const void* x, const void* w_gate, co
       t.B1 = w_up;
       t.kseg = s.fp;
       t.kval = p->inner;
-      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dx), KMAJ, MNMAJ, t, store_to<T>(grad_x, p->ldgx, s.dx.cols), part, st));
+      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dx), KMAJ, MNMAJ, t, store_to<T>(grad_x, p->ldgx, grad_cols(p->ldgx, p->hidden, p->dtype)), part, st));
     }
     if (grad_gate && grad_up) {  // one launch: its tiles fill the chip's last round better than two launches' do
       TileParams t = product<T>(d, 2 * s.fp, x, p->ldx, p->inner, s.dw2.cols, p->tokens);
       t.pair = s.fp;
-      EpiLinear<T> e = store_to<T>(grad_gate, p->ldgw, s.dw2.cols);
+      EpiLinear<T> e = store_to<T>(grad_gate, p->ldgw, grad_cols(p->ldgw, p->hidden, p->dtype));
       e.y1 = static_cast<T*>(grad_up);
       OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw2), MNMAJ, MNMAJ, t, e, part, st));
     } else if (grad_gate || grad_up) {
       const TileParams t = product<T>(d + (grad_up ? s.fp * (int64_t)sizeof(T) : 0), 2 * s.fp, x, p->ldx, p->inner, s.dw.cols, p->tokens);
-      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw), MNMAJ, MNMAJ, t, store_to<T>(grad_up ? grad_up : grad_gate, p->ldgw, s.dw.cols), part, st));
+      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dw), MNMAJ, MNMAJ, t, store_to<T>(grad_up ? grad_up : grad_gate, p->ldgw, grad_cols(p->ldgw, p->hidden, p->dtype)), part, st));
     }
     if (grad_down) {
       const TileParams t = product<T>(grad_output, p->ldg, h, s.fp, p->out_features, s.dd.cols, p->tokens);
-      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dd), MNMAJ, MNMAJ, t, store_to<T>(grad_down, p->ldgd, s.dd.cols), part, st));
+      OP_LAUNCH(launch_op_linear<T>(plan_of(s.dd), MNMAJ, MNMAJ, t, store_to<T>(grad_down, p->ldgd, grad_cols(p->ldgd, p->inner, p->dtype)), part, st));
     }
     return ORDA_OK;
   });

@@ -173,14 +173,11 @@ Tensor rows_of(const Tensor& given, ScalarType type) {
   return t;
 }
 
+// Dense, so that accumulating it into a leaf copies nothing.
 Tensor gradient(const Tensor& like, int64_t rows, int64_t cols, ScalarType type) {
-  return at::empty({rows, padded(cols, type)}, like.options().dtype(type));
+  return at::empty({rows, cols}, like.options().dtype(type));
 }
-Tensor trimmed(const Tensor& g, int64_t cols, ScalarType type) {
-  if (!g.defined()) return g;
-  Tensor t = g.size(1) == cols ? g : g.narrow(1, 0, cols);
-  return t.scalar_type() == type ? t : t.to(type);
-}
+Tensor as_type(const Tensor& g, ScalarType type) { return !g.defined() || g.scalar_type() == type ? g : g.to(type); }
 
 // Gradients of a node that is differentiable once: with create_graph (`graph`)
 // a second backward through them raises.
@@ -238,7 +235,7 @@ LinearCall linear_run(const Tensor& x, const Tensor& w, const Tensor& bias, cons
   const Tensor b = bias.defined() ? bias.to(type).contiguous() : Tensor();
   const Tensor r = res.defined() ? rows_of(res, type) : Tensor();
   c.p = {ORDA_ABI_VERSION, code(type), (int32_t)act, 0, x.size(0), x.size(1), w.size(0), pitch(c.x), pitch(c.w),
-         r.defined() ? pitch(r) : 0, padded(x.size(1), type), padded(x.size(1), type)};
+         r.defined() ? pitch(r) : 0, x.size(1), x.size(1)};
   c.y = at::empty({x.size(0), w.size(0)}, x.options().dtype(type));
   if (keep && act != ORDA_ACT_NONE) c.d = bytes(size_of(api.linear_saved_bytes(&c.p), "orda_linear_saved_bytes"), x);
   const size_t n = size_of(api.linear_workspace_bytes(&c.p, 0), "orda_linear_workspace_bytes");
@@ -290,9 +287,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
       const size_t n = size_of(api.linear_workspace_bytes(&p, 1), "orda_linear_workspace_bytes");
       const Tensor ws = bytes(n, dy);
       check(api.linear_backward(&p, ptr(x), ptr(w), ptr(d), ptr(dy), out(g[0]), out(g[1]), out(g[2]), out(ws), n, s), "orda_linear_backward");
-      g[0] = trimmed(g[0], p.in_features, type(1));
-      g[1] = trimmed(g[1], p.in_features, type(2));
-      if (nb) g[2] = g[2].to(type(3));
+      for (int i = 0; i < 3; ++i) g[i] = as_type(g[i], type(i + 1));
     }
     return once(std::move(g), graph);
   }
@@ -322,7 +317,7 @@ FfnCall ffn_run(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tenso
   const Tensor r = res.defined() ? rows_of(res, type) : Tensor();
   const int64_t N = x.size(0), H = x.size(1), F = wg.size(0), O = wd.size(0);
   c.p = {ORDA_ABI_VERSION, code(type), (int32_t)act, 0, N, H, F, O, pitch(c.x), pitch(c.gate), pitch(c.down),
-         r.defined() ? pitch(r) : 0, padded(O, type), padded(H, type), padded(H, type), padded(F, type)};
+         r.defined() ? pitch(r) : 0, padded(O, type), H, H, F};
   c.y = at::empty({N, O}, x.options().dtype(type));
   c.h = at::empty({N, (int64_t)size_of((size_t)api.ffn_inner_pitch(&c.p), "orda_ffn_inner_pitch")}, c.y.options());
   if (keep) {
@@ -384,7 +379,7 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
       const Tensor ws = bytes(n, dy);
       check(api.ffn_backward(&p, ptr(x), ptr(gate), ptr(up), ptr(down), ptr(h), ptr(da), ptr(db), ptr(dy), out(g[0]), out(g[1]), out(g[2]),
                              out(g[3]), out(ws), n, s), "orda_ffn_backward");
-      for (int i = 0; i < 4; ++i) g[i] = trimmed(g[i], cols[i], type(i + 1));
+      for (int i = 0; i < 4; ++i) g[i] = as_type(g[i], type(i + 1));
     }
     return once(std::move(g), graph);
   }
