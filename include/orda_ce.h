@@ -372,7 +372,7 @@ typedef struct orda_linear {
 } orda_linear_t;
 
 /* Bytes of d = act'(x W^T + bias) as orda_linear_forward keeps it for the
- * backward pass (fp32; for 16-bit tensors the upper 24 bits of fp32 values). */
+ * backward pass (fp32; for 16-bit tensors rounded to the upper 24 bits). */
 size_t orda_linear_saved_bytes(const orda_linear_t* p);
 
 /* Scratch bytes of the forward (backward = 0) or the backward call (1). */
@@ -418,7 +418,7 @@ typedef struct orda_ffn {
 /* Elements between the rows of h ([tokens x this], in dtype). */
 int64_t orda_ffn_inner_pitch(const orda_ffn_t* p);
 /* Bytes of each factor that the forward call keeps for the backward pass (fp32;
- * for 16-bit tensors the upper 24 bits of fp32 values). */
+ * for 16-bit tensors rounded to the upper 24 bits). */
 size_t orda_ffn_saved_bytes(const orda_ffn_t* p);
 size_t orda_ffn_workspace_bytes(const orda_ffn_t* p, int32_t backward);
 

@@ -175,11 +175,15 @@ struct RawRow {
 };
 
 // Factors that the backward pass multiplies by.  For 16-bit tensors they are
-// kept as the upper 24 bits of the fp32 value (15 bits after the leading one,
-// fp32's range), in a plane of 16-bit halves and a plane of bytes: rounded to
-// bf16 they made the gradients of the feed-forward block 1.8 times as far off
-// float64 as one rounding at the end, with 24 bits 1.4 times (da and db are
-// rounded as operands).  fp32: as is, in the first plane.
+// kept in 24 bits, an fp32 value's sign, exponent and first 15 bits, in a plane
+// of 16-bit halves and a plane of bytes: rounded to bf16 they made the gradients
+// of the feed-forward block 1.8 times as far off float64 as one rounding at the
+// end, with 24 bits 1.4 times (da and db are rounded as operands).  Rounded to
+// nearest, ties away from zero, so that sums over many tokens see no one-sided
+// error; half a step is 2^-16 of the value.  (Adding half a step to the bits
+// carries into the exponent as it should and leaves infinities; a NaN that came
+// from 16-bit operands or from arithmetic has zeros in the bits it could carry
+// out of.)  fp32: as is, in the first plane.
 // i: index of the first of W values, a multiple of W.
 template <class T>
 constexpr int kKeptBytes = sizeof(T) == 4 ? 4 : 3;
@@ -202,14 +206,15 @@ __device__ __forceinline__ void keep(const Planes& p, uint32_t i, const float (&
   if constexpr (sizeof(T) == 4) {
     st_row<float, W>(reinterpret_cast<float*>(p.hi + i * 4), v, W);
   } else {
-    uint32_t h[W / 2], l[W / 4];
+    uint32_t r[W], h[W / 2], l[W / 4];
 #pragma unroll
-    for (int e = 0; e < W / 2; ++e)
-      h[e] = __builtin_amdgcn_perm(__float_as_uint(v[2 * e + 1]), __float_as_uint(v[2 * e]), 0x07060302u);
+    for (int e = 0; e < W; ++e) r[e] = __float_as_uint(v[e]) + 0x80u;
+#pragma unroll
+    for (int e = 0; e < W / 2; ++e) h[e] = __builtin_amdgcn_perm(r[2 * e + 1], r[2 * e], 0x07060302u);
 #pragma unroll
     for (int e = 0; e < W / 4; ++e) {
-      const uint32_t a = __builtin_amdgcn_perm(__float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e]), 0x0c0c0501u);
-      const uint32_t b = __builtin_amdgcn_perm(__float_as_uint(v[4 * e + 3]), __float_as_uint(v[4 * e + 2]), 0x0c0c0501u);
+      const uint32_t a = __builtin_amdgcn_perm(r[4 * e + 1], r[4 * e], 0x0c0c0501u);
+      const uint32_t b = __builtin_amdgcn_perm(r[4 * e + 3], r[4 * e + 2], 0x0c0c0501u);
       l[e] = a | (b << 16);
     }
     if constexpr (W == 4) {

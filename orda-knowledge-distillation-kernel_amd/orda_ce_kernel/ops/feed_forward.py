@@ -11,7 +11,7 @@ A training call also keeps the factors p = b act'(a) and q = act(a).  Backward, 
     dWg = da^T x    dWu = db^T x    dWd = dy^T h
 
 h, da and db are rounded to the compute dtype as operands of the next product; p and q are kept in fp32, for 16-bit tensors
-in its upper 24 bits; products accumulate in fp32.  The operands, workspaces and the autograd node are in
+rounded to its upper 24 bits; products accumulate in fp32.  The operands, workspaces and the autograd node are in
 csrc/torch_ops.cpp.  No counterpart in the reference, whose models use torch.
 """
 from __future__ import annotations

@@ -4,7 +4,7 @@
 
 One kernel computes it (few rows: one that streams W; more: tiles of the matrix cores, with K split over workgroups where
 there are few tiles); for the backward pass it also keeps d = act'(x W^T + bias) where there is an activation (fp32; for
-16-bit tensors the upper 24 bits of the fp32 values).  Backward: dz = dy d and the bias gradient in one pass over dy and d,
+16-bit tensors rounded to the upper 24 bits).  Backward: dz = dy d and the bias gradient in one pass over dy and d,
 then dx = dz W and dW = dz^T x; the residual's gradient is dy.  Products accumulate in fp32, every output is rounded once.
 The operands, workspaces and the autograd node are in csrc/torch_ops.cpp.  No counterpart in the reference, whose models use
 torch.
