@@ -172,7 +172,7 @@ template <class T, class O, int KIND, int ROWS>
 __global__ __launch_bounds__(256) void k_clip(SpanTable<ROWS> S, ClipParams P) {
   // 16 bytes a lane and access on the wider side: 16 in and 2 x 16 out leave
   // half of each line to another store (bf16 into fp32: 5.1 TB/s, 6.5 so)
-  constexpr int VE = sizeof(O) == 4 ? 4 : 16 / (int)sizeof(T), U = 4;
+  constexpr int VE = sizeof(O) == 4 ? 4 : 16 / (int)sizeof(T);
   typedef T in_vec __attribute__((ext_vector_type(VE)));
   // (outputs at any element: the hardware's unaligned stores)
   typedef O out_vec __attribute__((ext_vector_type(VE), aligned(sizeof(O))));
@@ -194,16 +194,8 @@ __global__ __launch_bounds__(256) void k_clip(SpanTable<ROWS> S, ClipParams P) {
   };
   for_chunks<T>(S, [&](int t, int row, const T* p, int64_t lo, int64_t hi) {
     O* o = static_cast<O*>(S.t[t].out) + row * S.t[t].ld_out;
-    int64_t e = lo + (int64_t)threadIdx.x * VE;
-    for (; e + (U - 1) * 256 * VE + VE <= hi && lo >= 0; e += U * 256 * VE) {
-      in_vec v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const in_vec*>(p + e + u * 256 * VE);
-#pragma unroll
-      for (int u = 0; u < U; ++u) put(o + e + u * 256 * VE, v[u]);
-    }
 #pragma unroll 2
-    for (; e < hi; e += 256 * VE) {
+    for (int64_t e = lo + (int64_t)threadIdx.x * VE; e < hi; e += 256 * VE) {
       if (e >= 0 && e + VE <= hi) {
         put(o + e, *reinterpret_cast<const in_vec*>(p + e));
       } else {

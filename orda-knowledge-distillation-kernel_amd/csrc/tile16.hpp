@@ -139,13 +139,11 @@ struct TileDma {
     chunk = (uint32_t)((i % kPer) ^ (L == KMAJ ? kswz((int)row) : mn_f<R>((int)row) << 1));
   }
   static constexpr int kRowStep = 256 / kPer;
-  // The thread's offset for chunk q (added by the caller: q kRowStep rows), or
+  // The thread's offset (chunk q lies q kRowStep rows on, the caller adds them), or
   // past every resource.  K-major: left = bytes of K from the step on;
   // MN-major: left = valid columns.
-  __device__ __forceinline__ uint32_t off(uint32_t ldb, int left, int q) const {
-    // (MN-major rows of 512 bytes: K rows 8 apart differ in f's third bit)
-    const uint32_t c = L == MNMAJ && R == 256 && (q & 1) ? chunk ^ 8u : chunk;
-    return (int)(c * (L == KMAJ ? 16 : 8)) < left ? row * ldb + c * 16 : kOob;
+  __device__ __forceinline__ uint32_t off(uint32_t ldb, int left) const {
+    return (int)(chunk * (L == KMAJ ? 16 : 8)) < left ? row * ldb + chunk * 16 : kOob;
   }
   static __device__ __forceinline__ void go(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t soff, int q, char* tile) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(tile + (q * 4 + wave_id()) * 1024),
@@ -205,32 +203,24 @@ __global__ __launch_bounds__(256) void k_tile(TileParams P, Epi E0) {
   const int seg = (int)lmin((P.kseg - kb0 + 63) / 64, 0x7fffffff);  // B1's first step
   const int kbytes = (int)(klen * 2);
   const int mleft = (int)lmin(P.M - m0, BM), nleft = (int)lmin(P.N - n0, BN);
-  uint32_t offa[TileDma<T, LA, BM>::NQ], offb[TileDma<T, LB, BN>::NQ];
-  if constexpr (LA == MNMAJ) {
-#pragma unroll
-    for (int q = 0; q < TileDma<T, LA, BM>::NQ; ++q) offa[q] = da.off(ldab, mleft, q);
-  }
-  if constexpr (LB == MNMAJ) {
-#pragma unroll
-    for (int q = 0; q < TileDma<T, LB, BN>::NQ; ++q) offb[q] = db.off(ldbb, nleft, q);
-  }
+  const uint32_t offa = da.off(ldab, mleft), offb = db.off(ldbb, nleft);  // (MN-major)
   auto issue = [&](int kt, char* st) __attribute__((always_inline)) {
     const int left = kbytes - kt * 128;  // (past the end: <= 0, zeros; the count of DMAs stays the same)
     {
-      const uint32_t o = LA == KMAJ ? da.off(ldab, left, 0) : 0u;
+      const uint32_t o = LA == KMAJ ? da.off(ldab, left) : left > 0 ? offa : kOob;
       const uint32_t so = LA == KMAJ ? (uint32_t)kt * 128u : left > 0 ? (uint32_t)kt * 64u * ldab : 0u;
 #pragma unroll
       for (int q = 0; q < TileDma<T, LA, BM>::NQ; ++q)
-        da.go(ra, LA == KMAJ ? o : (left > 0 ? offa[q] : kOob), so + (uint32_t)(q * TileDma<T, LA, BM>::kRowStep) * ldab, q, st);
+        da.go(ra, o, so + (uint32_t)(q * TileDma<T, LA, BM>::kRowStep) * ldab, q, st);
     }
     {
-      const uint32_t o = LB == KMAJ ? db.off(ldbb, left, 0) : 0u;
+      const uint32_t o = LB == KMAJ ? db.off(ldbb, left) : left > 0 ? offb : kOob;
       const uint32_t so = LB == KMAJ ? (uint32_t)kt * 128u : left > 0 ? (uint32_t)kt * 64u * ldbb : 0u;
       constexpr int H = TileDma<T, LB, BN>::NQ / 2;
 #pragma unroll
       for (int q = 0; q < TileDma<T, LB, BN>::NQ; ++q) {
         const bool two = DUAL ? q >= H : (LB == MNMAJ && LA == KMAJ && kt >= seg);
-        db.go(two ? rb1 : rb0, LB == KMAJ ? o : (left > 0 ? offb[q] : kOob),
+        db.go(two ? rb1 : rb0, o,
               so + (uint32_t)((DUAL && q >= H ? q - H : q) * TileDma<T, LB, BN>::kRowStep) * ldbb, q, st + kA);
       }
     }
