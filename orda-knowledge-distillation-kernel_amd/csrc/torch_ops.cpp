@@ -153,16 +153,16 @@ std::pair<Tensor, Tensor> add_pair(Operands& ops, const Tensor& a, const Tensor&
 
 // What a node saved, as the backward pass reads it.  Saved-tensor hooks
 // (offloading to the host, for one) may hand back a copy, dense where the saved
-// tensor's rows were apart, so that pitches and alignment are taken from what
-// they hand back; its shape and device have to be the saved one's.
+// tensor's rows were apart, so that pitches, alignment and dtype are taken from
+// what they hand back; its shape and device have to be the saved one's.
 const Tensor& restored(const Tensor& t, at::IntArrayRef sizes, const c10::Device& device) {
   TORCH_CHECK(t.defined() && t.sizes() == sizes && t.device() == device, "a saved tensor of shape ", sizes, " on ", device,
               " came back from its hooks ", t.defined() ? "with another shape or on another device" : "undefined");
   return t;
 }
 // Kept factors and h: dense and 16-byte aligned.
-Tensor restored_dense(const Tensor& t, at::IntArrayRef sizes, const c10::Device& device) {
-  Tensor d = restored(t, sizes, device).contiguous();
+Tensor restored_dense(const Tensor& t, at::IntArrayRef sizes, ScalarType type, const c10::Device& device) {
+  Tensor d = restored(t, sizes, device).to(type).contiguous();
   return aligned(d) ? d : d.clone();
 }
 
@@ -280,7 +280,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
       if (nx) p.ldw = pitch(w = ops.add(restored(saved[1], {p.out_features, kp}, dy.device())));
       ops.copy(s);
       if (p.activation != ORDA_ACT_NONE)
-        d = restored_dense(saved[2], {(int64_t)size_of(api.linear_saved_bytes(&p), "orda_linear_saved_bytes")}, dy.device());
+        d = restored_dense(saved[2], {(int64_t)size_of(api.linear_saved_bytes(&p), "orda_linear_saved_bytes")}, at::kByte, dy.device());
       if (nx) g[0] = gradient(dy, p.tokens, p.in_features, t);
       if (nw) g[1] = gradient(dy, p.out_features, p.in_features, t);
       if (nb) g[2] = at::empty({p.out_features}, dy.options());
@@ -367,8 +367,8 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
       const auto [gate, up] = add_pair(ops, restored(v[1], {p.inner, hp}, device), restored(v[2], {p.inner, hp}, device));
       const Tensor down = ops.add(restored(v[3], {p.out_features, padded(p.inner, t)}, device));
       ops.copy(s);
-      const Tensor h = restored_dense(v[4], {p.tokens, api.ffn_inner_pitch(&p)}, device);
-      const Tensor da = restored_dense(v[5], {kept}, device), db = restored_dense(v[6], {kept}, device);
+      const Tensor h = restored_dense(v[4], {p.tokens, api.ffn_inner_pitch(&p)}, t, device);
+      const Tensor da = restored_dense(v[5], {kept}, at::kByte, device), db = restored_dense(v[6], {kept}, at::kByte, device);
       p.ldg = pitch(dy);
       p.ldx = pitch(x);
       p.ldw = pitch(gate);

@@ -82,6 +82,17 @@ def test_padded_operands_and_one_gate_weight_handed_back_apart():
     check({"y": y, **got}, want_ffn(t, "silu", torch.bfloat16))
 
 
+def test_hooks_that_hand_back_another_dtype():
+    """Values that a hook keeps in fp32 (or, bytes, as int32) and hands back so."""
+    t = ffn_case(90, 96, 72, 88, torch.bfloat16, "silu", False, seed=43)
+    names = ("x", "w_gate", "w_up", "w_down")
+    leaves = [t[n].cuda().requires_grad_(True) for n in names]
+    wide = lambda v: v.int() if v.dtype == torch.uint8 else v.float()  # noqa: E731
+    with torch.autograd.graph.saved_tensors_hooks(wide, lambda v: v):
+        y = orda.gated_feed_forward(*leaves)
+    check({"y": y, **dict(zip(names, torch.autograd.grad(y, leaves, t["dy"].cuda())))}, want_ffn(t, "silu", torch.bfloat16))
+
+
 def test_hooks_that_hand_back_something_else_are_refused():
     x, w = (torch.randn(40, 16, device="cuda", requires_grad=True) for _ in range(2))
     for other in (lambda t: t[:-1], lambda t: t.cpu(), lambda t: t.reshape(-1)):
