@@ -26,9 +26,12 @@ __device__ __forceinline__ float sigmoid_of(float x) {
 // Phi(x) = erfc(-x / sqrt 2) / 2, which keeps its relative accuracy where
 // 1 + erf cancels, and e = exp(-x^2 / 2).  For 16-bit outputs erfc(u) exp(u^2),
 // u = |x| / sqrt 2, is t P(t) with t = 1 / (1 + u / 2) and P of degree 6 fitted
-// to least relative error on u in [0, 9.5] (iterated reweighted least squares;
-// 1.4e-6 in fp32 arithmetic): a dozen instructions, where the library's erfc
-// made the epilogue of an 8192 x 2048 x 4096 product 80 us of its 186.
+// to least relative error on u in [0, 9.5] (iterated reweighted least squares):
+// a dozen instructions, where the library's erfc made the epilogue of an 8192 x
+// 2048 x 4096 product 80 us of its 186.  The polynomial errs by 1.4e-6 in fp32
+// arithmetic; Phi by 1.9e-6 of its value above x = -5 and, through the rounding
+// of the exponent's argument, by up to 8.2e-6 down to x = -13 (half a step of
+// fp16 is 2.4e-4 or more).
 template <class T>
 __device__ __forceinline__ float normal_cdf(float x, float& e) {
   if constexpr (sizeof(T) == 4) {
