@@ -1,17 +1,17 @@
 #!/usr/bin/env python
 """Benchmark: fused CE + distillation loss, forward + backward, on one MI355X.
 
-Default workload is BASELINE config 2 (tied teacher, bf16, N=8192 tokens
+The default workload is a tied teacher (bf16, N=8192 tokens
 (B=4 x T=2048), hidden 4096, vocab 128256, forward KL, T=1, kl_weight 1,
 student and teacher CE weight 1, gradients for student hidden and W; the
 teacher hidden is frozen).  A step is ``loss = distillation_loss(...);
 loss.backward()`` on inputs resident in HBM.  Prints ONE JSON line.
 
-Extra fields beyond the driver contract:
+Extra fields beyond metric, value, times and configuration:
   roofline      dominant kernel class: algorithmic flops per launch / mean
                 launch time (hipEvents recorded by the library on its launch
                 stream during the timed steps) against 2.5 PFLOP/s bf16
-  step_roofline whole step: algorithmic flops (5 x 2NVH at config 2) / step time
+  step_roofline whole step: algorithmic flops (5 x 2NVH by default) / step time
   kernels       per kernel class: launches, ms per step, executed and
                 algorithmic TFLOP/s
   peak_extra_hbm_gb  max_memory_allocated - memory_allocated before a step
