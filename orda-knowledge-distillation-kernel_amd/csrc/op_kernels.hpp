@@ -7,9 +7,11 @@
 namespace orda {
 
 // The projection's backward pass in front of its products: dz = dy act'(z) and
-// the column sums of dz, one pass over dy and the kept derivative.  A wave takes 1 KiB (64 lanes x 16 bytes) of a
-// row, the four waves of a workgroup alternate rows; bias gradients are summed
-// per workgroup and added up by k_colsum, in a fixed order.  Bound by memory.
+// the column sums of dz, one pass over dy and the kept derivative.  dz is rounded
+// to T, being an operand of the matrix cores next; the sums take it unrounded.  A
+// wave takes 1 KiB (64 lanes x 16 bytes) of a row, the four waves of a workgroup
+// alternate rows; bias gradients are summed per workgroup and added up by
+// k_colsum, in a fixed order.  Bound by memory.
 template <class T>
 __global__ __launch_bounds__(256) void k_dz(DzParams P) {
   constexpr int W = 16 / (int)sizeof(T);

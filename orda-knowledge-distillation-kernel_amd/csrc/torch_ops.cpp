@@ -177,6 +177,9 @@ Tensor rows_of(const Tensor& given, ScalarType type) {
 Tensor gradient(const Tensor& like, int64_t rows, int64_t cols, ScalarType type) {
   return at::empty({rows, cols}, like.options().dtype(type));
 }
+// A gradient in its own tensor's dtype.  Beside 16-bit operands that of an fp32
+// tensor has the compute dtype's value, as under torch's autocast: a second set
+// of epilogues would be needed to write the accumulators themselves.
 Tensor as_type(const Tensor& g, ScalarType type) { return !g.defined() || g.scalar_type() == type ? g : g.to(type); }
 
 // Gradients of a node that is differentiable once: with create_graph (`graph`)

@@ -16,6 +16,8 @@ def test_a_sum_of_partials_of_2_to_32_threads():
     2^30): the sum of the ranges' partials takes four elements a thread.  Small whole numbers, exact sums."""
     N, K, O, ld = 8192, 1 << 21, 72, 1 << 22
     bf, lib = torch.bfloat16, _native.library()
+    if torch.cuda.mem_get_info()[0] < 190 << 30:
+        pytest.skip("needs 175 GB of device memory")
     p = _native.Linear(_native.ABI_VERSION, 0, 0, 0, N, K, O, K, ld, O, K, K)
     plan = _native.ProductPlan()
     assert lib.orda_linear_plan(ctypes.byref(p), 1, ctypes.byref(plan)) == 0 and plan.splits == 2
