@@ -493,6 +493,112 @@ int orda_clip_grad_norm(const orda_grad_t* grads, int64_t n, double norm_type, d
  * call must not overlap (ORDA_EINVAL). */
 int orda_clip_grads(const orda_grad_t* grads, int64_t n, const float* total, double max_norm, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * What a student's step has around its projections: token embedding, dropout,
+ * layer norm, masked self-attention (no counterpart in the reference, whose
+ * models use torch).  Problems start with the ABI version; pitches and strides
+ * are in elements, at most 2^22 (attention: rows) or as stated; outputs are
+ * dense and meet no input. */
+
+/* The token embedding, y[n] = scale W[t_n] (a row of zeros for t_n outside [0,
+ * vocab)), and its gradient dW[v] = scale sum of dy[n] over t_n = v, zeros for v
+ * = padding_idx and for rows that no token names. */
+typedef struct orda_embedding {
+  int32_t abi_version;
+  int32_t dtype;       /* of the weight and its gradient: enum orda_dtype       */
+  int32_t out_dtype;   /* of y and dy                                           */
+  int32_t wide_ids;    /* ids are int64 (else int32)                            */
+  int64_t tokens;      /* up to 2^30                                            */
+  int64_t vocab;       /* up to 2^31 - 2                                        */
+  int64_t hidden;      /* up to 2^21                                            */
+  int64_t ldw;         /* pitch of the weight's rows                            */
+  int64_t ldg;         /* pitch of dy's rows                                    */
+  int64_t padding_idx; /* -1: none                                              */
+  float scale;
+  int32_t reserved;    /* 0 */
+} orda_embedding_t;
+int orda_embedding_forward(const orda_embedding_t* p, const void* ids, const void* weight, void* y, void* stream);
+size_t orda_embedding_workspace_bytes(const orda_embedding_t* p); /* backward */
+int orda_embedding_backward(const orda_embedding_t* p, const void* ids, const void* grad_output, void* grad_weight,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* Dropout.  Element e of the row-major tensor is dropped where 16 bits of
+ * Philox4x32-10 (key: the seed; counter: e / 8 in its low 64 bits, `site` in its
+ * high ones; bits 16 (e % 8).. of the 128) are below threshold = floor(65536 p +
+ * 0.5); the others are multiplied by 65536 / (65536 - threshold). */
+typedef struct orda_dropout {
+  double p;            /* in [0, 1]                                             */
+  uint64_t seed;
+  const int64_t* seed_on_device; /* not NULL: the seed is read there            */
+  uint64_t site;       /* calls that share a seed                               */
+} orda_dropout_t;
+
+/* y = residual + dropout(x) on rows of cols elements (dense tensors: one row).
+ * The backward pass is the same call on dy, without residual. */
+typedef struct orda_rows_problem {
+  int32_t abi_version;
+  int32_t dtype;
+  int64_t rows, cols;  /* up to 2^30 and 2^40, 2^42 elements in all             */
+  int64_t ldx, ldr;    /* pitches of x and of the residual                      */
+} orda_rows_problem_t;
+int orda_dropout_add(const orda_rows_problem_t* p, const orda_dropout_t* d, const void* x, const void* residual, void* y,
+                     void* stream);
+
+/* Layer norm with dropout and residual in front of it:
+ *   s = residual + dropout(x), y = (s - mean) / sqrt(variance + eps) w + b.
+ * s (NULL: not wanted) and stats (rows x (mean, rstd) fp32; NULL: no backward
+ * pass) are what the backward pass reads; without residual and dropout it may
+ * read x as s.  With fp32 parameters beside 16-bit tensors it may be given x (as
+ * s) and the residual instead, and computes s again in fp32.  Gradients: ds' = ds + that through the norm, dx = dropout(ds')
+ * without residual, dr = ds'; dw, db.  Any gradient may be NULL; without dropout
+ * dx and dr are one and only one of them may be asked for. */
+typedef struct orda_layer_norm {
+  int32_t abi_version;
+  int32_t dtype;
+  int32_t param_dtype; /* of weight, bias and their gradients: dtype or fp32    */
+  float eps;
+  int64_t rows, cols;  /* up to 2^30 and 2^21                                   */
+  int64_t ldx, ldr;    /* forward                                               */
+  int64_t ld_s, ld_dy, ld_ds; /* backward                                       */
+} orda_layer_norm_t;
+int orda_layer_norm_forward(const orda_layer_norm_t* p, const orda_dropout_t* d, const void* x, const void* residual,
+                            const void* weight, const void* bias, void* y, void* s, float* stats, void* stream);
+size_t orda_layer_norm_workspace_bytes(const orda_layer_norm_t* p); /* backward */
+int orda_layer_norm_backward(const orda_layer_norm_t* p, const orda_dropout_t* d, const void* s, const void* residual,
+                             const float* stats, const void* weight, const void* grad_y, const void* grad_s, void* grad_x, void* grad_residual,
+                             void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Masked self-attention on (batch, length, heads, head_dim) tensors.
+ *   z = scale q.k; with softcap > 0 softcap tanh(z / softcap); less slopes[h] |i - j|
+ * Query i sees key j if (not causal, or j <= i, or j < prefix[b]) and, with
+ * documents, both have the same number, 0 or above.  A query that sees nothing
+ * gives zeros and no gradient.  Query head h reads key and value head h /
+ * (heads / kv_heads).  Rows of a head are 16-byte aligned (all strides multiples
+ * of 8). */
+typedef struct orda_attention {
+  int32_t abi_version;
+  int32_t dtype;       /* ORDA_BF16 or ORDA_F16                                 */
+  int32_t heads, kv_heads;
+  int32_t head_dim;    /* a multiple of 8 up to 128                             */
+  int32_t causal;
+  int64_t batch, length; /* length up to 2^24                                   */
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* of batch, position, head    */
+  int64_t g_stride[3]; /* of grad_output                                        */
+  int64_t documents_stride; /* of the batch                                     */
+  double scale, softcap;
+} orda_attention_t;
+/* What a call keeps for its backward pass (in `saved`; without one it needs
+ * orda_attention_saved_bytes(p, with_documents, 0) of it as a workspace). */
+size_t orda_attention_saved_bytes(const orda_attention_t* p, int32_t with_documents, int32_t training);
+int orda_attention_forward(const orda_attention_t* p, const void* q, const void* k, const void* v, const float* slopes,
+                           const int32_t* documents, const int32_t* prefix, void* out, void* saved, size_t saved_bytes,
+                           int32_t training, void* stream);
+size_t orda_attention_workspace_bytes(const orda_attention_t* p); /* backward */
+int orda_attention_backward(const orda_attention_t* p, const void* q, const void* k, const void* v, const float* slopes,
+                            int32_t with_documents, const int32_t* prefix, const void* out, const void* saved,
+                            size_t saved_bytes, const void* grad_output, void* grad_q, void* grad_k, void* grad_v,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 /* Per-kernel-class timing, for benchmarks.  No counterpart in the reference,
  * whose benchmarks bracket whole steps with torch.cuda.Event
  * (test/benchmark/src/_train.py:410-419); this hook brackets each launch

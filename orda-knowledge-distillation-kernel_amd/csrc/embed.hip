@@ -1,0 +1,382 @@
+// embed.hip -- the token embedding: rows of the weight, scaled, and the
+// weight's gradient by sorted tokens.
+//
+// Forward: y[n] = scale W[t_n], one piece of 8 columns a thread, bound by
+// memory.  A token outside [0, V) gives a row of zeros and no gradient.
+//
+// Backward: dW[v] = scale sum of dy[n] over t_n = v, and zeros in all other
+// rows (most of the bytes with a large vocabulary).  Four launches:
+//   sort   segments of 4096 tokens, each by one workgroup in LDS (radix, 8 bits
+//          a pass, stable); the other workgroups fill dW with zeros meanwhile
+//   merge  up to 16 sorted segments a round: an element's place is the sum of
+//          its places in the others, found by 16 searches side by side (more
+//          than 4096 tokens)
+//   sum    a wave takes 512 columns of `chunk` sorted entries and adds up their
+//          rows of dy in fp32; a run of one token that lies in the chunk goes
+//          out rounded, one that reaches past it as an fp32 partial sum
+//   join   the partial sums of such runs, in order
+// Equal tokens stay in their order throughout, so the sums do not depend on the
+// run, and a token that fills the batch is added up by as many waves as any
+// other.
+#include <algorithm>
+
+#include "epilogue.hpp"
+#include "step_launch.hpp"
+
+namespace orda {
+
+__device__ __forceinline__ int64_t token_at(const void* ids, int wide, int64_t i) {
+  return wide ? static_cast<const int64_t*>(ids)[i] : (int64_t) static_cast<const int32_t*>(ids)[i];
+}
+
+// ------------------------------------------------------------- forward
+template <class W, class T>
+__global__ __launch_bounds__(256) void k_embed(EmbedParams P, int64_t per_row, int64_t pieces) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = pieces <= 0xffffffffll ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row;
+    const int64_t c = (i - row * per_row) * 8;
+    const int cnt = (int)lmin(8, P.hidden - c);
+    const int64_t t = token_at(P.ids, P.wide, row);
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (t >= 0 && t < P.vocab) {
+      ld_row<W, 8>(static_cast<const W*>(P.weight) + t * P.ldw + c, v, cnt);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= P.scale;
+    }
+    st_row<T, 8>(static_cast<T*>(P.y) + row * P.hidden + c, v, cnt);
+  }
+}
+
+// ------------------------------------------------------------- sort
+constexpr int kSegment = 4096;  // tokens of one workgroup
+
+// Keys: the token, V for one that has no gradient (it sorts behind all others).
+// Entries past the last token have all bits set and stay behind them.
+__global__ __launch_bounds__(1024) void k_embed_sort(EmbedGradParams P, int passes, int segments, uint32_t* tokens, uint32_t* places, int64_t fill_bytes) {
+  if ((int)blockIdx.x >= segments) {
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    const int64_t n = fill_bytes / 16, step = (int64_t)(gridDim.x - segments) * 1024;
+    const int64_t at = (int64_t)(blockIdx.x - segments) * 1024 + threadIdx.x;
+    uint4* out = static_cast<uint4*>(P.dw);
+    for (int64_t i = at; i < n; i += step) out[i] = zero;
+    const int64_t tail = (fill_bytes % 16) / 2;  // (elements of 2 or 4 bytes)
+    if (at < tail) reinterpret_cast<uint16_t*>(out + n)[at] = 0;
+    return;
+  }
+  __shared__ uint32_t key[2][kSegment];
+  __shared__ uint16_t from[2][kSegment];
+  __shared__ uint32_t hist[16][256];
+  __shared__ uint32_t total[16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t base = (int64_t)blockIdx.x * kSegment;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = w * 256 + i * 64 + lane;
+    uint32_t k = 0xffffffffu;
+    if (base + at < P.tokens) {
+      const int64_t t = token_at(P.ids, P.wide, base + at);
+      k = t >= 0 && t < P.vocab && t != P.padding ? (uint32_t)t : (uint32_t)P.vocab;
+    }
+    key[0][at] = k;
+    from[0][at] = (uint16_t)at;
+  }
+  int cur = 0;
+  for (int pass = 0; pass < passes; ++pass, cur ^= 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(hist)[threadIdx.x + 1024 * i] = 0;
+    __syncthreads();
+    // a key's rank among the keys of its wave's 256 with the same digit: those
+    // of earlier rows of 64 (counted in hist), and of lower lanes
+    uint32_t k[4], rank[4];
+    uint16_t f[4];
+    volatile uint32_t* mine = hist[w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = w * 256 + i * 64 + lane;
+      k[i] = key[cur][at];
+      f[i] = from[cur][at];
+      const uint32_t d = (k[i] >> (8 * pass)) & 255u;
+      uint64_t same = ~0ull;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        const uint64_t m = __ballot((d >> b) & 1);
+        same &= (d >> b) & 1 ? m : ~m;
+      }
+      const uint32_t before = __popcll(same & ((1ull << lane) - 1)), old = mine[d];
+      rank[i] = old + before;
+      __builtin_amdgcn_wave_barrier();
+      if (before == 0) mine[d] = old + (uint32_t)__popcll(same);
+      __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    // exclusive sums over digits, within a digit over waves: 4 waves a thread
+    const int d = threadIdx.x >> 2, q = (threadIdx.x & 3) * 4;
+    uint32_t c[4], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c[j] = hist[q + j][d];
+      sum += c[j];
+    }
+    uint32_t run = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t up = __shfl_up(run, o);
+      if (lane >= o) run += up;
+    }
+    if (lane == 63) total[w] = run;
+    __syncthreads();
+    run -= sum;
+    for (int i = 0; i < w; ++i) run += total[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      hist[q + j][d] = run;
+      run += c[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t to = hist[w][(k[i] >> (8 * pass)) & 255u] + rank[i];
+      key[cur ^ 1][to] = k[i];
+      from[cur ^ 1][to] = f[i];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = threadIdx.x + 1024 * i;
+    if (base + at < P.tokens) {
+      tokens[base + at] = key[cur][at];
+      places[base + at] = (uint32_t)(base + from[cur][at]);
+    }
+  }
+}
+
+// Groups of 16 sorted segments of `len` (a power of two) entries to one each.
+__global__ __launch_bounds__(256) void k_embed_merge(const uint32_t* tokens, const uint32_t* places, uint32_t* tokens_out, uint32_t* places_out, int64_t n, int64_t len) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= n) return;
+  const uint32_t t = tokens[e];
+  const int64_t group = e / (16 * len) * (16 * len);
+  const int own = (int)((e - group) / len);
+  int64_t pos[16];
+#pragma unroll
+  for (int b = 0; b < 16; ++b) pos[b] = 0;
+  for (int64_t s = len; s > 0; s >>= 1) {
+#pragma unroll
+    for (int b = 0; b < 16; ++b) {
+      const int64_t first = group + b * len, at = first + pos[b] + s - 1;
+      if (b == own || pos[b] + s > len || at >= n) continue;
+      const uint32_t v = tokens[at];
+      if (b < own ? v <= t : v < t) pos[b] += s;  // (equal ones of earlier segments come first)
+    }
+  }
+  int64_t to = group + (e - group - own * len);
+#pragma unroll
+  for (int b = 0; b < 16; ++b) to += b == own ? 0 : pos[b];
+  tokens_out[to] = t;
+  places_out[to] = places[e];
+}
+
+// ------------------------------------------------------------- sums
+struct EmbedSums {
+  const uint32_t* tokens;
+  const uint32_t* places;
+  float* part;  // [chunks][2][hidden]: of a run that began before the chunk, and of one that goes on behind it
+  int chunk;
+  int slabs;    // of 512 columns
+  int64_t chunks;
+};
+
+template <class W, class T>
+__global__ __launch_bounds__(256) void k_embed_sum(EmbedGradParams P, EmbedSums S) {
+  constexpr int kAhead = 8;  // rows in flight
+  const int lane = threadIdx.x & 63;
+  const int64_t units = S.chunks * S.slabs;
+  for (int64_t u = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < units; u += (int64_t)gridDim.x * 4) {
+    const int64_t chunk = u / S.slabs, first = chunk * S.chunk;
+    const int n = (int)lmin(S.chunk, P.tokens - first);
+    const int64_t c = (u - chunk * S.slabs) * 512 + lane * 8;
+    const int cnt = (int)(c < P.hidden ? lmin(8, P.hidden - c) : 0);
+    uint32_t tok = (uint32_t)P.vocab, place = 0;
+    if (lane < n) {
+      tok = S.tokens[first + lane];
+      place = S.places[first + lane];
+    }
+    const uint32_t before = first > 0 ? S.tokens[first - 1] : 0xffffffffu;
+    const uint32_t after = first + n < P.tokens ? S.tokens[first + n] : 0xffffffffu;
+    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    bool from_before = (uint32_t)__builtin_amdgcn_readlane((int)tok, 0) == before;
+    for (int i0 = 0; i0 < n; i0 += kAhead) {
+      RawRow<T, 8> v[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = i0 + k < n ? i0 + k : n - 1;
+        const int64_t row = (uint32_t)__builtin_amdgcn_readlane((int)place, i);
+        const bool has = i0 + k < n && (uint32_t)__builtin_amdgcn_readlane((int)tok, i) < (uint32_t)P.vocab;
+        v[k].load(static_cast<const T*>(P.dy) + row * P.ldg + c, has ? cnt : 0);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = i0 + k;
+        if (i >= n) break;
+        const uint32_t t = (uint32_t)__builtin_amdgcn_readlane((int)tok, i);
+        if (t >= (uint32_t)P.vocab) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] += v[k][e];
+        const bool last = i + 1 == n;
+        const uint32_t next = last ? after : (uint32_t)__builtin_amdgcn_readlane((int)tok, last ? i : i + 1);
+        if (!last && next == t) continue;
+        // the run's end in this chunk
+        if (from_before || next == t) {
+          if (cnt) st_row<float, 8>(S.part + (2 * chunk + (from_before ? 0 : 1)) * P.hidden + c, acc, cnt);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] *= P.scale;
+          if (cnt) st_row<W, 8>(static_cast<W*>(P.dw) + (int64_t)t * P.hidden + c, acc, cnt);
+        }
+        from_before = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
+      }
+    }
+  }
+}
+
+// A run that begins in chunk c and goes on: its sum in c and those of the
+// chunks that it reaches, every eighth of them by one wave.
+template <class W>
+__global__ __launch_bounds__(512) void k_embed_join(EmbedGradParams P, EmbedSums S) {
+  __shared__ float join[8][64][8];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t units = S.chunks * S.slabs;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int64_t chunk = u / S.slabs, first = chunk * S.chunk, end = first + S.chunk;
+    if (end >= P.tokens) continue;
+    const uint32_t t = S.tokens[end];
+    if (t >= (uint32_t)P.vocab || S.tokens[end - 1] != t) continue;
+    if (first > 0 && S.tokens[first] == t && S.tokens[first - 1] == t) continue;  // (it began before)
+    int64_t lo = end, hi = P.tokens;  // the last entry of the run: tokens[lo] == t, tokens[hi] > t
+    while (hi - lo > 1) {
+      const int64_t m = (lo + hi) / 2;
+      if (S.tokens[m] == t) lo = m;
+      else hi = m;
+    }
+    const int64_t more = lo / S.chunk - chunk;
+    const int64_t c = (u - chunk * S.slabs) * 512 + lane * 8;
+    const int cnt = (int)(c < P.hidden ? lmin(8, P.hidden - c) : 0);
+    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8];
+    if (w == 0) ld_row<float, 8>(S.part + (2 * chunk + 1) * P.hidden + c, acc, cnt);
+#pragma unroll 4
+    for (int64_t k = 1 + w; k <= more; k += 8) {
+      ld_row<float, 8>(S.part + 2 * (chunk + k) * P.hidden + c, v, cnt);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += v[e];
+    }
+    __syncthreads();  // (the turn before has read join)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) join[w][lane][e] = acc[e];
+    __syncthreads();
+    if (w) continue;
+#pragma unroll
+    for (int i = 1; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += join[i][lane][e];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= P.scale;
+    if (cnt) st_row<W, 8>(static_cast<W*>(P.dw) + (int64_t)t * P.hidden + c, acc, cnt);
+  }
+}
+
+// ------------------------------------------------------------- launches
+template <class W, class T>
+static hipError_t embed_go(const EmbedParams& P, hipStream_t s) {
+  const int64_t per_row = (P.hidden + 7) / 8, pieces = per_row * P.tokens;
+  hipLaunchKernelGGL((k_embed<W, T>), dim3((unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 23)), dim3(256), 0, s, P, per_row, pieces);
+  return hipGetLastError();
+}
+template <class W>
+static hipError_t embed_out(const EmbedParams& P, int out_dtype, hipStream_t s) {
+  switch (out_dtype) {
+    case DT_BF16: return embed_go<W, bf16>(P, s);
+    case DT_F16: return embed_go<W, f16>(P, s);
+    default: return embed_go<W, float>(P, s);
+  }
+}
+hipError_t launch_embed(const EmbedParams& P, int dtype, int out_dtype, hipStream_t s) {
+  switch (dtype) {
+    case DT_BF16: return embed_out<bf16>(P, out_dtype, s);
+    case DT_F16: return embed_out<f16>(P, out_dtype, s);
+    default: return embed_out<float>(P, out_dtype, s);
+  }
+}
+
+// Sorted entries of a wave's chunk: 32, fewer where that would leave less than
+// 16 waves to a CU.
+static EmbedSums sums_of(int64_t tokens, int64_t hidden) {
+  EmbedSums S{};
+  S.slabs = (int)((hidden + 511) / 512);
+  S.chunk = 32;
+  while (S.chunk > 4 && (tokens + S.chunk - 1) / S.chunk * S.slabs < 4096) S.chunk /= 2;
+  S.chunks = (tokens + S.chunk - 1) / S.chunk;
+  return S;
+}
+static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+static size_t list_bytes(int64_t tokens) { return up256((size_t)tokens * 4); }
+size_t embed_grad_workspace(int64_t tokens, int64_t hidden) {
+  const EmbedSums S = sums_of(tokens, hidden);
+  return list_bytes(tokens) * (tokens > kSegment ? 4 : 2) + up256((size_t)S.chunks * 2 * hidden * 4);
+}
+
+template <class W, class T>
+static hipError_t sum_go(const EmbedGradParams& P, const EmbedSums& S, hipStream_t s) {
+  const int64_t units = S.chunks * S.slabs;
+  hipLaunchKernelGGL((k_embed_sum<W, T>), dim3((unsigned)std::min<int64_t>((units + 3) / 4, 1 << 22)), dim3(256), 0, s, P, S);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || S.chunks == 1) return e;
+  hipLaunchKernelGGL((k_embed_join<W>), dim3((unsigned)std::min<int64_t>(units, 1 << 20)), dim3(512), 0, s, P, S);
+  return hipGetLastError();
+}
+template <class W>
+static hipError_t sum_out(const EmbedGradParams& P, const EmbedSums& S, int out_dtype, hipStream_t s) {
+  switch (out_dtype) {
+    case DT_BF16: return sum_go<W, bf16>(P, S, s);
+    case DT_F16: return sum_go<W, f16>(P, S, s);
+    default: return sum_go<W, float>(P, S, s);
+  }
+}
+
+hipError_t launch_embed_grad(const EmbedGradParams& P, int dtype, int out_dtype, void* workspace, hipStream_t s) {
+  EmbedSums S = sums_of(P.tokens, P.hidden);
+  const size_t list = list_bytes(P.tokens);
+  char* ws = static_cast<char*>(workspace);
+  uint32_t* tokens[2];
+  uint32_t* places[2];
+  const int lists = P.tokens > kSegment ? 2 : 1;
+  for (int i = 0; i < 2; ++i) {
+    tokens[i] = reinterpret_cast<uint32_t*>(ws + (i % lists) * 2 * list);
+    places[i] = reinterpret_cast<uint32_t*>(ws + (i % lists) * 2 * list + list);
+  }
+  S.part = reinterpret_cast<float*>(ws + lists * 2 * list);
+  int passes = 1;
+  while (passes < 4 && (P.vocab >> (8 * passes)) != 0) ++passes;
+  const int segments = (int)((P.tokens + kSegment - 1) / kSegment);
+  const int64_t bytes = P.vocab * P.hidden * (dtype == DT_F32 ? 4 : 2);
+  const int fill = (int)std::min<int64_t>(1024, (bytes + 65535) / 65536);
+  hipLaunchKernelGGL(k_embed_sort, dim3((unsigned)(segments + fill)), dim3(1024), 0, s, P, passes, segments, tokens[0], places[0], bytes);
+  hipError_t e = hipGetLastError();
+  int at = 0;
+  for (int64_t len = kSegment; e == hipSuccess && len < P.tokens; len *= 16, at ^= 1) {
+    hipLaunchKernelGGL(k_embed_merge, dim3((unsigned)((P.tokens + 255) / 256)), dim3(256), 0, s, tokens[at], places[at], tokens[at ^ 1], places[at ^ 1], P.tokens, len);
+    e = hipGetLastError();
+  }
+  if (e != hipSuccess) return e;
+  S.tokens = tokens[at];
+  S.places = places[at];
+  switch (dtype) {
+    case DT_BF16: return sum_out<bf16>(P, S, out_dtype, s);
+    case DT_F16: return sum_out<f16>(P, S, out_dtype, s);
+    default: return sum_out<float>(P, S, out_dtype, s);
+  }
+}
+
+}  // namespace orda

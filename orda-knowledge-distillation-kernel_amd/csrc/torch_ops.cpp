@@ -1,5 +1,6 @@
 // torch_ops.cpp -- the binding of orda_linear_*, orda_ffn_*, orda_grad_norm and
-// orda_clip_grads to torch: operands as the kernels read them, workspaces and
+// orda_clip_grads (and, in torch_step.hpp, of the embedding, dropout, layer norm
+// and attention) to torch: operands as the kernels read them, workspaces and
 // outputs from torch's allocator, autograd nodes, tables of gradients.  Host
 // code only; it reaches the C entry points through the addresses that
 // _native.py hands over, so one library is loaded.  Measured against the same
@@ -53,6 +54,17 @@ struct Api {
   decltype(&orda_grad_norm) grad_norm;
   decltype(&orda_clip_grads) clip_grads;
   decltype(&orda_clip_grad_norm) clip_grad_norm;
+  decltype(&orda_embedding_forward) embedding_forward;
+  decltype(&orda_embedding_workspace_bytes) embedding_workspace_bytes;
+  decltype(&orda_embedding_backward) embedding_backward;
+  decltype(&orda_dropout_add) dropout_add;
+  decltype(&orda_layer_norm_forward) layer_norm_forward;
+  decltype(&orda_layer_norm_workspace_bytes) layer_norm_workspace_bytes;
+  decltype(&orda_layer_norm_backward) layer_norm_backward;
+  decltype(&orda_attention_saved_bytes) attention_saved_bytes;
+  decltype(&orda_attention_forward) attention_forward;
+  decltype(&orda_attention_workspace_bytes) attention_workspace_bytes;
+  decltype(&orda_attention_backward) attention_backward;
 } api;
 
 void bind(const std::map<std::string, uintptr_t>& at) {
@@ -72,6 +84,17 @@ void bind(const std::map<std::string, uintptr_t>& at) {
   ORDA_BIND(grad_norm);
   ORDA_BIND(clip_grads);
   ORDA_BIND(clip_grad_norm);
+  ORDA_BIND(embedding_forward);
+  ORDA_BIND(embedding_workspace_bytes);
+  ORDA_BIND(embedding_backward);
+  ORDA_BIND(dropout_add);
+  ORDA_BIND(layer_norm_forward);
+  ORDA_BIND(layer_norm_workspace_bytes);
+  ORDA_BIND(layer_norm_backward);
+  ORDA_BIND(attention_saved_bytes);
+  ORDA_BIND(attention_forward);
+  ORDA_BIND(attention_workspace_bytes);
+  ORDA_BIND(attention_backward);
 #undef ORDA_BIND
 }
 
@@ -550,6 +573,8 @@ Tensor clip(const std::vector<Tensor>& params, double max_norm, double norm_type
   return total;
 }
 
+#include "torch_step.hpp"
+
 }  // namespace
 
 PYBIND11_MODULE(orda_torch, m) {
@@ -558,4 +583,8 @@ PYBIND11_MODULE(orda_torch, m) {
   m.def("feed_forward", &feed_forward);
   m.def("grad_norm", &grad_norm);
   m.def("clip", &clip);
+  m.def("embedding", &embedding);
+  m.def("dropout", &dropout);
+  m.def("layer_norm", &layer_norm);
+  m.def("attention", &attention);
 }

@@ -21,7 +21,7 @@ __all__ = [
     "saved_bytes", "forward_workspace_bytes", "backward_workspace_bytes", "gemm_abt", "gemm",
     "MODE", "DTYPE", "FLAG", "KERNEL_CLASSES", "timing_enable", "timing_collect",
     "ACTIVATION", "Linear", "FeedForward", "torch_ops", "linear_plan",
-    "feed_forward_plan",
+    "feed_forward_plan", "Embedding", "Dropout", "RowsProblem", "LayerNorm", "Attention",
 ]
 
 ABI_VERSION = 4
@@ -167,6 +167,46 @@ class Rows(ctypes.Structure):
     ]
 
 
+class Embedding(ctypes.Structure):
+    """orda_embedding_t"""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "dtype", "out_dtype", "wide_ids")] + [
+        (n, ctypes.c_int64) for n in ("tokens", "vocab", "hidden", "ldw", "ldg", "padding_idx")
+    ] + [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class Dropout(ctypes.Structure):
+    """orda_dropout_t"""
+
+    _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("seed_on_device", ctypes.c_void_p), ("site", ctypes.c_uint64)]
+
+
+class RowsProblem(ctypes.Structure):
+    """orda_rows_problem_t"""
+
+    _fields_ = [("abi_version", ctypes.c_int32), ("dtype", ctypes.c_int32)] + [
+        (n, ctypes.c_int64) for n in ("rows", "cols", "ldx", "ldr")
+    ]
+
+
+class LayerNorm(ctypes.Structure):
+    """orda_layer_norm_t"""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "dtype", "param_dtype")] + [("eps", ctypes.c_float)] + [
+        (n, ctypes.c_int64) for n in ("rows", "cols", "ldx", "ldr", "ld_s", "ld_dy", "ld_ds")
+    ]
+
+
+class Attention(ctypes.Structure):
+    """orda_attention_t"""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "dtype", "heads", "kv_heads", "head_dim", "causal")] + [
+        ("batch", ctypes.c_int64), ("length", ctypes.c_int64)
+    ] + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "g_stride")] + [
+        ("documents_stride", ctypes.c_int64), ("scale", ctypes.c_double), ("softcap", ctypes.c_double)
+    ]
+
+
 _LOCK = threading.Lock()
 _LIB = None
 
@@ -245,6 +285,19 @@ def library() -> ctypes.CDLL:
         lib.orda_clip_grad_norm.argtypes = [vp, ctypes.c_int64, ctypes.c_double, ctypes.c_double, vp, vp, sz, vp]
         lib.orda_clip_grads.restype = ctypes.c_int
         lib.orda_clip_grads.argtypes = [vp, ctypes.c_int64, vp, ctypes.c_double, vp]
+        E, D, R, N, A = (ctypes.POINTER(c) for c in (Embedding, Dropout, RowsProblem, LayerNorm, Attention))
+        i32 = ctypes.c_int32
+        for name, args in (("orda_embedding_forward", [E] + [vp] * 4), ("orda_embedding_backward", [E] + [vp] * 4 + [sz, vp]),
+                           ("orda_dropout_add", [R, D] + [vp] * 4), ("orda_layer_norm_forward", [N, D] + [vp] * 8),
+                           ("orda_layer_norm_backward", [N, D] + [vp] * 11 + [sz, vp]),
+                           ("orda_attention_forward", [A] + [vp] * 8 + [sz, i32, vp]),
+                           ("orda_attention_backward", [A] + [vp] * 4 + [i32] + [vp] * 3 + [sz] + [vp] * 5 + [sz, vp])):
+            fn = getattr(lib, name)
+            fn.restype, fn.argtypes = ctypes.c_int, args
+        for name, args in (("orda_embedding_workspace_bytes", [E]), ("orda_layer_norm_workspace_bytes", [N]),
+                           ("orda_attention_saved_bytes", [A, i32, i32]), ("orda_attention_workspace_bytes", [A])):
+            fn = getattr(lib, name)
+            fn.restype, fn.argtypes = sz, args
         lib.orda_timing_enable.restype = ctypes.c_int
         lib.orda_timing_enable.argtypes = [ctypes.c_int]
         lib.orda_timing_collect.restype = ctypes.c_int
@@ -406,12 +459,14 @@ _TORCH_API = (
     "orda_last_error", "orda_pad_rows", "orda_linear_saved_bytes", "orda_linear_workspace_bytes", "orda_linear_forward",
     "orda_linear_backward", "orda_ffn_inner_pitch", "orda_ffn_saved_bytes", "orda_ffn_workspace_bytes",
     "orda_ffn_forward", "orda_ffn_backward", "orda_grad_norm_workspace_bytes", "orda_grad_norm", "orda_clip_grads",
-    "orda_clip_grad_norm",
+    "orda_clip_grad_norm", "orda_embedding_forward", "orda_embedding_workspace_bytes", "orda_embedding_backward",
+    "orda_dropout_add", "orda_layer_norm_forward", "orda_layer_norm_workspace_bytes", "orda_layer_norm_backward",
+    "orda_attention_saved_bytes", "orda_attention_forward", "orda_attention_workspace_bytes", "orda_attention_backward",
 )
 
 
 def torch_ops():
-    """The native binding of the layers and the gradient norm (``_lib/orda_torch.so``, built from ``csrc/torch_ops.cpp``),
+    """The native binding of the layers, the other operators of a student's step and the gradient norm (``_lib/orda_torch.so``, built from ``csrc/torch_ops.cpp``),
     loaded once and given the loaded library's entry points; RuntimeError if it cannot be loaded."""
     global _TORCH_OPS
     if _TORCH_OPS is not None:

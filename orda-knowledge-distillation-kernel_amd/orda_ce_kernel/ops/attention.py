@@ -1,0 +1,118 @@
+"""Masked self-attention.
+
+    z = scale q.k;  cap tanh(z / cap);  less slope_h |i - j|;      P = softmax over the keys that a query sees;      o = P v
+    dv = P^T do      dz = P (do v^T - sum(do o))      dq = scale dz k      dk = scale dz^T q
+
+One kernel forward, two backward, on the matrix cores, with the softmax in one pass over the keys; scores never reach
+memory, and tiles that no query sees are not read (csrc/attn.hpp).  No counterpart in the reference, whose models use torch.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from .. import _native
+from .._runtime import default_compute_dtype
+from ._layers import check_shape, check_tensors, needs_function, use_kernels
+
+__all__ = ["masked_attention"]
+
+
+def _seen(B, S, causal, documents, prefix, device):
+    """(B, S, S): whether query i sees key j."""
+    at = torch.arange(S, device=device)
+    seen = torch.ones(B, S, S, dtype=torch.bool, device=device)
+    if causal:
+        seen = (at[:, None] >= at[None]).expand(B, S, S)
+        if prefix is not None:
+            seen = seen | (at[None, None] < prefix[:, None, None])
+    if documents is not None:
+        seen = seen & (documents[:, :, None] == documents[:, None]) & (documents >= 0)[:, :, None]
+    return seen
+
+
+def _torch(q, k, v, causal, scale, softcap, slopes, documents, prefix, dtype):
+    B, S, H, D = q.shape
+    G = H // k.shape[2]
+    seen = _seen(B, S, causal, documents, prefix, q.device)[:, None]
+    if documents is not None:  # (padding rows may hold anything)
+        real = (documents >= 0)[:, :, None, None]
+        q, k, v = (torch.where(real, t, torch.zeros((), dtype=t.dtype, device=t.device)) for t in (q, k, v))
+    qf = q.to(dtype).float().transpose(1, 2)
+    kf, vf = (t.to(dtype).float().transpose(1, 2).repeat_interleave(G, 1) for t in (k, v))
+    z = torch.matmul(qf, kf.transpose(2, 3).contiguous()) * scale
+    if softcap:
+        z = softcap * torch.tanh(z / softcap)
+    if slopes is not None:
+        at = torch.arange(S, device=q.device)
+        z = z - slopes.view(1, H, 1, 1) * (at[:, None] - at[None]).abs()
+    some = seen.any(-1, keepdim=True)
+    z = torch.where(seen, z, -math.inf)
+    p = torch.softmax(torch.where(some, z, 0.0), -1)
+    return torch.matmul(torch.where(some, p, 0.0), vf).transpose(1, 2).to(dtype)
+
+
+def _integers(entry, name, t, shape, device):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{entry}: {name} must be an int32 or int64 tensor, got {getattr(t, 'dtype', type(t).__name__)}")
+    check_shape(entry, name, t, shape)
+    if t.device != device:
+        raise ValueError(f"{entry}: {name} is on {t.device}, q on {device}")
+    return t.clamp(-1, 2**31 - 1).to(torch.int32).contiguous() if t.dtype == torch.int64 else t.contiguous()
+
+
+@torch._dynamo.disable
+def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = True, scale: float | None = None,
+                     softcap: float = 0.0, slopes: torch.Tensor | None = None, documents: torch.Tensor | None = None,
+                     prefix: torch.Tensor | None = None, backend: str = "auto") -> torch.Tensor:
+    """Self-attention over whole sequences, with its backward pass.
+
+    ``q`` is ``(batch, length, heads, head_dim)``, ``k`` and ``v`` ``(batch, length, kv_heads, head_dim)`` with ``heads`` a
+    multiple of ``kv_heads`` (query head h reads head ``h // (heads // kv_heads)``); slices of one projection's output serve
+    as they are.  The result is ``(batch, length, heads, head_dim)``.  ``scale`` (default ``head_dim ** -0.5``) multiplies the
+    products; ``softcap`` > 0 caps them to ``softcap * tanh(z / softcap)``; ``slopes`` (``(heads,)``) takes ``slopes[h] *
+    |i - j|`` off.  ``causal``: query i sees the keys up to i, and with ``prefix`` (``(batch,)``) also those below
+    ``prefix[b]``.  ``documents`` (``(batch, length)``): only keys with the query's own number; a negative number is padding,
+    which sees nothing and is not seen, whatever it holds: zeros come out, and zero gradients.
+
+    On the kernels bf16 and fp16 with head_dim up to 128 (multiples of 8 are read in place, others are copied).  The compute
+    dtype is the loss's rule; fp32 tensors run on ``backend="torch"`` or under autocast.  Probabilities and their gradients
+    are rounded to the compute dtype as operands of products; sums are fp32.  A non-finite value in a row that a query does
+    not see may still reach it where both are in one tile of 64 rows (padding excepted).  Once differentiable, in q, k and v.
+    ``backend`` as :func:`distillation_loss` has it."""
+    entry = "masked_attention"
+    check_tensors(entry, "none", q, k=k, v=v, slopes=slopes)
+    if q.ndim != 4:
+        raise ValueError(f"{entry}: q must have shape (batch, length, heads, head_dim), got {tuple(q.shape)}")
+    B, S, H, D = q.shape
+    if k.ndim != 4 or k.shape[2] == 0 or H % k.shape[2] != 0:
+        raise ValueError(f"{entry}: k must have shape ({B}, {S}, kv_heads, {D}) with kv_heads a divisor of {H}, got {tuple(k.shape)}")
+    check_shape(entry, "k", k, (B, S, k.shape[2], D))
+    check_shape(entry, "v", v, k.shape)
+    check_shape(entry, "slopes", slopes, (H,))
+    if slopes is not None and slopes.requires_grad:
+        raise ValueError(f"{entry}: slopes are constants; they have no gradient")
+    documents = _integers(entry, "documents", documents, (B, S), q.device)
+    prefix = _integers(entry, "prefix", prefix, (B,), q.device)
+    if prefix is not None and not causal:
+        raise ValueError(f"{entry}: prefix widens the causal mask; it needs causal=True")
+    scale = D ** -0.5 if scale is None else float(scale)
+    softcap = float(softcap)
+    if not math.isfinite(scale):
+        raise ValueError(f"{entry}: scale must be finite, got {scale}")
+    if not (softcap >= 0.0 and math.isfinite(softcap)):
+        raise ValueError(f"{entry}: softcap must be finite and >= 0, got {softcap}")
+    kernels = use_kernels(backend, q, entry)
+    dtype = default_compute_dtype(q, k, v)
+    slopes = None if slopes is None else slopes.detach().float().contiguous()
+    if not kernels or q.numel() == 0:
+        return _torch(q, k, v, causal, scale, softcap, slopes, documents, prefix, dtype)
+    if dtype == torch.float32:
+        raise ValueError(f"{entry}: the kernels take bfloat16 and float16; cast, use autocast, or pass backend='torch'")
+    if D > 128:
+        raise ValueError(f"{entry}: the kernels take head_dim up to 128, got {D}; pass backend='torch'")
+    return _native.torch_ops().attention(q, k, v, slopes, documents, prefix, bool(causal), scale, softcap, dtype,
+                                         needs_function(q, k, v))
