@@ -46,28 +46,50 @@ __device__ __forceinline__ int attn_swz(int r) {
   return HD == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
 }
 
+// Workgroup -> (head of the batch, tile of its rows).  An XCD takes whole heads,
+// so that its L2 holds their keys and values.  With a causal mask a tile's work
+// grows (or falls) with its number: of 8 heads of an XCD together the longest
+// tiles come first, so that the last to end are short ones.
+__device__ __forceinline__ void attn_place(const AttnParams& P, int heads, bool last_first, int& head, int& tile) {
+  constexpr int kTogether = 8;
+  if (P.causal && heads % 8 == 0) {
+    const int per = heads / 8, local = blockIdx.x / 8;
+    const int g = local / (kTogether * P.tiles) * kTogether, n = min(kTogether, per - g), in = local - g * P.tiles;
+    head = blockIdx.x % 8 * per + g + in % n;
+    tile = in / n;
+  } else {
+    const int t = xcd_order(blockIdx.x, gridDim.x);
+    head = t / P.tiles;
+    tile = t - head * P.tiles;
+  }
+  if (last_first) tile = P.tiles - 1 - tile;
+}
+
 // A tile of 64 rows to LDS, 16 bytes a lane.  Rows from `rows` on and columns
 // from D on arrive as zeros.
-template <int HD>
+template <int HD, int WAVES = 4>
 struct AttnDma {
-  static constexpr int kChunks = HD / 8, kIssues = 64 * kChunks / 256, kStep = 256 / kChunks;
-  uint32_t off, step;
+  static constexpr int kChunks = HD / 8, kIssues = kChunks / WAVES, kStep = 64 * WAVES / kChunks;
+  static_assert(kIssues > 0 && kStep % 16 == 0, "rows kStep apart have one swizzle");
+  uint32_t off[kIssues];
   int row;
-  bool in;
   __device__ __forceinline__ void init(int64_t ss, int D) {
     const int p = wave_id() * 64 + (threadIdx.x & 63);
     row = p / kChunks;
-    const int c = (p % kChunks) ^ attn_swz<HD>(row);  // (rows kStep apart have one swizzle)
-    in = c * 8 < D;
-    off = (uint32_t)row * (uint32_t)(ss * 2) + (uint32_t)c * 16;
-    step = (uint32_t)kStep * (uint32_t)(ss * 2);
+    const int c = (p % kChunks) ^ attn_swz<HD>(row);
+#pragma unroll
+    for (int i = 0; i < kIssues; ++i) off[i] = c * 8 < D ? (uint32_t)(row + i * kStep) * (uint32_t)(ss * 2) + (uint32_t)c * 16 : kOob;
   }
-  __device__ __forceinline__ void issue(const void* p, int64_t rows, char* tile) const {
+  __device__ __forceinline__ void issue(const void* p, int rows, char* tile) const {
     const auto rs = rsrc_of(p);
     const int w = wave_id();
+    if (rows >= kAttnTile) {
 #pragma unroll
-    for (int i = 0; i < kIssues; ++i)
-      dma16(rs, in && row + i * kStep < rows ? off + i * step : kOob, tile + (i * 4 + w) * 1024);
+      for (int i = 0; i < kIssues; ++i) dma16(rs, off[i], tile + (i * WAVES + w) * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kIssues; ++i) dma16(rs, row + i * kStep < rows ? off[i] : kOob, tile + (i * WAVES + w) * 1024);
+    }
   }
 };
 
@@ -83,53 +105,69 @@ struct AttnFrags {
     lo = (uint32_t)(k * kRow + (((m >> 3) ^ attn_swz<HD>(k)) << 4) + (m & 7) * 2);
     hi = (uint32_t)((k + 8) * kRow + (((m >> 3) ^ attn_swz<HD>(k + 8)) << 4) + (m & 7) * 2);
   }
-  // rows 32 block + lane % 32, columns 16 ks + 8 (lane / 32)..
-  __device__ __forceinline__ typename Traits<T>::Frag rows(const char* tile, int block, int ks) const {
-    return *reinterpret_cast<const typename Traits<T>::Frag*>(tile + block * 32 * kRow + (row_at ^ (uint32_t)(ks << 5)));
+  // rows lane % 32 of the 32 at `block`, columns 16 ks + 8 (lane / 32)..
+  __device__ __forceinline__ typename Traits<T>::Frag rows(const char* block, int ks) const {
+    return *reinterpret_cast<const typename Traits<T>::Frag*>(block + (row_at ^ (uint32_t)(ks << 5)));
   }
-  // column 32 d + lane % 32 for all d, rows 16 KS + the permuted 8 of lane / 32
-  template <int KS>
-  __device__ __forceinline__ void cols(uint32_t tile, typename Traits<T>::Frag (&out)[kBlocks]) const {
-    constexpr int kOff = KS * 16 * kRow;
-    tr_s4 x[kBlocks][2];
+  // column 32 d + lane % 32 for all d, the 32 rows at LDS address `block` in two
+  // operands of 16 (of each the permuted 8 of lane / 32).  Assembly that waits
+  // for its own reads: the compiler's transposed read waits for the DMA too.
+  __device__ __forceinline__ void cols(uint32_t block, typename Traits<T>::Frag (&out)[2][kBlocks]) const {
+    constexpr int kOff = 16 * kRow;
+    const uint32_t a = block + lo, b = block + hi;  // (blocks are aligned: the exclusive or below stays in the row)
+    tr_s4 x[2][kBlocks][2];
     if constexpr (kBlocks == 4) {
       asm volatile(
-          "ds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\t"
-          "ds_read_b64_tr_b16 %2, %10 offset:%16\n\tds_read_b64_tr_b16 %3, %11 offset:%16\n\t"
-          "ds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
-          "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%16\n\t"
+          "ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %17\n\t"
+          "ds_read_b64_tr_b16 %2, %18\n\tds_read_b64_tr_b16 %3, %19\n\t"
+          "ds_read_b64_tr_b16 %4, %20\n\tds_read_b64_tr_b16 %5, %21\n\t"
+          "ds_read_b64_tr_b16 %6, %22\n\tds_read_b64_tr_b16 %7, %23\n\t"
+          "ds_read_b64_tr_b16 %8, %16 offset:%24\n\tds_read_b64_tr_b16 %9, %17 offset:%24\n\t"
+          "ds_read_b64_tr_b16 %10, %18 offset:%24\n\tds_read_b64_tr_b16 %11, %19 offset:%24\n\t"
+          "ds_read_b64_tr_b16 %12, %20 offset:%24\n\tds_read_b64_tr_b16 %13, %21 offset:%24\n\t"
+          "ds_read_b64_tr_b16 %14, %22 offset:%24\n\tds_read_b64_tr_b16 %15, %23 offset:%24\n\t"
           "s_waitcnt lgkmcnt(0)"
-          : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1]), "=&v"(x[2][0]), "=&v"(x[2][1]),
-            "=&v"(x[3][0]), "=&v"(x[3][1])
-          : "v"(tile + lo), "v"(tile + hi), "v"(tile + (lo ^ 64u)), "v"(tile + (hi ^ 64u)), "v"(tile + (lo ^ 128u)),
-            "v"(tile + (hi ^ 128u)), "v"(tile + (lo ^ 192u)), "v"(tile + (hi ^ 192u)), "n"(kOff)
+          : "=&v"(x[0][0][0]), "=&v"(x[0][0][1]), "=&v"(x[0][1][0]), "=&v"(x[0][1][1]), "=&v"(x[0][2][0]), "=&v"(x[0][2][1]),
+            "=&v"(x[0][3][0]), "=&v"(x[0][3][1]), "=&v"(x[1][0][0]), "=&v"(x[1][0][1]), "=&v"(x[1][1][0]), "=&v"(x[1][1][1]),
+            "=&v"(x[1][2][0]), "=&v"(x[1][2][1]), "=&v"(x[1][3][0]), "=&v"(x[1][3][1])
+          : "v"(a), "v"(b), "v"(a ^ 64u), "v"(b ^ 64u), "v"(a ^ 128u), "v"(b ^ 128u), "v"(a ^ 192u), "v"(b ^ 192u), "n"(kOff)
           : "memory");
     } else {
       asm volatile(
-          "ds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %5 offset:%8\n\t"
-          "ds_read_b64_tr_b16 %2, %6 offset:%8\n\tds_read_b64_tr_b16 %3, %7 offset:%8\n\t"
+          "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\t"
+          "ds_read_b64_tr_b16 %2, %10\n\tds_read_b64_tr_b16 %3, %11\n\t"
+          "ds_read_b64_tr_b16 %4, %8 offset:%12\n\tds_read_b64_tr_b16 %5, %9 offset:%12\n\t"
+          "ds_read_b64_tr_b16 %6, %10 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
           "s_waitcnt lgkmcnt(0)"
-          : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1])
-          : "v"(tile + lo), "v"(tile + hi), "v"(tile + (lo ^ 64u)), "v"(tile + (hi ^ 64u)), "n"(kOff)
+          : "=&v"(x[0][0][0]), "=&v"(x[0][0][1]), "=&v"(x[0][1][0]), "=&v"(x[0][1][1]), "=&v"(x[1][0][0]), "=&v"(x[1][0][1]),
+            "=&v"(x[1][1][0]), "=&v"(x[1][1][1])
+          : "v"(a), "v"(b), "v"(a ^ 64u), "v"(b ^ 64u), "n"(kOff)
           : "memory");
     }
 #pragma unroll
-    for (int d = 0; d < kBlocks; ++d)
-      out[d] = __builtin_bit_cast(typename Traits<T>::Frag, __builtin_shufflevector(x[d][0], x[d][1], 0, 1, 2, 3, 4, 5, 6, 7));
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d)
+        out[k][d] = __builtin_bit_cast(typename Traits<T>::Frag, __builtin_shufflevector(x[k][d][0], x[k][d][1], 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };
 
 // The wave's own 32 rows as operands: row lane % 32, columns 16 ks + 8 h.. .
+// negate: with their signs turned.
 template <class T, int HD>
-__device__ __forceinline__ void own_rows(const T* p, int64_t ss, int64_t row0, int64_t rows, int D, typename Traits<T>::Frag (&f)[HD / 16]) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = row0 + (lane & 31);
+__device__ __forceinline__ void own_rows(const T* p, int64_t ss, int row0, int rows, int D, typename Traits<T>::Frag (&f)[HD / 16], bool negate = false) {
+  const int lane = threadIdx.x & 63, r = row0 + (lane & 31);
   const T* at = p + r * ss + 8 * (lane >> 5);
+  const uint32_t turn = negate ? 0x80008000u : 0u;
 #pragma unroll
   for (int ks = 0; ks < HD / 16; ++ks) {
-    const bool in = r < rows && ks * 16 + 8 * (lane >> 5) < D;
-    const s16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-    f[ks] = in ? *reinterpret_cast<const typename Traits<T>::Frag*>(at + ks * 16) : __builtin_bit_cast(typename Traits<T>::Frag, zero);
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (r < rows && ks * 16 + 8 * (lane >> 5) < D) u = *reinterpret_cast<const uint4*>(at + ks * 16);
+    u.x ^= turn;
+    u.y ^= turn;
+    u.z ^= turn;
+    u.w ^= turn;
+    f[ks] = __builtin_bit_cast(typename Traits<T>::Frag, u);
   }
 }
 
@@ -189,13 +227,8 @@ __device__ __forceinline__ void store_own(const f32x16 (&acc)[HD / 32], float mu
 }
 
 // ------------------------------------------------------------- masks
-// The tiles [base, base + 64) of one side against the rows [r0, r0 + 128) of the
-// other: seen by any, with elements that are not seen, with padding rows.
-struct AttnTiles {
-  uint64_t seen, part, pad;
-};
-// What the workgroup's rows have of documents: the smallest and largest number
-// and whether there is padding.
+// What the workgroup's 128 rows have of documents: the smallest and largest
+// number and whether there is padding.
 struct DocRange {
   int lo, hi, pad;
   __device__ __forceinline__ void join(const int4& o) {
@@ -204,485 +237,692 @@ struct DocRange {
     pad |= o.z;
   }
 };
+// The tiles of the other side that a workgroup's rows meet, in order.  `part`:
+// each element has to be looked at; `pad`: some rows are padding.
+struct AttnTile {
+  int first;  // its first row, -1 behind the last tile
+  bool part, pad;
+  int head;   // (queries: of the heads that share the keys)
+};
 template <bool KEYS>  // the tiles are keys (else queries)
-__device__ __forceinline__ AttnTiles attn_tiles(const AttnParams& P, int base, int64_t r0, int64_t prefix, const int4* ranges, const DocRange& own) {
-  const int t = base + (threadIdx.x & 63);
-  const int64_t a = (int64_t)t * kAttnTile, b = lmin(a + kAttnTile, P.S), r1 = lmin(r0 + kAttnRows, P.S);  // [a, b) against [r0, r1)
-  bool seen = a < P.S, part = KEYS && a + kAttnTile > P.S, pad = false;
-  if (P.causal) {
-    const int64_t q0 = KEYS ? r0 : a, q1 = KEYS ? r1 : b, k0 = KEYS ? a : r0, k1 = KEYS ? b : r1;
-    if (k0 >= q1 && k0 >= prefix) seen = false;
-    if (k1 - 1 > q0 && k1 > prefix) part = true;
+struct AttnWalk {
+  int S, r0, prefix, causal, base;
+  int head, heads;  // the walk's turn, and how many
+  const int4* ranges;
+  DocRange own;
+  uint64_t seen, part, pad;
+  __device__ __forceinline__ void look() {
+    const int t = base + (threadIdx.x & 63);
+    const int a = t * kAttnTile, b = min(a + kAttnTile, S), r1 = min(r0 + kAttnRows, S);  // [a, b) against [r0, r1)
+    bool s = a < S, p = KEYS && a + kAttnTile > S, d = false;
+    if (causal) {
+      const int q0 = KEYS ? r0 : a, q1 = KEYS ? r1 : b, k0 = KEYS ? a : r0, k1 = KEYS ? b : r1;
+      if (k0 >= q1 && k0 >= prefix) s = false;
+      if (k1 - 1 > q0 && k1 > prefix) p = true;
+    }
+    if (ranges && s) {
+      const int4 v = ranges[t];
+      if (v.x > own.hi || v.y < own.lo) s = false;
+      if (v.x != v.y || own.lo != own.hi || v.x != own.lo || v.z || own.pad) p = true;
+      d = v.z != 0;
+    }
+    seen = __ballot(s);
+    part = __ballot(p);
+    pad = __ballot(d);
   }
-  if (ranges && seen) {
-    const int4 d = ranges[t];
-    if (d.x > own.hi || d.y < own.lo) seen = false;
-    if (d.x != d.y || own.lo != own.hi || d.x != own.lo || d.z || own.pad) part = true;
-    pad = d.z != 0;
+  __device__ __forceinline__ void init(const AttnParams& P, int b, int row0, int turns = 1) {
+    head = 0;
+    heads = turns;
+    S = (int)P.S;
+    r0 = row0;
+    causal = P.causal;
+    prefix = P.prefix ? P.prefix[b] : 0;
+    ranges = nullptr;
+    own = DocRange{0x7fffffff, -1, 0};
+    if (P.docs) {
+      ranges = P.ranges + (int64_t)b * (P.padded / kAttnTile);
+      own.join(ranges[r0 / kAttnTile]);
+      own.join(ranges[r0 / kAttnTile + 1]);
+    }
+    base = -64;
+    seen = 0;
   }
-  return {__ballot(seen), __ballot(seen && part), __ballot(seen && pad)};
-}
+  __device__ __forceinline__ AttnTile next() {
+    while (!seen) {
+      base += 64;
+      if (base * kAttnTile >= S) {
+        if (++head >= heads) {
+          head = heads;  // (stays behind the last)
+          base -= 64;
+          return {-1, false, false, 0};
+        }
+        base = 0;
+      }
+      look();
+    }
+    const int j = __builtin_ctzll(seen);
+    seen &= seen - 1;
+    return {(base + j) * kAttnTile, (bool)((part >> j) & 1), (bool)((pad >> j) & 1), head};
+  }
+};
 
 // Rows without a document: zeros in LDS, so that whatever they hold (nothing, for
 // what lies behind a batch's sequences) is not multiplied by a probability of 0.
 template <int HD>
 __device__ __forceinline__ void clear_padding(const int* docs, char* one, char* two) {
   constexpr int kChunks = HD / 8;
-  for (int p = threadIdx.x; p < kAttnTile * kChunks; p += 256)
+  for (int p = threadIdx.x; p < kAttnTile * kChunks; p += (int)blockDim.x)
     if (docs[p / kChunks] < 0) {
       reinterpret_cast<uint4*>(one)[p] = make_uint4(0, 0, 0, 0);
-      if (two) reinterpret_cast<uint4*>(two)[p] = make_uint4(0, 0, 0, 0);
+      reinterpret_cast<uint4*>(two)[p] = make_uint4(0, 0, 0, 0);
     }
   __syncthreads();
 }
 
-// Document numbers of the tile's rows that the lane's 16 elements of block
-// `block` belong to.
-__device__ __forceinline__ void tile_docs(const int* docs, int block, int (&d)[16]) {
-  const int h = (threadIdx.x & 63) >> 5;
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int4 v = *reinterpret_cast<const int4*>(docs + 32 * block + 8 * g + 4 * h);
-    d[4 * g] = v.x;
-    d[4 * g + 1] = v.y;
-    d[4 * g + 2] = v.z;
-    d[4 * g + 3] = v.w;
-  }
-}
-// The tile's row, relative to the tile, of element r of block `block`.
-__device__ __forceinline__ int tile_row(int block, int r) {
-  return 32 * block + (r >> 2) * 8 + ((threadIdx.x & 63) >> 5) * 4 + (r & 3);
-}
+// The row, relative to a block of 32, of element r of the lane's 16.
+__device__ __forceinline__ int block_row(int r) { return (r >> 2) * 8 + ((threadIdx.x & 63) >> 5) * 4 + (r & 3); }
 
-// Scores in units of log2 from products: z[r] = log2(e) (cap tanh(scale s / cap)
-// - slope |i - j|), and with CAP the tanh.  dist: the lane's row less the tile's
-// first.  tanh u = 1 - 2 / (1 + e^2u) on the hardware's exp2 and reciprocal, off
-// by 2e-7, a cap of 50 by 1e-5, below half a step of a 16-bit probability.
-template <bool CAP, bool BIAS>
-__device__ __forceinline__ void scores(const f32x16& s, float (&z)[16], float (&th)[16], const AttnParams& P, float slope, int dist, int block) {
+// z = -inf for what is not seen.  Keys in the rows: those below `bound` (behind
+// the query and its prefix, the sequence's end) are seen; queries in the rows:
+// those from `bound` on.  Relative to the block; docs: the numbers of its rows,
+// read by scalar loads (a vector load would wait for the DMA in flight), of which
+// the lower half of a wave compares four and the upper half the next four.
+template <bool KEYS>
+__device__ __forceinline__ void hide(f32x16& z, int bound, const int* docs, int doc) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    if constexpr (CAP) {
-      const float e = __builtin_amdgcn_exp2f(s[r] * P.cap_in);
-      th[r] = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e);
-      z[r] = th[r] * P.cap_out;
-    } else {
-      z[r] = s[r] * P.scale_log2;
+    const int row = block_row(r);
+    z[r] = (KEYS ? row < bound : row >= bound) ? z[r] : -kInf;
+  }
+  if (docs) {
+    const __attribute__((address_space(4))) int* d = (const __attribute__((address_space(4))) int*)(uintptr_t)docs;
+    const int own = doc < 0 ? -2 : doc;  // (padding sees nothing, padding neither)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int at = (r >> 2) * 8 + (r & 3);
+      const uint64_t low = __ballot(own == d[at]), high = __ballot(own == d[at + 4]);
+      const uint64_t seen = (low & 0xffffffffull) | (high & 0xffffffff00000000ull);
+      z[r] = __builtin_amdgcn_inverse_ballot_w64(seen) ? z[r] : -kInf;
     }
-    if constexpr (BIAS) z[r] = fmaf(-slope, fabsf((float)(dist - tile_row(block, r))), z[r]);
+  }
+}
+
+// Scores from products s = q.k.  Plain ones stay as they are, and what uses them
+// multiplies by mul = |scale| log2(e); capped or biased ones are formed here, in
+// units of log2 (mul = 1): log2(e) (cap tanh(scale s / cap) - slope |i - j|),
+// with CAP also the tanh.  dist: the lane's row less the block's first.
+// tanh u = 1 - 2 / (1 + e^2u) on the hardware's exp2 and reciprocal, off by 2e-7,
+// a cap of 50 by 1e-5, below half a step of a 16-bit probability.  (A negative
+// scale is turned over to one of the operands.)
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ void scores(f32x16& z, float (&th)[16], const AttnParams& P, float slope, int dist) {
+  if constexpr (CAP || BIAS) {
+    const float from = (float)(dist - block_row(0));  // (exact: lengths are below 2^24)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if constexpr (CAP) {
+        const float e = __builtin_amdgcn_exp2f(z[r] * P.cap_in);
+        th[r] = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e);
+        z[r] = th[r] * P.cap_out;
+      } else {
+        z[r] *= P.scale_log2;
+      }
+      if constexpr (BIAS) z[r] = fmaf(-slope, fabsf(from - (float)((r >> 2) * 8 + (r & 3))), z[r]);
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t lds_at(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
+
+// ------------------------------------------------------------- the pipeline
+// The walk over a workgroup's tiles, block by block of 32 rows, with the products
+// of the next block (`ahead`) in the same straight piece of code as the softmax
+// of this one, so that the matrix cores run under it.
+//
+// Operands that only `ahead` reads have two slots in LDS, those that the products
+// behind the softmax read too three.  Half way through a tile the workgroup
+// meets: then the next tile has arrived (it was sent for a tile earlier), and
+// nobody reads the tile before this one any more, nor this one's `ahead`
+// operands, so that the tile after the next goes there.
+//
+// f.issue(tile, n), f.ready(tile, n): the n-th tile sent for; arrived.
+// f.hidden(row): whether none of the wave's rows meets the 32 from `row` on.
+// f.ahead<BLOCK>(n): products of that block of the n-th tile, into the BLOCK-th
+// set of registers.  f.work<BLOCK>(tile, n, then): the block's softmax and what
+// follows, beside `ahead` of the next block, which is in the `then`-th tile
+// (behind the last tile: of what lies in LDS, unused).
+template <class F>
+__device__ __forceinline__ void attn_walk(AttnWalk<true>& walk, F& f) {
+  AttnTile t0 = walk.next();
+  if (t0.first < 0) return;
+  AttnTile t1 = walk.next();
+  f.issue(t0, 0);
+  if (t1.first >= 0) f.issue(t1, 1);
+  wait_vmem<0>();
+  tile_barrier();
+  f.ready(t0, 0);
+  if (t1.first >= 0) f.ready(t1, 1);
+  f.template ahead<0>(0);
+  bool sent = true;  // (the first two tiles have arrived)
+  for (int n = 0;; ++n) {
+    if (!f.hidden(t0.first)) f.template work<0>(t0, n, n);  // (blocks that are hidden are followed by none that are not)
+    AttnTile t2{-1, false, false, 0};
+    if (t1.first >= 0) {
+      t2 = walk.next();
+      wait_vmem<0>();
+      tile_barrier();
+      if (t2.first >= 0) f.issue(t2, n + 2);
+      if (!sent) f.ready(t1, n + 1);
+      sent = false;
+    }
+    if (!f.hidden(t0.first + 32)) f.template work<1>(t0, n, n + 1);
+    if (t1.first < 0) return;
+    t0 = t1;
+    t1 = t2;
+  }
+}
+
+// The same without products ahead, where the registers do not hold them and two
+// waves of a SIMD run beside each other: two slots, f.work<BLOCK>(tile, n).
+template <class F>
+__device__ __forceinline__ void attn_walk_plain(AttnWalk<true>& walk, F& f) {
+  AttnTile t = walk.next();
+  if (t.first < 0) return;
+  f.issue(t, 0);
+  for (int n = 0;; ++n) {
+    const AttnTile then = walk.next();
+    wait_vmem<0>();
+    tile_barrier();
+    if (then.first >= 0) f.issue(then, n + 1);
+    f.ready(t, n);
+    if (!f.hidden(t.first)) f.template work<0>(t, n);
+    if (!f.hidden(t.first + 32)) f.template work<1>(t, n);
+    if (then.first < 0) return;
+    t = then;
   }
 }
 
 // ------------------------------------------------------------- forward
 template <class T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void k_attn(AttnParams P) {
+struct AttnForward {
   using Frag = typename Traits<T>::Frag;
-  constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][kTile];
-  const int t = xcd_order(blockIdx.x, gridDim.x);
-  const int bh = t / P.tiles, q0 = (P.tiles - 1 - t % P.tiles) * kAttnRows;  // (long rows first)
-  const int b = bh / P.H, head = bh - b * P.H, kv = head / P.group;
-  const int lane = threadIdx.x & 63, w = wave_id();
-  const int64_t row0 = q0 + w * 32, i = row0 + (lane & 31);
-  const T* K = static_cast<const T*>(P.k) + b * P.kb + kv * P.kh;
-  const T* V = static_cast<const T*>(P.v) + b * P.vb + kv * P.vh;
-  Frag q[HD / 16];
-  own_rows<T, HD>(static_cast<const T*>(P.q) + b * P.qb + head * P.qh, P.qs, row0, P.S, P.D, q);
-  const int64_t prefix = P.prefix ? P.prefix[b] : 0;
-  const float slope = BIAS ? P.slopes[head] * kLog2e : 0.0f;
-  const int* docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
-  const int4* ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / kAttnTile) : nullptr;
-  DocRange own{0x7fffffff, -1, 0};
-  int doc = 0;
-  if (docs) {
-    own.join(ranges[q0 / kAttnTile]);
-    own.join(ranges[q0 / kAttnTile + 1]);
-    doc = docs[i];
-  }
+  static constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32, kHalf = kTile / 2;
+  const AttnParams& P;
+  char *klds, *vlds;  // two slots of K, three of V
+  const T *K, *V;
+  const int* docs;
   AttnDma<HD> kd, vd;
-  kd.init(P.ks, P.D);
-  vd.init(P.vs, P.D);
   AttnFrags<T, HD> fr;
-  fr.init();
-  const uint32_t base_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0][0];
-
+  Frag q[HD / 16], rows[HD / 16];
   f32x16 o[kBlocks];
+  f32x16 s[2];
+  float m, l, slope;
+  int row0, i, bound, doc, prefix;
+  __device__ __forceinline__ AttnForward(const AttnParams& p) : P(p) {}
+  __device__ __forceinline__ void issue(const AttnTile& t, int n) {
+    kd.issue(K + t.first * P.ks, (int)P.S - t.first, klds + (n & 1) * kTile);
+    vd.issue(V + t.first * P.vs, (int)P.S - t.first, vlds + (n % 3) * kTile);
+  }
+  __device__ __forceinline__ void ready(const AttnTile& t, int n) {
+    if (t.pad) clear_padding<HD>(docs + t.first, klds + (n & 1) * kTile, vlds + (n % 3) * kTile);
+  }
+  __device__ __forceinline__ bool hidden(int row) const { return P.causal && row > row0 + 31 && row >= prefix; }
+  template <int BLOCK>
+  __device__ __forceinline__ void fetch(int n) {
+    const char* kt = klds + (n & 1) * kTile + BLOCK * kHalf;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) rows[ks] = fr.rows(kt, ks);
+  }
+  template <int BLOCK>
+  __device__ __forceinline__ void products() {
+    f32x16& z = s[BLOCK];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) z = Traits<T>::mma(rows[ks], q[ks], z);
+  }
+  template <int BLOCK>
+  __device__ __forceinline__ void ahead(int n) {
+    fetch<BLOCK>(n);
+    products<BLOCK>();
+  }
+  template <int BLOCK>
+  __device__ __forceinline__ void work(const AttnTile& t, int n, int then) {
+    const int at = t.first + 32 * BLOCK;
+    f32x16& x = s[BLOCK];
+    fetch<1 - BLOCK>(then);
+    float th[16];
+    scores<CAP, BIAS>(x, th, P, slope, i - at);
+    if (t.part) hide<true>(x, bound - at, docs ? docs + at : nullptr, doc);
+    float top = fmaxf(x[0], x[1]);
+#pragma unroll
+    for (int r = 2; r < 16; ++r) top = fmaxf(top, x[r]);
+    top = halves_max(top);
+    const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
+    // The maximum follows only where it grows by more than 2^8: sums and products
+    // of probabilities up to 2^8 lose nothing in fp32.
+    if (__any(top * mul > m * mul + 8.0f)) {
+      const float to = fmaxf(m, top), by = to == -kInf ? 1.0f : __builtin_amdgcn_exp2f((m - to) * mul);
+      m = to;
+      l *= by;
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= by;
+    }
+    const float off = m == -kInf ? 0.0f : -m * mul;
+    products<1 - BLOCK>();
+    float p[16], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      p[r] = __builtin_amdgcn_exp2f(fmaf(x[r], mul, off));
+      sum[r & 1] += p[r];
+    }
+    l += sum[0] + sum[1];
+    // P is rounded to 16 bits as an operand of the product, its sum is not
+    Frag pf[2], vf[2][kBlocks];
+    as_operand<T>(p, pf);
+    fr.cols(lds_at(vlds) + (uint32_t)((n % 3) * kTile + BLOCK * kHalf), vf);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d) o[d] = Traits<T>::mma(vf[k][d], pf[k], o[d]);
+  }
+};
+
+template <class T, int HD, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void k_attn(AttnParams P) {
+  constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32;
+  __shared__ __attribute__((aligned(1024))) char lds[5 * kTile];
+  int bh, q0;
+  attn_place(P, P.B * P.H, true, bh, q0);
+  q0 *= kAttnRows;
+  const int b = bh / P.H, head = bh - b * P.H, kv = head / P.group;
+  const int lane = threadIdx.x & 63, S = (int)P.S;
+  AttnForward<T, HD, CAP, BIAS> f(P);
+  f.klds = lds;
+  f.vlds = lds + 2 * kTile;
+  f.row0 = q0 + wave_id() * 32;
+  f.i = f.row0 + (lane & 31);
+  f.K = static_cast<const T*>(P.k) + b * P.kb + kv * P.kh;
+  f.V = static_cast<const T*>(P.v) + b * P.vb + kv * P.vh;
+  f.slope = BIAS ? P.slopes[head] * kLog2e : 0.0f;
+  f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
+  f.doc = P.docs ? f.docs[f.i] : 0;
+  AttnWalk<true> walk;
+  walk.init(P, b, q0);
+  f.prefix = walk.prefix;
+  f.bound = P.causal ? min(S, max(f.i + 1, walk.prefix)) : S;
+  own_rows<T, HD>(static_cast<const T*>(P.q) + b * P.qb + head * P.qh, P.qs, f.row0, S, P.D, f.q, P.scale < 0.0f);
+  f.kd.init(P.ks, P.D);
+  f.vd.init(P.vs, P.D);
+  f.fr.init();
 #pragma unroll
   for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
-  float m = -kInf, l = 0.0f;
-  int stage = 0;
-  auto issue = [&](int tile, int st) {
-    const int64_t k0 = (int64_t)tile * kAttnTile;
-    kd.issue(K + k0 * P.ks, P.S - k0, lds[st][0]);
-    vd.issue(V + k0 * P.vs, P.S - k0, lds[st][1]);
-  };
-  const int all = (int)((P.S + kAttnTile - 1) / kAttnTile);
-  for (int base = 0; base < all; base += 64) {
-    AttnTiles tiles = attn_tiles<true>(P, base, q0, prefix, ranges, own);
-    if (!tiles.seen) continue;
-    int j = __builtin_ctzll(tiles.seen);
-    issue(base + j, stage);
-    while (true) {
-      const uint64_t rest = tiles.seen & (tiles.seen - 1);
-      const int next = rest ? __builtin_ctzll(rest) : -1;
-      wait_vmem<0>();
-      tile_barrier();
-      if (next >= 0) issue(base + next, stage ^ 1);
-      const int64_t k0 = (int64_t)(base + j) * kAttnTile;
-      const bool part = (tiles.part >> j) & 1;
-      if ((tiles.pad >> j) & 1) clear_padding<HD>(docs + k0, lds[stage][1], nullptr);
-      const bool hidden = P.causal && k0 > row0 + 31 && k0 >= prefix;  // (for this wave's rows)
-      if (!hidden) {
-        const char* kt = lds[stage][0];
-        const uint32_t vt = base_lds + (uint32_t)(stage * 2 + 1) * kTile;
-        float p[2][16], top = -kInf;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          f32x16 s;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = 0.0f;
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) s = Traits<T>::mma(fr.rows(kt, n, ks), q[ks], s);
-          float th[16];
-          scores<CAP, BIAS>(s, p[n], th, P, slope, (int)(i - k0), n);
-          if (part) {
-            int dk[16];
-            if (docs) tile_docs(docs + k0, n, dk);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int64_t key = k0 + tile_row(n, r);
-              bool see = key < P.S && (!P.causal || key <= i || key < prefix);
-              if (docs) see = see && dk[r] == doc && doc >= 0;
-              p[n][r] = see ? p[n][r] : -kInf;
-            }
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, p[n][r]);
-        }
-        top = halves_max(top);
-        // The maximum follows only where it grows by more than 2^8: sums and
-        // products of probabilities up to 2^8 lose nothing in fp32.
-        if (__any(top > m + 8.0f)) {
-          const float to = fmaxf(m, top), by = to == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - to);
-          m = to;
-          l *= by;
-#pragma unroll
-          for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] *= by;
-        }
-        const float at = m == -kInf ? 0.0f : m;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            p[n][r] = __builtin_amdgcn_exp2f(p[n][r] - at);
-            l += p[n][r];
-          }
-          // P is rounded to 16 bits as an operand of the product, its sum is not
-          Frag pf[2], vf[kBlocks];
-          as_operand<T>(p[n], pf);
-          static_for<0, 2>([&](auto k) {
-            constexpr int KS = decltype(k)::value;
-            if (n == 0) fr.template cols<KS>(vt, vf);
-            else fr.template cols<2 + KS>(vt, vf);
-#pragma unroll
-            for (int d = 0; d < kBlocks; ++d) o[d] = Traits<T>::mma(vf[d], pf[KS], o[d]);
-          });
-        }
-      }
-      stage ^= 1;
-      if (next < 0) break;
-      tiles.seen = rest;
-      j = next;
-    }
-  }
-  l = halves_sum(l);
+    for (int r = 0; r < 16; ++r) f.o[d][r] = 0.0f;
+  f.m = -kInf;
+  f.l = 0.0f;
+  attn_walk(walk, f);
+  const float l = halves_sum(f.l), mul = CAP || BIAS ? 1.0f : P.scale_log2;
   const bool empty = !(l > 0.0f) && l == l;
-  if (P.lse && lane < 32)
-    P.lse[(int64_t)bh * P.padded + i] = i >= P.S || empty ? kInf : m + __builtin_amdgcn_logf(l);
-  const int64_t at = ((b * P.S + i) * P.H + head) * P.D;
+  if (P.lse && lane < 32) P.lse[(int64_t)bh * P.padded + f.i] = f.i >= S || empty ? kInf : f.m * mul + __builtin_amdgcn_logf(l);
+  const int64_t at = (((int64_t)b * S + f.i) * P.H + head) * P.D;
   const float inv = empty ? 0.0f : 1.0f / l;
-  store_own<T, HD>(o, inv, static_cast<T*>(P.o) + at, P.D, i < P.S);
+  store_own<T, HD>(f.o, inv, static_cast<T*>(P.o) + at, P.D, f.i < S);
   // dz = P (dP - delta) cancels where P is near 1, and delta = sum(do o) would be
   // as far off as o's rounding: for the backward pass o is kept in both halves
   // (8 short rows: dq and dk off by 2.4e-3 of their norm instead of 3.4e-3 in bf16).
-  if (P.o_low) store_own<T, HD, true>(o, inv, static_cast<T*>(P.o_low) + at, P.D, i < P.S);
+  if (P.o_low) store_own<T, HD, true>(f.o, inv, static_cast<T*>(P.o_low) + at, P.D, f.i < S);
 }
 
 // ------------------------------------------------------------- dq
 // Also delta = sum(do o) of each query, which the next kernel reads.
 template <class T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void k_attn_dq(AttnParams P) {
+struct AttnGradQ {
   using Frag = typename Traits<T>::Frag;
-  constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][kTile];
-  const int t = xcd_order(blockIdx.x, gridDim.x);
-  const int bh = t / P.tiles, q0 = (P.tiles - 1 - t % P.tiles) * kAttnRows;
-  const int b = bh / P.H, head = bh - b * P.H, kv = head / P.group;
-  const int lane = threadIdx.x & 63, w = wave_id();
-  const int64_t row0 = q0 + w * 32, i = row0 + (lane & 31);
-  const T* K = static_cast<const T*>(P.k) + b * P.kb + kv * P.kh;
-  const T* V = static_cast<const T*>(P.v) + b * P.vb + kv * P.vh;
-  const int64_t prefix = P.prefix ? P.prefix[b] : 0;
-  const float slope = BIAS ? P.slopes[head] * kLog2e : 0.0f;
-  const int* docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
-  const int4* ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / kAttnTile) : nullptr;
-  DocRange own{0x7fffffff, -1, 0};
-  int doc = 0;
-  if (docs) {
-    own.join(ranges[q0 / kAttnTile]);
-    own.join(ranges[q0 / kAttnTile + 1]);
-    doc = docs[i];
-  }
+  static constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32, kHalf = kTile / 2;
+  const AttnParams& P;
+  char *klds, *vlds;  // two slots each
+  const T *K, *V;
+  const int* docs;
+  AttnDma<HD> kd, vd;
+  AttnFrags<T, HD> fr;
   Frag q[HD / 16], g[HD / 16];
-  own_rows<T, HD>(static_cast<const T*>(P.q) + b * P.qb + head * P.qh, P.qs, row0, P.S, P.D, q);
-  own_rows<T, HD>(static_cast<const T*>(P.dout) + b * P.gb + head * P.gh, P.gs, row0, P.S, P.D, g);
-  float delta = 0.0f;
+  f32x16 dq[kBlocks];
+  float lse, delta, slope;
+  int row0, i, bound, doc, prefix;
+  __device__ __forceinline__ AttnGradQ(const AttnParams& p) : P(p) {}
+  __device__ __forceinline__ void issue(const AttnTile& t, int n) {
+    kd.issue(K + t.first * P.ks, (int)P.S - t.first, klds + (n & 1) * kTile);
+    vd.issue(V + t.first * P.vs, (int)P.S - t.first, vlds + (n & 1) * kTile);
+  }
+  __device__ __forceinline__ void ready(const AttnTile& t, int n) {
+    if (t.pad) clear_padding<HD>(docs + t.first, klds + (n & 1) * kTile, vlds + (n & 1) * kTile);
+  }
+  __device__ __forceinline__ bool hidden(int row) const { return P.causal && row > row0 + 31 && row >= prefix; }
+  template <int BLOCK>
+  __device__ __forceinline__ void work(const AttnTile& t, int n) {
+    const int at = t.first + 32 * BLOCK;
+    const char *kt = klds + (n & 1) * kTile + BLOCK * kHalf, *vt = vlds + (n & 1) * kTile + BLOCK * kHalf;
+    f32x16 x, dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = dp[r] = 0.0f;
+    Frag krows[HD / 16], vrows[HD / 16];
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) krows[ks] = fr.rows(kt, ks);
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      x = Traits<T>::mma(krows[ks], q[ks], x);
+      vrows[ks] = fr.rows(vt, ks);
+    }
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) dp = Traits<T>::mma(vrows[ks], g[ks], dp);
+    float th[16];
+    scores<CAP, BIAS>(x, th, P, slope, i - at);
+    if (t.part) hide<true>(x, bound - at, docs ? docs + at : nullptr, doc);
+    const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
+    float z[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      z[r] = __builtin_amdgcn_exp2f(fmaf(x[r], mul, -lse)) * (dp[r] - delta);
+      if constexpr (CAP) z[r] *= 1.0f - th[r] * th[r];
+    }
+    Frag zf[2], kf[2][kBlocks];
+    as_operand<T>(z, zf);  // (dz in 16 bits, as an operand of the product)
+    fr.cols(lds_at(klds) + (uint32_t)((n & 1) * kTile + BLOCK * kHalf), kf);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d) dq[d] = Traits<T>::mma(kf[k][d], zf[k], dq[d]);
+  }
+};
+
+template <class T, int HD, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void k_attn_dq(AttnParams P) {
+  constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kTile];
+  int bh, q0;
+  attn_place(P, P.B * P.H, true, bh, q0);
+  q0 *= kAttnRows;
+  const int b = bh / P.H, head = bh - b * P.H, kv = head / P.group;
+  const int lane = threadIdx.x & 63, S = (int)P.S;
+  AttnGradQ<T, HD, CAP, BIAS> f(P);
+  f.klds = lds;
+  f.vlds = lds + 2 * kTile;
+  f.row0 = q0 + wave_id() * 32;
+  f.i = f.row0 + (lane & 31);
+  f.K = static_cast<const T*>(P.k) + b * P.kb + kv * P.kh;
+  f.V = static_cast<const T*>(P.v) + b * P.vb + kv * P.vh;
+  f.slope = BIAS ? P.slopes[head] * kLog2e : 0.0f;
+  f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
+  f.doc = P.docs ? f.docs[f.i] : 0;
+  own_rows<T, HD>(static_cast<const T*>(P.dout) + b * P.gb + head * P.gh, P.gs, f.row0, S, P.D, f.g);
   {
-    Frag o[HD / 16], low[HD / 16];
-    const int64_t at = (b * P.S * P.H + head) * P.D;
-    own_rows<T, HD>(static_cast<const T*>(P.o) + at, P.H * P.D, row0, P.S, P.D, o);
-    own_rows<T, HD>(static_cast<const T*>(P.o_low) + at, P.H * P.D, row0, P.S, P.D, low);
+    typename Traits<T>::Frag o[HD / 16];
+    const int64_t at = ((int64_t)b * S * P.H + head) * P.D;
+    f.delta = 0.0f;
 #pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks)
+    for (int part = 0; part < 2; ++part) {
+      own_rows<T, HD>(static_cast<const T*>(part ? P.o_low : P.o) + at, P.H * P.D, f.row0, S, P.D, o);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta = fmaf(to_f32(g[ks][e]), to_f32(o[ks][e]) + to_f32(low[ks][e]), delta);
-    delta = halves_sum(delta);
-    if (doc < 0) delta = 0.0f;
-    if (lane < 32) P.delta[(int64_t)bh * P.padded + i] = delta;
+      for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f.delta = fmaf(to_f32(f.g[ks][e]), to_f32(o[ks][e]), f.delta);
+    }
+    f.delta = f.doc < 0 ? 0.0f : halves_sum(f.delta);
+    if (lane < 32) P.delta[(int64_t)bh * P.padded + f.i] = f.delta;
   }
   if (!P.dq) return;
-  const float lse = P.lse[(int64_t)bh * P.padded + i];
-  AttnDma<HD> kd, vd;
-  kd.init(P.ks, P.D);
-  vd.init(P.vs, P.D);
-  AttnFrags<T, HD> fr;
-  fr.init();
-  const uint32_t base_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0][0];
-  f32x16 dq[kBlocks];
+  f.lse = P.lse[(int64_t)bh * P.padded + f.i];
+  AttnWalk<true> walk;
+  walk.init(P, b, q0);
+  f.prefix = walk.prefix;
+  f.bound = P.causal ? min(S, max(f.i + 1, walk.prefix)) : S;
+  own_rows<T, HD>(static_cast<const T*>(P.q) + b * P.qb + head * P.qh, P.qs, f.row0, S, P.D, f.q, P.scale < 0.0f);
+  f.kd.init(P.ks, P.D);
+  f.vd.init(P.vs, P.D);
+  f.fr.init();
 #pragma unroll
   for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dq[d][r] = 0.0f;
-  int stage = 0;
-  auto issue = [&](int tile, int st) {
-    const int64_t k0 = (int64_t)tile * kAttnTile;
-    kd.issue(K + k0 * P.ks, P.S - k0, lds[st][0]);
-    vd.issue(V + k0 * P.vs, P.S - k0, lds[st][1]);
-  };
-  const int all = (int)((P.S + kAttnTile - 1) / kAttnTile);
-  for (int base = 0; base < all; base += 64) {
-    AttnTiles tiles = attn_tiles<true>(P, base, q0, prefix, ranges, own);
-    if (!tiles.seen) continue;
-    int j = __builtin_ctzll(tiles.seen);
-    issue(base + j, stage);
-    while (true) {
-      const uint64_t rest = tiles.seen & (tiles.seen - 1);
-      const int next = rest ? __builtin_ctzll(rest) : -1;
-      wait_vmem<0>();
-      tile_barrier();
-      if (next >= 0) issue(base + next, stage ^ 1);
-      const int64_t k0 = (int64_t)(base + j) * kAttnTile;
-      const bool part = (tiles.part >> j) & 1;
-      if ((tiles.pad >> j) & 1) clear_padding<HD>(docs + k0, lds[stage][0], lds[stage][1]);
-      const bool hidden = P.causal && k0 > row0 + 31 && k0 >= prefix;
-      if (!hidden) {
-        const char *kt = lds[stage][0], *vt = lds[stage][1];
-        const uint32_t ktr = base_lds + (uint32_t)(stage * 2) * kTile;
-        static_for<0, 2>([&](auto nn) {
-          constexpr int n = decltype(nn)::value;
-          f32x16 s, dp;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) {
-            s = Traits<T>::mma(fr.rows(kt, n, ks), q[ks], s);
-            dp = Traits<T>::mma(fr.rows(vt, n, ks), g[ks], dp);
-          }
-          float z[16], th[16];
-          scores<CAP, BIAS>(s, z, th, P, slope, (int)(i - k0), n);
-          if (part) {
-            int dk[16];
-            if (docs) tile_docs(docs + k0, n, dk);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int64_t key = k0 + tile_row(n, r);
-              bool see = key < P.S && (!P.causal || key <= i || key < prefix);
-              if (docs) see = see && dk[r] == doc && doc >= 0;
-              z[r] = see ? z[r] : -kInf;
-            }
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            z[r] = __builtin_amdgcn_exp2f(z[r] - lse) * (dp[r] - delta);
-            if constexpr (CAP) z[r] *= 1.0f - th[r] * th[r];
-          }
-          Frag zf[2], kf[kBlocks];
-          as_operand<T>(z, zf);  // (dz in 16 bits, as an operand of the product)
-          static_for<0, 2>([&](auto k) {
-            constexpr int KS = decltype(k)::value;
-            fr.template cols<2 * n + KS>(ktr, kf);
-#pragma unroll
-            for (int d = 0; d < kBlocks; ++d) dq[d] = Traits<T>::mma(kf[d], zf[KS], dq[d]);
-          });
-        });
-      }
-      stage ^= 1;
-      if (next < 0) break;
-      tiles.seen = rest;
-      j = next;
-    }
-  }
-  if (doc < 0)  // (what a padding row holds may not be finite)
+    for (int r = 0; r < 16; ++r) f.dq[d][r] = 0.0f;
+  attn_walk_plain(walk, f);
+  if (f.doc < 0)  // (what a padding row holds may not be finite)
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dq[d][r] = 0.0f;
-  T* out = static_cast<T*>(P.dq) + ((b * P.S + i) * P.H + head) * P.D;
-  store_own<T, HD>(dq, P.scale, out, P.D, i < P.S);
+      for (int r = 0; r < 16; ++r) f.dq[d][r] = 0.0f;
+  T* out = static_cast<T*>(P.dq) + (((int64_t)b * S + f.i) * P.H + head) * P.D;
+  store_own<T, HD>(f.dq, P.scale, out, P.D, f.i < S);
 }
 
 // ------------------------------------------------------------- dk and dv
-// A workgroup's 128 keys against the queries of all heads that share them.
+// A workgroup's 128 keys against the queries of all heads that share them: two
+// waves for every 32 keys, on one SIMD.  The first makes P from S = Q k^T and adds
+// up dv = P^T do; the second makes dz from P, which it gets through LDS in fp32,
+// and dP = do v^T, and adds up dk = dz^T Q.  Each has half of the matrix products
+// and half of the registers (dk and dv of 32 keys are 128 of 256).
+//
+// A phase takes 32 queries, and the workgroup meets behind it.  In phase p the
+// first wave starts with the softmax of block p and goes on with the products
+// dv of p and S of p + 1; the second starts with the products dk of p - 2 and dP of
+// p - 1, whose operands it read in the phase before, and goes on with dz of p - 1:
+// while one has the matrix cores the other has the vector unit.
 template <class T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 1) void k_attn_dkv(AttnParams P) {
+struct AttnGradKV {
   using Frag = typename Traits<T>::Frag;
-  constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][kTile];
-  __shared__ __attribute__((aligned(16))) float stats[2][2][kAttnTile];  // L and delta of the tile's queries
-  const int t = xcd_order(blockIdx.x, gridDim.x);
-  const int bk = t / P.tiles, r0 = (t % P.tiles) * kAttnRows;  // (with a causal mask the first keys have the most queries)
-  const int b = bk / P.KV, kv = bk - b * P.KV;
-  const int lane = threadIdx.x & 63, w = wave_id();
-  const int64_t row0 = r0 + w * 32, key = row0 + (lane & 31);
-  const int64_t prefix = P.prefix ? P.prefix[b] : 0;
-  const int* docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
-  const int4* ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / kAttnTile) : nullptr;
-  DocRange own{0x7fffffff, -1, 0};
-  int doc = 0;
-  if (docs) {
-    own.join(ranges[r0 / kAttnTile]);
-    own.join(ranges[r0 / kAttnTile + 1]);
-    doc = docs[key];
-  }
-  Frag kf[HD / 16], vf[HD / 16];
-  own_rows<T, HD>(static_cast<const T*>(P.k) + b * P.kb + kv * P.kh, P.ks, row0, P.S, P.D, kf);
-  own_rows<T, HD>(static_cast<const T*>(P.v) + b * P.vb + kv * P.vh, P.vs, row0, P.S, P.D, vf);
-  AttnDma<HD> qd, gd;
-  qd.init(P.qs, P.D);
-  gd.init(P.gs, P.D);
+  static constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32, kHalf = kTile / 2;
+  static constexpr int kStats = 2 * kAttnTile * 4, kProbs = 4 * 4096;
+  static constexpr int kLds = 6 * kTile + 2 * kProbs + 3 * kStats;
+  const AttnParams& P;
+  // (one object: between two the compiler waits for the DMA into either before it reads the other)
+  char *qlds, *glds;  // three slots of Q and of do
+  char *probs;        // two blocks of P
+  char *stats;        // three of (L, delta) of the queries
+  const T *Q, *G;     // of the first head
+  const float *lse, *delta, *slopes;
+  const int* docs;
+  AttnDma<HD, 8> qd, gd;
   AttnFrags<T, HD> fr;
-  fr.init();
-  const uint32_t base_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0][0];
-  f32x16 dk[kBlocks], dv[kBlocks];
+  Frag own[HD / 16];  // the wave's keys, or their values
+  f32x16 acc[kBlocks];
+  f32x16 x;                              // first: S of the next phase's block
+  Frag rows[HD / 16], cf[2][kBlocks];    // second: operands of the next phase
+  Frag zf[2];                            // second: dz of the last phase's block
+  int row0, key, bound, doc, prefix;
+  __device__ __forceinline__ AttnGradKV(const AttnParams& p) : P(p) {}
+  __device__ __forceinline__ void issue(const AttnTile& t, int n) {
+    qd.issue(Q + t.head * P.qh + t.first * P.qs, (int)P.S - t.first, qlds + (n % 3) * kTile);
+    gd.issue(G + t.head * P.gh + t.first * P.gs, (int)P.S - t.first, glds + (n % 3) * kTile);
+    const int w = wave_id();
+    if (w < 2)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of((w ? delta : lse) + t.head * P.padded + t.first),
+                                               (__attribute__((address_space(3))) void*)(stats + (n % 3) * kStats + w * (kStats / 2)), 4,
+                                               (threadIdx.x & 63) * 4, 0, 0, 0);
+  }
+  __device__ __forceinline__ void ready(const AttnTile& t, int n) {
+    if (t.pad) clear_padding<HD>(docs + t.first, qlds + (n % 3) * kTile, glds + (n % 3) * kTile);
+  }
+  __device__ __forceinline__ bool hidden(int row) const { return P.causal && row0 > row + 31 && row0 >= prefix; }
+  __device__ __forceinline__ char* qrows(int n, int block) const { return qlds + (n % 3) * kTile + block * kHalf; }
+  __device__ __forceinline__ char* grows(int n, int block) const { return glds + (n % 3) * kTile + block * kHalf; }
+  __device__ __forceinline__ void fetch(const char* at) {
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) rows[ks] = fr.rows(at, ks);
+  }
+  __device__ __forceinline__ void product(f32x16& z) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) z = Traits<T>::mma(rows[ks], own[ks], z);
+  }
+  __device__ __forceinline__ void add_up(const Frag (&f)[2]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d) acc[d] = Traits<T>::mma(cf[j][d], f[j], acc[d]);
+  }
+  // four consecutive queries of the lane's rows at a time
+  __device__ __forceinline__ const char* stat(int n, int block, int which) const {
+    return stats + (n % 3) * kStats + which * (kStats / 2) + 128 * block + ((threadIdx.x & 63) >> 5) * 16;
+  }
+  __device__ __forceinline__ char* prob(int buffer) const { return probs + buffer * kProbs + (wave_id() & 3) * 4096 + (threadIdx.x & 63) * 16; }
+  // The first wave's phase: block BLOCK of tile t; `then`: S of the block behind
+  // it, block 1 - BLOCK of tile tn.
+  template <int BLOCK>
+  __device__ __forceinline__ void lead(const AttnTile& t, int n, bool then, int tn) {
+    const int at = t.first + 32 * BLOCK;
+    if (then) fetch(qrows(tn, 1 - BLOCK));
+    if (!hidden(at)) {
+      f4v L[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) L[g] = *reinterpret_cast<const f4v*>(stat(n, BLOCK, 0) + 32 * g);
+      fr.cols(lds_at(grows(n, BLOCK)), cf);
+      float th[16], p[16];
+      scores<CAP, BIAS>(x, th, P, BIAS ? slopes[t.head] * kLog2e : 0.0f, key - at);
+      if (t.part) hide<false>(x, bound - at, docs ? docs + at : nullptr, doc);
+      const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f4v out;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          p[r] = __builtin_amdgcn_exp2f(fmaf(x[r], mul, -L[g][e]));  // (queries behind the last, or that see nothing: L = inf)
+          out[e] = CAP ? p[r] * (1.0f - th[r] * th[r]) : p[r];
+        }
+        *reinterpret_cast<f4v*>(prob(BLOCK) + g * 1024) = out;
+      }
+      Frag pf[2];
+      as_operand<T>(p, pf);
+      add_up(pf);
+    }
+    if (then) product(x);
+  }
+  // The second wave's: dk of block BLOCK of tile u (has: there is one), dz of
+  // block 1 - BLOCK of tile t, and the operands of the next phase, dP of block
+  // BLOCK of tile next (more: there is one) and dk of the block whose dz this is.
+  template <int BLOCK>
+  __device__ __forceinline__ void follow(const AttnTile& u, bool has, const AttnTile& t, int n, bool here, int next, bool more) {
+    constexpr int kOther = 1 - BLOCK;
+    if (has && !hidden(u.first + 32 * BLOCK)) add_up(zf);
+    if (here && !hidden(t.first + 32 * kOther)) {
+      f32x16 dp;
+      f4v dl[4], p[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        dl[g] = *reinterpret_cast<const f4v*>(stat(n, kOther, 1) + 32 * g);
+        p[g] = *reinterpret_cast<const f4v*>(prob(kOther) + g * 1024);
+      }
+      product(dp);
+      float z[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) z[r] = p[r >> 2][r & 3] * (dp[r] - dl[r >> 2][r & 3]);
+      as_operand<T>(z, zf);
+    }
+    if (more) fetch(grows(next, BLOCK));
+    if (here) fr.cols(lds_at(qrows(n, kOther)), cf);
+  }
+  // (a loop of its own for each of the two: in one, what either holds would take
+  // registers of both)
+  template <bool LEADS>
+  __device__ __forceinline__ void walk(AttnWalk<false>& w) {
+    AttnTile t0 = w.next(), last = t0;
+    if (t0.first < 0) return;
+    AttnTile t1 = w.next();
+    issue(t0, 0);
+    if (t1.first >= 0) issue(t1, 1);
+    wait_vmem<0>();
+    tile_barrier();
+    ready(t0, 0);
+    if constexpr (LEADS) {
+      if (!hidden(t0.first)) {
+        fetch(qrows(0, 0));
+        product(x);
+      }
+    }
+    int n = 0;
+    for (;; ++n) {
+      if constexpr (LEADS) lead<0>(t0, n, !hidden(t0.first + 32), n);
+      else follow<0>(last, n > 0, last, n + 2, n > 0, n, true);  // (n + 2: the slots of n - 1)
+      wait_vmem<0>();  // (t1, sent for two phases ago)
+      tile_barrier();
+      const AttnTile t2 = w.next();
+      if (t2.first >= 0) issue(t2, n + 2);  // (over the tile before t0, whose last block was read in the phase before)
+      const bool more = t1.first >= 0;
+      if (more) ready(t1, n + 1);
+      if constexpr (LEADS) lead<1>(t0, n, more && !hidden(t1.first), n + 1);
+      else follow<1>(last, n > 0, t0, n, true, n, true);
+      tile_barrier();
+      last = t0;
+      if (!more) break;
+      t0 = t1;
+      t1 = t2;
+    }
+    if constexpr (!LEADS) {
+      follow<0>(last, true, last, n, true, n, false);
+      if (!hidden(last.first + 32)) add_up(zf);
+    }
+  }
+};
+
+template <class T, int HD, bool CAP, bool BIAS>
+__global__ __launch_bounds__(512, 2) void k_attn_dkv(AttnParams P) {
+  using F = AttnGradKV<T, HD, CAP, BIAS>;
+  constexpr int kBlocks = HD / 32;
+  __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
+  int bk, r0;
+  attn_place(P, P.B * P.KV, false, bk, r0);
+  r0 *= kAttnRows;
+  const int b = bk / P.KV, kv = bk - b * P.KV, head = kv * P.group;
+  const int lane = threadIdx.x & 63, S = (int)P.S, w = wave_id();
+  const bool leads = w < 4;
+  F f(P);
+  f.qlds = lds;
+  f.glds = lds + 3 * F::kTile;
+  f.probs = lds + 6 * F::kTile;
+  f.stats = f.probs + 2 * F::kProbs;
+  f.row0 = r0 + (w & 3) * 32;
+  f.key = f.row0 + (lane & 31);
+  f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
+  f.doc = P.docs ? f.docs[f.key] : 0;
+  f.prefix = P.prefix ? P.prefix[b] : 0;
+  f.bound = P.causal && f.key >= f.prefix ? f.key : 0;
+  f.Q = static_cast<const T*>(P.q) + b * P.qb + head * P.qh;
+  f.G = static_cast<const T*>(P.dout) + b * P.gb + head * P.gh;
+  f.lse = P.lse + ((int64_t)b * P.H + head) * P.padded;
+  f.delta = P.delta + ((int64_t)b * P.H + head) * P.padded;
+  f.slopes = BIAS ? P.slopes + head : nullptr;
+  f.qd.init(P.qs, P.D);
+  f.gd.init(P.gs, P.D);
+  f.fr.init();
 #pragma unroll
   for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.0f;
-  int stage = 0;
-  const int all = (int)((P.S + kAttnTile - 1) / kAttnTile);
-  for (int head = kv * P.group; head < (kv + 1) * P.group; ++head) {
-    const T* Q = static_cast<const T*>(P.q) + b * P.qb + head * P.qh;
-    const T* G = static_cast<const T*>(P.dout) + b * P.gb + head * P.gh;
-    const float* lse = P.lse + ((int64_t)b * P.H + head) * P.padded;
-    const float* delta = P.delta + ((int64_t)b * P.H + head) * P.padded;
-    const float slope = BIAS ? P.slopes[head] * kLog2e : 0.0f;
-    auto issue = [&](int tile, int st) {
-      const int64_t a = (int64_t)tile * kAttnTile;
-      qd.issue(Q + a * P.qs, P.S - a, lds[st][0]);
-      gd.issue(G + a * P.gs, P.S - a, lds[st][1]);
-      if (w < 2)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of((w ? delta : lse) + a), (__attribute__((address_space(3))) void*)stats[st][w], 4,
-                                                 lane * 4, 0, 0, 0);
-    };
-    for (int base = 0; base < all; base += 64) {
-      AttnTiles tiles = attn_tiles<false>(P, base, r0, prefix, ranges, own);
-      if (!tiles.seen) continue;
-      int j = __builtin_ctzll(tiles.seen);
-      issue(base + j, stage);
-      while (true) {
-        const uint64_t rest = tiles.seen & (tiles.seen - 1);
-        const int next = rest ? __builtin_ctzll(rest) : -1;
-        wait_vmem<0>();
-        tile_barrier();
-        if (next >= 0) issue(base + next, stage ^ 1);
-        const int64_t a = (int64_t)(base + j) * kAttnTile;
-        const bool part = (tiles.part >> j) & 1;
-        if ((tiles.pad >> j) & 1) clear_padding<HD>(docs + a, lds[stage][0], lds[stage][1]);
-        const bool hidden = P.causal && row0 > a + kAttnTile - 1 && row0 >= prefix;
-        if (!hidden) {
-          const char *qt = lds[stage][0], *gt = lds[stage][1];
-          const uint32_t qtr = base_lds + (uint32_t)(stage * 2) * kTile, gtr = qtr + kTile;
-          static_for<0, 2>([&](auto nn) {
-            constexpr int n = decltype(nn)::value;
-            f32x16 s, dp;
+    for (int r = 0; r < 16; ++r) f.acc[d][r] = 0.0f;
+  AttnWalk<false> walk;
+  walk.init(P, b, r0, P.group);
+  const int64_t at = (((int64_t)b * S + f.key) * P.KV + kv) * P.D;
+  const bool live = f.key < S;
+  // (zeros for a padding row: what it holds may not be finite)
+  auto finish = [&](T* out, float mul) {
+    if (f.doc < 0)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+      for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-            for (int ks = 0; ks < HD / 16; ++ks) {
-              s = Traits<T>::mma(fr.rows(qt, n, ks), kf[ks], s);
-              dp = Traits<T>::mma(fr.rows(gt, n, ks), vf[ks], dp);
-            }
-            float z[16], th[16], p[16];
-            scores<CAP, BIAS>(s, z, th, P, slope, (int)(key - a), n);
-            if (part) {
-              int dq[16];
-              if (docs) tile_docs(docs + a, n, dq);
-#pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                const int64_t i = a + tile_row(n, r);
-                bool see = !P.causal || key <= i || key < prefix;
-                if (docs) see = see && dq[r] == doc && doc >= 0;
-                z[r] = see ? z[r] : -kInf;
-              }
-            }
-            // queries behind the last, or that see nothing, have L = inf
-#pragma unroll
-            for (int gq = 0; gq < 4; ++gq) {
-              const int at = tile_row(n, 4 * gq);
-              const float4 L = *reinterpret_cast<const float4*>(&stats[stage][0][at]);
-              const float4 dl = *reinterpret_cast<const float4*>(&stats[stage][1][at]);
-              const float Lr[4] = {L.x, L.y, L.z, L.w}, dr[4] = {dl.x, dl.y, dl.z, dl.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int r = 4 * gq + e;
-                p[r] = __builtin_amdgcn_exp2f(z[r] - Lr[e]);
-                z[r] = p[r] * (dp[r] - dr[e]);
-                if constexpr (CAP) z[r] *= 1.0f - th[r] * th[r];
-              }
-            }
-            Frag pf[2], zf[2], cf[kBlocks];
-            as_operand<T>(p, pf);
-            as_operand<T>(z, zf);
-            static_for<0, 2>([&](auto k) {
-              constexpr int KS = decltype(k)::value;
-              fr.template cols<2 * n + KS>(gtr, cf);
-#pragma unroll
-              for (int d = 0; d < kBlocks; ++d) dv[d] = Traits<T>::mma(cf[d], pf[KS], dv[d]);
-              fr.template cols<2 * n + KS>(qtr, cf);
-#pragma unroll
-              for (int d = 0; d < kBlocks; ++d) dk[d] = Traits<T>::mma(cf[d], zf[KS], dk[d]);
-            });
-          });
-        }
-        stage ^= 1;
-        if (next < 0) break;
-        tiles.seen = rest;
-        j = next;
-      }
-    }
+        for (int r = 0; r < 16; ++r) f.acc[d][r] = 0.0f;
+    if (out) store_own<T, HD>(f.acc, mul, out + at, P.D, live);
+  };
+  if (leads) {
+    own_rows<T, HD>(static_cast<const T*>(P.k) + b * P.kb + kv * P.kh, P.ks, f.row0, S, P.D, f.own, P.scale < 0.0f);
+    f.template walk<true>(walk);
+    finish(static_cast<T*>(P.dv), 1.0f);
+  } else {
+    own_rows<T, HD>(static_cast<const T*>(P.v) + b * P.vb + kv * P.vh, P.vs, f.row0, S, P.D, f.own);
+    f.template walk<false>(walk);
+    finish(static_cast<T*>(P.dk), P.scale);
   }
-  if (doc < 0)
-#pragma unroll
-    for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.0f;
-  const int64_t at = ((b * P.S + key) * P.KV + kv) * P.D;
-  if (P.dk) store_own<T, HD>(dk, P.scale, static_cast<T*>(P.dk) + at, P.D, key < P.S);
-  if (P.dv) store_own<T, HD>(dv, 1.0f, static_cast<T*>(P.dv) + at, P.D, key < P.S);
 }
 
 // ------------------------------------------------------------- launches
@@ -693,7 +933,7 @@ static hipError_t attn_go(AttnParams P, AttnPass pass, hipStream_t s) {
   switch (pass) {
     case ATTN_FORWARD: hipLaunchKernelGGL((k_attn<T, HD, CAP, BIAS>), grid, dim3(256), 0, s, P); break;
     case ATTN_DQ: hipLaunchKernelGGL((k_attn_dq<T, HD, CAP, BIAS>), grid, dim3(256), 0, s, P); break;
-    default: hipLaunchKernelGGL((k_attn_dkv<T, HD, CAP, BIAS>), grid, dim3(256), 0, s, P);
+    default: hipLaunchKernelGGL((k_attn_dkv<T, HD, CAP, BIAS>), grid, dim3(512), 0, s, P);
   }
   return hipGetLastError();
 }

@@ -179,10 +179,13 @@ AttnParams attn_params(const orda_attention_t* p, const void* q, const void* k, 
   a.D = p->head_dim;
   a.causal = p->causal;
   const double log2e = 1.4426950408889634;
+  // (magnitudes: the kernels turn the sign of one operand; a scale of 0 is 1e-30,
+  // so that the -inf of what is not seen stays one)
+  const double size = std::fmax(std::fabs(p->scale), 1e-30);
   a.scale = (float)p->scale;
-  a.scale_log2 = (float)(p->scale * log2e);
+  a.scale_log2 = (float)(size * log2e);
   if (p->softcap > 0.0) {
-    a.cap_in = (float)(2.0 * log2e * p->scale / p->softcap);
+    a.cap_in = (float)(2.0 * log2e * size / p->softcap);
     a.cap_out = (float)(p->softcap * log2e);
   }
   return a;

@@ -97,8 +97,8 @@ struct AttnParams {
   int64_t S, padded;      // padded: S up to a multiple of 128
   int64_t qb, qs, qh, kb, ks, kh, vb, vs, vh, gb, gs, gh;
   int B, H, KV, group, D, causal, tiles;
-  float scale, scale_log2;  // scale_log2 = scale log2(e)
-  float cap_in, cap_out;    // 2 scale log2(e) / cap and cap log2(e); 0: no cap
+  float scale, scale_log2;  // scale_log2 = |scale| log2(e)
+  float cap_in, cap_out;    // 2 |scale| log2(e) / cap and cap log2(e); 0: no cap
 };
 enum AttnPass { ATTN_FORWARD, ATTN_DQ, ATTN_DKV };
 template <class T, int HD> hipError_t launch_attn(const AttnParams& P, AttnPass pass, hipStream_t s);
