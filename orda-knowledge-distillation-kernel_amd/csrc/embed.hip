@@ -20,7 +20,7 @@
 // other.
 #include <algorithm>
 
-#include "epilogue.hpp"
+#include "pieces.hpp"
 #include "step_launch.hpp"
 
 namespace orda {
@@ -30,37 +30,42 @@ __device__ __forceinline__ int64_t token_at(const void* ids, int wide, int64_t i
 }
 
 // ------------------------------------------------------------- forward
-template <class W, class T>
+template <class W, class T, bool EVEN>
 __global__ __launch_bounds__(256) void k_embed(EmbedParams P, int64_t per_row, int64_t pieces) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
     const int64_t row = pieces <= 0xffffffffll ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row;
-    const int64_t c = (i - row * per_row) * 8;
-    const int cnt = (int)lmin(8, P.hidden - c);
+    const Piece<EVEN> p(i - row * per_row, P.hidden);
     const int64_t t = token_at(P.ids, P.wide, row);
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (t >= 0 && t < P.vocab) {
-      ld_row<W, 8>(static_cast<const W*>(P.weight) + t * P.ldw + c, v, cnt);
+    const bool known = t >= 0 && t < P.vocab;
+    Raw8<W> w;
+    w.get(static_cast<const W*>(P.weight) + (known ? t : 0) * P.ldw, p);
+    float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= P.scale;
-    }
-    st_row<T, 8>(static_cast<T*>(P.y) + row * P.hidden + c, v, cnt);
+    for (int e = 0; e < 8; ++e) v[e] = known ? w[e] * P.scale : 0.0f;
+    put8(static_cast<T*>(P.y) + row * P.hidden, p, v);
   }
 }
 
 // ------------------------------------------------------------- sort
 constexpr int kSegment = 4096;  // tokens of one workgroup
+constexpr int kFill = 4096;     // 16-byte stores of one that fills
 
 // Keys: the token, V for one that has no gradient (it sorts behind all others).
 // Entries past the last token have all bits set and stay behind them.
 __global__ __launch_bounds__(1024) void k_embed_sort(EmbedGradParams P, int passes, int segments, uint32_t* tokens, uint32_t* places, int64_t fill_bytes) {
   if ((int)blockIdx.x >= segments) {
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    const int64_t n = fill_bytes / 16, step = (int64_t)(gridDim.x - segments) * 1024;
-    const int64_t at = (int64_t)(blockIdx.x - segments) * 1024 + threadIdx.x;
     uint4* out = static_cast<uint4*>(P.dw);
-    for (int64_t i = at; i < n; i += step) out[i] = zero;
-    const int64_t tail = (fill_bytes % 16) / 2;  // (elements of 2 or 4 bytes)
-    if (at < tail) reinterpret_cast<uint16_t*>(out + n)[at] = 0;
+    const int64_t n = fill_bytes / 16, groups = gridDim.x - segments;
+    // (64 KB of a workgroup in a row)
+    for (int64_t b = blockIdx.x - segments; b * kFill < n; b += groups)
+#pragma unroll
+      for (int i = 0; i < kFill / 1024; ++i) {
+        const int64_t at = b * kFill + i * 1024 + threadIdx.x;
+        if (at < n) out[at] = zero;
+      }
+    const int tail = (int)(fill_bytes % 16) / 2;  // (elements of 2 or 4 bytes)
+    if ((int)blockIdx.x == segments && (int)threadIdx.x < tail) reinterpret_cast<uint16_t*>(out + n)[threadIdx.x] = 0;
     return;
   }
   __shared__ uint32_t key[2][kSegment];
@@ -187,16 +192,15 @@ struct EmbedSums {
   int64_t chunks;
 };
 
-template <class W, class T>
+template <class W, class T, bool EVEN>
 __global__ __launch_bounds__(256) void k_embed_sum(EmbedGradParams P, EmbedSums S) {
   constexpr int kAhead = 8;  // rows in flight
   const int lane = threadIdx.x & 63;
   const int64_t units = S.chunks * S.slabs;
-  for (int64_t u = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < units; u += (int64_t)gridDim.x * 4) {
+  for (int64_t u = (int64_t)blockIdx.x * 4 + wave_id(); u < units; u += (int64_t)gridDim.x * 4) {
     const int64_t chunk = u / S.slabs, first = chunk * S.chunk;
     const int n = (int)lmin(S.chunk, P.tokens - first);
-    const int64_t c = (u - chunk * S.slabs) * 512 + lane * 8;
-    const int cnt = (int)(c < P.hidden ? lmin(8, P.hidden - c) : 0);
+    const Piece<EVEN> at((u - chunk * S.slabs) * 64 + lane, P.hidden);
     uint32_t tok = (uint32_t)P.vocab, place = 0;
     if (lane < n) {
       tok = S.tokens[first + lane];
@@ -207,20 +211,17 @@ __global__ __launch_bounds__(256) void k_embed_sum(EmbedGradParams P, EmbedSums 
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     bool from_before = (uint32_t)__builtin_amdgcn_readlane((int)tok, 0) == before;
     for (int i0 = 0; i0 < n; i0 += kAhead) {
-      RawRow<T, 8> v[kAhead];
+      Raw8<T> v[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int i = i0 + k < n ? i0 + k : n - 1;
-        const int64_t row = (uint32_t)__builtin_amdgcn_readlane((int)place, i);
-        const bool has = i0 + k < n && (uint32_t)__builtin_amdgcn_readlane((int)tok, i) < (uint32_t)P.vocab;
-        v[k].load(static_cast<const T*>(P.dy) + row * P.ldg + c, has ? cnt : 0);
+      for (int k = 0; k < kAhead; ++k) {  // (without a condition, so that none waits for another; behind the last entry its row again)
+        const int64_t row = (uint32_t)__builtin_amdgcn_readlane((int)place, min(i0 + k, n - 1));
+        v[k].get(static_cast<const T*>(P.dy) + row * P.ldg, at);
       }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         const int i = i0 + k;
-        if (i >= n) break;
-        const uint32_t t = (uint32_t)__builtin_amdgcn_readlane((int)tok, i);
-        if (t >= (uint32_t)P.vocab) continue;
+        const uint32_t t = (uint32_t)__builtin_amdgcn_readlane((int)tok, min(i, n - 1));
+        if (i >= n || t >= (uint32_t)P.vocab) break;  // (those without a gradient are the last)
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] += v[k][e];
         const bool last = i + 1 == n;
@@ -228,11 +229,11 @@ __global__ __launch_bounds__(256) void k_embed_sum(EmbedGradParams P, EmbedSums 
         if (!last && next == t) continue;
         // the run's end in this chunk
         if (from_before || next == t) {
-          if (cnt) st_row<float, 8>(S.part + (2 * chunk + (from_before ? 0 : 1)) * P.hidden + c, acc, cnt);
+          put8(S.part + (2 * chunk + (from_before ? 0 : 1)) * P.hidden, at, acc);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) acc[e] *= P.scale;
-          if (cnt) st_row<W, 8>(static_cast<W*>(P.dw) + (int64_t)t * P.hidden + c, acc, cnt);
+          put8(static_cast<W*>(P.dw) + (int64_t)t * P.hidden, at, acc);
         }
         from_before = false;
 #pragma unroll
@@ -244,54 +245,65 @@ __global__ __launch_bounds__(256) void k_embed_sum(EmbedGradParams P, EmbedSums 
 
 // A run that begins in chunk c and goes on: its sum in c and those of the
 // chunks that it reaches, every eighth of them by one wave.
-template <class W>
+template <class W, bool EVEN>
 __global__ __launch_bounds__(512) void k_embed_join(EmbedGradParams P, EmbedSums S) {
-  __shared__ float join[8][64][8];
+  __shared__ float join[8][8][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t units = S.chunks * S.slabs;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int64_t chunk = u / S.slabs, first = chunk * S.chunk, end = first + S.chunk;
     if (end >= P.tokens) continue;
-    const uint32_t t = S.tokens[end];
-    if (t >= (uint32_t)P.vocab || S.tokens[end - 1] != t) continue;
-    if (first > 0 && S.tokens[first] == t && S.tokens[first - 1] == t) continue;  // (it began before)
-    int64_t lo = end, hi = P.tokens;  // the last entry of the run: tokens[lo] == t, tokens[hi] > t
-    while (hi - lo > 1) {
-      const int64_t m = (lo + hi) / 2;
-      if (S.tokens[m] == t) lo = m;
-      else hi = m;
+    const uint32_t t = S.tokens[end], last = S.tokens[end - 1], start = S.tokens[first], before = first > 0 ? S.tokens[first - 1] : 0xffffffffu;
+    if (t >= (uint32_t)P.vocab || last != t) continue;
+    if (start == t && before == t) continue;  // (it began before)
+    // the chunks that begin with t
+    int64_t more = 0;
+    while (true) {
+      const int64_t e = end + (more + lane) * S.chunk;
+      const uint64_t same = __ballot(e < P.tokens && S.tokens[lmin(e, P.tokens - 1)] == t);
+      if (~same) {
+        more += __builtin_ctzll(~same);
+        break;
+      }
+      more += 64;
     }
-    const int64_t more = lo / S.chunk - chunk;
-    const int64_t c = (u - chunk * S.slabs) * 512 + lane * 8;
-    const int cnt = (int)(c < P.hidden ? lmin(8, P.hidden - c) : 0);
-    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8];
-    if (w == 0) ld_row<float, 8>(S.part + (2 * chunk + 1) * P.hidden + c, acc, cnt);
+    const Piece<EVEN> at((u - chunk * S.slabs) * 64 + lane, P.hidden);
+    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (w == 0) {
+      Raw8<float> v;
+      v.get(S.part + (2 * chunk + 1) * P.hidden, at);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = v[e];
+    }
 #pragma unroll 4
     for (int64_t k = 1 + w; k <= more; k += 8) {
-      ld_row<float, 8>(S.part + 2 * (chunk + k) * P.hidden + c, v, cnt);
+      Raw8<float> v;
+      v.get(S.part + 2 * (chunk + k) * P.hidden, at);
 #pragma unroll
       for (int e = 0; e < 8; ++e) acc[e] += v[e];
     }
     __syncthreads();  // (the turn before has read join)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) join[w][lane][e] = acc[e];
+    for (int e = 0; e < 8; ++e) join[w][e][lane] = acc[e];
     __syncthreads();
     if (w) continue;
 #pragma unroll
     for (int i = 1; i < 8; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += join[i][lane][e];
+      for (int e = 0; e < 8; ++e) acc[e] += join[i][e][lane];
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] *= P.scale;
-    if (cnt) st_row<W, 8>(static_cast<W*>(P.dw) + (int64_t)t * P.hidden + c, acc, cnt);
+    put8(static_cast<W*>(P.dw) + (int64_t)t * P.hidden, at, acc);
   }
 }
 
 // ------------------------------------------------------------- launches
 template <class W, class T>
 static hipError_t embed_go(const EmbedParams& P, hipStream_t s) {
-  const int64_t per_row = (P.hidden + 7) / 8, pieces = per_row * P.tokens;
-  hipLaunchKernelGGL((k_embed<W, T>), dim3((unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 23)), dim3(256), 0, s, P, per_row, pieces);
+  const int64_t per_row = pieces_of(P.hidden), pieces = per_row * P.tokens;
+  const unsigned groups = (unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 23);
+  if (P.hidden % 8 == 0) hipLaunchKernelGGL((k_embed<W, T, true>), dim3(groups), dim3(256), 0, s, P, per_row, pieces);
+  else hipLaunchKernelGGL((k_embed<W, T, false>), dim3(groups), dim3(256), 0, s, P, per_row, pieces);
   return hipGetLastError();
 }
 template <class W>
@@ -327,14 +339,18 @@ size_t embed_grad_workspace(int64_t tokens, int64_t hidden) {
   return list_bytes(tokens) * (tokens > kSegment ? 4 : 2) + up256((size_t)S.chunks * 2 * hidden * 4);
 }
 
-template <class W, class T>
-static hipError_t sum_go(const EmbedGradParams& P, const EmbedSums& S, hipStream_t s) {
+template <class W, class T, bool EVEN>
+static hipError_t sum_even(const EmbedGradParams& P, const EmbedSums& S, hipStream_t s) {
   const int64_t units = S.chunks * S.slabs;
-  hipLaunchKernelGGL((k_embed_sum<W, T>), dim3((unsigned)std::min<int64_t>((units + 3) / 4, 1 << 22)), dim3(256), 0, s, P, S);
+  hipLaunchKernelGGL((k_embed_sum<W, T, EVEN>), dim3((unsigned)std::min<int64_t>((units + 3) / 4, 1 << 22)), dim3(256), 0, s, P, S);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || S.chunks == 1) return e;
-  hipLaunchKernelGGL((k_embed_join<W>), dim3((unsigned)std::min<int64_t>(units, 1 << 20)), dim3(512), 0, s, P, S);
+  hipLaunchKernelGGL((k_embed_join<W, EVEN>), dim3((unsigned)std::min<int64_t>(units, 1 << 20)), dim3(512), 0, s, P, S);
   return hipGetLastError();
+}
+template <class W, class T>
+static hipError_t sum_go(const EmbedGradParams& P, const EmbedSums& S, hipStream_t s) {
+  return P.hidden % 8 == 0 ? sum_even<W, T, true>(P, S, s) : sum_even<W, T, false>(P, S, s);
 }
 template <class W>
 static hipError_t sum_out(const EmbedGradParams& P, const EmbedSums& S, int out_dtype, hipStream_t s) {
@@ -361,7 +377,7 @@ hipError_t launch_embed_grad(const EmbedGradParams& P, int dtype, int out_dtype,
   while (passes < 4 && (P.vocab >> (8 * passes)) != 0) ++passes;
   const int segments = (int)((P.tokens + kSegment - 1) / kSegment);
   const int64_t bytes = P.vocab * P.hidden * (dtype == DT_F32 ? 4 : 2);
-  const int fill = (int)std::min<int64_t>(1024, (bytes + 65535) / 65536);
+  const int fill = (int)std::min<int64_t>(1 << 20, (bytes + kFill * 16 - 1) / (kFill * 16));
   hipLaunchKernelGGL(k_embed_sort, dim3((unsigned)(segments + fill)), dim3(1024), 0, s, P, passes, segments, tokens[0], places[0], bytes);
   hipError_t e = hipGetLastError();
   int at = 0;

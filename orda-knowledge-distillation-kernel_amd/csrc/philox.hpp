@@ -51,10 +51,11 @@ __device__ __forceinline__ uint32_t keep_block(uint64_t block, uint64_t seed, ui
 }
 
 // Bit e: element `index` + e is kept, e < 8.  An index inside a block of 8 (rows
-// of odd lengths) takes two.
+// of odd lengths; never where EVEN) takes two.
+template <bool EVEN>
 __device__ __forceinline__ uint32_t keep8(int64_t index, uint64_t seed, uint64_t site, uint32_t threshold) {
   const uint64_t block = (uint64_t)index >> 3;
-  const int skip = (int)(index & 7);
+  const int skip = EVEN ? 0 : (int)(index & 7);
   uint32_t m = keep_block(block, seed, site, threshold);
   if (skip) m = (m | keep_block(block + 1, seed, site, threshold) << 8) >> skip;
   return m;

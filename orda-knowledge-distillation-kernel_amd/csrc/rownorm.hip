@@ -15,17 +15,17 @@
 // run.
 //
 // A row has LPR lanes (8, a wave, 256 or 1024 threads) with NP pieces of 8
-// consecutive elements each, piece k of lane l at 8 (l + k LPR).
+// consecutive elements each, the k-th of lane l piece l + k LPR.
 #include <algorithm>
 
-#include "epilogue.hpp"
+#include "pieces.hpp"
 #include "step_launch.hpp"
 
 namespace orda {
 
 // ------------------------------------------------------------- dropout
 // One piece a thread: 256 threads 2048 elements, as clipping has it.
-template <class T, bool RES>
+template <class T, bool RES, bool EVEN>
 __global__ __launch_bounds__(256) void k_dropout(DropoutParams P, int64_t per_row, int64_t pieces) {
   const uint64_t seed = seed_of(P.drop);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
@@ -34,29 +34,32 @@ __global__ __launch_bounds__(256) void k_dropout(DropoutParams P, int64_t per_ro
       row = pieces <= 0xffffffffll ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row;
       k -= row * per_row;
     }
-    const int64_t c = k * 8;
-    const int cnt = (int)lmin(8, P.cols - c);
-    float x[8], r[8];
-    ld_row<T, 8>(static_cast<const T*>(P.x) + row * P.ldx + c, x, cnt);
-    if constexpr (RES) ld_row<T, 8>(static_cast<const T*>(P.residual) + row * P.ldr + c, r, cnt);
-    const int64_t index = row * P.cols + c;
-    const uint32_t m = keep8(index, seed, P.drop.site, P.drop.threshold);
+    const Piece<EVEN> p(k, P.cols);
+    Raw8<T> x, r;
+    x.get(static_cast<const T*>(P.x) + row * P.ldx, p);
+    if constexpr (RES) r.get(static_cast<const T*>(P.residual) + row * P.ldr, p);
+    const uint32_t m = keep8<EVEN>(row * P.cols + p.c, seed, P.drop.site, P.drop.threshold);
+    float y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {  // (a dropped infinity or NaN leaves nothing)
-      x[e] = (m >> e) & 1 ? x[e] * P.drop.factor : 0.0f;
-      if constexpr (RES) x[e] += r[e];
+      y[e] = (m >> e) & 1 ? x[e] * P.drop.factor : 0.0f;
+      if constexpr (RES) y[e] += r[e];
     }
-    st_row<T, 8>(static_cast<T*>(P.y) + index, x, cnt);
+    put8(static_cast<T*>(P.y) + row * P.cols, p, y);
   }
 }
 
 template <class T>
 static hipError_t dropout_go(const DropoutParams& P, hipStream_t s) {
-  const int64_t per_row = (P.cols + 7) / 8, pieces = per_row * P.rows;
+  const int64_t per_row = pieces_of(P.cols), pieces = per_row * P.rows;
   // (a launch has fewer than 2^32 threads; past them a thread takes several pieces)
   const unsigned groups = (unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 23);
-  if (P.residual) hipLaunchKernelGGL((k_dropout<T, true>), dim3(groups), dim3(256), 0, s, P, per_row, pieces);
-  else hipLaunchKernelGGL((k_dropout<T, false>), dim3(groups), dim3(256), 0, s, P, per_row, pieces);
+  auto go = [&](auto residual, auto even) {
+    hipLaunchKernelGGL((k_dropout<T, decltype(residual)::value, decltype(even)::value>), dim3(groups), dim3(256), 0, s, P, per_row, pieces);
+  };
+  const bool even = P.cols % 8 == 0;
+  if (P.residual) even ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+  else even ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
   return hipGetLastError();
 }
 hipError_t launch_dropout(const DropoutParams& P, int dtype, hipStream_t s) {
@@ -68,8 +71,8 @@ hipError_t launch_dropout(const DropoutParams& P, int dtype, hipStream_t s) {
 }
 
 // ------------------------------------------------------------- row sums
-// v of all lanes of the row's LPR added up, in every lane; `red`: one float per
-// wave, another one for every call between two barriers.
+// v of all lanes of the row's LPR added up, in every lane; `red`: N floats per
+// wave, others for every call between two barriers.
 template <int LPR>
 __device__ __forceinline__ float lanes_sum(float v) {
   v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, false));   // lane ^ 1
@@ -77,8 +80,10 @@ __device__ __forceinline__ float lanes_sum(float v) {
   v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xF, 0xF, false));  // the other quad of 8
   if constexpr (LPR > 8) {
     v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xF, 0xF, false));  // the other 8 of 16
-    v += __shfl_xor(v, 16);
-    v += __shfl_xor(v, 32);
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(b[0]) + __uint_as_float(b[1]);
   }
   return v;
 }
@@ -92,7 +97,7 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* red) {
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
       for (int i = 0; i < N; ++i) red[i * kWaves + w] = v[i];
-    __syncthreads();
+    tile_barrier();  // (no wait for loads and stores in flight)
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       float t = 0.0f;
@@ -106,61 +111,64 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* red) {
 constexpr int group_threads(int lpr) { return lpr > 256 ? lpr : 256; }
 
 // s of one piece: residual + keep(x) factor
-template <class T>
-__device__ __forceinline__ void drop_piece(float (&x)[8], const float* r, int64_t index, const DropParams& d, uint64_t seed) {
+template <bool EVEN, class T>
+__device__ __forceinline__ void stream_piece(float (&s)[8], const Raw8<T>& x, const Raw8<T>& r, bool residual, int64_t index, const DropParams& d, uint64_t seed) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[e] = x[e];
   if (d.threshold) {
-    const uint32_t m = keep8(index, seed, d.site, d.threshold);
+    const uint32_t m = keep8<EVEN>(index, seed, d.site, d.threshold);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (m >> e) & 1 ? x[e] * d.factor : 0.0f;
+    for (int e = 0; e < 8; ++e) s[e] = (m >> e) & 1 ? s[e] * d.factor : 0.0f;
   }
-  if (r)
+  if (residual)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] += r[e];
+    for (int e = 0; e < 8; ++e) s[e] += r[e];
 }
 
 // ------------------------------------------------------------- forward
-template <class T, class W, int LPR, int NP>
+// The next row is loaded while this one is worked on.
+template <class T, class W, int LPR, int NP, bool EVEN>
 __global__ __launch_bounds__(group_threads(LPR)) void k_layer_norm(LayerNormParams P) {
   constexpr int kRows = group_threads(LPR) / LPR, kWaves = group_threads(LPR) / 64;
   __shared__ float red[2][2][kWaves];
   const int lane = threadIdx.x % LPR;
   const uint64_t seed = P.drop.threshold ? seed_of(P.drop) : 0;
   const float n_cols = (float)P.cols;
-  int cnt[NP];
-  RawRow<W, 8> w[NP], b[NP];
+  Piece<EVEN> at[NP];
+  Raw8<W> w[NP], b[NP];
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const int64_t c = 8 * (int64_t)(lane + k * LPR);
-    cnt[k] = (int)(P.cols - c < 0 ? 0 : lmin(8, P.cols - c));
-    w[k].load(static_cast<const W*>(P.weight) + c, cnt[k]);
-    if (P.bias) b[k].load(static_cast<const W*>(P.bias) + c, cnt[k]);
+    at[k] = Piece<EVEN>(lane + k * LPR, P.cols);
+    w[k].get(static_cast<const W*>(P.weight), at[k]);
+    if (P.bias) b[k].get(static_cast<const W*>(P.bias), at[k]);
   }
-  int turn = 0;
-  const int64_t steps = (P.rows + kRows - 1) / kRows;
-  for (int64_t step = blockIdx.x; step < steps; step += gridDim.x, turn ^= 1) {
-    const int64_t row = step * kRows + threadIdx.x / LPR;
-    const bool live = row < P.rows;
-    float v[NP][8], sum[1] = {0.0f};
-    RawRow<T, 8> x[NP], r[NP];
+  const bool residual = P.residual != nullptr;
+  struct Loaded {
+    Raw8<T> x[NP], r[NP];
+  };
+  const int64_t steps = (P.rows + kRows - 1) / kRows, own = threadIdx.x / LPR;
+  // (behind the last row: the last row again, not stored)
+  auto load = [&](int64_t step, Loaded& q) {
+    const int64_t row = lmin(step * kRows + own, P.rows - 1);
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      const int n = live ? cnt[k] : 0;
-      const int64_t c = 8 * (int64_t)(lane + k * LPR);
-      x[k].load(static_cast<const T*>(P.x) + row * P.ldx + c, n);
-      if (P.residual) r[k].load(static_cast<const T*>(P.residual) + row * P.ldr + c, n);
+      q.x[k].get(static_cast<const T*>(P.x) + row * P.ldx, at[k]);
+      if (residual) q.r[k].get(static_cast<const T*>(P.residual) + row * P.ldr, at[k]);
     }
+  };
+  int turn = 0;
+  Loaded next;
+  load(blockIdx.x, next);
+  for (int64_t step = blockIdx.x; step < steps; step += gridDim.x, turn ^= 1) {
+    const Loaded q = next;
+    if (step + gridDim.x < steps) load(step + gridDim.x, next);
+    const int64_t row = step * kRows + own;
+    float v[NP][8], sum[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      const int64_t c = 8 * (int64_t)(lane + k * LPR);
-      float add[8];
+      stream_piece<EVEN>(v[k], q.x[k], q.r[k], residual, row * P.cols + at[k].c, P.drop, seed);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[k][e] = x[k][e];
-        add[e] = P.residual ? r[k][e] : 0.0f;
-      }
-      if (live && cnt[k]) drop_piece<T>(v[k], P.residual ? add : nullptr, row * P.cols + c, P.drop, seed);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum[0] += e < cnt[k] ? v[k][e] : 0.0f;
+      for (int e = 0; e < 8; ++e) sum[0] += at[k].own(e) ? v[k][e] : 0.0f;
     }
     row_sums<LPR>(sum, red[turn][0]);
     const float mean = sum[0] / n_cols;
@@ -169,92 +177,91 @@ __global__ __launch_bounds__(group_threads(LPR)) void k_layer_norm(LayerNormPara
     for (int k = 0; k < NP; ++k)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float d = e < cnt[k] ? v[k][e] - mean : 0.0f;
+        const float d = at[k].own(e) ? v[k][e] - mean : 0.0f;
         sum[0] = fmaf(d, d, sum[0]);
       }
     row_sums<LPR>(sum, red[turn][1]);
     const float rstd = 1.0f / sqrtf(sum[0] / n_cols + P.eps);
-    if (!live) continue;
+    if (row >= P.rows) continue;
     if (P.stats && lane == 0) *reinterpret_cast<float2*>(P.stats + 2 * row) = make_float2(mean, rstd);
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      if (!cnt[k]) continue;
-      const int64_t at = row * P.cols + 8 * (int64_t)(lane + k * LPR);
-      if (P.s) st_row<T, 8>(static_cast<T*>(P.s) + at, v[k], cnt[k]);
+      if (P.s) put8(static_cast<T*>(P.s) + row * P.cols, at[k], v[k]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float h = (v[k][e] - mean) * rstd;
         v[k][e] = P.bias ? fmaf(h, w[k][e], b[k][e]) : h * w[k][e];
       }
-      st_row<T, 8>(static_cast<T*>(P.y) + at, v[k], cnt[k]);
+      put8(static_cast<T*>(P.y) + row * P.cols, at[k], v[k]);
     }
   }
 }
 
 // Rows longer than a workgroup's registers hold: 1024 threads read the row three
 // times (the second and third time from the caches).
-template <class T, class W>
+template <class T, class W, bool EVEN>
 __global__ __launch_bounds__(1024) void k_layer_norm_long(LayerNormParams P) {
   __shared__ float red[2][2][16];
   const uint64_t seed = P.drop.threshold ? seed_of(P.drop) : 0;
   const float n_cols = (float)P.cols;
+  const int64_t pieces = pieces_of(P.cols);
   int turn = 0;
   for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x, turn ^= 1) {
-    auto piece = [&](int64_t c, float (&v)[8], int n) {
-      float r[8];
-      ld_row<T, 8>(static_cast<const T*>(P.x) + row * P.ldx + c, v, n);
-      if (P.residual) ld_row<T, 8>(static_cast<const T*>(P.residual) + row * P.ldr + c, r, n);
-      drop_piece<T>(v, P.residual ? r : nullptr, row * P.cols + c, P.drop, seed);
+    auto piece = [&](const Piece<EVEN>& at, float (&v)[8]) {
+      Raw8<T> x, r;
+      x.get(static_cast<const T*>(P.x) + row * P.ldx, at);
+      if (P.residual) r.get(static_cast<const T*>(P.residual) + row * P.ldr, at);
+      stream_piece<EVEN>(v, x, r, P.residual != nullptr, row * P.cols + at.c, P.drop, seed);
     };
     float sum[1] = {0.0f}, v[8];
-    for (int64_t c = 8 * threadIdx.x; c < P.cols; c += 8192) {
-      const int n = (int)lmin(8, P.cols - c);
-      piece(c, v, n);
+    for (int64_t i = threadIdx.x; i < pieces; i += 1024) {
+      const Piece<EVEN> at(i, P.cols);
+      piece(at, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[0] += e < n ? v[e] : 0.0f;
-      if (P.s) st_row<T, 8>(static_cast<T*>(P.s) + row * P.cols + c, v, n);
+      for (int e = 0; e < 8; ++e) sum[0] += at.own(e) ? v[e] : 0.0f;
+      if (P.s) put8(static_cast<T*>(P.s) + row * P.cols, at, v);
     }
     row_sums<1024>(sum, red[turn][0]);
     const float mean = sum[0] / n_cols;
     sum[0] = 0.0f;
-    for (int64_t c = 8 * threadIdx.x; c < P.cols; c += 8192) {
-      const int n = (int)lmin(8, P.cols - c);
-      piece(c, v, n);
+    for (int64_t i = threadIdx.x; i < pieces; i += 1024) {
+      const Piece<EVEN> at(i, P.cols);
+      piece(at, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float d = e < n ? v[e] - mean : 0.0f;
+        const float d = at.own(e) ? v[e] - mean : 0.0f;
         sum[0] = fmaf(d, d, sum[0]);
       }
     }
     row_sums<1024>(sum, red[turn][1]);
     const float rstd = 1.0f / sqrtf(sum[0] / n_cols + P.eps);
     if (P.stats && threadIdx.x == 0) *reinterpret_cast<float2*>(P.stats + 2 * row) = make_float2(mean, rstd);
-    for (int64_t c = 8 * threadIdx.x; c < P.cols; c += 8192) {
-      const int n = (int)lmin(8, P.cols - c);
-      float w[8], b[8];
-      piece(c, v, n);
-      ld_row<W, 8>(static_cast<const W*>(P.weight) + c, w, n);
-      if (P.bias) ld_row<W, 8>(static_cast<const W*>(P.bias) + c, b, n);
+    for (int64_t i = threadIdx.x; i < pieces; i += 1024) {
+      const Piece<EVEN> at(i, P.cols);
+      Raw8<W> w, b;
+      piece(at, v);
+      w.get(static_cast<const W*>(P.weight), at);
+      if (P.bias) b.get(static_cast<const W*>(P.bias), at);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float h = (v[e] - mean) * rstd;
         v[e] = P.bias ? fmaf(h, w[e], b[e]) : h * w[e];
       }
-      st_row<T, 8>(static_cast<T*>(P.y) + row * P.cols + c, v, n);
+      put8(static_cast<T*>(P.y) + row * P.cols, at, v);
     }
   }
 }
 
 // ------------------------------------------------------------- backward
 // ds' of one piece to dr, and what dropout leaves of it to dx.
-template <class T>
-__device__ __forceinline__ void grad_piece(const LayerNormGradParams& P, float (&t)[8], int64_t at, int n, uint32_t kept) {
-  if (P.dr) st_row<T, 8>(static_cast<T*>(P.dr) + at, t, n);
+template <class T, bool EVEN>
+__device__ __forceinline__ void grad_piece(const LayerNormGradParams& P, float (&t)[8], int64_t row, const Piece<EVEN>& at, uint32_t kept) {
+  if (P.dr) put8(static_cast<T*>(P.dr) + row * P.cols, at, t);
   if (!P.dx) return;
   if (P.drop.threshold)
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] = (kept >> e) & 1 ? t[e] * P.drop.factor : 0.0f;
-  st_row<T, 8>(static_cast<T*>(P.dx) + at, t, n);
+  put8(static_cast<T*>(P.dx) + row * P.cols, at, t);
 }
 
 // AGAIN: s is computed again from x and the residual, in fp32.  fp32 parameters
@@ -262,66 +269,63 @@ __device__ __forceinline__ void grad_piece(const LayerNormGradParams& P, float (
 // read of 16 to 20; from s as it was rounded dw is off by half a step of the
 // 16-bit type (2e-4 of its norm in fp16, 2.4e-3 in bf16, where 1.7e-3 come from
 // its own rounding).
-template <class T, class W, int LPR, int NP, bool AGAIN>
+template <class T, class W, int LPR, int NP, bool EVEN, bool AGAIN>
 __global__ __launch_bounds__(group_threads(LPR)) void k_layer_norm_grad(LayerNormGradParams P) {
   constexpr int kRows = group_threads(LPR) / LPR, kWaves = group_threads(LPR) / 64;
   __shared__ float red[2][2 * kWaves];
   const int lane = threadIdx.x % LPR;
   const uint64_t seed = P.drop.threshold ? seed_of(P.drop) : 0;
   const float n_cols = (float)P.cols;
-  int cnt[NP];
-  RawRow<W, 8> w[NP];
+  Piece<EVEN> at[NP];
+  Raw8<W> w[NP];
   float dw[NP][8], db[NP][8];
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const int64_t c = 8 * (int64_t)(lane + k * LPR);
-    cnt[k] = (int)(P.cols - c < 0 ? 0 : lmin(8, P.cols - c));
-    w[k].load(static_cast<const W*>(P.weight) + c, cnt[k]);
+    at[k] = Piece<EVEN>(lane + k * LPR, P.cols);
+    w[k].get(static_cast<const W*>(P.weight), at[k]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[k][e] = db[k][e] = 0.0f;
   }
-  // a row's pieces are loaded while the row before is worked on
   struct Loaded {
-    RawRow<T, 8> s[NP], dy[NP], ds[NP], r[AGAIN ? NP : 1];
+    Raw8<T> s[NP], dy[NP], ds[NP], r[AGAIN ? NP : 1];
     float2 st;
   };
-  auto load = [&](int64_t row, Loaded& q) {
-    const bool live = row < P.rows;
-    q.st = live ? *reinterpret_cast<const float2*>(P.stats + 2 * row) : make_float2(0.0f, 0.0f);
+  const int64_t steps = (P.rows + kRows - 1) / kRows, own = threadIdx.x / LPR;
+  auto load = [&](int64_t step, Loaded& q) {
+    const int64_t row = lmin(step * kRows + own, P.rows - 1);
+    q.st = *reinterpret_cast<const float2*>(P.stats + 2 * row);
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      const int n = live ? cnt[k] : 0;
-      const int64_t c = 8 * (int64_t)(lane + k * LPR);
-      q.s[k].load(static_cast<const T*>(P.s) + row * P.ld_s + c, n);
-      if constexpr (AGAIN) q.r[k].load(static_cast<const T*>(P.residual) + row * P.ldr + c, n);
-      q.dy[k].load(static_cast<const T*>(P.dy) + row * P.ldy + c, n);
-      if (P.ds) q.ds[k].load(static_cast<const T*>(P.ds) + row * P.ldd + c, n);
+      q.s[k].get(static_cast<const T*>(P.s) + row * P.ld_s, at[k]);
+      if constexpr (AGAIN) q.r[k].get(static_cast<const T*>(P.residual) + row * P.ldr, at[k]);
+      q.dy[k].get(static_cast<const T*>(P.dy) + row * P.ldy, at[k]);
+      if (P.ds) q.ds[k].get(static_cast<const T*>(P.ds) + row * P.ldd, at[k]);
     }
   };
-  const int64_t steps = (P.rows + kRows - 1) / kRows;
   int turn = 0;
   Loaded next;
-  load((int64_t)blockIdx.x * kRows + threadIdx.x / LPR, next);
+  load(blockIdx.x, next);
   for (int64_t step = blockIdx.x; step < steps; step += gridDim.x, turn ^= 1) {
-    const int64_t row = step * kRows + threadIdx.x / LPR;
     const Loaded q = next;
-    if (step + gridDim.x < steps) load(row + (int64_t)gridDim.x * kRows, next);
+    if (step + gridDim.x < steps) load(step + gridDim.x, next);
+    const int64_t row = step * kRows + own;
     const bool live = row < P.rows;
     float h[NP][8], sum[2] = {0.0f, 0.0f};
     uint32_t kept[NP];
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
       kept[k] = 0xff;
-      if (P.drop.threshold && live && cnt[k]) kept[k] = keep8(row * P.cols + 8 * (int64_t)(lane + k * LPR), seed, P.drop.site, P.drop.threshold);
+      if (P.drop.threshold) kept[k] = keep8<EVEN>(row * P.cols + at[k].c, seed, P.drop.site, P.drop.threshold);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float s = q.s[k][e];
         if constexpr (AGAIN) s = ((kept[k] >> e) & 1 ? s * P.drop.factor : 0.0f) + q.r[k][e];
-        h[k][e] = e < cnt[k] ? (s - q.st.x) * q.st.y : 0.0f;
-        const float g = q.dy[k][e], gw = g * w[k][e];
+        h[k][e] = (s - q.st.x) * q.st.y;
+        const float g = live ? q.dy[k][e] : 0.0f, gw = at[k].own(e) ? g * w[k][e] : 0.0f;
         sum[0] += gw;
         sum[1] = fmaf(gw, h[k][e], sum[1]);
-        dw[k][e] = fmaf(g, h[k][e], dw[k][e]);
+        // (a row that is read twice, behind the last, has g = 0; h may not be finite there)
+        dw[k][e] = live ? fmaf(g, h[k][e], dw[k][e]) : dw[k][e];
         db[k][e] += g;
       }
     }
@@ -331,14 +335,13 @@ __global__ __launch_bounds__(group_threads(LPR)) void k_layer_norm_grad(LayerNor
       if (live)
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
-          if (!cnt[k]) continue;
           float t[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             t[e] = q.st.y * (fmaf(q.dy[k][e], w[k][e], -mg) - h[k][e] * mgh);
             if (P.ds) t[e] += q.ds[k][e];
           }
-          grad_piece<T>(P, t, row * P.cols + 8 * (int64_t)(lane + k * LPR), cnt[k], kept[k]);
+          grad_piece<T, EVEN>(P, t, row, at[k], kept[k]);
         }
     }
   }
@@ -366,75 +369,73 @@ __global__ __launch_bounds__(group_threads(LPR)) void k_layer_norm_grad(LayerNor
   float* out = P.partial + (int64_t)blockIdx.x * 2 * P.cols;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const int64_t c = 8 * (int64_t)(lane + k * LPR);
-    if (!cnt[k]) continue;
-    st_row<float, 8>(out + c, dw[k], cnt[k]);
-    st_row<float, 8>(out + P.cols + c, db[k], cnt[k]);
+    put8(out, at[k], dw[k]);
+    put8(out + P.cols, at[k], db[k]);
   }
 }
 
 // Long rows: sums of dw and db in the workgroup's own rows of `partial`, which
-// each thread reads and writes at its own columns only.
-template <class T, class W>
+// each thread reads and writes at its own columns only (of two pieces that
+// overlap the second adds up its own elements).
+template <class T, class W, bool EVEN>
 __global__ __launch_bounds__(1024) void k_layer_norm_grad_long(LayerNormGradParams P) {
   __shared__ float red[2][32];
   const uint64_t seed = P.drop.threshold ? seed_of(P.drop) : 0;
   const float n_cols = (float)P.cols;
+  const int64_t pieces = pieces_of(P.cols);
   float* part = P.partial ? P.partial + (int64_t)blockIdx.x * 2 * P.cols : nullptr;
   int turn = 0;
   bool first = true;
   for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x, turn ^= 1, first = false) {
     const float2 st = *reinterpret_cast<const float2*>(P.stats + 2 * row);
-    float sum[2] = {0.0f, 0.0f}, s[8], g[8], w[8];
+    float sum[2] = {0.0f, 0.0f}, s[8];
+    Raw8<T> g;
+    Raw8<W> w;
     uint32_t kept = 0xff;
-    auto piece = [&](int64_t c, int n) {
-      ld_row<T, 8>(static_cast<const T*>(P.s) + row * P.ld_s + c, s, n);
-      if (P.drop.threshold) kept = keep8(row * P.cols + c, seed, P.drop.site, P.drop.threshold);
-      if (P.residual) {
-        float r[8];
-        ld_row<T, 8>(static_cast<const T*>(P.residual) + row * P.ldr + c, r, n);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = ((kept >> e) & 1 ? s[e] * P.drop.factor : 0.0f) + r[e];
-      }
-      ld_row<T, 8>(static_cast<const T*>(P.dy) + row * P.ldy + c, g, n);
-      ld_row<W, 8>(static_cast<const W*>(P.weight) + c, w, n);
-    };
-    for (int64_t c = 8 * threadIdx.x; c < P.cols; c += 8192) {
-      const int n = (int)lmin(8, P.cols - c);
-      piece(c, n);
-      float a[8], b[8];
-      if (part) {
-        ld_row<float, 8>(part + c, a, first ? 0 : n);
-        ld_row<float, 8>(part + P.cols + c, b, first ? 0 : n);
-      }
+    auto piece = [&](const Piece<EVEN>& at) {
+      Raw8<T> x, r;
+      x.get(static_cast<const T*>(P.s) + row * P.ld_s, at);
+      if (P.residual) r.get(static_cast<const T*>(P.residual) + row * P.ldr, at);
+      g.get(static_cast<const T*>(P.dy) + row * P.ldy, at);
+      w.get(static_cast<const W*>(P.weight), at);
+      if (P.drop.threshold) kept = keep8<EVEN>(row * P.cols + at.c, seed, P.drop.site, P.drop.threshold);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float h = e < n ? (s[e] - st.x) * st.y : 0.0f;
-        sum[0] = fmaf(g[e], w[e], sum[0]);
-        sum[1] = fmaf(g[e] * w[e], h, sum[1]);
-        a[e] = fmaf(g[e], h, a[e]);
-        b[e] += g[e];
+        s[e] = x[e];
+        if (P.residual) s[e] = ((kept >> e) & 1 ? s[e] * P.drop.factor : 0.0f) + r[e];
       }
-      if (part) {
-        st_row<float, 8>(part + c, a, n);
-        st_row<float, 8>(part + P.cols + c, b, n);
+    };
+    for (int64_t i = threadIdx.x; i < pieces; i += 1024) {
+      const Piece<EVEN> at(i, P.cols);
+      piece(at);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!at.own(e)) continue;
+        const float h = (s[e] - st.x) * st.y, gw = g[e] * w[e];
+        sum[0] += gw;
+        sum[1] = fmaf(gw, h, sum[1]);
+        if (part) {
+          float* a = part + at.c + e;
+          a[0] = fmaf(g[e], h, first ? 0.0f : a[0]);
+          a[P.cols] = g[e] + (first ? 0.0f : a[P.cols]);
+        }
       }
     }
     if (!P.dx && !P.dr) continue;
     row_sums<1024>(sum, red[turn]);
     const float mg = sum[0] / n_cols, mgh = sum[1] / n_cols;
-    for (int64_t c = 8 * threadIdx.x; c < P.cols; c += 8192) {
-      const int n = (int)lmin(8, P.cols - c);
-      piece(c, n);
+    for (int64_t i = threadIdx.x; i < pieces; i += 1024) {
+      const Piece<EVEN> at(i, P.cols);
+      piece(at);
       float t[8];
+      Raw8<T> ds;
+      if (P.ds) ds.get(static_cast<const T*>(P.ds) + row * P.ldd, at);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) t[e] = st.y * (fmaf(g[e], w[e], -mg) - (s[e] - st.x) * st.y * mgh);
-      if (P.ds) {
-        ld_row<T, 8>(static_cast<const T*>(P.ds) + row * P.ldd + c, s, n);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] += s[e];
+      for (int e = 0; e < 8; ++e) {
+        t[e] = st.y * (fmaf(g[e], w[e], -mg) - (s[e] - st.x) * st.y * mgh);
+        if (P.ds) t[e] += ds[e];
       }
-      grad_piece<T>(P, t, row * P.cols + c, n, kept);
+      grad_piece<T, EVEN>(P, t, row, at, kept);
     }
   }
 }
@@ -448,8 +449,11 @@ __global__ __launch_bounds__(1024) void k_layer_norm_params(const float* partial
   W* out = blockIdx.y ? db : dw;
   if (!out) return;
   float v = 0.0f;
-  if (c < cols)
-    for (int64_t g = wave; g < groups; g += 16) v += partial[(2 * g + blockIdx.y) * cols + c];
+  if (c < cols) {
+    const float* p = partial + blockIdx.y * cols + c;
+#pragma unroll 8
+    for (int64_t g = wave; g < groups; g += 16) v += p[2 * g * cols];
+  }
   join[wave][lane] = v;
   __syncthreads();
   if (wave || c >= cols) return;
@@ -459,11 +463,12 @@ __global__ __launch_bounds__(1024) void k_layer_norm_params(const float* partial
 }
 
 // ------------------------------------------------------------- launches
-// f(LPR, NP) of a row length; (0, 0): the long kernels.
+// f(LPR, NP, EVEN) of a row length; LPR 0: the long kernels.
 template <class F>
 static hipError_t for_width(int64_t cols, const F& f) {
   using std::integral_constant;
-#define ORDA_ROW(L, N) f(integral_constant<int, L>{}, integral_constant<int, N>{})
+#define ORDA_ROW(L, N) (cols % 8 == 0 ? f(integral_constant<int, L>{}, integral_constant<int, N>{}, std::true_type{}) \
+                                      : f(integral_constant<int, L>{}, integral_constant<int, N>{}, std::false_type{}))
   if (cols <= 64) return ORDA_ROW(8, 1);
   if (cols <= 512) return ORDA_ROW(64, 1);
   if (cols <= 1024) return ORDA_ROW(64, 2);
@@ -476,32 +481,46 @@ static hipError_t for_width(int64_t cols, const F& f) {
 static int64_t rows_per_group(int64_t cols) { return cols <= 64 ? 32 : cols <= 1024 ? 4 : 1; }
 static int64_t threads_of(int64_t cols) { return cols <= 4096 ? 256 : 1024; }
 
+#ifndef GRAD_GROUPS
+#define GRAD_GROUPS 512
+#endif
+#ifndef NORM_GROUPS
+#define NORM_GROUPS 2048
+#endif
 int64_t layer_norm_groups(int64_t rows, int64_t cols) {
   const int64_t steps = (rows + rows_per_group(cols) - 1) / rows_per_group(cols);
-  return std::min<int64_t>(steps, threads_of(cols) == 256 ? 512 : 256);
+  return std::min<int64_t>(steps, threads_of(cols) == 256 ? GRAD_GROUPS : 256);
 }
 
 template <class T, class W>
 static hipError_t norm_go(const LayerNormParams& P, hipStream_t s) {
   const int64_t steps = (P.rows + rows_per_group(P.cols) - 1) / rows_per_group(P.cols);
-  const unsigned groups = (unsigned)std::min<int64_t>(steps, threads_of(P.cols) == 256 ? 2048 : 512);
-  return for_width(P.cols, [&](auto l, auto n) {
+  const unsigned groups = (unsigned)std::min<int64_t>(steps, threads_of(P.cols) == 256 ? NORM_GROUPS : 512);
+  return for_width(P.cols, [&](auto l, auto n, auto even) {
     constexpr int L = decltype(l)::value, N = decltype(n)::value;
-    if constexpr (L == 0) hipLaunchKernelGGL((k_layer_norm_long<T, W>), dim3(groups), dim3(1024), 0, s, P);
-    else hipLaunchKernelGGL((k_layer_norm<T, W, L, N>), dim3(groups), dim3(group_threads(L)), 0, s, P);
+    constexpr bool E = decltype(even)::value;
+    if constexpr (L == 0) hipLaunchKernelGGL((k_layer_norm_long<T, W, E>), dim3(groups), dim3(1024), 0, s, P);
+    else hipLaunchKernelGGL((k_layer_norm<T, W, L, N, E>), dim3(groups), dim3(group_threads(L)), 0, s, P);
     return hipGetLastError();
   });
 }
 template <class T, class W>
 static hipError_t norm_grad_go(const LayerNormGradParams& P, hipStream_t s) {
   const unsigned groups = (unsigned)layer_norm_groups(P.rows, P.cols);
-  return for_width(P.cols, [&](auto l, auto n) {
+  return for_width(P.cols, [&](auto l, auto n, auto even) {
     constexpr int L = decltype(l)::value, N = decltype(n)::value;
-    if constexpr (L == 0) hipLaunchKernelGGL((k_layer_norm_grad_long<T, W>), dim3(groups), dim3(1024), 0, s, P);
-    else if constexpr (sizeof(T) < sizeof(W)) {
-      if (P.residual) hipLaunchKernelGGL((k_layer_norm_grad<T, W, L, N, true>), dim3(groups), dim3(group_threads(L)), 0, s, P);
-      else hipLaunchKernelGGL((k_layer_norm_grad<T, W, L, N, false>), dim3(groups), dim3(group_threads(L)), 0, s, P);
-    } else hipLaunchKernelGGL((k_layer_norm_grad<T, W, L, N, false>), dim3(groups), dim3(group_threads(L)), 0, s, P);
+    constexpr bool E = decltype(even)::value;
+    auto go = [&](auto again) {
+      hipLaunchKernelGGL((k_layer_norm_grad<T, W, L, N, E, decltype(again)::value>), dim3(groups), dim3(group_threads(L)), 0, s, P);
+    };
+    if constexpr (L == 0) {
+      hipLaunchKernelGGL((k_layer_norm_grad_long<T, W, E>), dim3(groups), dim3(1024), 0, s, P);
+    } else if constexpr (sizeof(T) < sizeof(W)) {
+      if (P.residual) go(std::true_type{});
+      else go(std::false_type{});
+    } else {
+      go(std::false_type{});
+    }
     return hipGetLastError();
   });
 }
