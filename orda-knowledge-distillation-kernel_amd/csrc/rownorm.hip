@@ -481,21 +481,19 @@ static hipError_t for_width(int64_t cols, const F& f) {
 static int64_t rows_per_group(int64_t cols) { return cols <= 64 ? 32 : cols <= 1024 ? 4 : 1; }
 static int64_t threads_of(int64_t cols) { return cols <= 4096 ? 256 : 1024; }
 
-#ifndef GRAD_GROUPS
-#define GRAD_GROUPS 512
-#endif
-#ifndef NORM_GROUPS
-#define NORM_GROUPS 2048
-#endif
+// Workgroups of a pass: at 16384 x 4096 any number from 256 to 1024 backward and
+// from 1024 to 16384 forward takes the same time (130 to 143 us, 92 to 96); fewer
+// backward are fewer sums to add up.
+constexpr int64_t kGradGroups = 512, kNormGroups = 2048;
 int64_t layer_norm_groups(int64_t rows, int64_t cols) {
   const int64_t steps = (rows + rows_per_group(cols) - 1) / rows_per_group(cols);
-  return std::min<int64_t>(steps, threads_of(cols) == 256 ? GRAD_GROUPS : 256);
+  return std::min<int64_t>(steps, threads_of(cols) == 256 ? kGradGroups : 256);
 }
 
 template <class T, class W>
 static hipError_t norm_go(const LayerNormParams& P, hipStream_t s) {
   const int64_t steps = (P.rows + rows_per_group(P.cols) - 1) / rows_per_group(P.cols);
-  const unsigned groups = (unsigned)std::min<int64_t>(steps, threads_of(P.cols) == 256 ? NORM_GROUPS : 512);
+  const unsigned groups = (unsigned)std::min<int64_t>(steps, threads_of(P.cols) == 256 ? kNormGroups : 512);
   return for_width(P.cols, [&](auto l, auto n, auto even) {
     constexpr int L = decltype(l)::value, N = decltype(n)::value;
     constexpr bool E = decltype(even)::value;

@@ -28,11 +28,15 @@ Tensor embedding_run(const Tensor& ids, const Tensor& weight, double scale, int6
 }
 
 struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
+  struct Kept {
+    orda_embedding_t p;
+    int64_t type, weight_type;
+  };
   static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale, int64_t padding, int64_t type) {
     const Tensor y = embedding_run(ids, weight, scale, padding, static_cast<ScalarType>(type));
     ctx->save_for_backward({ids});
-    ctx->saved_data["scale"] = scale;
-    ctx->saved_data["n"] = std::vector<int64_t>{ids.numel(), weight.size(0), weight.size(1), padding, type, (int64_t)weight.scalar_type()};
+    ctx->saved_data["kept"] = packed(Kept{embedding_problem(ids.numel(), ids, weight.size(0), weight.size(1), weight.scalar_type(),
+                                                            static_cast<ScalarType>(type), scale, padding), type, (int64_t)weight.scalar_type()});
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -42,15 +46,15 @@ struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
     const at::AutoGradMode off(false);
     const c10::DeviceGuard guard(grads[0].device());
     check_capture("token_embedding");
-    const std::vector<int64_t> n = ctx->saved_data["n"].toIntVector();
-    Tensor ids = restored(ctx->get_saved_variables()[0], {n[0]}, grads[0].device());
-    if (ids.scalar_type() != at::kInt) ids = ids.to(at::kLong);
+    const Kept kept = unpacked<Kept>(ctx->saved_data["kept"].toStringRef());
+    orda_embedding_t p = kept.p;
+    Tensor ids = restored(ctx->get_saved_variables()[0], {p.tokens}, grads[0].device());
+    if (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) ids = ids.to(at::kLong);
     ids = ids.contiguous();
-    const ScalarType type = static_cast<ScalarType>(n[4]), wt = static_cast<ScalarType>(n[5]);
-    const Tensor dy = rows_of(grads[0], type);
-    orda_embedding_t p = embedding_problem(n[0], ids, n[1], n[2], wt, type, ctx->saved_data["scale"].toDouble(), n[3]);
+    p.wide_ids = ids.scalar_type() == at::kLong;
+    const Tensor dy = rows_of(grads[0], static_cast<ScalarType>(kept.type));
     p.ldg = pitch(dy);
-    g[1] = at::empty({n[1], n[2]}, dy.options().dtype(wt));
+    g[1] = at::empty({p.vocab, p.hidden}, dy.options().dtype(static_cast<ScalarType>(kept.weight_type)));
     const size_t bytes_needed = size_of(api.embedding_workspace_bytes(&p), "orda_embedding_workspace_bytes");
     const Tensor ws = bytes(bytes_needed, dy);
     check(api.embedding_backward(&p, ptr(ids), ptr(dy), out(g[1]), out(ws), bytes_needed, stream_of(dy)), "orda_embedding_backward");
@@ -73,14 +77,16 @@ struct Drop {
   Tensor on_device;  // or undefined
   orda_dropout_t c() const { return {p, seed, on_device.defined() ? on_device.const_data_ptr<int64_t>() : nullptr, site}; }
 };
-void save_drop(AutogradContext* ctx, const Drop& d) {
-  ctx->saved_data["p"] = d.p;
-  ctx->saved_data["drop"] = std::vector<int64_t>{(int64_t)d.seed, (int64_t)d.site, d.on_device.defined()};
-}
+// What a node keeps of it beside the seed's tensor.
+struct KeptDrop {
+  double p;
+  uint64_t seed, site;
+  int64_t on_device;
+};
+KeptDrop kept_drop(const Drop& d) { return {d.p, d.seed, d.site, d.on_device.defined()}; }
 // seed: what the node saved of the seed's tensor
-Drop restored_drop(AutogradContext* ctx, const Tensor& seed, const c10::Device& device) {
-  const std::vector<int64_t> v = ctx->saved_data["drop"].toIntVector();
-  return {ctx->saved_data["p"].toDouble(), (uint64_t)v[0], (uint64_t)v[1], v[2] ? restored_dense(seed, {1}, at::kLong, device) : Tensor()};
+Drop restored_drop(const KeptDrop& k, const Tensor& seed, const c10::Device& device) {
+  return {k.p, k.seed, k.site, k.on_device ? restored_dense(seed, {1}, at::kLong, device) : Tensor()};
 }
 
 Tensor dropout_run(const Tensor& x_, const Tensor& res_, const Drop& d, ScalarType type) {
@@ -102,13 +108,16 @@ Tensor dropout_run(const Tensor& x_, const Tensor& res_, const Drop& d, ScalarTy
 }
 
 struct DropoutNode : torch::autograd::Function<DropoutNode> {
+  struct Kept {
+    KeptDrop drop;
+    int64_t types[4];
+  };
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& res_, double p, int64_t seed, int64_t site, const OptTensor& on_device, int64_t type) {
     const ScalarType t = static_cast<ScalarType>(type);
     const Drop d{p, (uint64_t)seed, (uint64_t)site, given(on_device)};
     const Tensor res = given(res_);
-    save_drop(ctx, d);
     ctx->save_for_backward({d.on_device});
-    ctx->saved_data["types"] = std::vector<int64_t>{type, type_or(x, t), type_or(res, t), res.defined()};
+    ctx->saved_data["kept"] = packed(Kept{kept_drop(d), {type, type_or(x, t), type_or(res, t), res.defined()}});
     return dropout_run(x, res, d, t);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -116,13 +125,13 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
     if (!grads[0].defined()) return g;
     const bool graph = at::GradMode::is_enabled();
     const at::AutoGradMode off(false);
-    const std::vector<int64_t> types = ctx->saved_data["types"].toIntVector();
-    auto type = [&](int i) { return static_cast<ScalarType>(types[i]); };
-    if (types[3] && ctx->needs_input_grad(1)) g[1] = grads[0].to(type(2));
+    const Kept kept = unpacked<Kept>(ctx->saved_data["kept"].toStringRef());
+    auto type = [&](int i) { return static_cast<ScalarType>(kept.types[i]); };
+    if (kept.types[3] && ctx->needs_input_grad(1)) g[1] = grads[0].to(type(2));
     if (ctx->needs_input_grad(0)) {
       const c10::DeviceGuard guard(grads[0].device());
       check_capture("counter_dropout");
-      const Drop d = restored_drop(ctx, ctx->get_saved_variables()[0], grads[0].device());
+      const Drop d = restored_drop(kept.drop, ctx->get_saved_variables()[0], grads[0].device());
       g[0] = as_type(dropout_run(grads[0], Tensor(), d, type(0)), type(1));
     }
     return once(std::move(g), graph);
@@ -173,6 +182,11 @@ NormCall norm_run(const Tensor& x_, const Tensor& w, const Tensor& b_, const Ten
 }
 
 struct NormNode : torch::autograd::Function<NormNode> {
+  struct Kept {
+    orda_layer_norm_t p;
+    KeptDrop drop;
+    int64_t types[7];
+  };
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& b_, const OptTensor& res_, double eps, double p,
                                int64_t seed, int64_t site, const OptTensor& on_device, int64_t type) {
     const ScalarType t = static_cast<ScalarType>(type);
@@ -180,10 +194,8 @@ struct NormNode : torch::autograd::Function<NormNode> {
     const Drop d{p, (uint64_t)seed, (uint64_t)site, given(on_device)};
     NormCall c = norm_run(x, w, b, res, eps, d, t, true);
     ctx->set_materialize_grads(false);
-    save_drop(ctx, d);
     ctx->save_for_backward({c.s, c.stats, c.w, d.on_device, c.r});
-    ctx->saved_data["norm"] = packed(c.p);
-    ctx->saved_data["types"] = std::vector<int64_t>{type, type_or(x, t), type_or(w, t), type_or(b, t), type_or(res, t), b.defined(), res.defined()};
+    ctx->saved_data["kept"] = packed(Kept{c.p, kept_drop(d), {type, type_or(x, t), type_or(w, t), type_or(b, t), type_or(res, t), b.defined(), res.defined()}});
     return res.defined() ? variable_list{c.y, c.stream} : variable_list{c.y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -194,11 +206,11 @@ struct NormNode : torch::autograd::Function<NormNode> {
     const at::AutoGradMode off(false);
     const c10::Device device = any.device();
     const c10::DeviceGuard guard(device);
-    orda_layer_norm_t p = unpacked<orda_layer_norm_t>(ctx->saved_data["norm"].toStringRef());
-    const std::vector<int64_t> types = ctx->saved_data["types"].toIntVector();
-    auto type = [&](int i) { return static_cast<ScalarType>(types[i]); };
+    const Kept kept = unpacked<Kept>(ctx->saved_data["kept"].toStringRef());
+    orda_layer_norm_t p = kept.p;
+    auto type = [&](int i) { return static_cast<ScalarType>(kept.types[i]); };
     const ScalarType t = type(0), pt = p.param_dtype == ORDA_F32 ? at::kFloat : t;
-    const bool has_b = types[5] != 0, has_r = types[6] != 0;
+    const bool has_b = kept.types[5] != 0, has_r = kept.types[6] != 0;
     // (edges are numbered over the tensors that were given)
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = has_b && ctx->needs_input_grad(2);
     const bool nr = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
@@ -208,7 +220,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     const Tensor s = rows_of(restored(v[0], {p.rows, p.cols}, device), t);
     const Tensor stats = restored_dense(v[1], {p.rows, 2}, at::kFloat, device), w = restored_dense(v[2], {p.cols}, pt, device);
     const Tensor r = has_r && pt != t ? rows_of(restored(v[4], {p.rows, p.cols}, device), t) : Tensor();
-    const Drop d = restored_drop(ctx, v[3], device);
+    const Drop d = restored_drop(kept.drop, v[3], device);
     const Tensor dy = grads[0].defined() ? rows_of(grads[0], t) : at::zeros({p.rows, p.cols}, any.options().dtype(t));
     const Tensor ds = has_r && grads[1].defined() ? rows_of(grads[1], t) : Tensor();
     p.ld_s = pitch(s);
@@ -297,6 +309,10 @@ AttentionCall attention_run(const Tensor& q, const Tensor& k, const Tensor& v, c
 Tensor without_padding(const Tensor& t, int64_t D) { return t.size(3) == D ? t : t.narrow(3, 0, D).contiguous(); }
 
 struct AttentionNode : torch::autograd::Function<AttentionNode> {
+  struct Kept {
+    orda_attention_t p;
+    int64_t types[8];
+  };
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& slopes_, const OptTensor& docs_,
                         const OptTensor& prefix_, bool causal, double scale, double softcap, int64_t type) {
     const ScalarType t = static_cast<ScalarType>(type);
@@ -304,8 +320,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     AttentionCall c = attention_run(q, k, v, slopes, docs, prefix, causal, scale, softcap, t, true);
     const Tensor y = without_padding(c.o, q.size(3));
     ctx->save_for_backward({c.q, c.k, c.v, c.o, c.saved, slopes, prefix});
-    ctx->saved_data["p"] = packed(c.p);
-    ctx->saved_data["types"] = std::vector<int64_t>{type, type_or(q, t), type_or(k, t), type_or(v, t), docs.defined(), slopes.defined(), prefix.defined(), q.size(3)};
+    ctx->saved_data["kept"] = packed(Kept{c.p, {type, type_or(q, t), type_or(k, t), type_or(v, t), docs.defined(), slopes.defined(), prefix.defined(), q.size(3)}});
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -318,8 +333,9 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     const bool n[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2)};
     if (!n[0] && !n[1] && !n[2]) return g;
     check_capture("masked_attention");
-    orda_attention_t p = unpacked<orda_attention_t>(ctx->saved_data["p"].toStringRef());
-    const std::vector<int64_t> types = ctx->saved_data["types"].toIntVector();
+    const Kept node = unpacked<Kept>(ctx->saved_data["kept"].toStringRef());
+    orda_attention_t p = node.p;
+    const int64_t(&types)[8] = node.types;
     const ScalarType t = static_cast<ScalarType>(types[0]);
     const variable_list s = ctx->get_saved_variables();
     const int64_t width = p.head_dim, rows[4] = {p.batch, p.length, p.heads, width}, kv[4] = {p.batch, p.length, p.kv_heads, width};
