@@ -385,58 +385,63 @@ __device__ __forceinline__ uint32_t lds_at(const void* p) { return (uint32_t)(ui
 // nobody reads the tile before this one any more, nor this one's `ahead`
 // operands, so that the tile after the next goes there.
 //
-// f.issue(tile, n), f.ready(tile, n): the n-th tile sent for; arrived.
-// f.hidden(row): whether none of the wave's rows meets the 32 from `row` on.
-// f.ahead<BLOCK>(n): products of that block of the n-th tile, into the BLOCK-th
-// set of registers.  f.work<BLOCK>(tile, n, then): the block's softmax and what
-// follows, beside `ahead` of the next block, which is in the `then`-th tile
-// (behind the last tile: of what lies in LDS, unused).
+// f.issue(tile, two, three), f.ready(tile, two, three): the tile sent for, in that
+// slot of the two and of the three; arrived.  f.hidden(row): whether none of the
+// wave's rows meets the 32 from `row` on.  f.ahead<BLOCK>(two): products of that
+// block of the tile, into the BLOCK-th set of registers.  f.work<BLOCK>(tile,
+// three, two): the block's softmax and what follows, beside `ahead` of the next
+// block, which is in slot `two` (behind the last tile: of what lies in LDS,
+// unused).
 template <class F>
 __device__ __forceinline__ void attn_walk(AttnWalk<true>& walk, F& f) {
   AttnTile t0 = walk.next();
   if (t0.first < 0) return;
   AttnTile t1 = walk.next();
-  f.issue(t0, 0);
-  if (t1.first >= 0) f.issue(t1, 1);
+  int two = 0, three = 0, after = 1, behind = 2;
+  f.issue(t0, 0, 0);
+  if (t1.first >= 0) f.issue(t1, 1, 1);
   wait_vmem<0>();
   tile_barrier();
-  f.ready(t0, 0);
-  if (t1.first >= 0) f.ready(t1, 1);
+  f.ready(t0, 0, 0);
+  if (t1.first >= 0) f.ready(t1, 1, 1);
   f.template ahead<0>(0);
-  bool sent = true;  // (the first two tiles have arrived)
-  for (int n = 0;; ++n) {
-    if (!f.hidden(t0.first)) f.template work<0>(t0, n, n);  // (blocks that are hidden are followed by none that are not)
+  for (bool sent = true;; sent = false) {  // (sent: the first two tiles have arrived)
+    if (!f.hidden(t0.first)) f.template work<0>(t0, three, two);  // (blocks that are hidden are followed by none that are not)
     AttnTile t2{-1, false, false, 0};
     if (t1.first >= 0) {
       t2 = walk.next();
       wait_vmem<0>();
       tile_barrier();
-      if (t2.first >= 0) f.issue(t2, n + 2);
-      if (!sent) f.ready(t1, n + 1);
-      sent = false;
+      if (t2.first >= 0) f.issue(t2, two, behind);
+      if (!sent) f.ready(t1, two ^ 1, after);
     }
-    if (!f.hidden(t0.first + 32)) f.template work<1>(t0, n, n + 1);
+    if (!f.hidden(t0.first + 32)) f.template work<1>(t0, three, two ^ 1);
     if (t1.first < 0) return;
     t0 = t1;
     t1 = t2;
+    two ^= 1;
+    const int free = three;
+    three = after;
+    after = behind;
+    behind = free;
   }
 }
 
 // The same without products ahead, where the registers do not hold them and two
-// waves of a SIMD run beside each other: two slots, f.work<BLOCK>(tile, n).
+// waves of a SIMD run beside each other: two slots, f.work<BLOCK>(tile, slot).
 template <class F>
 __device__ __forceinline__ void attn_walk_plain(AttnWalk<true>& walk, F& f) {
   AttnTile t = walk.next();
   if (t.first < 0) return;
   f.issue(t, 0);
-  for (int n = 0;; ++n) {
+  for (int slot = 0;; slot ^= 1) {
     const AttnTile then = walk.next();
     wait_vmem<0>();
     tile_barrier();
-    if (then.first >= 0) f.issue(then, n + 1);
-    f.ready(t, n);
-    if (!f.hidden(t.first)) f.template work<0>(t, n);
-    if (!f.hidden(t.first + 32)) f.template work<1>(t, n);
+    if (then.first >= 0) f.issue(then, slot ^ 1);
+    f.ready(t, slot);
+    if (!f.hidden(t.first)) f.template work<0>(t, slot);
+    if (!f.hidden(t.first + 32)) f.template work<1>(t, slot);
     if (then.first < 0) return;
     t = then;
   }
@@ -459,17 +464,17 @@ struct AttnForward {
   float m, l, slope;
   int row0, i, bound, doc, prefix;
   __device__ __forceinline__ AttnForward(const AttnParams& p) : P(p) {}
-  __device__ __forceinline__ void issue(const AttnTile& t, int n) {
-    kd.issue(K + t.first * P.ks, (int)P.S - t.first, klds + (n & 1) * kTile);
-    vd.issue(V + t.first * P.vs, (int)P.S - t.first, vlds + (n % 3) * kTile);
+  __device__ __forceinline__ void issue(const AttnTile& t, int two, int three) {
+    kd.issue(K + t.first * P.ks, (int)P.S - t.first, klds + two * kTile);
+    vd.issue(V + t.first * P.vs, (int)P.S - t.first, vlds + three * kTile);
   }
-  __device__ __forceinline__ void ready(const AttnTile& t, int n) {
-    if (t.pad) clear_padding<HD>(docs + t.first, klds + (n & 1) * kTile, vlds + (n % 3) * kTile);
+  __device__ __forceinline__ void ready(const AttnTile& t, int two, int three) {
+    if (t.pad) clear_padding<HD>(docs + t.first, klds + two * kTile, vlds + three * kTile);
   }
   __device__ __forceinline__ bool hidden(int row) const { return P.causal && row > row0 + 31 && row >= prefix; }
   template <int BLOCK>
-  __device__ __forceinline__ void fetch(int n) {
-    const char* kt = klds + (n & 1) * kTile + BLOCK * kHalf;
+  __device__ __forceinline__ void fetch(int two) {
+    const char* kt = klds + two * kTile + BLOCK * kHalf;
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) rows[ks] = fr.rows(kt, ks);
   }
@@ -482,15 +487,17 @@ struct AttnForward {
     for (int ks = 0; ks < HD / 16; ++ks) z = Traits<T>::mma(rows[ks], q[ks], z);
   }
   template <int BLOCK>
-  __device__ __forceinline__ void ahead(int n) {
-    fetch<BLOCK>(n);
+  __device__ __forceinline__ void ahead(int two) {
+    fetch<BLOCK>(two);
     products<BLOCK>();
   }
   template <int BLOCK>
-  __device__ __forceinline__ void work(const AttnTile& t, int n, int then) {
+  __device__ __forceinline__ void work(const AttnTile& t, int three, int two) {
     const int at = t.first + 32 * BLOCK;
     f32x16& x = s[BLOCK];
-    fetch<1 - BLOCK>(then);
+    fetch<1 - BLOCK>(two);
+    Frag vf[2][kBlocks];
+    fr.cols(lds_at(vlds) + (uint32_t)(three * kTile + BLOCK * kHalf), vf);  // (one wait for both)
     float th[16];
     scores<CAP, BIAS>(x, th, P, slope, i - at);
     if (t.part) hide<true>(x, bound - at, docs ? docs + at : nullptr, doc);
@@ -520,9 +527,8 @@ struct AttnForward {
     }
     l += sum[0] + sum[1];
     // P is rounded to 16 bits as an operand of the product, its sum is not
-    Frag pf[2], vf[2][kBlocks];
+    Frag pf[2];
     as_operand<T>(p, pf);
-    fr.cols(lds_at(vlds) + (uint32_t)((n % 3) * kTile + BLOCK * kHalf), vf);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -531,7 +537,7 @@ struct AttnForward {
 };
 
 template <class T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void k_attn(AttnParams P) {
+__global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
   constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32;
   __shared__ __attribute__((aligned(1024))) char lds[5 * kTile];
   int bh, q0;
@@ -593,18 +599,18 @@ struct AttnGradQ {
   float lse, delta, slope;
   int row0, i, bound, doc, prefix;
   __device__ __forceinline__ AttnGradQ(const AttnParams& p) : P(p) {}
-  __device__ __forceinline__ void issue(const AttnTile& t, int n) {
-    kd.issue(K + t.first * P.ks, (int)P.S - t.first, klds + (n & 1) * kTile);
-    vd.issue(V + t.first * P.vs, (int)P.S - t.first, vlds + (n & 1) * kTile);
+  __device__ __forceinline__ void issue(const AttnTile& t, int slot) {
+    kd.issue(K + t.first * P.ks, (int)P.S - t.first, klds + slot * kTile);
+    vd.issue(V + t.first * P.vs, (int)P.S - t.first, vlds + slot * kTile);
   }
-  __device__ __forceinline__ void ready(const AttnTile& t, int n) {
-    if (t.pad) clear_padding<HD>(docs + t.first, klds + (n & 1) * kTile, vlds + (n & 1) * kTile);
+  __device__ __forceinline__ void ready(const AttnTile& t, int slot) {
+    if (t.pad) clear_padding<HD>(docs + t.first, klds + slot * kTile, vlds + slot * kTile);
   }
   __device__ __forceinline__ bool hidden(int row) const { return P.causal && row > row0 + 31 && row >= prefix; }
   template <int BLOCK>
-  __device__ __forceinline__ void work(const AttnTile& t, int n) {
+  __device__ __forceinline__ void work(const AttnTile& t, int slot) {
     const int at = t.first + 32 * BLOCK;
-    const char *kt = klds + (n & 1) * kTile + BLOCK * kHalf, *vt = vlds + (n & 1) * kTile + BLOCK * kHalf;
+    const char *kt = klds + slot * kTile + BLOCK * kHalf, *vt = vlds + slot * kTile + BLOCK * kHalf;
     f32x16 x, dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = dp[r] = 0.0f;
@@ -630,7 +636,7 @@ struct AttnGradQ {
     }
     Frag zf[2], kf[2][kBlocks];
     as_operand<T>(z, zf);  // (dz in 16 bits, as an operand of the product)
-    fr.cols(lds_at(klds) + (uint32_t)((n & 1) * kTile + BLOCK * kHalf), kf);
+    fr.cols(lds_at(klds) + (uint32_t)(slot * kTile + BLOCK * kHalf), kf);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -639,7 +645,7 @@ struct AttnGradQ {
 };
 
 template <class T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void k_attn_dq(AttnParams P) {
+__global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P) {
   constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32;
   __shared__ __attribute__((aligned(1024))) char lds[4 * kTile];
   int bh, q0;
@@ -732,21 +738,21 @@ struct AttnGradKV {
   Frag zf[2];                            // second: dz of the last phase's block
   int row0, key, bound, doc, prefix;
   __device__ __forceinline__ AttnGradKV(const AttnParams& p) : P(p) {}
-  __device__ __forceinline__ void issue(const AttnTile& t, int n) {
-    qd.issue(Q + t.head * P.qh + t.first * P.qs, (int)P.S - t.first, qlds + (n % 3) * kTile);
-    gd.issue(G + t.head * P.gh + t.first * P.gs, (int)P.S - t.first, glds + (n % 3) * kTile);
+  __device__ __forceinline__ void issue(const AttnTile& t, int slot) {
+    qd.issue(Q + t.head * P.qh + t.first * P.qs, (int)P.S - t.first, qlds + slot * kTile);
+    gd.issue(G + t.head * P.gh + t.first * P.gs, (int)P.S - t.first, glds + slot * kTile);
     const int w = wave_id();
     if (w < 2)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of((w ? delta : lse) + t.head * P.padded + t.first),
-                                               (__attribute__((address_space(3))) void*)(stats + (n % 3) * kStats + w * (kStats / 2)), 4,
+                                               (__attribute__((address_space(3))) void*)(stats + slot * kStats + w * (kStats / 2)), 4,
                                                (threadIdx.x & 63) * 4, 0, 0, 0);
   }
-  __device__ __forceinline__ void ready(const AttnTile& t, int n) {
-    if (t.pad) clear_padding<HD>(docs + t.first, qlds + (n % 3) * kTile, glds + (n % 3) * kTile);
+  __device__ __forceinline__ void ready(const AttnTile& t, int slot) {
+    if (t.pad) clear_padding<HD>(docs + t.first, qlds + slot * kTile, glds + slot * kTile);
   }
   __device__ __forceinline__ bool hidden(int row) const { return P.causal && row0 > row + 31 && row0 >= prefix; }
-  __device__ __forceinline__ char* qrows(int n, int block) const { return qlds + (n % 3) * kTile + block * kHalf; }
-  __device__ __forceinline__ char* grows(int n, int block) const { return glds + (n % 3) * kTile + block * kHalf; }
+  __device__ __forceinline__ char* qrows(int slot, int block) const { return qlds + slot * kTile + block * kHalf; }
+  __device__ __forceinline__ char* grows(int slot, int block) const { return glds + slot * kTile + block * kHalf; }
   __device__ __forceinline__ void fetch(const char* at) {
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) rows[ks] = fr.rows(at, ks);
@@ -764,21 +770,21 @@ struct AttnGradKV {
       for (int d = 0; d < kBlocks; ++d) acc[d] = Traits<T>::mma(cf[j][d], f[j], acc[d]);
   }
   // four consecutive queries of the lane's rows at a time
-  __device__ __forceinline__ const char* stat(int n, int block, int which) const {
-    return stats + (n % 3) * kStats + which * (kStats / 2) + 128 * block + ((threadIdx.x & 63) >> 5) * 16;
+  __device__ __forceinline__ const char* stat(int slot, int block, int which) const {
+    return stats + slot * kStats + which * (kStats / 2) + 128 * block + ((threadIdx.x & 63) >> 5) * 16;
   }
   __device__ __forceinline__ char* prob(int buffer) const { return probs + buffer * kProbs + (wave_id() & 3) * 4096 + (threadIdx.x & 63) * 16; }
-  // The first wave's phase: block BLOCK of tile t; `then`: S of the block behind
-  // it, block 1 - BLOCK of tile tn.
+  // The first wave's phase: block BLOCK of tile t in `slot`; `then`: S of the block
+  // behind it, block 1 - BLOCK of the tile in slot `to`.
   template <int BLOCK>
-  __device__ __forceinline__ void lead(const AttnTile& t, int n, bool then, int tn) {
+  __device__ __forceinline__ void lead(const AttnTile& t, int slot, bool then, int to) {
     const int at = t.first + 32 * BLOCK;
-    if (then) fetch(qrows(tn, 1 - BLOCK));
+    if (then) fetch(qrows(to, 1 - BLOCK));
     if (!hidden(at)) {
       f4v L[4];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) L[g] = *reinterpret_cast<const f4v*>(stat(n, BLOCK, 0) + 32 * g);
-      fr.cols(lds_at(grows(n, BLOCK)), cf);
+      for (int g = 0; g < 4; ++g) L[g] = *reinterpret_cast<const f4v*>(stat(slot, BLOCK, 0) + 32 * g);
+      fr.cols(lds_at(grows(slot, BLOCK)), cf);
       float th[16], p[16];
       scores<CAP, BIAS>(x, th, P, BIAS ? slopes[t.head] * kLog2e : 0.0f, key - at);
       if (t.part) hide<false>(x, bound - at, docs ? docs + at : nullptr, doc);
@@ -801,10 +807,11 @@ struct AttnGradKV {
     if (then) product(x);
   }
   // The second wave's: dk of block BLOCK of tile u (has: there is one), dz of
-  // block 1 - BLOCK of tile t, and the operands of the next phase, dP of block
-  // BLOCK of tile next (more: there is one) and dk of the block whose dz this is.
+  // block 1 - BLOCK of tile t in `slot` (here: there is one), and the operands of
+  // the next phase, dP of block BLOCK of the tile in slot `to` (more: there is
+  // one) and dk of the block whose dz this is.
   template <int BLOCK>
-  __device__ __forceinline__ void follow(const AttnTile& u, bool has, const AttnTile& t, int n, bool here, int next, bool more) {
+  __device__ __forceinline__ void follow(const AttnTile& u, bool has, const AttnTile& t, int slot, bool here, int to, bool more) {
     constexpr int kOther = 1 - BLOCK;
     if (has && !hidden(u.first + 32 * BLOCK)) add_up(zf);
     if (here && !hidden(t.first + 32 * kOther)) {
@@ -812,7 +819,7 @@ struct AttnGradKV {
       f4v dl[4], p[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        dl[g] = *reinterpret_cast<const f4v*>(stat(n, kOther, 1) + 32 * g);
+        dl[g] = *reinterpret_cast<const f4v*>(stat(slot, kOther, 1) + 32 * g);
         p[g] = *reinterpret_cast<const f4v*>(prob(kOther) + g * 1024);
       }
       product(dp);
@@ -821,8 +828,8 @@ struct AttnGradKV {
       for (int r = 0; r < 16; ++r) z[r] = p[r >> 2][r & 3] * (dp[r] - dl[r >> 2][r & 3]);
       as_operand<T>(z, zf);
     }
-    if (more) fetch(grows(next, BLOCK));
-    if (here) fr.cols(lds_at(qrows(n, kOther)), cf);
+    if (more) fetch(grows(to, BLOCK));
+    if (here) fr.cols(lds_at(qrows(slot, kOther)), cf);
   }
   // (a loop of its own for each of the two: in one, what either holds would take
   // registers of both)
@@ -842,26 +849,30 @@ struct AttnGradKV {
         product(x);
       }
     }
-    int n = 0;
-    for (;; ++n) {
-      if constexpr (LEADS) lead<0>(t0, n, !hidden(t0.first + 32), n);
-      else follow<0>(last, n > 0, last, n + 2, n > 0, n, true);  // (n + 2: the slots of n - 1)
+    int slot = 0, after = 1, behind = 2;  // of t0, t1, and the tile before t0
+    for (bool first = true;; first = false) {
+      if constexpr (LEADS) lead<0>(t0, slot, !hidden(t0.first + 32), slot);
+      else follow<0>(last, !first, last, behind, !first, slot, true);
       wait_vmem<0>();  // (t1, sent for two phases ago)
       tile_barrier();
       const AttnTile t2 = w.next();
-      if (t2.first >= 0) issue(t2, n + 2);  // (over the tile before t0, whose last block was read in the phase before)
+      if (t2.first >= 0) issue(t2, behind);  // (whose last block was read in the phase before)
       const bool more = t1.first >= 0;
-      if (more) ready(t1, n + 1);
-      if constexpr (LEADS) lead<1>(t0, n, more && !hidden(t1.first), n + 1);
-      else follow<1>(last, n > 0, t0, n, true, n, true);
+      if (more) ready(t1, after);
+      if constexpr (LEADS) lead<1>(t0, slot, more && !hidden(t1.first), after);
+      else follow<1>(last, !first, t0, slot, true, slot, true);
       tile_barrier();
       last = t0;
       if (!more) break;
       t0 = t1;
       t1 = t2;
+      const int free = behind;
+      behind = slot;
+      slot = after;
+      after = free;
     }
     if constexpr (!LEADS) {
-      follow<0>(last, true, last, n, true, n, false);
+      follow<0>(last, true, last, slot, true, slot, false);
       if (!hidden(last.first + 32)) add_up(zf);
     }
   }
