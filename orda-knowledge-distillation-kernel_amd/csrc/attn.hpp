@@ -24,10 +24,10 @@
 // five that one kernel would need, whose gradients of q would have to be added
 // up by atomics in an order that changes from run to run.
 //
-// LDS: a tile's rows of HD elements (64 or 128; a head of D < HD is zero-padded
-// on the way in), chunk c (16 bytes) of row r at c ^ swz(r), so that neither 16
-// rows at one chunk (row reads) nor 4 rows at 64 bytes (transposed reads) meet
-// in a bank.
+// LDS: a tile's rows of 64 or 128 elements, of which HD (64, 96, 128) go through
+// the products (a head of D < HD is zero-padded on the way in), chunk c (16 bytes)
+// of row r at c ^ swz(r), so that neither 16 rows at one chunk (row reads) nor 4
+// rows at 64 bytes (transposed reads) meet in a bank.
 //
 // Which tiles are walked: 64 tiles at a time, lane t looks at tile t (causal
 // bound, prefix, the ranges of document numbers on both sides) and a ballot
@@ -42,23 +42,26 @@ constexpr int kAttnRows = 128;  // queries (forward, dq) or keys (dk, dv) of a w
 constexpr int kAttnTile = 64;   // rows of the other side that one step takes
 
 template <int HD>
+constexpr int kAttnLd = HD <= 64 ? 64 : 128;  // elements of a row in LDS
+
+template <int LD>
 __device__ __forceinline__ int attn_swz(int r) {
-  return HD == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  return LD == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
 }
 
 // Workgroup -> (head of the batch, tile of its rows).  An XCD takes whole heads,
 // so that its L2 holds their keys and values.  With a causal mask a tile's work
 // grows (or falls) with its number: of 8 heads of an XCD together the longest
 // tiles come first, so that the last to end are short ones.
-__device__ __forceinline__ void attn_place(const AttnParams& P, int heads, bool last_first, int& head, int& tile) {
+__device__ __forceinline__ void attn_place(const AttnParams& P, int id, int heads, bool last_first, int& head, int& tile) {
   constexpr int kTogether = 8;
   if (P.causal && heads % 8 == 0) {
-    const int per = heads / 8, local = blockIdx.x / 8;
+    const int per = heads / 8, local = id / 8;
     const int g = local / (kTogether * P.tiles) * kTogether, n = min(kTogether, per - g), in = local - g * P.tiles;
-    head = blockIdx.x % 8 * per + g + in % n;
+    head = id % 8 * per + g + in % n;
     tile = in / n;
   } else {
-    const int t = xcd_order(blockIdx.x, gridDim.x);
+    const int t = xcd_order(id, gridDim.x);
     head = t / P.tiles;
     tile = t - head * P.tiles;
   }
@@ -67,16 +70,16 @@ __device__ __forceinline__ void attn_place(const AttnParams& P, int heads, bool 
 
 // A tile of 64 rows to LDS, 16 bytes a lane.  Rows from `rows` on and columns
 // from D on arrive as zeros.
-template <int HD, int WAVES = 4>
+template <int LD, int WAVES = 4>
 struct AttnDma {
-  static constexpr int kChunks = HD / 8, kIssues = kChunks / WAVES, kStep = 64 * WAVES / kChunks;
+  static constexpr int kChunks = LD / 8, kIssues = kChunks / WAVES, kStep = 64 * WAVES / kChunks;
   static_assert(kIssues > 0 && kStep % 16 == 0, "rows kStep apart have one swizzle");
   uint32_t off[kIssues];
   int row;
   __device__ __forceinline__ void init(int64_t ss, int D) {
     const int p = wave_id() * 64 + (threadIdx.x & 63);
     row = p / kChunks;
-    const int c = (p % kChunks) ^ attn_swz<HD>(row);
+    const int c = (p % kChunks) ^ attn_swz<LD>(row);
 #pragma unroll
     for (int i = 0; i < kIssues; ++i) off[i] = c * 8 < D ? (uint32_t)(row + i * kStep) * (uint32_t)(ss * 2) + (uint32_t)c * 16 : kOob;
   }
@@ -96,14 +99,14 @@ struct AttnDma {
 // Fragments of a tile in LDS.
 template <class T, int HD>
 struct AttnFrags {
-  static constexpr int kRow = HD * 2, kBlocks = HD / 32;
+  static constexpr int kRow = kAttnLd<HD> * 2, kBlocks = HD / 32;
   uint32_t row_at, lo, hi;  // byte offsets in a tile
   __device__ __forceinline__ void init() {
     const int lane = threadIdx.x & 63, h = lane >> 5, r = lane & 31;
-    row_at = (uint32_t)(r * kRow + ((h ^ attn_swz<HD>(r)) << 4));
+    row_at = (uint32_t)(r * kRow + ((h ^ attn_swz<kAttnLd<HD>>(r)) << 4));
     const int s = lane & 15, k = 4 * h + (s >> 2), m = 16 * ((lane >> 4) & 1) + 4 * (s & 3);
-    lo = (uint32_t)(k * kRow + (((m >> 3) ^ attn_swz<HD>(k)) << 4) + (m & 7) * 2);
-    hi = (uint32_t)((k + 8) * kRow + (((m >> 3) ^ attn_swz<HD>(k + 8)) << 4) + (m & 7) * 2);
+    lo = (uint32_t)(k * kRow + (((m >> 3) ^ attn_swz<kAttnLd<HD>>(k)) << 4) + (m & 7) * 2);
+    hi = (uint32_t)((k + 8) * kRow + (((m >> 3) ^ attn_swz<kAttnLd<HD>>(k + 8)) << 4) + (m & 7) * 2);
   }
   // rows lane % 32 of the 32 at `block`, columns 16 ks + 8 (lane / 32)..
   __device__ __forceinline__ typename Traits<T>::Frag rows(const char* block, int ks) const {
@@ -132,6 +135,19 @@ struct AttnFrags {
             "=&v"(x[1][2][0]), "=&v"(x[1][2][1]), "=&v"(x[1][3][0]), "=&v"(x[1][3][1])
           : "v"(a), "v"(b), "v"(a ^ 64u), "v"(b ^ 64u), "v"(a ^ 128u), "v"(b ^ 128u), "v"(a ^ 192u), "v"(b ^ 192u), "n"(kOff)
           : "memory");
+    } else if constexpr (kBlocks == 3) {
+      asm volatile(
+          "ds_read_b64_tr_b16 %0, %12\n\tds_read_b64_tr_b16 %1, %13\n\t"
+          "ds_read_b64_tr_b16 %2, %14\n\tds_read_b64_tr_b16 %3, %15\n\t"
+          "ds_read_b64_tr_b16 %4, %16\n\tds_read_b64_tr_b16 %5, %17\n\t"
+          "ds_read_b64_tr_b16 %6, %12 offset:%18\n\tds_read_b64_tr_b16 %7, %13 offset:%18\n\t"
+          "ds_read_b64_tr_b16 %8, %14 offset:%18\n\tds_read_b64_tr_b16 %9, %15 offset:%18\n\t"
+          "ds_read_b64_tr_b16 %10, %16 offset:%18\n\tds_read_b64_tr_b16 %11, %17 offset:%18\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(x[0][0][0]), "=&v"(x[0][0][1]), "=&v"(x[0][1][0]), "=&v"(x[0][1][1]), "=&v"(x[0][2][0]), "=&v"(x[0][2][1]),
+            "=&v"(x[1][0][0]), "=&v"(x[1][0][1]), "=&v"(x[1][1][0]), "=&v"(x[1][1][1]), "=&v"(x[1][2][0]), "=&v"(x[1][2][1])
+          : "v"(a), "v"(b), "v"(a ^ 64u), "v"(b ^ 64u), "v"(a ^ 128u), "v"(b ^ 128u), "n"(kOff)
+          : "memory");
     } else {
       asm volatile(
           "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\t"
@@ -151,6 +167,19 @@ struct AttnFrags {
         out[k][d] = __builtin_bit_cast(typename Traits<T>::Frag, __builtin_shufflevector(x[k][d][0], x[k][d][1], 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };
+
+// acc^T as it is, to a row of fp32.
+template <int HD>
+__device__ __forceinline__ void store_part(const f32x16 (&acc)[HD / 32], float* p, int D, bool live) {
+  const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * d + 8 * g + 4 * h;
+      if (live && col < D) *reinterpret_cast<f4v*>(p + col) = f4v{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+    }
+}
 
 // The wave's own 32 rows as operands: row lane % 32, columns 16 ks + 8 h.. .
 // negate: with their signs turned.
@@ -308,9 +337,9 @@ struct AttnWalk {
 
 // Rows without a document: zeros in LDS, so that whatever they hold (nothing, for
 // what lies behind a batch's sequences) is not multiplied by a probability of 0.
-template <int HD>
+template <int LD>
 __device__ __forceinline__ void clear_padding(const int* docs, char* one, char* two) {
-  constexpr int kChunks = HD / 8;
+  constexpr int kChunks = LD / 8;
   for (int p = threadIdx.x; p < kAttnTile * kChunks; p += (int)blockDim.x)
     if (docs[p / kChunks] < 0) {
       reinterpret_cast<uint4*>(one)[p] = make_uint4(0, 0, 0, 0);
@@ -451,12 +480,12 @@ __device__ __forceinline__ void attn_walk_plain(AttnWalk<KEYS>& walk, F& f) {
 template <class T, int HD, bool CAP, bool BIAS>
 struct AttnForward {
   using Frag = typename Traits<T>::Frag;
-  static constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32, kHalf = kTile / 2;
+  static constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32, kHalf = kTile / 2;
   const AttnParams& P;
   char *klds, *vlds;  // two slots of K, three of V
   const T *K, *V;
   const int* docs;
-  AttnDma<HD> kd, vd;
+  AttnDma<kAttnLd<HD>> kd, vd;
   AttnFrags<T, HD> fr;
   Frag q[HD / 16], rows[HD / 16];
   f32x16 o[kBlocks];
@@ -469,7 +498,7 @@ struct AttnForward {
     vd.issue(V + t.first * P.vs, (int)P.S - t.first, vlds + three * kTile);
   }
   __device__ __forceinline__ void ready(const AttnTile& t, int two, int three) {
-    if (t.pad) clear_padding<HD>(docs + t.first, klds + two * kTile, vlds + three * kTile);
+    if (t.pad) clear_padding<kAttnLd<HD>>(docs + t.first, klds + two * kTile, vlds + three * kTile);
   }
   __device__ __forceinline__ bool hidden(int row) const { return P.causal && row > row0 + 31 && row >= prefix; }
   template <int BLOCK>
@@ -538,10 +567,10 @@ struct AttnForward {
 
 template <class T, int HD, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
-  constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32;
+  constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32;
   __shared__ __attribute__((aligned(1024))) char lds[5 * kTile];
   int bh, q0;
-  attn_place(P, P.B * P.H, true, bh, q0);
+  attn_place(P, blockIdx.x, P.B * P.H, true, bh, q0);
   q0 *= kAttnRows;
   const int b = bh / P.H, head = bh - b * P.H, kv = head / P.group;
   const int lane = threadIdx.x & 63, S = (int)P.S;
@@ -587,12 +616,12 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
 template <class T, int HD, bool CAP, bool BIAS>
 struct AttnGradQ {
   using Frag = typename Traits<T>::Frag;
-  static constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32, kHalf = kTile / 2;
+  static constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32, kHalf = kTile / 2;
   const AttnParams& P;
   char *klds, *vlds;  // two slots each
   const T *K, *V;
   const int* docs;
-  AttnDma<HD> kd, vd;
+  AttnDma<kAttnLd<HD>> kd, vd;
   AttnFrags<T, HD> fr;
   Frag q[HD / 16], g[HD / 16];
   f32x16 dq[kBlocks];
@@ -604,7 +633,7 @@ struct AttnGradQ {
     vd.issue(V + t.first * P.vs, (int)P.S - t.first, vlds + slot * kTile);
   }
   __device__ __forceinline__ void ready(const AttnTile& t, int slot) {
-    if (t.pad) clear_padding<HD>(docs + t.first, klds + slot * kTile, vlds + slot * kTile);
+    if (t.pad) clear_padding<kAttnLd<HD>>(docs + t.first, klds + slot * kTile, vlds + slot * kTile);
   }
   __device__ __forceinline__ bool hidden(int row) const { return P.causal && row > row0 + 31 && row >= prefix; }
   template <int BLOCK>
@@ -646,10 +675,10 @@ struct AttnGradQ {
 
 template <class T, int HD, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P) {
-  constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32;
+  constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32;
   __shared__ __attribute__((aligned(1024))) char lds[4 * kTile];
   int bh, q0;
-  attn_place(P, P.B * P.H, true, bh, q0);
+  attn_place(P, blockIdx.x, P.B * P.H, true, bh, q0);
   q0 *= kAttnRows;
   const int b = bh / P.H, head = bh - b * P.H, kv = head / P.group;
   const int lane = threadIdx.x & 63, S = (int)P.S;
@@ -715,10 +744,26 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P)
 // dv of p and S of p + 1; the second starts with the products dk of p - 2 and dP of
 // p - 1, whose operands it read in the phase before, and goes on with dz of p - 1:
 // while one has the matrix cores the other has the vector unit.
+struct AttnKeys {  // of a workgroup: batch, key head, first row, the heads it takes (of all that share these keys, or one part)
+  int b, kv, part, r0, head, heads;
+  __device__ __forceinline__ AttnKeys(const AttnParams& P, int id) {
+    int at;
+    attn_place(P, id, P.B * P.KV * P.parts, false, at, r0);
+    r0 *= kAttnRows;
+    part = at % P.parts;
+    b = at / P.parts / P.KV;
+    kv = at / P.parts - b * P.KV;
+    head = kv * P.group + part * P.share;
+    heads = min(P.share, P.group - part * P.share);
+  }
+  __device__ __forceinline__ int64_t row(const AttnParams& P, int key) const { return ((b * P.S + key) * P.KV + kv) * P.D; }
+  __device__ __forceinline__ float* partial(const AttnParams& P, int which) const { return P.partial + (which * P.parts + part) * (P.B * P.S * P.KV * P.D); }
+};
+
 template <class T, int HD, bool CAP, bool BIAS>
 struct AttnGradKV {
   using Frag = typename Traits<T>::Frag;
-  static constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32, kHalf = kTile / 2;
+  static constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32, kHalf = kTile / 2;
   static constexpr int kStats = 2 * kAttnTile * 4, kProbs = 4 * 4096;
   static constexpr int kLds = 6 * kTile + 2 * kProbs + 3 * kStats;
   const AttnParams& P;
@@ -729,7 +774,7 @@ struct AttnGradKV {
   const T *Q, *G;     // of the first head
   const float *lse, *delta, *slopes;
   const int* docs;
-  AttnDma<HD, 8> qd, gd;
+  AttnDma<kAttnLd<HD>, 8> qd, gd;
   AttnFrags<T, HD> fr;
   Frag own[HD / 16];  // the wave's keys, or their values
   f32x16 acc[kBlocks];
@@ -748,7 +793,7 @@ struct AttnGradKV {
                                                (threadIdx.x & 63) * 4, 0, 0, 0);
   }
   __device__ __forceinline__ void ready(const AttnTile& t, int slot) {
-    if (t.pad) clear_padding<HD>(docs + t.first, qlds + slot * kTile, glds + slot * kTile);
+    if (t.pad) clear_padding<kAttnLd<HD>>(docs + t.first, qlds + slot * kTile, glds + slot * kTile);
   }
   __device__ __forceinline__ bool hidden(int row) const { return P.causal && row0 > row + 31 && row0 >= prefix; }
   __device__ __forceinline__ char* qrows(int slot, int block) const { return qlds + slot * kTile + block * kHalf; }
@@ -883,10 +928,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_dkv(AttnParams P) {
   using F = AttnGradKV<T, HD, CAP, BIAS>;
   constexpr int kBlocks = HD / 32;
   __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
-  int bk, r0;
-  attn_place(P, P.B * P.KV, false, bk, r0);
-  r0 *= kAttnRows;
-  const int b = bk / P.KV, kv = bk - b * P.KV, head = kv * P.group;
+  const AttnKeys at(P, blockIdx.x);
+  const int b = at.b, kv = at.kv, r0 = at.r0, head = at.head;
   const int lane = threadIdx.x & 63, S = (int)P.S, w = wave_id();
   const bool leads = w < 4;
   F f(P);
@@ -913,37 +956,42 @@ __global__ __launch_bounds__(512, 2) void k_attn_dkv(AttnParams P) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) f.acc[d][r] = 0.0f;
   AttnWalk<false> walk;
-  walk.init(P, b, r0, P.group);
-  const int64_t at = (((int64_t)b * S + f.key) * P.KV + kv) * P.D;
-  const bool live = f.key < S;
+  walk.init(P, b, r0, at.heads);
   // (zeros for a padding row: what it holds may not be finite)
-  auto finish = [&](T* out, float mul) {
+  auto finish = [&](T* out, int which, float mul) {
     if (f.doc < 0)
 #pragma unroll
       for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) f.acc[d][r] = 0.0f;
-    if (out) store_own<T, HD>(f.acc, mul, out + at, P.D, live);
+    int id = blockIdx.x;
+    asm volatile("" : "+s"(id));  // (where the sums go is worked out again: the loop has no registers for it)
+    const AttnKeys to(P, id);
+    const int64_t row = to.row(P, f.key);
+    if (P.partial) store_part<HD>(f.acc, to.partial(P, which) + row, P.D, f.key < P.S);
+    else if (out) store_own<T, HD>(f.acc, mul, out + row, P.D, f.key < P.S);
   };
   if (leads) {
     own_rows<T, HD>(static_cast<const T*>(P.k) + b * P.kb + kv * P.kh, P.ks, f.row0, S, P.D, f.own, P.scale < 0.0f);
     f.template walk<true>(walk);
-    finish(static_cast<T*>(P.dv), 1.0f);
+    finish(static_cast<T*>(P.dv), 1, 1.0f);
   } else {
     own_rows<T, HD>(static_cast<const T*>(P.v) + b * P.vb + kv * P.vh, P.vs, f.row0, S, P.D, f.own);
     f.template walk<false>(walk);
-    finish(static_cast<T*>(P.dk), P.scale);
+    finish(static_cast<T*>(P.dk), 0, P.scale);
   }
 }
 
 // Heads of up to 64: both sums fit one wave's registers, no P goes through LDS, and
-// two workgroups of a CU run beside each other (4096 tokens and 16 heads: 152 us
-// instead of 202, 64 heads: 616 instead of 788).
+// two workgroups of a CU run beside each other (4096 tokens and 16 heads: 151 us
+// instead of 202, 64 heads: 594 instead of 788).  96 columns would not fit: 23
+// registers in scratch, and 202 us instead of 141 for 8 heads of 80, 1036 instead of
+// 1072 for 64.
 template <class T, bool CAP, bool BIAS>
 struct AttnGradBoth {
   static constexpr int HD = 64;
   using Frag = typename Traits<T>::Frag;
-  static constexpr int kTile = kAttnTile * HD * 2, kBlocks = HD / 32, kHalf = kTile / 2;
+  static constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32, kHalf = kTile / 2;
   static constexpr int kStats = 2 * kAttnTile * 4, kLds = 4 * kTile + 2 * kStats;
   const AttnParams& P;
   char *qlds, *glds;  // two slots of Q and of do
@@ -951,7 +999,7 @@ struct AttnGradBoth {
   const T *Q, *G;     // of the first head
   const float *lse, *delta, *slopes;
   const int* docs;
-  AttnDma<HD> qd, gd;
+  AttnDma<kAttnLd<HD>> qd, gd;
   AttnFrags<T, HD> fr;
   Frag k[HD / 16], v[HD / 16];
   f32x16 dk[kBlocks], dv[kBlocks];
@@ -967,7 +1015,7 @@ struct AttnGradBoth {
                                                (threadIdx.x & 63) * 4, 0, 0, 0);
   }
   __device__ __forceinline__ void ready(const AttnTile& t, int slot) {
-    if (t.pad) clear_padding<HD>(docs + t.first, qlds + slot * kTile, glds + slot * kTile);
+    if (t.pad) clear_padding<kAttnLd<HD>>(docs + t.first, qlds + slot * kTile, glds + slot * kTile);
   }
   __device__ __forceinline__ bool hidden(int row) const { return P.causal && row0 > row + 31 && row0 >= prefix; }
   template <int BLOCK>
@@ -978,59 +1026,58 @@ struct AttnGradBoth {
     f32x16 x, dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = dp[r] = 0.0f;
-    Frag qrows[HD / 16], grows[HD / 16];
+    Frag rows[HD / 16], cf[2][kBlocks];
+    f4v stat[4];
+    auto fetch = [&](const char* from, Frag (&to)[HD / 16]) {
 #pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) qrows[ks] = fr.rows(qt, ks);
+      for (int ks = 0; ks < HD / 16; ++ks) to[ks] = fr.rows(from, ks);
+    };
+    auto stats_of = [&](int which) {
 #pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) {
-      x = Traits<T>::mma(qrows[ks], k[ks], x);
-      grows[ks] = fr.rows(gt, ks);
-    }
-    f4v L[4], dl[4];
+      for (int g = 0; g < 4; ++g) stat[g] = *reinterpret_cast<const f4v*>(st + which * (kStats / 2) + 32 * g);
+    };
+    fetch(qt, rows);
+    stats_of(0);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      L[g] = *reinterpret_cast<const f4v*>(st + 32 * g);
-      dl[g] = *reinterpret_cast<const f4v*>(st + kStats / 2 + 32 * g);
-    }
-#pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) dp = Traits<T>::mma(grows[ks], v[ks], dp);
-    Frag gf[2][kBlocks], qf[2][kBlocks];
-    fr.cols(lds_at(gt), gf);
-    float th[16], p[16], z[16];
+    for (int ks = 0; ks < HD / 16; ++ks) x = Traits<T>::mma(rows[ks], k[ks], x);
+    fetch(gt, rows);
+    fr.cols(lds_at(gt), cf);
+    float th[16], p[16];
     scores<CAP, BIAS>(x, th, P, BIAS ? slopes[t.head] * kLog2e : 0.0f, key - at);
     if (t.part) hide<false>(x, bound - at, docs ? docs + at : nullptr, doc);
     const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(fmaf(x[r], mul, -L[r >> 2][r & 3]));  // (queries behind the last, or that see nothing: L = inf)
-    Frag pf[2], zf[2];
-    as_operand<T>(p, pf);
+    for (int ks = 0; ks < HD / 16; ++ks) dp = Traits<T>::mma(rows[ks], v[ks], dp);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(fmaf(x[r], mul, -stat[r >> 2][r & 3]));  // (queries behind the last, or that see nothing: L = inf)
+    Frag f[2];
+    as_operand<T>(p, f);
+    if constexpr (CAP)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[r] *= 1.0f - th[r] * th[r];
+    stats_of(1);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int d = 0; d < kBlocks; ++d) dv[d] = Traits<T>::mma(gf[j][d], pf[j], dv[d]);
-    fr.cols(lds_at(qt), qf);
+      for (int d = 0; d < kBlocks; ++d) dv[d] = Traits<T>::mma(cf[j][d], f[j], dv[d]);
+    fr.cols(lds_at(qt), cf);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      z[r] = p[r] * (dp[r] - dl[r >> 2][r & 3]);
-      if constexpr (CAP) z[r] *= 1.0f - th[r] * th[r];
-    }
-    as_operand<T>(z, zf);
+    for (int r = 0; r < 16; ++r) p[r] *= dp[r] - stat[r >> 2][r & 3];
+    as_operand<T>(p, f);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int d = 0; d < kBlocks; ++d) dk[d] = Traits<T>::mma(qf[j][d], zf[j], dk[d]);
+      for (int d = 0; d < kBlocks; ++d) dk[d] = Traits<T>::mma(cf[j][d], f[j], dk[d]);
   }
 };
 
 template <class T, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void k_attn_dkv64(AttnParams P) {
+__global__ __launch_bounds__(256, 2) void k_attn_dkv_one(AttnParams P) {
   using F = AttnGradBoth<T, CAP, BIAS>;
   constexpr int HD = F::HD, kBlocks = F::kBlocks;
   __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
-  int bk, r0;
-  attn_place(P, P.B * P.KV, false, bk, r0);
-  r0 *= kAttnRows;
-  const int b = bk / P.KV, kv = bk - b * P.KV, head = kv * P.group;
+  const AttnKeys at(P, blockIdx.x);
+  const int b = at.b, kv = at.kv, r0 = at.r0, head = at.head;
   const int lane = threadIdx.x & 63, S = (int)P.S;
   F f(P);
   f.qlds = lds;
@@ -1057,29 +1104,34 @@ __global__ __launch_bounds__(256, 2) void k_attn_dkv64(AttnParams P) {
   own_rows<T, HD>(static_cast<const T*>(P.k) + b * P.kb + kv * P.kh, P.ks, f.row0, S, P.D, f.k, P.scale < 0.0f);
   own_rows<T, HD>(static_cast<const T*>(P.v) + b * P.vb + kv * P.vh, P.vs, f.row0, S, P.D, f.v);
   AttnWalk<false> walk;
-  walk.init(P, b, r0, P.group);
+  walk.init(P, b, r0, at.heads);
   attn_walk_plain(walk, f);
-  const int64_t at = (((int64_t)b * S + f.key) * P.KV + kv) * P.D;
+  const int64_t row = at.row(P, f.key);
   const bool live = f.key < S;
   if (f.doc < 0)  // (zeros for a padding row: what it holds may not be finite)
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) f.dk[d][r] = f.dv[d][r] = 0.0f;
-  if (P.dk) store_own<T, HD>(f.dk, P.scale, static_cast<T*>(P.dk) + at, P.D, live);
-  if (P.dv) store_own<T, HD>(f.dv, 1.0f, static_cast<T*>(P.dv) + at, P.D, live);
+  if (P.partial) {
+    store_part<HD>(f.dk, at.partial(P, 0) + row, P.D, live);
+    store_part<HD>(f.dv, at.partial(P, 1) + row, P.D, live);
+    return;
+  }
+  if (P.dk) store_own<T, HD>(f.dk, P.scale, static_cast<T*>(P.dk) + row, P.D, live);
+  if (P.dv) store_own<T, HD>(f.dv, 1.0f, static_cast<T*>(P.dv) + row, P.D, live);
 }
 
 // ------------------------------------------------------------- launches
 template <class T, int HD, bool CAP, bool BIAS>
 static hipError_t attn_go(AttnParams P, AttnPass pass, hipStream_t s) {
   P.tiles = (int)((P.S + kAttnRows - 1) / kAttnRows);
-  const dim3 grid((unsigned)(P.tiles * P.B * (pass == ATTN_DKV ? P.KV : P.H)));
+  const dim3 grid((unsigned)(P.tiles * P.B * (pass == ATTN_DKV ? P.KV * P.parts : P.H)));
   switch (pass) {
     case ATTN_FORWARD: hipLaunchKernelGGL((k_attn<T, HD, CAP, BIAS>), grid, dim3(256), 0, s, P); break;
     case ATTN_DQ: hipLaunchKernelGGL((k_attn_dq<T, HD, CAP, BIAS>), grid, dim3(256), 0, s, P); break;
     default:
-      if constexpr (HD == 64) hipLaunchKernelGGL((k_attn_dkv64<T, CAP, BIAS>), grid, dim3(256), 0, s, P);
+      if constexpr (HD == 64) hipLaunchKernelGGL((k_attn_dkv_one<T, CAP, BIAS>), grid, dim3(256), 0, s, P);
       else hipLaunchKernelGGL((k_attn_dkv<T, HD, CAP, BIAS>), grid, dim3(512), 0, s, P);
   }
   return hipGetLastError();

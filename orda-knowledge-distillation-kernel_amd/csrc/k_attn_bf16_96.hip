@@ -1,0 +1,6 @@
+// The attention kernels of bf16 tensors with heads of 65 to 96 elements.
+#include "attn.hpp"
+
+namespace orda {
+template hipError_t launch_attn<bf16, 96>(const AttnParams&, AttnPass, hipStream_t);
+}  // namespace orda

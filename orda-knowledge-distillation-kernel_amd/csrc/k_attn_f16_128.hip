@@ -1,4 +1,4 @@
-// The attention kernels of f16 tensors with heads of up to 128 elements.
+// The attention kernels of f16 tensors with heads of 97 to 128 elements.
 #include "attn.hpp"
 
 namespace orda {

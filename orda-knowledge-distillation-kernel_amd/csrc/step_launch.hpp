@@ -96,12 +96,15 @@ struct AttnParams {
   const int4* ranges;     // [B][padded / 64]
   int64_t S, padded;      // padded: S up to a multiple of 128
   int64_t qb, qs, qh, kb, ks, kh, vb, vs, vh, gb, gs, gh;
+  float* partial;         // dk and dv of each part, [2][parts][B S KV D], or null (one part)
   int B, H, KV, group, D, causal, tiles;
+  int parts, share;         // workgroups that take the heads of a tile of keys, heads of each
   float scale, scale_log2;  // scale_log2 = |scale| log2(e)
   float cap_in, cap_out;    // 2 |scale| log2(e) / cap and cap log2(e); 0: no cap
 };
 enum AttnPass { ATTN_FORWARD, ATTN_DQ, ATTN_DKV };
 template <class T, int HD> hipError_t launch_attn(const AttnParams& P, AttnPass pass, hipStream_t s);
+hipError_t launch_attn_join(const AttnParams& P, int dtype, hipStream_t s);
 hipError_t launch_attn_docs(const int32_t* ids, int64_t ld, int64_t B, int64_t S, int64_t padded, int* docs, int4* ranges, hipStream_t s);
 
 }  // namespace orda

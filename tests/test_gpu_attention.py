@@ -78,6 +78,23 @@ def test_shared_heads(H, KV, D):
     compare(case(2, 190, H, KV, D, BF, H + D), BF)
 
 
+@pytest.mark.parametrize("B,S,H,KV,D", [
+    (32, 130, 16, 8, 40),   # 512 tiles of keys: a workgroup takes all heads of its keys
+    (16, 130, 24, 8, 64),   # 256: two take three heads, one of them one
+    (16, 130, 32, 8, 96),   # 256: two take two heads each
+    (16, 130, 16, 8, 128),  # 256: two take one each
+    (18, 150, 20, 4, 112),  # 144: four for five heads, by twos: three
+])
+def test_parts_of_shared_heads(B, S, H, KV, D):
+    """Heads that share keys one after the other in a workgroup, each in one of its own, and between the two."""
+    compare(case(B, S, H, KV, D, BF, H + D), BF, documents=documents(B, S, D), prefix=torch.arange(B, dtype=torch.int32) * 9)
+
+
+@pytest.mark.parametrize("D", [65, 68, 81, 88, 95, 96, 97, 104])
+def test_head_dims_around_96(D):
+    compare(case(2, 140, 4, 2, D, BF, D), BF, causal=False, softcap=3.0)
+
+
 @pytest.mark.parametrize("D", [32, 128])
 @pytest.mark.parametrize("kw", [
     dict(softcap=2.0), dict(slopes=True), dict(softcap=5.0, slopes=True, causal=False), dict(prefix=[0, 70]), dict(prefix=[190, -4]),
