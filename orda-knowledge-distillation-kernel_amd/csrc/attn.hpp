@@ -70,14 +70,15 @@ __device__ __forceinline__ void attn_place(const AttnParams& P, int id, int head
 
 // A tile of 64 rows to LDS, 16 bytes a lane.  Rows from `rows` on and columns
 // from D on arrive as zeros.
-template <int LD, int WAVES = 4>
+template <int LD>
 struct AttnDma {
+  static constexpr int WAVES = 4;
   static constexpr int kChunks = LD / 8, kIssues = kChunks / WAVES, kStep = 64 * WAVES / kChunks;
   static_assert(kIssues > 0 && kStep % 16 == 0, "rows kStep apart have one swizzle");
   uint32_t off[kIssues];
   int row;
   __device__ __forceinline__ void init(int64_t ss, int D) {
-    const int p = wave_id() * 64 + (threadIdx.x & 63);
+    const int p = threadIdx.x & 255;
     row = p / kChunks;
     const int c = (p % kChunks) ^ attn_swz<LD>(row);
 #pragma unroll
@@ -85,7 +86,7 @@ struct AttnDma {
   }
   __device__ __forceinline__ void issue(const void* p, int rows, char* tile) const {
     const auto rs = rsrc_of(p);
-    const int w = wave_id();
+    const int w = wave_id() & 3;
     if (rows >= kAttnTile) {
 #pragma unroll
       for (int i = 0; i < kIssues; ++i) dma16(rs, off[i], tile + (i * WAVES + w) * 1024);
@@ -774,7 +775,7 @@ struct AttnGradKV {
   const T *Q, *G;     // of the first head
   const float *lse, *delta, *slopes;
   const int* docs;
-  AttnDma<kAttnLd<HD>, 8> qd, gd;
+  AttnDma<kAttnLd<HD>> qd, gd;  // of the second waves, which have the matrix cores while they send for a tile
   AttnFrags<T, HD> fr;
   Frag own[HD / 16];  // the wave's keys, or their values
   f32x16 acc[kBlocks];
@@ -786,7 +787,7 @@ struct AttnGradKV {
   __device__ __forceinline__ void issue(const AttnTile& t, int slot) {
     qd.issue(Q + t.head * P.qh + t.first * P.qs, (int)P.S - t.first, qlds + slot * kTile);
     gd.issue(G + t.head * P.gh + t.first * P.gs, (int)P.S - t.first, glds + slot * kTile);
-    const int w = wave_id();
+    const int w = wave_id() & 3;
     if (w < 2)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of((w ? delta : lse) + t.head * P.padded + t.first),
                                                (__attribute__((address_space(3))) void*)(stats + slot * kStats + w * (kStats / 2)), 4,
@@ -883,9 +884,11 @@ struct AttnGradKV {
     AttnTile t0 = w.next(), last = t0;
     if (t0.first < 0) return;
     AttnTile t1 = w.next();
-    issue(t0, 0);
-    if (t1.first >= 0) issue(t1, 1);
-    wait_vmem<0>();
+    if constexpr (!LEADS) {
+      issue(t0, 0);
+      if (t1.first >= 0) issue(t1, 1);
+      wait_vmem<0>();
+    }
     tile_barrier();
     ready(t0, 0);
     if constexpr (LEADS) {
@@ -898,10 +901,11 @@ struct AttnGradKV {
     for (bool first = true;; first = false) {
       if constexpr (LEADS) lead<0>(t0, slot, !hidden(t0.first + 32), slot);
       else follow<0>(last, !first, last, behind, !first, slot, true);
-      wait_vmem<0>();  // (t1, sent for two phases ago)
+      if constexpr (!LEADS) wait_vmem<0>();  // (t1, sent for two phases ago)
       tile_barrier();
       const AttnTile t2 = w.next();
-      if (t2.first >= 0) issue(t2, behind);  // (whose last block was read in the phase before)
+      if constexpr (!LEADS)
+        if (t2.first >= 0) issue(t2, behind);  // (whose last block was read in the phase before)
       const bool more = t1.first >= 0;
       if (more) ready(t1, after);
       if constexpr (LEADS) lead<1>(t0, slot, more && !hidden(t1.first), after);
