@@ -7,17 +7,20 @@
 // Backward: dW[v] = scale sum of dy[n] over t_n = v, and zeros in all other
 // rows (most of the bytes with a large vocabulary).  Four launches:
 //   sort   segments of 4096 tokens, each by one workgroup in LDS (radix, 8 bits
-//          a pass, stable); the other workgroups fill dW with zeros meanwhile
+//          a pass, stable); the other workgroups fill the first rows of dW with
+//          zeros meanwhile
 //   merge  up to 16 sorted segments a round: an element's place is the sum of
 //          its places in the others, found by 16 searches side by side (more
-//          than 4096 tokens)
+//          than 4096 tokens); beside the first round, the next rows of zeros
 //   sum    a wave takes 512 columns of `chunk` sorted entries and adds up their
 //          rows of dy in fp32; a run of one token that lies in the chunk goes
-//          out rounded, one that reaches past it as an fp32 partial sum
+//          out rounded, one that reaches past it as an fp32 partial sum; other
+//          waves fill the remaining rows that no token names
 //   join   the partial sums of such runs, in order
 // Equal tokens stay in their order throughout, so the sums do not depend on the
 // run, and a token that fills the batch is added up by as many waves as any
-// other.
+// other.  Memory bounds it: 16384 tokens over 128256 rows of 4096 in bf16 are
+// FIGURE3.
 #include <algorithm>
 
 #include "pieces.hpp"
@@ -49,23 +52,30 @@ __global__ __launch_bounds__(256) void k_embed(EmbedParams P, int64_t per_row, i
 // ------------------------------------------------------------- sort
 constexpr int kSegment = 4096;  // tokens of one workgroup
 constexpr int kFill = 4096;     // 16-byte stores of one that fills
+constexpr int64_t kBeside = 128ll << 20;  // bytes of zeros beside the sort, and beside the merge
+
+// Zeros in the bytes [begin, end) of p (from the 16 that begin lies in on), 64 KB
+// of a workgroup of N threads in a row.
+template <int N>
+__device__ __forceinline__ void fill_zeros(void* p, int64_t begin, int64_t end, int64_t group, int64_t groups) {
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4* out = static_cast<uint4*>(p) + begin / 16;
+  const int64_t bytes = end - begin / 16 * 16, n = bytes / 16;
+  for (int64_t b = group; b * kFill < n; b += groups)
+#pragma unroll 4
+    for (int i = 0; i < kFill / N; ++i) {
+      const int64_t at = b * kFill + i * N + threadIdx.x;
+      if (at < n) out[at] = zero;
+    }
+  const int tail = (int)(bytes % 16) / 2;  // (elements of 2 or 4 bytes)
+  if (group == 0 && (int)threadIdx.x < tail) reinterpret_cast<uint16_t*>(out + n)[threadIdx.x] = 0;
+}
 
 // Keys: the token, V for one that has no gradient (it sorts behind all others).
 // Entries past the last token have all bits set and stay behind them.
-__global__ __launch_bounds__(1024) void k_embed_sort(EmbedGradParams P, int passes, int segments, uint32_t* tokens, uint32_t* places, int64_t fill_bytes) {
+__global__ __launch_bounds__(1024) void k_embed_sort(EmbedGradParams P, int passes, int segments, uint32_t* tokens, uint32_t* places, int64_t fill_end) {
   if ((int)blockIdx.x >= segments) {
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    uint4* out = static_cast<uint4*>(P.dw);
-    const int64_t n = fill_bytes / 16, groups = gridDim.x - segments;
-    // (64 KB of a workgroup in a row)
-    for (int64_t b = blockIdx.x - segments; b * kFill < n; b += groups)
-#pragma unroll
-      for (int i = 0; i < kFill / 1024; ++i) {
-        const int64_t at = b * kFill + i * 1024 + threadIdx.x;
-        if (at < n) out[at] = zero;
-      }
-    const int tail = (int)(fill_bytes % 16) / 2;  // (elements of 2 or 4 bytes)
-    if ((int)blockIdx.x == segments && (int)threadIdx.x < tail) reinterpret_cast<uint16_t*>(out + n)[threadIdx.x] = 0;
+    fill_zeros<1024>(P.dw, 0, fill_end, blockIdx.x - segments, gridDim.x - segments);
     return;
   }
   __shared__ uint32_t key[2][kSegment];
@@ -156,30 +166,47 @@ __global__ __launch_bounds__(1024) void k_embed_sort(EmbedGradParams P, int pass
   }
 }
 
-// Groups of 16 sorted segments of `len` (a power of two) entries to one each.
-__global__ __launch_bounds__(256) void k_embed_merge(const uint32_t* tokens, const uint32_t* places, uint32_t* tokens_out, uint32_t* places_out, int64_t n, int64_t len) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= n) return;
+// Groups of 16 sorted segments of `len` (a power of two) entries to one each.  A
+// wave's entries lie in one segment; the 16 searches of a lane have their loads in
+// flight together, step by step, none under a condition (16384 tokens and 128 MB of
+// zeros beside them: 21 us, what the zeros take; with conditional loads and
+// 64-bit places 30).
+__global__ __launch_bounds__(64) void k_embed_merge(const uint32_t* tokens, const uint32_t* places, uint32_t* tokens_out, uint32_t* places_out, int64_t n, int64_t len,
+                                                    int groups, void* dw, int64_t fill_begin, int64_t fill_end) {
+  if ((int)blockIdx.x >= groups) {
+    fill_zeros<64>(dw, fill_begin, fill_end, blockIdx.x - groups, gridDim.x - groups);
+    return;
+  }
+  const int64_t first = (int64_t)blockIdx.x * 64, group = first / (16 * len) * (16 * len), e = lmin(first + threadIdx.x, n - 1);
+  const int own = (int)((first - group) / len);
   const uint32_t t = tokens[e];
-  const int64_t group = e / (16 * len) * (16 * len);
-  const int own = (int)((e - group) / len);
-  int64_t pos[16];
+  uint32_t pos[16];
 #pragma unroll
   for (int b = 0; b < 16; ++b) pos[b] = 0;
-  for (int64_t s = len; s > 0; s >>= 1) {
+  for (uint32_t s = (uint32_t)len; s > 0; s >>= 1) {
+    uint32_t v[16];
+    auto size = [&](int b) { return (uint32_t)std::max<int64_t>(0, lmin(len, n - group - b * len)); };
+    // (four segments at a time, as long as there are any; of an empty one the group's
+    // first entry, unused)
 #pragma unroll
-    for (int b = 0; b < 16; ++b) {
-      const int64_t first = group + b * len, at = first + pos[b] + s - 1;
-      if (b == own || pos[b] + s > len || at >= n) continue;
-      const uint32_t v = tokens[at];
-      if (b < own ? v <= t : v < t) pos[b] += s;  // (equal ones of earlier segments come first)
-    }
+    for (int q = 0; q < 16; q += 4)
+      if (size(q))
+#pragma unroll
+        for (int b = q; b < q + 4; ++b) v[b] = tokens[group + (size(b) ? b * len : 0) + (max(min(pos[b] + s, size(b)), 1u) - 1)];
+#pragma unroll
+    for (int q = 0; q < 16; q += 4)
+      if (size(q))
+#pragma unroll
+        for (int b = q; b < q + 4; ++b)  // (equal ones of earlier segments come first)
+          if (pos[b] + s <= size(b) && v[b] < t + (b < own)) pos[b] += s;
   }
-  int64_t to = group + (e - group - own * len);
+  int64_t to = e - own * len;
 #pragma unroll
   for (int b = 0; b < 16; ++b) to += b == own ? 0 : pos[b];
-  tokens_out[to] = t;
-  places_out[to] = places[e];
+  if (first + threadIdx.x < n) {
+    tokens_out[to] = t;
+    places_out[to] = places[e];
+  }
 }
 
 // ------------------------------------------------------------- sums
@@ -190,14 +217,40 @@ struct EmbedSums {
   int chunk;
   int slabs;    // of 512 columns
   int64_t chunks;
+  int groups;      // workgroups that add up
+  int64_t filled;  // rows of dW that are zero already
 };
+
+// 64 rows of dW: zeros in those that no token names, every fourth by one wave.
+template <class W, bool EVEN>
+__device__ __forceinline__ void fill_unnamed(const EmbedGradParams& P, const EmbedSums& S, int64_t first) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = first + lane, per_row = pieces_of(P.hidden);
+  int64_t lo = 0, hi = P.tokens;  // the first entry that is not below `row` lies in [lo, hi]
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) / 2;
+    if ((int64_t)S.tokens[mid] < row) lo = mid + 1;
+    else hi = mid;
+  }
+  const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  const uint64_t unnamed = __ballot(row < P.vocab && (lo == P.tokens || (int64_t)S.tokens[lo] != row));
+  for (uint64_t to = unnamed & (0x1111111111111111ull << wave_id()); to; to &= to - 1) {
+    W* out = static_cast<W*>(P.dw) + (first + __builtin_ctzll(to)) * P.hidden;
+    for (int64_t i = lane; i < per_row; i += 64) put8(out, Piece<EVEN>(i, P.hidden), zero);
+  }
+}
 
 template <class W, class T, bool EVEN>
 __global__ __launch_bounds__(256) void k_embed_sum(EmbedGradParams P, EmbedSums S) {
   constexpr int kAhead = 8;  // rows in flight
   const int lane = threadIdx.x & 63;
+  if ((int)blockIdx.x >= S.groups) {
+    for (int64_t first = S.filled + (int64_t)(blockIdx.x - S.groups) * 64; first < P.vocab; first += (int64_t)(gridDim.x - S.groups) * 64)
+      fill_unnamed<W, EVEN>(P, S, first);
+    return;
+  }
   const int64_t units = S.chunks * S.slabs;
-  for (int64_t u = (int64_t)blockIdx.x * 4 + wave_id(); u < units; u += (int64_t)gridDim.x * 4) {
+  for (int64_t u = (int64_t)blockIdx.x * 4 + wave_id(); u < units; u += (int64_t)S.groups * 4) {
     const int64_t chunk = u / S.slabs, first = chunk * S.chunk;
     const int n = (int)lmin(S.chunk, P.tokens - first);
     const Piece<EVEN> at((u - chunk * S.slabs) * 64 + lane, P.hidden);
@@ -340,9 +393,11 @@ size_t embed_grad_workspace(int64_t tokens, int64_t hidden) {
 }
 
 template <class W, class T, bool EVEN>
-static hipError_t sum_even(const EmbedGradParams& P, const EmbedSums& S, hipStream_t s) {
+static hipError_t sum_even(const EmbedGradParams& P, EmbedSums S, hipStream_t s) {
   const int64_t units = S.chunks * S.slabs;
-  hipLaunchKernelGGL((k_embed_sum<W, T, EVEN>), dim3((unsigned)std::min<int64_t>((units + 3) / 4, 1 << 22)), dim3(256), 0, s, P, S);
+  S.groups = (int)std::min<int64_t>((units + 3) / 4, 1 << 22);
+  const int64_t fill = std::min<int64_t>((P.vocab - S.filled + 63) / 64, 1 << 20);
+  hipLaunchKernelGGL((k_embed_sum<W, T, EVEN>), dim3((unsigned)(S.groups + fill)), dim3(256), 0, s, P, S);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || S.chunks == 1) return e;
   hipLaunchKernelGGL((k_embed_join<W, EVEN>), dim3((unsigned)std::min<int64_t>(units, 1 << 20)), dim3(512), 0, s, P, S);
@@ -376,14 +431,20 @@ hipError_t launch_embed_grad(const EmbedGradParams& P, int dtype, int out_dtype,
   int passes = 1;
   while (passes < 4 && (P.vocab >> (8 * passes)) != 0) ++passes;
   const int segments = (int)((P.tokens + kSegment - 1) / kSegment);
-  const int64_t bytes = P.vocab * P.hidden * (dtype == DT_F32 ? 4 : 2);
-  const int fill = (int)std::min<int64_t>(1 << 20, (bytes + kFill * 16 - 1) / (kFill * 16));
-  hipLaunchKernelGGL(k_embed_sort, dim3((unsigned)(segments + fill)), dim3(1024), 0, s, P, passes, segments, tokens[0], places[0], bytes);
+  // As many rows as the card fills while it sorts, and while it merges.
+  const int64_t row_bytes = P.hidden * (dtype == DT_F32 ? 4 : 2), beside = (kBeside + row_bytes - 1) / row_bytes;
+  auto fill_groups = [&](int64_t rows) { return (rows * row_bytes + kFill * 16 - 1) / (kFill * 16); };
+  S.filled = std::min(P.vocab, beside);
+  hipLaunchKernelGGL(k_embed_sort, dim3((unsigned)(segments + fill_groups(S.filled))), dim3(1024), 0, s, P, passes, segments, tokens[0], places[0], S.filled * row_bytes);
   hipError_t e = hipGetLastError();
   int at = 0;
   for (int64_t len = kSegment; e == hipSuccess && len < P.tokens; len *= 16, at ^= 1) {
-    hipLaunchKernelGGL(k_embed_merge, dim3((unsigned)((P.tokens + 255) / 256)), dim3(256), 0, s, tokens[at], places[at], tokens[at ^ 1], places[at ^ 1], P.tokens, len);
+    const int64_t rows = len == kSegment ? std::min(P.vocab - S.filled, beside) : 0, begin = S.filled * row_bytes;
+    const int groups = (int)((P.tokens + 63) / 64);
+    hipLaunchKernelGGL(k_embed_merge, dim3((unsigned)(groups + fill_groups(rows))), dim3(64), 0, s, tokens[at], places[at], tokens[at ^ 1], places[at ^ 1], P.tokens,
+                       len, groups, P.dw, begin, begin + rows * row_bytes);
     e = hipGetLastError();
+    S.filled += rows;
   }
   if (e != hipSuccess) return e;
   S.tokens = tokens[at];

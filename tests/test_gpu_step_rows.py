@@ -255,6 +255,27 @@ def test_long_batches_are_merged_in_rounds():
     assert torch.equal(got.double(), want)
 
 
+@pytest.mark.parametrize("N,V,H,dtype", [(100, 40000, 4099, BF), (5000, 70001, 4096, BF), (4200, 150000, 1001, HF), (9, 12_000_000, 8, F), (70000, 90000, 1032, F)])
+def test_rows_that_no_token_names_are_zeros(N, V, H, dtype):
+    """Gradients of more bytes than are filled beside the sort and the merge, over memory that held NaN; whole numbers, exact sums."""
+    g = torch.Generator(device="cuda").manual_seed(N)
+    ids = torch.randint(-2, V + 2, (N,), generator=g, device="cuda")
+    ids[::3] = V - 1 - ids[::3].abs() % 7
+    ids[1::5] = 70
+    dy = torch.randint(-1, 2, (N, H), generator=g, device="cuda").to(dtype)
+    w = torch.zeros(V, H, dtype=dtype, device="cuda", requires_grad=True)
+    y = orda.token_embedding(ids, w, padding_idx=V // 2)
+    held = torch.full((V, H), float("nan"), dtype=dtype, device="cuda")
+    del held
+    (got,) = torch.autograd.grad(y, w, dy)
+    ok = (ids >= 0) & (ids < V) & (ids != V // 2)
+    rows, at = ids[ok].unique(return_inverse=True)
+    want = torch.zeros(len(rows), H, device="cuda", dtype=torch.float64).index_add_(0, at, dy[ok].double())
+    assert torch.equal(got[rows].double(), want.to(dtype).double())
+    got[rows] = 0
+    assert not got.any()
+
+
 def test_embedding_gradients_are_the_same_in_every_run():
     t = embed_case(6000, 200, 72, HF, 5, spread=4.0)
     first = run_embed(t)
