@@ -261,44 +261,70 @@ __device__ __forceinline__ void store_own(const f32x16 (&acc)[HD / 32], float mu
 // number and whether there is padding.
 struct DocRange {
   int lo, hi, pad;
-  __device__ __forceinline__ void join(const int4& o) {
-    lo = min(lo, o.x);
-    hi = max(hi, o.y);
-    pad |= o.z;
+  __device__ __forceinline__ DocRange(const int4& a) : lo(a.x), hi(a.y), pad(a.z) {}
+  __device__ __forceinline__ void join(const DocRange& o) {
+    lo = min(lo, o.lo);
+    hi = max(hi, o.hi);
+    pad |= o.pad;
   }
+  __device__ __forceinline__ bool meets(const DocRange& o) const { return lo <= o.hi && hi >= o.lo; }
+  __device__ __forceinline__ bool one(const DocRange& o) const { return lo == hi && o.lo == o.hi && lo == o.lo && !pad && !o.pad; }
 };
-// The tiles of the other side that a workgroup's rows meet, in order.  `part`:
-// each element has to be looked at; `pad`: some rows are padding.
+// A tile of the other side that a workgroup's rows meet, and for the wave's 32
+// rows and either block of 32 of the tile: whether they meet, and whether each
+// element has to be looked at.
 struct AttnTile {
   int first;  // its first row, -1 behind the last tile
-  bool part, pad;
+  int flags;
   int head;   // (queries: of the heads that share the keys)
+  __device__ __forceinline__ bool sees(int block) const { return (flags >> block) & 1; }
+  __device__ __forceinline__ bool part(int block) const { return (flags >> (2 + block)) & 1; }
+  __device__ __forceinline__ bool pad() const { return (flags >> 4) & 1; }  // (some of its rows are padding)
+  __device__ __forceinline__ bool done(int block) const { return (flags >> (5 + block)) & 1; }  // (the wave meets neither it nor any behind)
 };
 template <bool KEYS>  // the tiles are keys (else queries)
 struct AttnWalk {
   int S, r0, prefix, causal, base;
   int head, heads;  // the walk's turn, and how many
   const int4* ranges;
-  DocRange own;
-  uint64_t seen, part, pad;
+  uint64_t seen;  // tiles from `base` on that the workgroup meets
+  int flags;      // of tile base + lane
+  // rows [r, r1) of the workgroup and [a, b) of the other side
+  __device__ __forceinline__ bool meets(int a, int b, int r, int r1) const {
+    const int k0 = KEYS ? a : r, q1 = min(KEYS ? r1 : b, S);
+    return a < S && r < S && !(causal && k0 >= q1 && k0 >= prefix);
+  }
+  __device__ __forceinline__ bool in_part(int a, int b, int r, int r1) const {
+    const int q0 = KEYS ? r : a, k1 = min(KEYS ? b : r1, S);
+    return (KEYS && b > S) || (causal && k1 - 1 > q0 && k1 > prefix);
+  }
   __device__ __forceinline__ void look() {
-    const int t = base + (threadIdx.x & 63);
-    const int a = t * kAttnTile, b = min(a + kAttnTile, S), r1 = min(r0 + kAttnRows, S);  // [a, b) against [r0, r1)
-    bool s = a < S, p = KEYS && a + kAttnTile > S, d = false;
-    if (causal) {
-      const int q0 = KEYS ? r0 : a, q1 = KEYS ? r1 : b, k0 = KEYS ? a : r0, k1 = KEYS ? b : r1;
-      if (k0 >= q1 && k0 >= prefix) s = false;
-      if (k1 - 1 > q0 && k1 > prefix) p = true;
+    const int t = base + (threadIdx.x & 63), a = t * kAttnTile, w = wave_id() & 3, r = r0 + 32 * w;
+    bool any = meets(a, a + kAttnTile, r0, r0 + kAttnRows), s[2], p[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      s[k] = meets(a + 32 * k, a + 32 * k + 32, r, r + 32);
+      p[k] = in_part(a + 32 * k, a + 32 * k + 32, r, r + 32);
     }
-    if (ranges && s) {
-      const int4 v = ranges[t];
-      if (v.x > own.hi || v.y < own.lo) s = false;
-      if (v.x != v.y || own.lo != own.hi || v.x != own.lo || v.z || own.pad) p = true;
-      d = v.z != 0;
+    bool pad = false;
+    if (ranges && any) {
+      DocRange all(ranges[r0 / 32]), both(ranges[2 * t]);
+      const DocRange own(ranges[r0 / 32 + w]), tile[2] = {both, ranges[2 * t + 1]};
+#pragma unroll
+      for (int k = 1; k < 4; ++k) all.join(ranges[r0 / 32 + k]);
+      both.join(tile[1]);
+      any = all.meets(both);
+      pad = both.pad;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        s[k] = s[k] && own.meets(tile[k]);
+        p[k] = p[k] || !own.one(tile[k]);
+      }
     }
-    seen = __ballot(s);
-    part = __ballot(p);
-    pad = __ballot(d);
+    seen = __ballot(any);
+    const bool last = (base + 64) * kAttnTile >= S;
+    const uint64_t from = __ballot(s[0] || s[1]) >> (threadIdx.x & 63);  // (the wave's, from this tile on)
+    flags = s[0] | s[1] << 1 | p[0] << 2 | p[1] << 3 | pad << 4 | (last && !from) << 5 | (last && !s[1] && !(from >> 1)) << 6;
   }
   __device__ __forceinline__ void init(const AttnParams& P, int b, int row0, int turns = 1) {
     head = 0;
@@ -307,13 +333,7 @@ struct AttnWalk {
     r0 = row0;
     causal = P.causal;
     prefix = P.prefix ? P.prefix[b] : 0;
-    ranges = nullptr;
-    own = DocRange{0x7fffffff, -1, 0};
-    if (P.docs) {
-      ranges = P.ranges + (int64_t)b * (P.padded / kAttnTile);
-      own.join(ranges[r0 / kAttnTile]);
-      own.join(ranges[r0 / kAttnTile + 1]);
-    }
+    ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / 32) : nullptr;
     base = -64;
     seen = 0;
   }
@@ -324,7 +344,7 @@ struct AttnWalk {
         if (++head >= heads) {
           head = heads;  // (stays behind the last)
           base -= 64;
-          return {-1, false, false, 0};
+          return {-1, 0, 0};
         }
         base = 0;
       }
@@ -332,7 +352,7 @@ struct AttnWalk {
     }
     const int j = __builtin_ctzll(seen);
     seen &= seen - 1;
-    return {(base + j) * kAttnTile, (bool)((part >> j) & 1), (bool)((pad >> j) & 1), head};
+    return {(base + j) * kAttnTile, __builtin_amdgcn_readlane(flags, j), head};
   }
 };
 
@@ -354,23 +374,33 @@ __device__ __forceinline__ int block_row(int r) { return (r >> 2) * 8 + ((thread
 
 // z = -inf for what is not seen.  Keys in the rows: those below `bound` (behind
 // the query and its prefix, the sequence's end) are seen; queries in the rows:
-// those from `bound` on.  Relative to the block; docs: the numbers of its rows,
-// read by scalar loads (a vector load would wait for the DMA in flight), of which
-// the lower half of a wave compares four and the upper half the next four.
+// those from `bound` on.  Relative to the block of 32 at row `at`; docs, ranges:
+// the numbers and their ranges, or null, read by scalar loads (a vector load would
+// wait for the DMA in flight).  A block within one document takes one comparison
+// a lane; of others the lower half of a wave compares four rows and the upper half
+// the next four (12 heads of 80, 3 rows of one document of 1777: forward 49 us
+// instead of 76).
 template <bool KEYS>
-__device__ __forceinline__ void hide(f32x16& z, int bound, const int* docs, int doc) {
+__device__ __forceinline__ void hide(f32x16& z, int bound, const int* docs, const int4* ranges, int at, int doc) {
+  const int own = doc < 0 ? -2 : doc;  // (padding sees nothing, padding neither)
+  bound -= at;
+  bool mixed = false;
+  if (docs) {
+    const auto* range = (const __attribute__((address_space(4))) int*)(uintptr_t)(ranges + at / 32);
+    mixed = range[0] != range[1] || range[2];
+    if (!mixed && own != range[0]) bound = KEYS ? -1 : 32;
+  }
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     const int row = block_row(r);
     z[r] = (KEYS ? row < bound : row >= bound) ? z[r] : -kInf;
   }
-  if (docs) {
-    const __attribute__((address_space(4))) int* d = (const __attribute__((address_space(4))) int*)(uintptr_t)docs;
-    const int own = doc < 0 ? -2 : doc;  // (padding sees nothing, padding neither)
+  if (mixed) {
+    const auto* d = (const __attribute__((address_space(4))) int*)(uintptr_t)(docs + at);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int at = (r >> 2) * 8 + (r & 3);
-      const uint64_t low = __ballot(own == d[at]), high = __ballot(own == d[at + 4]);
+      const int i = (r >> 2) * 8 + (r & 3);
+      const uint64_t low = __ballot(own == d[i]), high = __ballot(own == d[i + 4]);
       const uint64_t seen = (low & 0xffffffffull) | (high & 0xffffffff00000000ull);
       z[r] = __builtin_amdgcn_inverse_ballot_w64(seen) ? z[r] : -kInf;
     }
@@ -416,8 +446,7 @@ __device__ __forceinline__ uint32_t lds_at(const void* p) { return (uint32_t)(ui
 // operands, so that the tile after the next goes there.
 //
 // f.issue(tile, two, three), f.ready(tile, two, three): the tile sent for, in that
-// slot of the two and of the three; arrived.  f.hidden(row): whether none of the
-// wave's rows meets the 32 from `row` on.  f.ahead<BLOCK>(two): products of that
+// slot of the two and of the three; arrived.  f.ahead<BLOCK>(two): products of that
 // block of the tile, into the BLOCK-th set of registers.  f.work<BLOCK>(tile,
 // three, two): the block's softmax and what follows, beside `ahead` of the next
 // block, which is in slot `two` (behind the last tile: of what lies in LDS,
@@ -436,8 +465,8 @@ __device__ __forceinline__ void attn_walk(AttnWalk<true>& walk, F& f) {
   if (t1.first >= 0) f.ready(t1, 1, 1);
   f.template ahead<0>(0);
   for (bool sent = true;; sent = false) {  // (sent: the first two tiles have arrived)
-    if (!f.hidden(t0.first)) f.template work<0>(t0, three, two);  // (blocks that are hidden are followed by none that are not)
-    AttnTile t2{-1, false, false, 0};
+    if (!t0.done(0)) f.template work<0>(t0, three, two);
+    AttnTile t2{-1, 0, 0};
     if (t1.first >= 0) {
       t2 = walk.next();
       wait_vmem<0>();
@@ -445,7 +474,7 @@ __device__ __forceinline__ void attn_walk(AttnWalk<true>& walk, F& f) {
       if (t2.first >= 0) f.issue(t2, two, behind);
       if (!sent) f.ready(t1, two ^ 1, after);
     }
-    if (!f.hidden(t0.first + 32)) f.template work<1>(t0, three, two ^ 1);
+    if (!t0.done(1)) f.template work<1>(t0, three, two ^ 1);
     if (t1.first < 0) return;
     t0 = t1;
     t1 = t2;
@@ -470,8 +499,8 @@ __device__ __forceinline__ void attn_walk_plain(AttnWalk<KEYS>& walk, F& f) {
     tile_barrier();
     if (then.first >= 0) f.issue(then, slot ^ 1);
     f.ready(t, slot);
-    if (!f.hidden(t.first)) f.template work<0>(t, slot);
-    if (!f.hidden(t.first + 32)) f.template work<1>(t, slot);
+    if (t.sees(0)) f.template work<0>(t, slot);
+    if (t.sees(1)) f.template work<1>(t, slot);
     if (then.first < 0) return;
     t = then;
   }
@@ -486,6 +515,7 @@ struct AttnForward {
   char *klds, *vlds;  // two slots of K, three of V
   const T *K, *V;
   const int* docs;
+  const int4* ranges;
   AttnDma<kAttnLd<HD>> kd, vd;
   AttnFrags<T, HD> fr;
   Frag q[HD / 16], rows[HD / 16];
@@ -499,9 +529,8 @@ struct AttnForward {
     vd.issue(V + t.first * P.vs, (int)P.S - t.first, vlds + three * kTile);
   }
   __device__ __forceinline__ void ready(const AttnTile& t, int two, int three) {
-    if (t.pad) clear_padding<kAttnLd<HD>>(docs + t.first, klds + two * kTile, vlds + three * kTile);
+    if (t.pad()) clear_padding<kAttnLd<HD>>(docs + t.first, klds + two * kTile, vlds + three * kTile);
   }
-  __device__ __forceinline__ bool hidden(int row) const { return P.causal && row > row0 + 31 && row >= prefix; }
   template <int BLOCK>
   __device__ __forceinline__ void fetch(int two) {
     const char* kt = klds + two * kTile + BLOCK * kHalf;
@@ -530,7 +559,12 @@ struct AttnForward {
     fr.cols(lds_at(vlds) + (uint32_t)(three * kTile + BLOCK * kHalf), vf);  // (one wait for both)
     float th[16];
     scores<CAP, BIAS>(x, th, P, slope, i - at);
-    if (t.part) hide<true>(x, bound - at, docs ? docs + at : nullptr, doc);
+    if (!t.sees(BLOCK)) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = -kInf;
+    } else if (t.part(BLOCK)) {
+      hide<true>(x, bound, docs, ranges, at, doc);
+    }
     float top = fmaxf(x[0], x[1]);
 #pragma unroll
     for (int r = 2; r < 16; ++r) top = fmaxf(top, x[r]);
@@ -584,6 +618,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
   f.V = static_cast<const T*>(P.v) + b * P.vb + kv * P.vh;
   f.slope = BIAS ? P.slopes[head] * kLog2e : 0.0f;
   f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
+  f.ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / 32) : nullptr;
   f.doc = P.docs ? f.docs[f.i] : 0;
   AttnWalk<true> walk;
   walk.init(P, b, q0);
@@ -622,6 +657,7 @@ struct AttnGradQ {
   char *klds, *vlds;  // two slots each
   const T *K, *V;
   const int* docs;
+  const int4* ranges;
   AttnDma<kAttnLd<HD>> kd, vd;
   AttnFrags<T, HD> fr;
   Frag q[HD / 16], g[HD / 16];
@@ -634,9 +670,8 @@ struct AttnGradQ {
     vd.issue(V + t.first * P.vs, (int)P.S - t.first, vlds + slot * kTile);
   }
   __device__ __forceinline__ void ready(const AttnTile& t, int slot) {
-    if (t.pad) clear_padding<kAttnLd<HD>>(docs + t.first, klds + slot * kTile, vlds + slot * kTile);
+    if (t.pad()) clear_padding<kAttnLd<HD>>(docs + t.first, klds + slot * kTile, vlds + slot * kTile);
   }
-  __device__ __forceinline__ bool hidden(int row) const { return P.causal && row > row0 + 31 && row >= prefix; }
   template <int BLOCK>
   __device__ __forceinline__ void work(const AttnTile& t, int slot) {
     const int at = t.first + 32 * BLOCK;
@@ -656,7 +691,7 @@ struct AttnGradQ {
     for (int ks = 0; ks < HD / 16; ++ks) dp = Traits<T>::mma(vrows[ks], g[ks], dp);
     float th[16];
     scores<CAP, BIAS>(x, th, P, slope, i - at);
-    if (t.part) hide<true>(x, bound - at, docs ? docs + at : nullptr, doc);
+    if (t.part(BLOCK)) hide<true>(x, bound, docs, ranges, at, doc);
     const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
     float z[16];
 #pragma unroll
@@ -692,6 +727,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P)
   f.V = static_cast<const T*>(P.v) + b * P.vb + kv * P.vh;
   f.slope = BIAS ? P.slopes[head] * kLog2e : 0.0f;
   f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
+  f.ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / 32) : nullptr;
   f.doc = P.docs ? f.docs[f.i] : 0;
   own_rows<T, HD>(static_cast<const T*>(P.dout) + b * P.gb + head * P.gh, P.gs, f.row0, S, P.D, f.g);
   {
@@ -775,6 +811,7 @@ struct AttnGradKV {
   const T *Q, *G;     // of the first head
   const float *lse, *delta, *slopes;
   const int* docs;
+  const int4* ranges;
   AttnDma<kAttnLd<HD>> qd, gd;  // of the second waves, which have the matrix cores while they send for a tile
   AttnFrags<T, HD> fr;
   Frag own[HD / 16];  // the wave's keys, or their values
@@ -794,9 +831,8 @@ struct AttnGradKV {
                                                (threadIdx.x & 63) * 4, 0, 0, 0);
   }
   __device__ __forceinline__ void ready(const AttnTile& t, int slot) {
-    if (t.pad) clear_padding<kAttnLd<HD>>(docs + t.first, qlds + slot * kTile, glds + slot * kTile);
+    if (t.pad()) clear_padding<kAttnLd<HD>>(docs + t.first, qlds + slot * kTile, glds + slot * kTile);
   }
-  __device__ __forceinline__ bool hidden(int row) const { return P.causal && row0 > row + 31 && row0 >= prefix; }
   __device__ __forceinline__ char* qrows(int slot, int block) const { return qlds + slot * kTile + block * kHalf; }
   __device__ __forceinline__ char* grows(int slot, int block) const { return glds + slot * kTile + block * kHalf; }
   __device__ __forceinline__ void fetch(const char* at) {
@@ -826,14 +862,14 @@ struct AttnGradKV {
   __device__ __forceinline__ void lead(const AttnTile& t, int slot, bool then, int to) {
     const int at = t.first + 32 * BLOCK;
     if (then) fetch(qrows(to, 1 - BLOCK));
-    if (!hidden(at)) {
+    if (t.sees(BLOCK)) {
       f4v L[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) L[g] = *reinterpret_cast<const f4v*>(stat(slot, BLOCK, 0) + 32 * g);
       fr.cols(lds_at(grows(slot, BLOCK)), cf);
       float th[16], p[16];
       scores<CAP, BIAS>(x, th, P, BIAS ? slopes[t.head] * kLog2e : 0.0f, key - at);
-      if (t.part) hide<false>(x, bound - at, docs ? docs + at : nullptr, doc);
+      if (t.part(BLOCK)) hide<false>(x, bound, docs, ranges, at, doc);
       const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -859,8 +895,8 @@ struct AttnGradKV {
   template <int BLOCK>
   __device__ __forceinline__ void follow(const AttnTile& u, bool has, const AttnTile& t, int slot, bool here, int to, bool more) {
     constexpr int kOther = 1 - BLOCK;
-    if (has && !hidden(u.first + 32 * BLOCK)) add_up(zf);
-    if (here && !hidden(t.first + 32 * kOther)) {
+    if (has && u.sees(BLOCK)) add_up(zf);
+    if (here && t.sees(kOther)) {
       f32x16 dp;
       f4v dl[4], p[4];
 #pragma unroll
@@ -892,14 +928,14 @@ struct AttnGradKV {
     tile_barrier();
     ready(t0, 0);
     if constexpr (LEADS) {
-      if (!hidden(t0.first)) {
+      if (t0.sees(0)) {
         fetch(qrows(0, 0));
         product(x);
       }
     }
     int slot = 0, after = 1, behind = 2;  // of t0, t1, and the tile before t0
     for (bool first = true;; first = false) {
-      if constexpr (LEADS) lead<0>(t0, slot, !hidden(t0.first + 32), slot);
+      if constexpr (LEADS) lead<0>(t0, slot, t0.sees(1), slot);
       else follow<0>(last, !first, last, behind, !first, slot, true);
       if constexpr (!LEADS) wait_vmem<0>();  // (t1, sent for two phases ago)
       tile_barrier();
@@ -908,7 +944,7 @@ struct AttnGradKV {
         if (t2.first >= 0) issue(t2, behind);  // (whose last block was read in the phase before)
       const bool more = t1.first >= 0;
       if (more) ready(t1, after);
-      if constexpr (LEADS) lead<1>(t0, slot, more && !hidden(t1.first), after);
+      if constexpr (LEADS) lead<1>(t0, slot, t1.sees(0), after);
       else follow<1>(last, !first, t0, slot, true, slot, true);
       tile_barrier();
       last = t0;
@@ -922,7 +958,7 @@ struct AttnGradKV {
     }
     if constexpr (!LEADS) {
       follow<0>(last, true, last, slot, true, slot, false);
-      if (!hidden(last.first + 32)) add_up(zf);
+      if (last.sees(1)) add_up(zf);
     }
   }
 };
@@ -944,6 +980,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_dkv(AttnParams P) {
   f.row0 = r0 + (w & 3) * 32;
   f.key = f.row0 + (lane & 31);
   f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
+  f.ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / 32) : nullptr;
   f.doc = P.docs ? f.docs[f.key] : 0;
   f.prefix = P.prefix ? P.prefix[b] : 0;
   f.bound = P.causal && f.key >= f.prefix ? f.key : 0;
@@ -1003,6 +1040,7 @@ struct AttnGradBoth {
   const T *Q, *G;     // of the first head
   const float *lse, *delta, *slopes;
   const int* docs;
+  const int4* ranges;
   AttnDma<kAttnLd<HD>> qd, gd;
   AttnFrags<T, HD> fr;
   Frag k[HD / 16], v[HD / 16];
@@ -1019,9 +1057,8 @@ struct AttnGradBoth {
                                                (threadIdx.x & 63) * 4, 0, 0, 0);
   }
   __device__ __forceinline__ void ready(const AttnTile& t, int slot) {
-    if (t.pad) clear_padding<kAttnLd<HD>>(docs + t.first, qlds + slot * kTile, glds + slot * kTile);
+    if (t.pad()) clear_padding<kAttnLd<HD>>(docs + t.first, qlds + slot * kTile, glds + slot * kTile);
   }
-  __device__ __forceinline__ bool hidden(int row) const { return P.causal && row0 > row + 31 && row0 >= prefix; }
   template <int BLOCK>
   __device__ __forceinline__ void work(const AttnTile& t, int slot) {
     const int at = t.first + 32 * BLOCK;
@@ -1048,7 +1085,7 @@ struct AttnGradBoth {
     fr.cols(lds_at(gt), cf);
     float th[16], p[16];
     scores<CAP, BIAS>(x, th, P, BIAS ? slopes[t.head] * kLog2e : 0.0f, key - at);
-    if (t.part) hide<false>(x, bound - at, docs ? docs + at : nullptr, doc);
+    if (t.part(BLOCK)) hide<false>(x, bound, docs, ranges, at, doc);
     const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) dp = Traits<T>::mma(rows[ks], v[ks], dp);
@@ -1090,6 +1127,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_dkv_one(AttnParams P) {
   f.row0 = r0 + wave_id() * 32;
   f.key = f.row0 + (lane & 31);
   f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
+  f.ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / 32) : nullptr;
   f.doc = P.docs ? f.docs[f.key] : 0;
   f.prefix = P.prefix ? P.prefix[b] : 0;
   f.bound = P.causal && f.key >= f.prefix ? f.key : 0;

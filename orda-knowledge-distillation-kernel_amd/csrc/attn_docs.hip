@@ -6,20 +6,21 @@
 namespace orda {
 
 // One wave per 64 positions: the numbers, -1 behind the last position and for
-// padding, and their range: (smallest, largest, whether there is padding, 0).
-// A block of padding has a range that no other meets.
+// padding, and the ranges of either half: (smallest, largest, whether there is
+// padding, 0).  A block of padding has a range that no other meets.  What lies
+// behind the last position counts for none of it: nothing there is loaded or kept.
 __global__ __launch_bounds__(64) void k_attn_docs(const int32_t* ids, int64_t ld, int64_t S, int64_t padded, int* docs, int4* ranges) {
   const int64_t at = (int64_t)blockIdx.x * 64 + threadIdx.x, row = blockIdx.y;
   int d = at < S ? ids[row * ld + at] : -1;
   if (d < 0) d = -1;
   docs[row * padded + at] = d;
   int lo = d < 0 ? 0x7fffffff : d, hi = d;
-  for (int o = 32; o; o >>= 1) {
+  for (int o = 16; o; o >>= 1) {
     lo = min(lo, __shfl_xor(lo, o));
     hi = max(hi, __shfl_xor(hi, o));
   }
-  const bool pad = __any(d < 0);
-  if (threadIdx.x == 0) ranges[row * (padded / 64) + blockIdx.x] = make_int4(lo, hi, pad, 0);
+  const int half = threadIdx.x / 32, pad = (uint32_t)(__ballot(at < S && d < 0) >> (32 * half)) != 0;
+  if (threadIdx.x % 32 == 0) ranges[row * (padded / 32) + 2 * blockIdx.x + half] = make_int4(lo, hi, pad, 0);
 }
 
 hipError_t launch_attn_docs(const int32_t* ids, int64_t ld, int64_t B, int64_t S, int64_t padded, int* docs, int4* ranges, hipStream_t s) {

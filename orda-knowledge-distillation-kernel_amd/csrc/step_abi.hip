@@ -145,7 +145,7 @@ struct Kept {
 Kept kept_of(const orda_attention_t* p, bool documents, bool training) {
   const size_t L = (size_t)padded_length(p);
   Kept k{};
-  k.docs = documents ? up256((size_t)p->batch * (L / 64) * sizeof(int4)) : 0;
+  k.docs = documents ? up256((size_t)p->batch * (L / 32) * sizeof(int4)) : 0;
   k.lse = k.docs + (documents ? up256((size_t)p->batch * L * 4) : 0);
   k.low = k.lse + (training ? up256((size_t)p->batch * p->heads * L * 4) : 0);
   k.bytes = k.low + (training ? (size_t)p->batch * p->length * p->heads * p->head_dim * 2 : 0) + 256;

@@ -93,7 +93,7 @@ struct AttnParams {
   const float* slopes;    // [H], or null
   const int32_t* prefix;  // [B], or null
   const int* docs;        // [B][padded], or null
-  const int4* ranges;     // [B][padded / 64]
+  const int4* ranges;     // [B][padded / 32]
   int64_t S, padded;      // padded: S up to a multiple of 128
   int64_t qb, qs, qh, kb, ks, kh, vb, vs, vh, gb, gs, gh;
   float* partial;         // dk and dv of each part, [2][parts][B S KV D], or null (one part)
