@@ -19,8 +19,12 @@
 //   join   the partial sums of such runs, in order
 // Equal tokens stay in their order throughout, so the sums do not depend on the
 // run, and a token that fills the batch is added up by as many waves as any
-// other.  Memory bounds it: 16384 tokens over 128256 rows of 4096 in bf16 are
-// FIGURE3.
+// other.
+//
+// Memory bounds both passes.  16384 tokens over 128256 rows of 4096 in bf16: forward
+// 268 MB in 53 us; backward 1.3 GB in 241 us (sort 23 and merge 21, with 128 MB of
+// zeros each, sums and the other 750 MB of zeros 181, join 16), where a fill of all
+// rows first and the sums behind it took 277.
 #include <algorithm>
 
 #include "pieces.hpp"
@@ -33,19 +37,33 @@ __device__ __forceinline__ int64_t token_at(const void* ids, int wide, int64_t i
 }
 
 // ------------------------------------------------------------- forward
-template <class W, class T, bool EVEN>
+// N pieces a thread, whose loads, each behind its token's, are in flight together
+// (16384 rows of 4096 in bf16: 53 us, one piece a thread 56).
+template <class W, class T, int N, bool EVEN>
 __global__ __launch_bounds__(256) void k_embed(EmbedParams P, int64_t per_row, int64_t pieces) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = pieces <= 0xffffffffll ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row;
-    const Piece<EVEN> p(i - row * per_row, P.hidden);
-    const int64_t t = token_at(P.ids, P.wide, row);
-    const bool known = t >= 0 && t < P.vocab;
-    Raw8<W> w;
-    w.get(static_cast<const W*>(P.weight) + (known ? t : 0) * P.ldw, p);
-    float v[8];
+  for (int64_t i0 = (int64_t)blockIdx.x * (256 * N) + threadIdx.x; i0 < pieces; i0 += (int64_t)gridDim.x * (256 * N)) {
+    int64_t row[N], t[N];
+    Piece<EVEN> p[N];
+    Raw8<W> w[N];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = known ? w[e] * P.scale : 0.0f;
-    put8(static_cast<T*>(P.y) + row * P.hidden, p, v);
+    for (int k = 0; k < N; ++k) {
+      const int64_t i = lmin(i0 + k * 256, pieces - 1);  // (the last piece again: the same values)
+      row[k] = pieces <= 0xffffffffll ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row;
+      p[k] = Piece<EVEN>(i - row[k] * per_row, P.hidden);
+      t[k] = token_at(P.ids, P.wide, row[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if (t[k] >= P.vocab) t[k] = -1;
+      w[k].get(static_cast<const W*>(P.weight) + (t[k] < 0 ? 0 : t[k]) * P.ldw, p[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = t[k] >= 0 ? w[k][e] * P.scale : 0.0f;
+      put8(static_cast<T*>(P.y) + row[k] * P.hidden, p[k], v);
+    }
   }
 }
 
@@ -354,9 +372,15 @@ __global__ __launch_bounds__(512) void k_embed_join(EmbedGradParams P, EmbedSums
 template <class W, class T>
 static hipError_t embed_go(const EmbedParams& P, hipStream_t s) {
   const int64_t per_row = pieces_of(P.hidden), pieces = per_row * P.tokens;
-  const unsigned groups = (unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 23);
-  if (P.hidden % 8 == 0) hipLaunchKernelGGL((k_embed<W, T, true>), dim3(groups), dim3(256), 0, s, P, per_row, pieces);
-  else hipLaunchKernelGGL((k_embed<W, T, false>), dim3(groups), dim3(256), 0, s, P, per_row, pieces);
+  auto go = [&](auto each, auto even) {
+    constexpr int N = decltype(each)::value;
+    const unsigned groups = (unsigned)std::min<int64_t>((pieces + 256 * N - 1) / (256 * N), 1 << 23);
+    hipLaunchKernelGGL((k_embed<W, T, N, decltype(even)::value>), dim3(groups), dim3(256), 0, s, P, per_row, pieces);
+  };
+  // (several pieces a thread where one each would be more workgroups than the card holds at a time)
+  const bool many = pieces > 256 * 2048, even = P.hidden % 8 == 0;
+  if (many) even ? go(std::integral_constant<int, 4>{}, std::true_type{}) : go(std::integral_constant<int, 4>{}, std::false_type{});
+  else even ? go(std::integral_constant<int, 1>{}, std::true_type{}) : go(std::integral_constant<int, 1>{}, std::false_type{});
   return hipGetLastError();
 }
 template <class W>

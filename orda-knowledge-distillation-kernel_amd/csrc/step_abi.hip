@@ -154,7 +154,7 @@ Kept kept_of(const orda_attention_t* p, bool documents, bool training) {
 // Parts that the heads of a tile of 128 keys are taken in, each by a workgroup of
 // its own: as many as bring two workgroups to a CU.  One whose keys' heads are one
 // after the other takes long on a card that these do not fill (3 x 1777 rows, 12
-// heads of 80, 4 of keys, documents: 111 us, by parts of one head 74 and 8 to add
+// heads of 80, 4 of keys, documents: 111 us, by parts of one head 74 and 9 to add
 // them up).
 struct Parts {
   int count, share;

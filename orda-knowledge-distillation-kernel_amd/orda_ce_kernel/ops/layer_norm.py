@@ -7,8 +7,8 @@
 One kernel forward, two backward (the second adds up dw's and db's partial sums, in order); csrc/rownorm.hip.  y is computed
 from s in fp32.  The backward pass reads s as it was written, rounded, with the row's mean and rstd in fp32; for fp32
 parameters beside 16-bit activations it computes s again from x and the residual, so that their gradients have fp32's
-precision.  No counterpart
-in the reference, whose models use torch (its student's RMS norm stands inside the loss: StudentRMSNorm).
+precision.  No counterpart in the reference, whose models use torch (its student's RMS norm stands inside the loss:
+StudentRMSNorm).
 """
 from __future__ import annotations
 
