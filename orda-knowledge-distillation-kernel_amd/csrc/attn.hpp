@@ -649,11 +649,15 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
   f.m = -kInf;
   f.l = 0.0f;
   attn_walk(walk, f);
-  const float l = halves_sum(f.l), mul = CAP || BIAS ? 1.0f : P.scale_log2;
+  const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
+  const float l = halves_sum(f.l);
+  // (one key alone: its 2^(m mul - m mul) is 1 but for the rounding of one of the
+  // two products; o is divided by what it was multiplied by, so that it is v)
+  const float one = __builtin_amdgcn_exp2f(fmaf(f.m, mul, -f.m * mul)), sum = l == one ? to_f32(from_f32<T>(one)) : l;
   const bool empty = !(l > 0.0f) && l == l;
   if (P.lse && lane < 32) P.lse[(int64_t)bh * P.padded + f.i] = f.i >= S || empty ? kInf : f.m * mul + __builtin_amdgcn_logf(l);
   const int64_t at = (((int64_t)b * S + f.i) * P.H + head) * P.D;
-  const float inv = empty ? 0.0f : 1.0f / l;
+  const float inv = empty ? 0.0f : 1.0f / sum;
   store_own<T, HD>(f.o, inv, static_cast<T*>(P.o) + at, P.D, f.i < S);
   // dz = P (dP - delta) cancels where P is near 1, and delta = sum(do o) would be
   // as far off as o's rounding: for the backward pass o is kept in both halves
@@ -770,17 +774,22 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P)
   f.doc = P.docs ? f.docs[f.i] : 0;
   own_rows<T, HD>(static_cast<const T*>(P.dout) + b * P.gb + head * P.gh, P.gs, f.row0, S, P.D, f.g);
   {
+    // The diagonal of o do^T, by the products that make dP: a query that sees one key
+    // has o = v, and dP - delta is 0 to the bit.
     typename Traits<T>::Frag o[HD / 16];
     const int64_t at = ((int64_t)b * S * P.H + head) * P.D;
-    f.delta = 0.0f;
+    f32x16 x;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = 0.0f;
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-      own_rows<T, HD>(static_cast<const T*>(part ? P.o_low : P.o) + at, P.H * P.D, f.row0, S, P.D, o);
+      own_rows<T, HD>(static_cast<const T*>(part ? P.o : P.o_low) + at, P.H * P.D, f.row0, S, P.D, o);
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f.delta = fmaf(to_f32(f.g[ks][e]), to_f32(o[ks][e]), f.delta);
+      for (int ks = 0; ks < HD / 16; ++ks) x = Traits<T>::mma(o[ks], f.g[ks], x);
     }
+    f.delta = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) f.delta = block_row(r) == (lane & 31) ? x[r] : f.delta;
     f.delta = f.doc < 0 ? 0.0f : halves_sum(f.delta);
     if (lane < 32) P.delta[(int64_t)bh * P.padded + f.i] = f.delta;
   }

@@ -155,6 +155,18 @@ def test_padding_may_hold_anything(kw):
         assert not any(got[n].cpu()[docs < 0].any() for n in got)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [1, 40, 64, 96, 128])
+def test_one_key_has_no_gradient_of_its_score(D, dtype):
+    """A probability of 1 whatever the score: o is v and dq and dk are zeros, not what is left of a difference."""
+    for B, S, kw in ((3, 1, dict()), (1, 1, dict(softcap=50.0, prefix=torch.tensor([1], dtype=torch.int32))),
+                     (2, 77, dict(documents=torch.arange(77)[None].expand(2, 77), causal=False))):
+        t = case(B, S, 8, 2, D, dtype, D + S)
+        got = run(t, **kw)
+        assert torch.equal(got["y"].cpu(), t["v"].repeat_interleave(4, 2)) and not got["q"].any() and not got["k"].any()
+        check({"v": got["v"]}, {"v": want(t, dtype, **kw)["v"]})
+
+
 def test_nothing_but_padding():
     t = case(1, 130, 2, 1, 64, BF, 13)
     got = run(t, documents=torch.full((1, 130), -1))
