@@ -549,9 +549,10 @@ int orda_dropout_add(const orda_rows_problem_t* p, const orda_dropout_t* d, cons
  * s (NULL: not wanted) and stats (rows x (mean, rstd) fp32; NULL: no backward
  * pass) are what the backward pass reads; without residual and dropout it may
  * read x as s.  With fp32 parameters beside 16-bit tensors it may be given x (as
- * s) and the residual instead, and computes s again in fp32.  Gradients: ds' = ds + that through the norm, dx = dropout(ds')
- * without residual, dr = ds'; dw, db.  Any gradient may be NULL; without dropout
- * dx and dr are one and only one of them may be asked for. */
+ * s) and the residual instead, and computes s again in fp32.  Gradients: ds' = ds
+ * + that through the norm, dx = dropout(ds') without residual, dr = ds'; dw, db.
+ * Any gradient may be NULL; without dropout dx and dr are one and only one of
+ * them may be asked for. */
 typedef struct orda_layer_norm {
   int32_t abi_version;
   int32_t dtype;

@@ -661,7 +661,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
   store_own<T, HD>(f.o, inv, static_cast<T*>(P.o) + at, P.D, f.i < S);
   // dz = P (dP - delta) cancels where P is near 1, and delta = sum(do o) would be
   // as far off as o's rounding: for the backward pass o is kept in both halves
-  // (8 short rows: dq and dk off by 2.4e-3 of their norm instead of 3.4e-3 in bf16).
+  // (8 short rows: dq and dk off by 2.5e-3 of their norm instead of 3.4e-3 in bf16).
   if (P.o_low) store_own<T, HD, true>(f.o, inv, static_cast<T*>(P.o_low) + at, P.D, f.i < S);
 }
 

@@ -75,13 +75,15 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causa
     as they are.  The result is ``(batch, length, heads, head_dim)``.  ``scale`` (default ``head_dim ** -0.5``) multiplies the
     products; ``softcap`` > 0 caps them to ``softcap * tanh(z / softcap)``; ``slopes`` (``(heads,)``) takes ``slopes[h] *
     |i - j|`` off.  ``causal``: query i sees the keys up to i, and with ``prefix`` (``(batch,)``) also those below
-    ``prefix[b]``.  ``documents`` (``(batch, length)``): only keys with the query's own number; a negative number is padding,
-    which sees nothing and is not seen, whatever it holds: zeros come out, and zero gradients.
+    ``prefix[b]`` (without ``causal`` it sees them all).  ``documents`` (``(batch, length)``): only keys with the query's own
+    number; a negative number is padding, which sees nothing and is not seen, whatever it holds: zeros come out, and zero
+    gradients.
 
     On the kernels bf16 and fp16 with head_dim up to 128 (multiples of 8 are read in place, others are copied).  The compute
     dtype is the loss's rule; fp32 tensors run on ``backend="torch"`` or under autocast.  Probabilities and their gradients
-    are rounded to the compute dtype as operands of products; sums are fp32.  A non-finite value in a row that a query does
-    not see may still reach it where both are in one tile of 64 rows (padding excepted).  Once differentiable, in q, k and v.
+    are rounded to the compute dtype as operands of products; sums are fp32.  A value that is not finite, in a row that a query
+    does not see, may still reach it where a query of the same 128 (from the sequence's start) sees a row of the value's 64
+    (padding excepted).  Once differentiable, in q, k and v.
     ``backend`` as :func:`distillation_loss` has it."""
     entry = "masked_attention"
     check_tensors(entry, "none", q, k=k, v=v, slopes=slopes)
@@ -97,8 +99,6 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causa
         raise ValueError(f"{entry}: slopes are constants; they have no gradient")
     documents = _integers(entry, "documents", documents, (B, S), q.device)
     prefix = _integers(entry, "prefix", prefix, (B,), q.device)
-    if prefix is not None and not causal:
-        raise ValueError(f"{entry}: prefix widens the causal mask; it needs causal=True")
     scale = D ** -0.5 if scale is None else float(scale)
     softcap = float(softcap)
     if not math.isfinite(scale):

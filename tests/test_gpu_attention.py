@@ -167,6 +167,16 @@ def test_one_key_has_no_gradient_of_its_score(D, dtype):
         check({"v": got["v"]}, {"v": want(t, dtype, **kw)["v"]})
 
 
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_a_prefix_says_nothing_without_the_causal_mask(D):
+    t = case(2, 150, 4, 2, D, BF, D)
+    docs = documents(2, 150, D)
+    for kw in (dict(), dict(documents=docs), dict(slopes=SLOPES(4), softcap=2.0)):
+        plain = run(t, causal=False, **kw)
+        got = run(t, causal=False, prefix=torch.tensor([70, -3]), **kw)
+        assert all(torch.equal(got[n], plain[n]) for n in plain)
+
+
 def test_nothing_but_padding():
     t = case(1, 130, 2, 1, 64, BF, 13)
     got = run(t, documents=torch.full((1, 130), -1))

@@ -199,7 +199,6 @@ Q = torch.zeros(2, 3, 4, 8)
     (lambda: orda.masked_attention(Q, Q, Q, documents=torch.zeros(2, 3)), ValueError, "documents must be an int32"),
     (lambda: orda.masked_attention(Q, Q, Q, documents=torch.zeros(3, 2, dtype=torch.int32)), ValueError, "documents must have shape"),
     (lambda: orda.masked_attention(Q, Q, Q, prefix=torch.zeros(3, dtype=torch.int32)), ValueError, "prefix must have shape"),
-    (lambda: orda.masked_attention(Q, Q, Q, causal=False, prefix=torch.zeros(2, dtype=torch.int32)), ValueError, "needs causal"),
     (lambda: orda.masked_attention(Q, Q, Q, softcap=-1.0), ValueError, "softcap must be"),
     (lambda: orda.masked_attention(Q, Q, Q, softcap=math.inf), ValueError, "softcap must be"),
     (lambda: orda.masked_attention(Q, Q, Q, scale=math.nan), ValueError, "scale must be finite"),
