@@ -76,8 +76,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causa
     products; ``softcap`` > 0 caps them to ``softcap * tanh(z / softcap)``; ``slopes`` (``(heads,)``) takes ``slopes[h] *
     |i - j|`` off.  ``causal``: query i sees the keys up to i, and with ``prefix`` (``(batch,)``) also those below
     ``prefix[b]`` (without ``causal`` it sees them all).  ``documents`` (``(batch, length)``): only keys with the query's own
-    number; a negative number is padding, which sees nothing and is not seen, whatever it holds: zeros come out, and zero
-    gradients.
+    number (int64 numbers past 2^31 - 1 count as that one); a negative number is padding, which sees nothing and is not
+    seen, whatever it holds: zeros come out, and zero gradients.
 
     On the kernels bf16 and fp16 with head_dim up to 128 (multiples of 8 are read in place, others are copied).  The compute
     dtype is the loss's rule; fp32 tensors run on ``backend="torch"`` or under autocast.  Probabilities and their gradients

@@ -124,6 +124,50 @@ def test_more_tiles_than_one_look():
     compare(t, BF, prefix=torch.tensor([4200], dtype=torch.int32))
 
 
+@pytest.mark.parametrize("D", [24, 72, 128])
+def test_long_sequences(D):
+    """Ten looks of 64 tiles and more, two heads that share keys, a prefix and documents, against sums in float64 that never
+    hold more than some rows of scores.  An operand of a product (P, dz) is off by half a step of bf16, 2^-8 of it (8 bits:
+    steps of 2^-7 of the power of two below), as is a result.  delta = do o takes o as the rounded P made it: it is off by
+    that of |do| P |v|, and dz by P times as much.  P = 2^(z - L) by the rounding of z and L in fp32, |z| and |L| below 64
+    here: 2^-24 * 128 ln 2 < 2^-17, and with it dz before it cancels, dP and delta being sums of D <= 128 products in fp32
+    (2^-17 of their absolute sums, as o's two halves)."""
+    S, H, step, half, tail = 41_000, 2, 500, torch.finfo(BF).eps / 2, 2.0 ** -16
+    t = case(1, S, H, 1, D, BF, D)
+    docs = (torch.arange(S, dtype=torch.int32) // 17_000)[None].clone()
+    docs[0, 30_000:30_100] = 0
+    docs[0, -70:] = -1
+    prefix = 2_500
+    got = {n: v[0].double() for n, v in run(t, documents=docs, prefix=torch.tensor([prefix], dtype=torch.int32)).items()}
+    q, k, v, dy = (t[n][0].cuda().double() for n in ("q", "k", "v", "dy"))
+    k, v, docs, at = k[:, 0], v[:, 0], docs[0].cuda(), torch.arange(S, device="cuda")
+    scale = D ** -0.5
+    dk, dv, dk_off, dv_off = (torch.zeros(S, D, dtype=torch.float64, device="cuda") for _ in range(4))
+
+    def near(a, b, off):
+        assert bool(((a - b).abs() <= off + half * (b.abs() + off) + 2.0 ** -120).all())
+
+    for i in range(0, S, step):
+        r = slice(i, i + step)
+        seen = ((at[r, None] >= at) | (at < prefix)) & (docs[r, None] == docs) & (docs[r, None] >= 0)
+        for h in range(H):
+            z = (q[r, h] @ k.t() * scale).masked_fill(~seen, -math.inf)
+            p = torch.softmax(z, -1).nan_to_num(0.0)
+            o, g = p @ v, dy[r, h]
+            near(got["y"][r, h], o, (half + tail) * (p @ v.abs()))
+            dp, delta = g @ v.t(), (g * o).sum(-1, keepdim=True)
+            dz = p * (dp - delta)
+            of_delta = (g.abs() * (p @ v.abs())).sum(-1, keepdim=True)
+            off = half * dz.abs() + p * (tail * (g.abs() @ v.abs().t()) + (half + tail) * of_delta)
+            near(got["q"][r, h], scale * dz @ k, scale * off @ k.abs())
+            dk += scale * dz.t() @ q[r, h]
+            dk_off += scale * off.t() @ q[r, h].abs()
+            dv += p.t() @ g
+            dv_off += (half + tail) * (p.t() @ g.abs())
+    near(got["k"][:, 0], dk, dk_off)
+    near(got["v"][:, 0], dv, dv_off)
+
+
 def test_packed_documents_are_their_own_sequences():
     """Each document's rows are, to the bit, not those of another batch, but within the bounds of its own sequence."""
     t = case(1, 330, 2, 2, 64, BF, 9)
