@@ -407,10 +407,11 @@ __device__ __forceinline__ void hide(f32x16& z, int bound, const int* docs, cons
   }
 }
 
-// Scores from products s = q.k.  Plain ones stay as they are, and what uses them
-// multiplies by mul = |scale| log2(e); capped or biased ones are formed here, in
-// units of log2 (mul = 1): log2(e) (cap tanh(scale s / cap) - slope |i - j|),
-// with CAP also the tanh.  dist: the lane's row less the block's first.
+// Scores from products s = q.k.  Without a cap in units of the products, s - slope
+// / |scale| |i - j|, and what uses them multiplies by mul = |scale| log2(e); with
+// one in units of log2 (mul = 1), log2(e) (cap tanh(scale s / cap) - slope |i - j|),
+// and also the tanh.  slope: times P.slope_mul.  dist: the lane's row less the
+// block's first.
 // tanh u = 1 - 2 / (1 + e^2u) on the hardware's exp2 and reciprocal, off by 2e-7,
 // a cap of 50 by 1e-5, below half a step of a 16-bit probability.  (A negative
 // scale is turned over to one of the operands.)
@@ -421,11 +422,9 @@ __device__ __forceinline__ void scores(f32x16& z, float (&th)[16], const AttnPar
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       if constexpr (CAP) {
-        const float e = __builtin_amdgcn_exp2f(z[r] * P.cap_in);
-        th[r] = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e);
-        z[r] = th[r] * P.cap_out;
-      } else {
-        z[r] *= P.scale_log2;
+        const float part = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z[r] * P.cap_in));
+        th[r] = fmaf(-2.0f, part, 1.0f);
+        z[r] = fmaf(-2.0f * P.cap_out, part, P.cap_out);
       }
       if constexpr (BIAS) z[r] = fmaf(-slope, fabsf(from - (float)((r >> 2) * 8 + (r & 3))), z[r]);
     }
@@ -573,7 +572,7 @@ struct AttnForward {
 #pragma unroll
     for (int r = 2; r < 16; ++r) top = fmaxf(top, x[r]);
     top = halves_max(top);
-    const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
+    const float mul = CAP ? 1.0f : P.scale_log2;
     // The maximum follows only where it grows by more than 2^8: sums and products
     // of probabilities up to 2^8 lose nothing in fp32.
     if (__any(top * mul > m * mul + 8.0f)) {
@@ -630,7 +629,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
   f.i = f.row0 + (lane & 31);
   f.K = static_cast<const T*>(P.k) + b * P.kb + kv * P.kh;
   f.V = static_cast<const T*>(P.v) + b * P.vb + kv * P.vh;
-  f.slope = BIAS ? P.slopes[head] * kLog2e : 0.0f;
+  f.slope = BIAS ? P.slopes[head] * P.slope_mul : 0.0f;
   f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
   f.ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / 32) : nullptr;
   f.doc = P.docs ? f.docs[f.i] : 0;
@@ -649,7 +648,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
   f.m = -kInf;
   f.l = 0.0f;
   attn_walk(walk, f);
-  const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
+  const float mul = CAP ? 1.0f : P.scale_log2;
   const float l = halves_sum(f.l);
   // (one key alone: its 2^(m mul - m mul) is 1 but for the rounding of one of the
   // two products; o is divided by what it was multiplied by, so that it is v)
@@ -727,7 +726,7 @@ struct AttnGradQ {
     scores<CAP, BIAS>(x, th, P, slope, i - at);
     if (t.part(BLOCK)) hide<true>(x, bound, docs, ranges, at, doc);
     if constexpr (kBeside) second();
-    const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
+    const float mul = CAP ? 1.0f : P.scale_log2;
     float z[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(x[r], mul, -lse));
@@ -768,7 +767,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P)
   f.i = f.row0 + (lane & 31);
   f.K = static_cast<const T*>(P.k) + b * P.kb + kv * P.kh;
   f.V = static_cast<const T*>(P.v) + b * P.vb + kv * P.vh;
-  f.slope = BIAS ? P.slopes[head] * kLog2e : 0.0f;
+  f.slope = BIAS ? P.slopes[head] * P.slope_mul : 0.0f;
   f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
   f.ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / 32) : nullptr;
   f.doc = P.docs ? f.docs[f.i] : 0;
@@ -922,9 +921,9 @@ struct AttnGradKV {
       for (int g = 0; g < 4; ++g) L[g] = *reinterpret_cast<const f4v*>(stat(slot, BLOCK, 0) + 32 * g);
       fr.cols(lds_at(grows(slot, BLOCK)), cf);
       float th[16], p[16];
-      scores<CAP, BIAS>(x, th, P, BIAS ? slopes[t.head] * kLog2e : 0.0f, key - at);
+      scores<CAP, BIAS>(x, th, P, BIAS ? slopes[t.head] * P.slope_mul : 0.0f, key - at);
       if (t.part(BLOCK)) hide<false>(x, bound, docs, ranges, at, doc);
-      const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
+      const float mul = CAP ? 1.0f : P.scale_log2;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         f4v out;
@@ -1138,9 +1137,9 @@ struct AttnGradBoth {
     fetch(gt, rows);
     fr.cols(lds_at(gt), cf);
     float th[16], p[16];
-    scores<CAP, BIAS>(x, th, P, BIAS ? slopes[t.head] * kLog2e : 0.0f, key - at);
+    scores<CAP, BIAS>(x, th, P, BIAS ? slopes[t.head] * P.slope_mul : 0.0f, key - at);
     if (t.part(BLOCK)) hide<false>(x, bound, docs, ranges, at, doc);
-    const float mul = CAP || BIAS ? 1.0f : P.scale_log2;
+    const float mul = CAP ? 1.0f : P.scale_log2;
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) dp = Traits<T>::mma(rows[ks], v[ks], dp);
 #pragma unroll

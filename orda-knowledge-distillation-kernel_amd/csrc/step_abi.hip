@@ -201,11 +201,12 @@ AttnParams attn_params(const orda_attention_t* p, const void* q, const void* k, 
   a.D = p->head_dim;
   a.causal = p->causal;
   const double log2e = 1.4426950408889634;
-  // (magnitudes: the kernels turn the sign of one operand; a scale of 0 is 1e-30,
+  // (magnitudes: the kernels turn the sign of one operand; a scale of 0 is 1e-24,
   // so that the -inf of what is not seen stays one)
-  const double size = std::fmax(std::fabs(p->scale), 1e-30);
+  const double size = std::fmax(std::fabs(p->scale), 1e-24);
   a.scale = (float)p->scale;
   a.scale_log2 = (float)(size * log2e);
+  a.slope_mul = (float)(p->softcap > 0.0 ? log2e : 1.0 / size);
   if (p->softcap > 0.0) {
     a.cap_in = (float)(2.0 * log2e * size / p->softcap);
     a.cap_out = (float)(p->softcap * log2e);

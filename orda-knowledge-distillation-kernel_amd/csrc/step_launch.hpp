@@ -100,6 +100,7 @@ struct AttnParams {
   int B, H, KV, group, D, causal, tiles;
   int parts, share;         // workgroups that take the heads of a tile of keys, heads of each
   float scale, scale_log2;  // scale_log2 = |scale| log2(e)
+  float slope_mul;          // 1 / |scale|, with a cap log2(e)
   float cap_in, cap_out;    // 2 |scale| log2(e) / cap and cap log2(e); 0: no cap
 };
 enum AttnPass { ATTN_FORWARD, ATTN_DQ, ATTN_DKV };

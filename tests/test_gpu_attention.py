@@ -221,6 +221,13 @@ def test_a_prefix_says_nothing_without_the_causal_mask(D):
         assert all(torch.equal(got[n], plain[n]) for n in plain)
 
 
+@pytest.mark.parametrize("scale,cap", [(0.0, 0.0), (1e-6, 0.0), (-30.0, 0.0), (0.0, 3.0)])
+def test_slopes_beside_small_and_large_scales(scale, cap):
+    """Slopes of either sign, none, and one so steep that a query sees itself alone."""
+    t = case(2, 140, 4, 2, 64, BF, 31, scale=0.4)
+    compare(t, BF, scale=scale, softcap=cap, slopes=torch.tensor([0.5, 0.0, -0.03, 1e6]))
+
+
 def test_nothing_but_padding():
     t = case(1, 130, 2, 1, 64, BF, 13)
     got = run(t, documents=torch.full((1, 130), -1))
