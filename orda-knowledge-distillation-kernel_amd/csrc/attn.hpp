@@ -506,7 +506,7 @@ __device__ __forceinline__ void attn_walk_plain(AttnWalk<KEYS>& walk, F& f) {
 }
 
 // ------------------------------------------------------------- forward
-// 2 x 4096 rows of 32 heads (8) of 128 in bf16, causal: 275 GFLOP in 326 us, 843
+// 2 x 4096 rows of 32 heads (8) of 128 in bf16, causal: 275 GFLOP in 322 us, 854
 // TFLOP/s; the matrix cores are busy for 47 % of it, at 1.9 GHz (16 heads without
 // others, no mask: 157 us, 875 TFLOP/s; 8 heads, a workgroup to a CU: 104 us, what
 // a workgroup's 128 blocks take one after the other).
@@ -666,8 +666,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
 
 // ------------------------------------------------------------- dq
 // Also delta = sum(do o) of each query, which the next kernel reads.  2 x 4096 rows
-// of 32 heads (8) of 128 in bf16, causal: 412 GFLOP in 420 us, 982 TFLOP/s, the
-// matrix cores busy for 56 % of it at 1.8 GHz.
+// of 32 heads (8) of 128 in bf16, causal: 412 GFLOP in 408 us, 1010 TFLOP/s,
+// the matrix cores busy for 56 % of it at 1.8 GHz.
 template <class T, int HD, bool CAP, bool BIAS>
 struct AttnGradQ {
   using Frag = typename Traits<T>::Frag;
@@ -847,7 +847,7 @@ struct AttnKeys {  // of a workgroup: batch, key head, first row, the heads it t
 // product beside its own vector work instead took 158 us against 136: 8 heads of
 // 80, 4096.)
 //
-// 2 x 4096 rows of 32 heads (8) of 128 in bf16, causal: 550 GFLOP in 655 us, 840
+// 2 x 4096 rows of 32 heads (8) of 128 in bf16, causal: 550 GFLOP in 640 us, 860
 // TFLOP/s; the matrix cores are busy for 46 % of it, at 1.9 GHz, LDS for 37 %, and a
 // phase waits for its two halves in turn.
 template <class T, int HD, bool CAP, bool BIAS>
