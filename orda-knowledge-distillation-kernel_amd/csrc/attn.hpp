@@ -525,7 +525,7 @@ struct AttnForward {
   f32x16 o[kBlocks];
   f32x16 s[2];
   float m, l, slope;
-  int row0, i, bound, doc, prefix;
+  int row0, i, bound, doc;
   __device__ __forceinline__ AttnForward(const AttnParams& p) : P(p) {}
   __device__ __forceinline__ void issue(const AttnTile& t, int two, int three) {
     kd.issue(K + t.first * P.ks, (int)P.S - t.first, klds + two * kTile);
@@ -635,7 +635,6 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
   f.doc = P.docs ? f.docs[f.i] : 0;
   AttnWalk<true> walk;
   walk.init(P, b, q0);
-  f.prefix = walk.prefix;
   f.bound = P.causal ? min(S, max(f.i + 1, walk.prefix)) : S;
   own_rows<T, HD>(static_cast<const T*>(P.q) + b * P.qb + head * P.qh, P.qs, f.row0, S, P.D, f.q, P.scale < 0.0f);
   f.kd.init(P.ks, P.D);
@@ -682,7 +681,7 @@ struct AttnGradQ {
   Frag q[HD / 16], g[HD / 16];
   f32x16 dq[kBlocks];
   float lse, delta, slope;
-  int row0, i, bound, doc, prefix;
+  int row0, i, bound, doc;
   __device__ __forceinline__ AttnGradQ(const AttnParams& p) : P(p) {}
   __device__ __forceinline__ void issue(const AttnTile& t, int slot) {
     kd.issue(K + t.first * P.ks, (int)P.S - t.first, klds + slot * kTile);
@@ -796,7 +795,6 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P)
   f.lse = P.lse[(int64_t)bh * P.padded + f.i];
   AttnWalk<true> walk;
   walk.init(P, b, q0);
-  f.prefix = walk.prefix;
   f.bound = P.causal ? min(S, max(f.i + 1, walk.prefix)) : S;
   own_rows<T, HD>(static_cast<const T*>(P.q) + b * P.qb + head * P.qh, P.qs, f.row0, S, P.D, f.q, P.scale < 0.0f);
   f.kd.init(P.ks, P.D);
@@ -872,7 +870,7 @@ struct AttnGradKV {
   f32x16 x;                              // first: S of the next phase's block
   Frag rows[HD / 16], cf[2][kBlocks];    // second: operands of the next phase
   Frag zf[2];                            // second: dz of the last phase's block
-  int row0, key, bound, doc, prefix;
+  int row0, key, bound, doc;
   __device__ __forceinline__ AttnGradKV(const AttnParams& p) : P(p) {}
   __device__ __forceinline__ void issue(const AttnTile& t, int slot) {
     qd.issue(Q + t.head * P.qh + t.first * P.qs, (int)P.S - t.first, qlds + slot * kTile);
@@ -1035,8 +1033,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_dkv(AttnParams P) {
   f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
   f.ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / 32) : nullptr;
   f.doc = P.docs ? f.docs[f.key] : 0;
-  f.prefix = P.prefix ? P.prefix[b] : 0;
-  f.bound = P.causal && f.key >= f.prefix ? f.key : 0;
+  const int prefix = P.prefix ? P.prefix[b] : 0;
+  f.bound = P.causal && f.key >= prefix ? f.key : 0;
   f.Q = static_cast<const T*>(P.q) + b * P.qb + head * P.qh;
   f.G = static_cast<const T*>(P.dout) + b * P.gb + head * P.gh;
   f.lse = P.lse + ((int64_t)b * P.H + head) * P.padded;
@@ -1098,7 +1096,7 @@ struct AttnGradBoth {
   AttnFrags<T, HD> fr;
   Frag k[HD / 16], v[HD / 16];
   f32x16 dk[kBlocks], dv[kBlocks];
-  int row0, key, bound, doc, prefix;
+  int row0, key, bound, doc;
   __device__ __forceinline__ AttnGradBoth(const AttnParams& p) : P(p) {}
   __device__ __forceinline__ void issue(const AttnTile& t, int slot) {
     qd.issue(Q + t.head * P.qh + t.first * P.qs, (int)P.S - t.first, qlds + slot * kTile);
@@ -1182,8 +1180,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_dkv_one(AttnParams P) {
   f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
   f.ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / 32) : nullptr;
   f.doc = P.docs ? f.docs[f.key] : 0;
-  f.prefix = P.prefix ? P.prefix[b] : 0;
-  f.bound = P.causal && f.key >= f.prefix ? f.key : 0;
+  const int prefix = P.prefix ? P.prefix[b] : 0;
+  f.bound = P.causal && f.key >= prefix ? f.key : 0;
   f.Q = static_cast<const T*>(P.q) + b * P.qb + head * P.qh;
   f.G = static_cast<const T*>(P.dout) + b * P.gb + head * P.gh;
   f.lse = P.lse + ((int64_t)b * P.H + head) * P.padded;

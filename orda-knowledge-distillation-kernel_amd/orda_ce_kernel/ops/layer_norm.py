@@ -49,8 +49,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     in fp32.  ``p``, ``seed`` and ``site`` as :func:`counter_dropout` has them (``p`` > 0 needs ``residual``).  The result has
     the compute dtype of ``x`` and ``residual`` (the loss's rule).  Gradients for every tensor, through y and s; once
     differentiable.  A training call keeps s (x without ``residual``, both with fp32 parameters beside 16-bit tensors) and two
-    fp32 numbers a row.  ``backend`` as
-    :func:`distillation_loss` has it."""
+    fp32 numbers a row.  ``backend`` as :func:`distillation_loss` has it."""
     entry = "layer_norm"
     check_tensors(entry, "none", x, weight=weight, bias=bias, residual=residual)
     check_shape(entry, "weight", weight, (x.shape[-1],))
