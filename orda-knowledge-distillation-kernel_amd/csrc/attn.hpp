@@ -232,6 +232,15 @@ __device__ __forceinline__ void as_operand(const float (&x)[16], typename Traits
   }
 }
 
+// What x's rounding to f left, as operands of their own: FINE, for short sequences.
+template <class T>
+__device__ __forceinline__ void rest_operand(const float (&x)[16], const typename Traits<T>::Frag (&f)[2], typename Traits<T>::Frag (&rest)[2]) {
+  float y[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) y[i] = x[i] - to_f32(f[i >> 3][i & 7]);
+  as_operand<T>(y, rest);
+}
+
 // acc^T (columns d, the lane's row) times `mul` to the lane's row at p: lanes l
 // and l + 32 exchange groups of 4 columns, so that each stores 8 in a row.  LOW:
 // what the rounding left instead, itself rounded.
@@ -667,7 +676,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
 // Also delta = sum(do o) of each query, which the next kernel reads.  2 x 4096 rows
 // of 32 heads (8) of 128 in bf16, causal: 412 GFLOP in 408 us, 1010 TFLOP/s,
 // the matrix cores busy for 56 % of it at 1.8 GHz.
-template <class T, int HD, bool CAP, bool BIAS>
+template <class T, int HD, bool CAP, bool BIAS, bool FINE>
 struct AttnGradQ {
   using Frag = typename Traits<T>::Frag;
   static constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32, kHalf = kTile / 2;
@@ -743,6 +752,14 @@ struct AttnGradQ {
     Frag zf[2], kf[2][kBlocks];
     as_operand<T>(z, zf);  // (dz in 16 bits, as an operand of the product)
     fr.cols(lds_at(klds) + (uint32_t)(slot * kTile + BLOCK * kHalf), kf);
+    if constexpr (FINE) {
+      Frag rest[2];
+      rest_operand<T>(z, zf, rest);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d) dq[d] = Traits<T>::mma(kf[k][d], rest[k], dq[d]);
+    }
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -750,7 +767,7 @@ struct AttnGradQ {
   }
 };
 
-template <class T, int HD, bool CAP, bool BIAS>
+template <class T, int HD, bool CAP, bool BIAS, bool FINE>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P) {
   constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32;
   __shared__ __attribute__((aligned(1024))) char lds[4 * kTile];
@@ -759,7 +776,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P)
   q0 *= kAttnRows;
   const int b = bh / P.H, head = bh - b * P.H, kv = head / P.group;
   const int lane = threadIdx.x & 63, S = (int)P.S;
-  AttnGradQ<T, HD, CAP, BIAS> f(P);
+  AttnGradQ<T, HD, CAP, BIAS, FINE> f(P);
   f.klds = lds;
   f.vlds = lds + 2 * kTile;
   f.row0 = q0 + wave_id() * 32;
@@ -946,8 +963,10 @@ struct AttnGradKV {
   template <int BLOCK>
   __device__ __forceinline__ void follow(const AttnTile& u, bool has, const AttnTile& t, int slot, bool here, int to, bool more) {
     constexpr int kOther = 1 - BLOCK;
+    float z[16];
+    const bool made = here && t.sees(kOther);
     if (has && u.sees(BLOCK)) add_up(zf);
-    if (here && t.sees(kOther)) {
+    if (made) {
       f32x16 dp;
       f4v dl[4], p[4];
 #pragma unroll
@@ -956,13 +975,17 @@ struct AttnGradKV {
         p[g] = *reinterpret_cast<const f4v*>(prob(kOther) + g * 1024);
       }
       product(dp);
-      float z[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) z[r] = p[r >> 2][r & 3] * (dp[r] - dl[r >> 2][r & 3]);
       as_operand<T>(z, zf);
     }
     if (more) fetch(grows(to, BLOCK));
     if (here) fr.cols(lds_at(qrows(slot, kOther)), cf);
+    if (P.fine && made) {
+      Frag rest[2];
+      rest_operand<T>(z, zf, rest);
+      add_up(rest);
+    }
   }
   // (a loop of its own for each of the two: in one, what either holds would take
   // registers of both)
@@ -1079,7 +1102,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_dkv(AttnParams P) {
 // instead of 202, 64 heads: 594 instead of 788).  96 columns would not fit: 23
 // registers in scratch, and 202 us instead of 141 for 8 heads of 80, 1036 instead of
 // 1072 for 64.
-template <class T, bool CAP, bool BIAS>
+template <class T, bool CAP, bool BIAS, bool FINE>
 struct AttnGradBoth {
   static constexpr int HD = 64;
   using Frag = typename Traits<T>::Frag;
@@ -1156,6 +1179,14 @@ struct AttnGradBoth {
 #pragma unroll
     for (int r = 0; r < 16; ++r) p[r] *= dp[r] - stat[r >> 2][r & 3];
     as_operand<T>(p, f);
+    if constexpr (FINE) {
+      Frag rest[2];
+      rest_operand<T>(p, f, rest);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d) dk[d] = Traits<T>::mma(cf[j][d], rest[j], dk[d]);
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -1163,9 +1194,9 @@ struct AttnGradBoth {
   }
 };
 
-template <class T, bool CAP, bool BIAS>
+template <class T, bool CAP, bool BIAS, bool FINE>
 __global__ __launch_bounds__(256, 2) void k_attn_dkv_one(AttnParams P) {
-  using F = AttnGradBoth<T, CAP, BIAS>;
+  using F = AttnGradBoth<T, CAP, BIAS, FINE>;
   constexpr int HD = F::HD, kBlocks = F::kBlocks;
   __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
   const AttnKeys at(P, blockIdx.x);
@@ -1222,10 +1253,17 @@ static hipError_t attn_go(AttnParams P, AttnPass pass, hipStream_t s) {
   const dim3 grid((unsigned)(P.tiles * P.B * (pass == ATTN_DKV ? P.KV * P.parts : P.H)));
   switch (pass) {
     case ATTN_FORWARD: hipLaunchKernelGGL((k_attn<T, HD, CAP, BIAS>), grid, dim3(256), 0, s, P); break;
-    case ATTN_DQ: hipLaunchKernelGGL((k_attn_dq<T, HD, CAP, BIAS>), grid, dim3(256), 0, s, P); break;
+    case ATTN_DQ:
+      if (P.fine) hipLaunchKernelGGL((k_attn_dq<T, HD, CAP, BIAS, true>), grid, dim3(256), 0, s, P);
+      else hipLaunchKernelGGL((k_attn_dq<T, HD, CAP, BIAS, false>), grid, dim3(256), 0, s, P);
+      break;
     default:
-      if constexpr (HD == 64) hipLaunchKernelGGL((k_attn_dkv_one<T, CAP, BIAS>), grid, dim3(256), 0, s, P);
-      else hipLaunchKernelGGL((k_attn_dkv<T, HD, CAP, BIAS>), grid, dim3(512), 0, s, P);
+      if constexpr (HD == 64) {
+        if (P.fine) hipLaunchKernelGGL((k_attn_dkv_one<T, CAP, BIAS, true>), grid, dim3(256), 0, s, P);
+        else hipLaunchKernelGGL((k_attn_dkv_one<T, CAP, BIAS, false>), grid, dim3(256), 0, s, P);
+      } else {
+        hipLaunchKernelGGL((k_attn_dkv<T, HD, CAP, BIAS>), grid, dim3(512), 0, s, P);
+      }
   }
   return hipGetLastError();
 }

@@ -196,6 +196,12 @@ AttnParams attn_params(const orda_attention_t* p, const void* q, const void* k, 
   a.H = p->heads;
   a.KV = p->kv_heads;
   a.group = p->heads / p->kv_heads;
+  // The rounding of dz does not average out over a few keys, and there is time for
+  // two products more: dq and dk of 8 rows in bf16 are off by 1.8e-3 of their norm
+  // instead of 2.5e-3, of 64 by 1.7e-3 instead of 2.4e-3 (1.7e-3 is their own
+  // rounding).  Over long sequences dq would take 200 us instead of 124 (8 heads of
+  // 128, 4096: the registers do not hold both).
+  a.fine = p->length <= 64;
   a.parts = parts_of(p).count;
   a.share = parts_of(p).share;
   a.D = p->head_dim;

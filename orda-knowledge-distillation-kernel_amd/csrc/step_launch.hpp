@@ -98,6 +98,7 @@ struct AttnParams {
   int64_t qb, qs, qh, kb, ks, kh, vb, vs, vh, gb, gs, gh;
   float* partial;         // dk and dv of each part, [2][parts][B S KV D], or null (one part)
   int B, H, KV, group, D, causal, tiles;
+  int fine;                 // dz goes into its products in two halves
   int parts, share;         // workgroups that take the heads of a tile of keys, heads of each
   float scale, scale_log2;  // scale_log2 = |scale| log2(e)
   float slope_mul;          // 1 / |scale|, with a cap log2(e)
