@@ -81,9 +81,9 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causa
 
     On the kernels bf16 and fp16 with head_dim up to 128 (multiples of 8 are read in place, others are copied).  The compute
     dtype is the loss's rule; fp32 tensors run on ``backend="torch"`` or under autocast.  Probabilities and their gradients
-    are rounded to the compute dtype as operands of products (the latter in two parts up to a length of 64); sums are fp32.  A value that is not finite, in a row that a query
-    does not see, may still reach it where a query of the same 128 (from the sequence's start) sees a row of the value's 64
-    (padding excepted).  Once differentiable, in q, k and v.
+    are rounded to the compute dtype as operands of products (the latter in two parts up to a length of 64); sums are fp32.
+    A value that is not finite, in a row that a query does not see, may still reach it where a query of the same 128 (from
+    the sequence's start) sees a row of the value's 64 (padding excepted).  Once differentiable, in q, k and v.
     ``backend`` as :func:`distillation_loss` has it."""
     entry = "masked_attention"
     check_tensors(entry, "none", q, k=k, v=v, slopes=slopes)
