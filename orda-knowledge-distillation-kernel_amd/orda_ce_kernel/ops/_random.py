@@ -34,7 +34,8 @@ def check_dropout(entry: str, p: float, seed, site: int, device: torch.device):
         if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{entry}: a captured call would repeat one seed with every replay; pass seed= as an int64 tensor "
                                "on the device and change it between replays")
-        return p, int(torch.randint(1 << 62, (), dtype=torch.int64)), None  # (torch.manual_seed; no device work)
+        # (torch.manual_seed; no device work, whatever torch.device() or the default device says)
+        return p, int(torch.randint(1 << 62, (), dtype=torch.int64, device="cpu")), None
     if isinstance(seed, bool) or not isinstance(seed, int) or not 0 <= seed < 1 << 64:
         raise ValueError(f"{entry}: seed must be an int in [0, 2^64) or an int64 tensor, got {seed!r}")
     return p, seed, None
