@@ -50,7 +50,9 @@ def _torch(q, k, v, causal, scale, softcap, slopes, documents, prefix, dtype):
     some = seen.any(-1, keepdim=True)
     z = torch.where(seen, z, -math.inf)
     p = torch.softmax(torch.where(some, z, 0.0), -1)
-    return torch.matmul(torch.where(some, p, 0.0), vf).transpose(1, 2).to(dtype)
+    o = torch.matmul(torch.where(some, p, 0.0), vf).transpose(1, 2).to(dtype)
+    # (the gradient from above of a padding row may hold anything too)
+    return o if documents is None else torch.where(real, o, torch.zeros((), dtype=dtype, device=o.device))
 
 
 def _integers(entry, name, t, shape, device):

@@ -1,6 +1,8 @@
 """What the docstrings of a student's operators promise beside their formulas, on the CPU."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -18,3 +20,20 @@ def test_a_drawn_seed_does_not_depend_on_the_default_device(call):
         torch.manual_seed(11)
         assert torch.equal(call(x), want)
     assert torch.equal(torch.get_rng_state(), state)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("kw", [dict(), dict(causal=False, softcap=3.0), dict(prefix=torch.tensor([4, 6])), dict(slopes=torch.ones(2))],
+                         ids=lambda kw: "-".join(kw) or "causal")
+def test_padding_of_the_gradient_from_above_may_hold_anything(kw, bad):
+    """The torch formulation: what dy holds in rows without a document reaches no gradient."""
+    docs = torch.tensor([[0, 0, 0, 0, -1, -1], [-3, 1, 1, -1, 2, 2]])
+    g = torch.Generator().manual_seed(4)
+    leaves = [torch.randn(2, 6, 2, 4, generator=g).requires_grad_(True) for _ in range(3)]
+    dy = torch.randn(2, 6, 2, 4, generator=g)
+    y = orda.masked_attention(*leaves, documents=docs, **kw)
+    want = torch.autograd.grad(y, leaves, torch.where((docs < 0)[:, :, None, None], 0.0, dy), retain_graph=True)
+    got = torch.autograd.grad(y, leaves, torch.where((docs < 0)[:, :, None, None], bad, dy))
+    assert not y[docs < 0].any()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b) and torch.isfinite(a).all() and not a[docs < 0].any()
