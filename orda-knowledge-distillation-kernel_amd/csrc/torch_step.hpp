@@ -94,7 +94,10 @@ Tensor dropout_run(const Tensor& x_, const Tensor& res_, const Drop& d, ScalarTy
   Tensor x = x_.scalar_type() == type ? x_ : x_.to(type), r = !res_.defined() || res_.scalar_type() == type ? res_ : res_.to(type);
   orda_rows_problem_t p{ORDA_ABI_VERSION, code(type), 1, x.numel(), 0, 0};
   Tensor y = at::empty(x.sizes(), x.options());
-  if (!x.is_contiguous() || (r.defined() && !r.is_contiguous())) {  // row by row
+  if (x.size(-1) > (1 << 22)) {  // (rows longer than a pitch may be: one dense row)
+    x = x.contiguous();
+    if (r.defined()) r = r.contiguous();
+  } else if (!x.is_contiguous() || (r.defined() && !r.is_contiguous())) {  // row by row
     x = rows_of(x.reshape({-1, x.size(-1)}), type);
     if (r.defined()) r = rows_of(r.reshape({-1, r.size(-1)}), type);
     p.rows = x.size(0);
