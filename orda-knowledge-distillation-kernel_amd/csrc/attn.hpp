@@ -419,21 +419,34 @@ __device__ __forceinline__ void hide(f32x16& z, int bound, const int* docs, cons
 // Scores from products s = q.k.  Without a cap in units of the products, s - slope
 // / |scale| |i - j|, and what uses them multiplies by mul = |scale| log2(e); with
 // one in units of log2 (mul = 1), log2(e) (cap tanh(scale s / cap) - slope |i - j|),
-// and also the tanh.  slope: times P.slope_mul.  dist: the lane's row less the
-// block's first.
-// tanh u = 1 - 2 / (1 + e^2u) on the hardware's exp2 and reciprocal, off by 2e-7,
-// a cap of 50 by 1e-5, below half a step of a 16-bit probability.  (A negative
-// scale is turned over to one of the operands.)
-template <bool CAP, bool BIAS>
+// and also the tanh.  slope: times P.slope_mul.  dist: the lane's row less the block's
+// first.  (A negative scale is turned over to one of the operands.)
+//
+// tanh u = 1 - 2 / (1 + e^2u) on the hardware's exp2 and reciprocal is off by 2e-7
+// whatever u is, and cap tanh u by 2e-7 cap.  CAP_SMALL takes that (128: 2e-5, a
+// 25th of half a step of an fp16 probability).  CAP_ANY has below |u| = 1/4 the
+// series u (1 - u^2/3 + 2 u^4/15 - 17 u^6/315 + 62 u^8/2835), whose next term is 9e-9
+// of it, so that the capped score is off by at most 2^-18 of itself at any cap.
+// (3 x 1777 rows of 12 heads of 80, forward, dq, dk and dv: 67, 82 and 122 us with
+// CAP_SMALL, 100, 119 and 171 with CAP_ANY.)
+template <int CAP, bool BIAS>
 __device__ __forceinline__ void scores(f32x16& z, float (&th)[16], const AttnParams& P, float slope, int dist) {
   if constexpr (CAP || BIAS) {
     const float from = (float)(dist - block_row(0));  // (exact: lengths are below 2^24)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       if constexpr (CAP) {
-        const float part = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z[r] * P.cap_in));
+        const float s = z[r], twice = s * P.cap_in, part = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(twice));
         th[r] = fmaf(-2.0f, part, 1.0f);
         z[r] = fmaf(-2.0f * P.cap_out, part, P.cap_out);
+        if constexpr (CAP == CAP_ANY) {
+          const float u = twice * 0.34657359f, w = u * u;  // (ln(2) / 2)
+          const float poly = fmaf(w, fmaf(w, fmaf(w, fmaf(w, 0.021869489f, -0.053968254f), 0.13333333f), -0.33333333f), 1.0f);
+          if (w < 0.0625f) {
+            th[r] = u * poly;
+            z[r] = s * P.scale_log2 * poly;
+          }
+        }
       }
       if constexpr (BIAS) z[r] = fmaf(-slope, fabsf(from - (float)((r >> 2) * 8 + (r & 3))), z[r]);
     }
@@ -519,7 +532,7 @@ __device__ __forceinline__ void attn_walk_plain(AttnWalk<KEYS>& walk, F& f) {
 // TFLOP/s; the matrix cores are busy for 47 % of it, at 1.9 GHz (16 heads without
 // others, no mask: 157 us, 875 TFLOP/s; 8 heads, a workgroup to a CU: 104 us, what
 // a workgroup's 128 blocks take one after the other).
-template <class T, int HD, bool CAP, bool BIAS>
+template <class T, int HD, int CAP, bool BIAS>
 struct AttnForward {
   using Frag = typename Traits<T>::Frag;
   static constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32, kHalf = kTile / 2;
@@ -622,7 +635,7 @@ struct AttnForward {
   }
 };
 
-template <class T, int HD, bool CAP, bool BIAS>
+template <class T, int HD, int CAP, bool BIAS>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
   constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32;
   __shared__ __attribute__((aligned(1024))) char lds[5 * kTile];
@@ -676,7 +689,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
 // Also delta = sum(do o) of each query, which the next kernel reads.  2 x 4096 rows
 // of 32 heads (8) of 128 in bf16, causal: 412 GFLOP in 408 us, 1010 TFLOP/s,
 // the matrix cores busy for 56 % of it at 1.8 GHz.
-template <class T, int HD, bool CAP, bool BIAS, bool FINE>
+template <class T, int HD, int CAP, bool BIAS, bool FINE>
 struct AttnGradQ {
   using Frag = typename Traits<T>::Frag;
   static constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32, kHalf = kTile / 2;
@@ -767,7 +780,7 @@ struct AttnGradQ {
   }
 };
 
-template <class T, int HD, bool CAP, bool BIAS, bool FINE>
+template <class T, int HD, int CAP, bool BIAS, bool FINE>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P) {
   constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32;
   __shared__ __attribute__((aligned(1024))) char lds[4 * kTile];
@@ -865,7 +878,7 @@ struct AttnKeys {  // of a workgroup: batch, key head, first row, the heads it t
 // 2 x 4096 rows of 32 heads (8) of 128 in bf16, causal: 550 GFLOP in 640 us, 860
 // TFLOP/s; the matrix cores are busy for 46 % of it, at 1.9 GHz, LDS for 37 %, and a
 // phase waits for its two halves in turn.
-template <class T, int HD, bool CAP, bool BIAS>
+template <class T, int HD, int CAP, bool BIAS>
 struct AttnGradKV {
   using Frag = typename Traits<T>::Frag;
   static constexpr int kTile = kAttnTile * kAttnLd<HD> * 2, kBlocks = HD / 32, kHalf = kTile / 2;
@@ -1037,7 +1050,7 @@ struct AttnGradKV {
   }
 };
 
-template <class T, int HD, bool CAP, bool BIAS>
+template <class T, int HD, int CAP, bool BIAS>
 __global__ __launch_bounds__(512, 2) void k_attn_dkv(AttnParams P) {
   using F = AttnGradKV<T, HD, CAP, BIAS>;
   constexpr int kBlocks = HD / 32;
@@ -1102,7 +1115,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_dkv(AttnParams P) {
 // instead of 202, 64 heads: 594 instead of 788).  96 columns would not fit: 23
 // registers in scratch, and 202 us instead of 141 for 8 heads of 80, 1036 instead of
 // 1072 for 64.
-template <class T, bool CAP, bool BIAS, bool FINE>
+template <class T, int CAP, bool BIAS, bool FINE>
 struct AttnGradBoth {
   static constexpr int HD = 64;
   using Frag = typename Traits<T>::Frag;
@@ -1194,7 +1207,7 @@ struct AttnGradBoth {
   }
 };
 
-template <class T, bool CAP, bool BIAS, bool FINE>
+template <class T, int CAP, bool BIAS, bool FINE>
 __global__ __launch_bounds__(256, 2) void k_attn_dkv_one(AttnParams P) {
   using F = AttnGradBoth<T, CAP, BIAS, FINE>;
   constexpr int HD = F::HD, kBlocks = F::kBlocks;
@@ -1247,7 +1260,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_dkv_one(AttnParams P) {
 }
 
 // ------------------------------------------------------------- launches
-template <class T, int HD, bool CAP, bool BIAS>
+template <class T, int HD, int CAP, bool BIAS>
 static hipError_t attn_go(AttnParams P, AttnPass pass, hipStream_t s) {
   P.tiles = (int)((P.S + kAttnRows - 1) / kAttnRows);
   const dim3 grid((unsigned)(P.tiles * P.B * (pass == ATTN_DKV ? P.KV * P.parts : P.H)));
@@ -1267,11 +1280,17 @@ static hipError_t attn_go(AttnParams P, AttnPass pass, hipStream_t s) {
   }
   return hipGetLastError();
 }
+template <class T, int HD, int CAP>
+static hipError_t attn_bias(const AttnParams& P, AttnPass pass, hipStream_t s) {
+  return P.slopes ? attn_go<T, HD, CAP, true>(P, pass, s) : attn_go<T, HD, CAP, false>(P, pass, s);
+}
 template <class T, int HD>
 hipError_t launch_attn(const AttnParams& P, AttnPass pass, hipStream_t s) {
-  const bool bias = P.slopes != nullptr;
-  if (P.cap_out > 0.0f) return bias ? attn_go<T, HD, true, true>(P, pass, s) : attn_go<T, HD, true, false>(P, pass, s);
-  return bias ? attn_go<T, HD, false, true>(P, pass, s) : attn_go<T, HD, false, false>(P, pass, s);
+  switch (P.cap) {
+    case CAP_NONE: return attn_bias<T, HD, CAP_NONE>(P, pass, s);
+    case CAP_SMALL: return attn_bias<T, HD, CAP_SMALL>(P, pass, s);
+    default: return attn_bias<T, HD, CAP_ANY>(P, pass, s);
+  }
 }
 
 }  // namespace orda

@@ -172,6 +172,10 @@ size_t attention_bytes(const orda_attention_t* p) {
   return delta_bytes(p) + (parts > 1 ? (size_t)2 * parts * p->batch * p->length * p->kv_heads * p->head_dim * 4 : 0) + 256;
 }
 
+// Caps up to which the shorter tanh serves (attn.hpp, scores: its error grows with
+// the cap; 2e-5 here, the other's time is 1.4 to 1.7 times as long).
+constexpr double kSmallCap = 128.0;
+
 AttnParams attn_params(const orda_attention_t* p, const void* q, const void* k, const void* v, const float* slopes, const int32_t* prefix) {
   AttnParams a{};
   a.q = q;
@@ -213,9 +217,13 @@ AttnParams attn_params(const orda_attention_t* p, const void* q, const void* k, 
   a.scale = (float)p->scale;
   a.scale_log2 = (float)(size * log2e);
   a.slope_mul = (float)(p->softcap > 0.0 ? log2e : 1.0 / size);
+  a.cap = CAP_NONE;
   if (p->softcap > 0.0) {
-    a.cap_in = (float)(2.0 * log2e * size / p->softcap);
-    a.cap_out = (float)(p->softcap * log2e);
+    // (a cap below 1e-24 leaves scores of 0 and one past 1e30 the scores as they are, in fp32)
+    const double cap = std::fmin(std::fmax(p->softcap, 1e-24), 1e30);
+    a.cap = cap <= kSmallCap ? CAP_SMALL : CAP_ANY;
+    a.cap_in = (float)std::fmin(2.0 * log2e * size / cap, 3e38);
+    a.cap_out = (float)(cap * log2e);
   }
   return a;
 }

@@ -98,12 +98,14 @@ struct AttnParams {
   int64_t qb, qs, qh, kb, ks, kh, vb, vs, vh, gb, gs, gh;
   float* partial;         // dk and dv of each part, [2][parts][B S KV D], or null (one part)
   int B, H, KV, group, D, causal, tiles;
+  int cap;                  // AttnCap
   int fine;                 // dz goes into its products in two halves
   int parts, share;         // workgroups that take the heads of a tile of keys, heads of each
   float scale, scale_log2;  // scale_log2 = |scale| log2(e)
   float slope_mul;          // 1 / |scale|, with a cap log2(e)
-  float cap_in, cap_out;    // 2 |scale| log2(e) / cap and cap log2(e); 0: no cap
+  float cap_in, cap_out;    // 2 |scale| log2(e) / cap and cap log2(e)
 };
+enum AttnCap { CAP_NONE, CAP_SMALL, CAP_ANY };  // (attn.hpp: scores)
 enum AttnPass { ATTN_FORWARD, ATTN_DQ, ATTN_DKV };
 template <class T, int HD> hipError_t launch_attn(const AttnParams& P, AttnPass pass, hipStream_t s);
 hipError_t launch_attn_join(const AttnParams& P, int dtype, hipStream_t s);

@@ -107,6 +107,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causa
         raise ValueError(f"{entry}: scale must be finite, got {scale}")
     if not (softcap >= 0.0 and math.isfinite(softcap)):
         raise ValueError(f"{entry}: softcap must be finite and >= 0, got {softcap}")
+    if softcap:  # (a cap below the one leaves scores of 0 and one past the other the scores as they are, in fp32)
+        softcap = min(max(softcap, 1e-24), 1e30)
     kernels = use_kernels(backend, q, entry)
     dtype = default_compute_dtype(q, k, v)
     slopes = None if slopes is None else slopes.detach().float().contiguous()

@@ -154,8 +154,10 @@ def seen(B, S, causal=True, documents=None, prefix=None):
     return m
 
 
-def attention64(dtype, q, k, v, causal=True, scale=None, softcap=0.0, slopes=None, documents=None, prefix=None, dy=None):
-    """{name: (value, bound)} of (B, S, H, D) tensors; all float64."""
+def attention64(dtype, q, k, v, causal=True, scale=None, softcap=0.0, slopes=None, documents=None, prefix=None, dy=None,
+                cap_error=None):
+    """{name: (value, bound)} of (B, S, H, D) tensors; all float64.  cap_error: what a capped score may be off, of itself
+    (default: 4e-7 of the cap)."""
     unit = Unit(dtype)
     B, S, H, D = q.shape
     G = H // k.shape[2]
@@ -177,7 +179,7 @@ def attention64(dtype, q, k, v, causal=True, scale=None, softcap=0.0, slopes=Non
     if softcap:
         t = torch.tanh(raw / softcap)
         z = softcap * t
-        e_z = e_z + 4e-7 * softcap
+        e_z = e_z + (4e-7 * softcap if cap_error is None else cap_error * z.abs())
     e_t = e_z / softcap if softcap else 0.0 * e_z
     if slopes is not None:
         i = torch.arange(S, dtype=torch.float64)

@@ -37,3 +37,14 @@ def test_padding_of_the_gradient_from_above_may_hold_anything(kw, bad):
     assert not y[docs < 0].any()
     for a, b in zip(got, want):
         assert torch.equal(a, b) and torch.isfinite(a).all() and not a[docs < 0].any()
+
+
+def test_caps_past_the_range_of_fp32():
+    """A cap that no score reaches leaves the scores, one below all of them nothing of them; in between it is the formula."""
+    g = torch.Generator().manual_seed(5)
+    q, k, v = (torch.randn(1, 9, 2, 4, generator=g).requires_grad_(True) for _ in range(3))
+    none, mean = orda.masked_attention(q, k, v), orda.masked_attention(q, k, v, scale=0.0)
+    for cap, want in ((1e39, none), (1e300, none), (1e30, none), (1e-300, mean), (1e-46, mean), (1e-30, mean)):
+        y = orda.masked_attention(q, k, v, softcap=cap)
+        assert torch.allclose(y, want, rtol=1e-6, atol=1e-6)
+        assert all(torch.isfinite(a).all() for a in torch.autograd.grad(y.sum(), (q, k, v)))
