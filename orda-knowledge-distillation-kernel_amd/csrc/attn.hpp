@@ -169,16 +169,16 @@ struct AttnFrags {
   }
 };
 
-// acc^T as it is, to a row of fp32.
+// acc^T times `mul`, to a row of fp32.
 template <int HD>
-__device__ __forceinline__ void store_part(const f32x16 (&acc)[HD / 32], float* p, int D, bool live) {
+__device__ __forceinline__ void store_part(const f32x16 (&acc)[HD / 32], float mul, float* p, int D, bool live) {
   const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int col = 32 * d + 8 * g + 4 * h;
-      if (live && col < D) *reinterpret_cast<f4v*>(p + col) = f4v{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+      if (live && col < D) *reinterpret_cast<f4v*>(p + col) = f4v{acc[d][4 * g] * mul, acc[d][4 * g + 1] * mul, acc[d][4 * g + 2] * mul, acc[d][4 * g + 3] * mul};
     }
 }
 
@@ -239,6 +239,45 @@ __device__ __forceinline__ void rest_operand(const float (&x)[16], const typenam
 #pragma unroll
   for (int i = 0; i < 16; ++i) y[i] = x[i] - to_f32(f[i >> 3][i & 7]);
   as_operand<T>(y, rest);
+}
+
+// fp16 operands.  Below 2^-14 fp16 has steps of 2^-24, and probabilities of long
+// rows and what small gradients from above make of them lie there: dz of 4096
+// keys with gradients of 1e-4 put dq off by 5 % of its norm.  Operands are lifted
+// by powers of two, which the results take out in fp32.  (bf16 has fp32's range.)
+// Forward: P, up to 2^8 of the running maximum's, by 2^7.  Backward: P, up to 1
+// (by the rounding of L at scores of 1e5 a little more), by 2^10, within L.  dz
+// has no bound that is known beforehand: it starts at another 2^30, and where the
+// lane's row (a query of dq, a key of dk) passes 2^15 goes down to 2^8, with its sum
+// so far.  (dq and dk in fp16 take up to 8 % longer for it: 3 x 1777 rows of 12 heads
+// of 80 with a cap 81 -> 85 and 120 -> 126 us, 2 x 4096 of 32 heads of 128 436 and 688
+// -> 718.)
+template <class T>
+constexpr bool kNarrow = std::is_same_v<T, f16>;
+template <class T>
+constexpr float kLiftForward = kNarrow<T> ? 7.0f : 0.0f;
+template <class T>
+constexpr float kLiftBackward = kNarrow<T> ? 10.0f : 0.0f;
+template <class T>
+constexpr float kLiftScores = kNarrow<T> ? 30.0f : 0.0f;
+// The exponent that dz of the lane's row goes down by, 0 nearly always.
+template <int N>
+__device__ __forceinline__ int keep_in_range(float (&z)[16], f32x16 (&acc)[N]) {
+  constexpr float kTop = 32768.0f;
+  float top = fabsf(z[0]);
+#pragma unroll
+  for (int r = 1; r < 16; ++r) top = fmaxf(top, fabsf(z[r]));
+  if (!__any(top > kTop)) return 0;
+  top = halves_max(top);
+  const int down = top > kTop && top < kInf ? __builtin_amdgcn_frexp_expf(top) - 8 : 0;
+  const float by = __builtin_amdgcn_ldexpf(1.0f, -down);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] *= by;
+#pragma unroll
+  for (int d = 0; d < N; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[d][r] *= by;
+  return down;
 }
 
 // acc^T (columns d, the lane's row) times `mul` to the lane's row at p: lanes l
@@ -575,6 +614,8 @@ struct AttnForward {
     fetch<BLOCK>(two);
     products<BLOCK>();
   }
+  // what the exponents of 2 have beside x mul
+  __device__ __forceinline__ float offset(float mul) const { return kNarrow<T> ? fmaf(-m, mul, kLiftForward<T>) : -m * mul; }
   template <int BLOCK>
   __device__ __forceinline__ void work(const AttnTile& t, int three, int two) {
     const int at = t.first + 32 * BLOCK;
@@ -606,7 +647,7 @@ struct AttnForward {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= by;
     }
-    const float off = m == -kInf ? 0.0f : -m * mul;
+    const float off = m == -kInf ? 0.0f : offset(mul);
     products<1 - BLOCK>();
     float p[16], sum[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -673,9 +714,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
   const float l = halves_sum(f.l);
   // (one key alone: its 2^(m mul - m mul) is 1 but for the rounding of one of the
   // two products; o is divided by what it was multiplied by, so that it is v)
-  const float one = __builtin_amdgcn_exp2f(fmaf(f.m, mul, -f.m * mul)), sum = l == one ? to_f32(from_f32<T>(one)) : l;
+  const float one = __builtin_amdgcn_exp2f(fmaf(f.m, mul, f.offset(mul))), sum = l == one ? to_f32(from_f32<T>(one)) : l;
   const bool empty = !(l > 0.0f) && l == l;
-  if (P.lse && lane < 32) P.lse[(int64_t)bh * P.padded + f.i] = f.i >= S || empty ? kInf : f.m * mul + __builtin_amdgcn_logf(l);
+  if (P.lse && lane < 32) P.lse[(int64_t)bh * P.padded + f.i] = f.i >= S || empty ? kInf : f.m * mul + (__builtin_amdgcn_logf(l) - (kLiftForward<T> + kLiftBackward<T>));
   const int64_t at = (((int64_t)b * S + f.i) * P.H + head) * P.D;
   const float inv = empty ? 0.0f : 1.0f / sum;
   store_own<T, HD>(f.o, inv, static_cast<T*>(P.o) + at, P.D, f.i < S);
@@ -703,6 +744,7 @@ struct AttnGradQ {
   Frag q[HD / 16], g[HD / 16];
   f32x16 dq[kBlocks];
   float lse, delta, slope;
+  float lift;  // exponent, of dz beside P's
   int row0, i, bound, doc;
   __device__ __forceinline__ AttnGradQ(const AttnParams& p) : P(p) {}
   __device__ __forceinline__ void issue(const AttnTile& t, int slot) {
@@ -749,8 +791,9 @@ struct AttnGradQ {
     if constexpr (kBeside) second();
     const float mul = CAP ? 1.0f : P.scale_log2;
     float z[16];
+    const float off = kNarrow<T> ? lift - lse : -lse;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(x[r], mul, -lse));
+    for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(x[r], mul, off));
     if constexpr (kBeside)
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks) {
@@ -762,6 +805,7 @@ struct AttnGradQ {
       z[r] *= dp[r] - delta;
       if constexpr (CAP) z[r] *= 1.0f - th[r] * th[r];
     }
+    if constexpr (kNarrow<T>) lift -= (float)keep_in_range(z, dq);
     Frag zf[2], kf[2][kBlocks];
     as_operand<T>(z, zf);  // (dz in 16 bits, as an operand of the product)
     fr.cols(lds_at(klds) + (uint32_t)(slot * kTile + BLOCK * kHalf), kf);
@@ -823,6 +867,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P)
   }
   if (!P.dq) return;
   f.lse = P.lse[(int64_t)bh * P.padded + f.i];
+  f.lift = kLiftScores<T>;
   AttnWalk<true> walk;
   walk.init(P, b, q0);
   f.bound = P.causal ? min(S, max(f.i + 1, walk.prefix)) : S;
@@ -841,7 +886,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P)
 #pragma unroll
       for (int r = 0; r < 16; ++r) f.dq[d][r] = 0.0f;
   T* out = static_cast<T*>(P.dq) + (((int64_t)b * S + f.i) * P.H + head) * P.D;
-  store_own<T, HD>(f.dq, P.scale, out, P.D, f.i < S);
+  const float unlift = kNarrow<T> ? __builtin_amdgcn_exp2f(-f.lift - kLiftBackward<T>) : 1.0f;
+  store_own<T, HD>(f.dq, P.scale * unlift, out, P.D, f.i < S);
 }
 
 // ------------------------------------------------------------- dk and dv
@@ -900,6 +946,7 @@ struct AttnGradKV {
   f32x16 x;                              // first: S of the next phase's block
   Frag rows[HD / 16], cf[2][kBlocks];    // second: operands of the next phase
   Frag zf[2];                            // second: dz of the last phase's block
+  float lift;                            // second: of dz beside P's
   int row0, key, bound, doc;
   __device__ __forceinline__ AttnGradKV(const AttnParams& p) : P(p) {}
   __device__ __forceinline__ void issue(const AttnTile& t, int slot) {
@@ -989,7 +1036,11 @@ struct AttnGradKV {
       }
       product(dp);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) z[r] = p[r >> 2][r & 3] * (dp[r] - dl[r >> 2][r & 3]);
+      for (int r = 0; r < 16; ++r) {
+        z[r] = p[r >> 2][r & 3] * (dp[r] - dl[r >> 2][r & 3]);
+        if constexpr (kNarrow<T>) z[r] *= lift;
+      }
+      if constexpr (kNarrow<T>) lift = __builtin_amdgcn_ldexpf(lift, -keep_in_range(z, acc));
       as_operand<T>(z, zf);
     }
     if (more) fetch(grows(to, BLOCK));
@@ -1054,6 +1105,7 @@ template <class T, int HD, int CAP, bool BIAS>
 __global__ __launch_bounds__(512, 2) void k_attn_dkv(AttnParams P) {
   using F = AttnGradKV<T, HD, CAP, BIAS>;
   constexpr int kBlocks = HD / 32;
+  constexpr float kUnlift = kNarrow<T> ? 1.0f / 1024.0f : 1.0f;  // 2^-kLiftBackward
   __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
   const AttnKeys at(P, blockIdx.x);
   const int b = at.b, kv = at.kv, r0 = at.r0, head = at.head;
@@ -1083,10 +1135,11 @@ __global__ __launch_bounds__(512, 2) void k_attn_dkv(AttnParams P) {
   for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) f.acc[d][r] = 0.0f;
+  f.lift = __builtin_amdgcn_exp2f(kLiftScores<T>);
   AttnWalk<false> walk;
   walk.init(P, b, r0, at.heads);
   // (zeros for a padding row: what it holds may not be finite)
-  auto finish = [&](T* out, int which, float mul) {
+  auto finish = [&](T* out, int which, float mul, float unlift) {
     if (f.doc < 0)
 #pragma unroll
       for (int d = 0; d < kBlocks; ++d)
@@ -1096,17 +1149,17 @@ __global__ __launch_bounds__(512, 2) void k_attn_dkv(AttnParams P) {
     asm volatile("" : "+s"(id));  // (where the sums go is worked out again: the loop has no registers for it)
     const AttnKeys to(P, id);
     const int64_t row = to.row(P, f.key);
-    if (P.partial) store_part<HD>(f.acc, to.partial(P, which) + row, P.D, f.key < P.S);
-    else if (out) store_own<T, HD>(f.acc, mul, out + row, P.D, f.key < P.S);
+    if (P.partial) store_part<HD>(f.acc, unlift, to.partial(P, which) + row, P.D, f.key < P.S);
+    else if (out) store_own<T, HD>(f.acc, mul * unlift, out + row, P.D, f.key < P.S);
   };
   if (leads) {
     own_rows<T, HD>(static_cast<const T*>(P.k) + b * P.kb + kv * P.kh, P.ks, f.row0, S, P.D, f.own, P.scale < 0.0f);
     f.template walk<true>(walk);
-    finish(static_cast<T*>(P.dv), 1, 1.0f);
+    finish(static_cast<T*>(P.dv), 1, 1.0f, kUnlift);
   } else {
     own_rows<T, HD>(static_cast<const T*>(P.v) + b * P.vb + kv * P.vh, P.vs, f.row0, S, P.D, f.own);
     f.template walk<false>(walk);
-    finish(static_cast<T*>(P.dk), 0, P.scale);
+    finish(static_cast<T*>(P.dk), 0, P.scale, kUnlift / f.lift);
   }
 }
 
@@ -1132,6 +1185,7 @@ struct AttnGradBoth {
   AttnFrags<T, HD> fr;
   Frag k[HD / 16], v[HD / 16];
   f32x16 dk[kBlocks], dv[kBlocks];
+  float lift;  // of dz beside P's
   int row0, key, bound, doc;
   __device__ __forceinline__ AttnGradBoth(const AttnParams& p) : P(p) {}
   __device__ __forceinline__ void issue(const AttnTile& t, int slot) {
@@ -1190,7 +1244,11 @@ struct AttnGradBoth {
       for (int d = 0; d < kBlocks; ++d) dv[d] = Traits<T>::mma(cf[j][d], f[j], dv[d]);
     fr.cols(lds_at(qt), cf);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) p[r] *= dp[r] - stat[r >> 2][r & 3];
+    for (int r = 0; r < 16; ++r) {
+      p[r] *= dp[r] - stat[r >> 2][r & 3];
+      if constexpr (kNarrow<T>) p[r] *= lift;
+    }
+    if constexpr (kNarrow<T>) lift = __builtin_amdgcn_ldexpf(lift, -keep_in_range(p, dk));
     as_operand<T>(p, f);
     if constexpr (FINE) {
       Frag rest[2];
@@ -1211,6 +1269,7 @@ template <class T, int CAP, bool BIAS, bool FINE>
 __global__ __launch_bounds__(256, 2) void k_attn_dkv_one(AttnParams P) {
   using F = AttnGradBoth<T, CAP, BIAS, FINE>;
   constexpr int HD = F::HD, kBlocks = F::kBlocks;
+  constexpr float kUnlift = kNarrow<T> ? 1.0f / 1024.0f : 1.0f;  // 2^-kLiftBackward
   __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
   const AttnKeys at(P, blockIdx.x);
   const int b = at.b, kv = at.kv, r0 = at.r0, head = at.head;
@@ -1240,6 +1299,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_dkv_one(AttnParams P) {
     for (int r = 0; r < 16; ++r) f.dk[d][r] = f.dv[d][r] = 0.0f;
   own_rows<T, HD>(static_cast<const T*>(P.k) + b * P.kb + kv * P.kh, P.ks, f.row0, S, P.D, f.k, P.scale < 0.0f);
   own_rows<T, HD>(static_cast<const T*>(P.v) + b * P.vb + kv * P.vh, P.vs, f.row0, S, P.D, f.v);
+  f.lift = __builtin_amdgcn_exp2f(kLiftScores<T>);
   AttnWalk<false> walk;
   walk.init(P, b, r0, at.heads);
   attn_walk_plain(walk, f);
@@ -1251,12 +1311,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_dkv_one(AttnParams P) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) f.dk[d][r] = f.dv[d][r] = 0.0f;
   if (P.partial) {
-    store_part<HD>(f.dk, at.partial(P, 0) + row, P.D, live);
-    store_part<HD>(f.dv, at.partial(P, 1) + row, P.D, live);
+    store_part<HD>(f.dk, kUnlift / f.lift, at.partial(P, 0) + row, P.D, live);
+    store_part<HD>(f.dv, kUnlift, at.partial(P, 1) + row, P.D, live);
     return;
   }
-  if (P.dk) store_own<T, HD>(f.dk, P.scale, static_cast<T*>(P.dk) + row, P.D, live);
-  if (P.dv) store_own<T, HD>(f.dv, 1.0f, static_cast<T*>(P.dv) + row, P.D, live);
+  if (P.dk) store_own<T, HD>(f.dk, P.scale * (kUnlift / f.lift), static_cast<T*>(P.dk) + row, P.D, live);
+  if (P.dv) store_own<T, HD>(f.dv, kUnlift, static_cast<T*>(P.dv) + row, P.D, live);
 }
 
 // ------------------------------------------------------------- launches
