@@ -458,7 +458,7 @@ __device__ __forceinline__ void hide(f32x16& z, int bound, const int* docs, cons
 // Scores from products s = q.k.  Without a cap in units of the products, s - slope
 // / |scale| |i - j|, and what uses them multiplies by mul = |scale| log2(e); with
 // one in units of log2 (mul = 1), log2(e) (cap tanh(scale s / cap) - slope |i - j|),
-// and also the tanh.  slope: times P.slope_mul.  dist: the lane's row less the block's
+// and also the tanh.  slope: slope_of's.  dist: the lane's row less the block's
 // first.  (A negative scale is turned over to one of the operands.)
 //
 // tanh u = 1 - 2 / (1 + e^2u) on the hardware's exp2 and reciprocal is off by 2e-7
@@ -468,6 +468,14 @@ __device__ __forceinline__ void hide(f32x16& z, int bound, const int* docs, cons
 // of it, so that the capped score is off by at most 2^-18 of itself at any cap.
 // (3 x 1777 rows of 12 heads of 80, forward, dq, dk and dv: 67, 82 and 122 us with
 // CAP_SMALL, 100, 119 and 171 with CAP_ANY.)
+// A slope is taken for what keeps a whole sequence's distance from it below 2^30 in
+// log2 (2^24 positions: 64 each), so that no exponent passes fp32's range, and a
+// negative one, whose far keys have the largest scores, below 2^22, where fp32 holds
+// a score to a quarter.
+__device__ __forceinline__ float slope_of(const AttnParams& P, float given) {
+  const float s = given * P.slope_mul;
+  return s > P.slope_high ? P.slope_high : s < P.slope_low ? P.slope_low : s;
+}
 template <int CAP, bool BIAS>
 __device__ __forceinline__ void scores(f32x16& z, float (&th)[16], const AttnParams& P, float slope, int dist) {
   if constexpr (CAP || BIAS) {
@@ -586,6 +594,7 @@ struct AttnForward {
   f32x16 o[kBlocks];
   f32x16 s[2];
   float m, l, slope;
+  float bar;  // (the score from which the maximum follows)
   int row0, i, bound, doc;
   __device__ __forceinline__ AttnForward(const AttnParams& p) : P(p) {}
   __device__ __forceinline__ void issue(const AttnTile& t, int two, int three) {
@@ -636,10 +645,16 @@ struct AttnForward {
     for (int r = 2; r < 16; ++r) top = fmaxf(top, x[r]);
     top = halves_max(top);
     const float mul = CAP ? 1.0f : P.scale_log2;
-    // The maximum follows only where it grows by more than 2^8: sums and products
-    // of probabilities up to 2^8 lose nothing in fp32.
-    if (__any(top * mul > m * mul + 8.0f)) {
-      const float to = fmaxf(m, top), by = to == -kInf ? 1.0f : __builtin_amdgcn_exp2f((m - to) * mul);
+    // The maximum follows only where it grows by more than 2^8: sums and products of
+    // probabilities up to 2^8 lose nothing in fp32.  Past 2^20 (far keys behind a steep
+    // slope) fp32 holds no eighth of a score, and the maximum's own exponent is the
+    // rounding of m mul: in fp16 it follows there wherever it grows, and is taken for 2
+    // to 4 steps more, so that no probability passes the type's largest value.
+    if (__any(top > bar)) {
+      const bool more = top > bar, far = kNarrow<T> && fabsf(top * mul) > 0x1p20f;
+      const float to = more ? (far ? fmaf(fabsf(top), 0x1p-22f, top) : top) : m;
+      const float by = more ? __builtin_amdgcn_exp2f((m - to) * mul) : 1.0f;
+      bar = more ? (far ? top : fmaf(8.0f, __builtin_amdgcn_rcpf(mul), top)) : bar;
       m = to;
       l *= by;
 #pragma unroll
@@ -692,7 +707,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
   f.i = f.row0 + (lane & 31);
   f.K = static_cast<const T*>(P.k) + b * P.kb + kv * P.kh;
   f.V = static_cast<const T*>(P.v) + b * P.vb + kv * P.vh;
-  f.slope = BIAS ? P.slopes[head] * P.slope_mul : 0.0f;
+  f.slope = BIAS ? slope_of(P, P.slopes[head]) : 0.0f;
   f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
   f.ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / 32) : nullptr;
   f.doc = P.docs ? f.docs[f.i] : 0;
@@ -707,16 +722,17 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
   for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) f.o[d][r] = 0.0f;
-  f.m = -kInf;
+  f.m = f.bar = -kInf;
   f.l = 0.0f;
   attn_walk(walk, f);
   const float mul = CAP ? 1.0f : P.scale_log2;
   const float l = halves_sum(f.l);
   // (one key alone: its 2^(m mul - m mul) is 1 but for the rounding of one of the
-  // two products; o is divided by what it was multiplied by, so that it is v)
-  const float one = __builtin_amdgcn_exp2f(fmaf(f.m, mul, f.offset(mul))), sum = l == one ? to_f32(from_f32<T>(one)) : l;
+  // two products; o is divided by what it was multiplied by, so that it is v.  The
+  // smaller of m and bar is the maximum itself)
+  const float off = f.offset(mul), one = __builtin_amdgcn_exp2f(fmaf(fminf(f.m, f.bar), mul, off)), sum = l == one ? to_f32(from_f32<T>(one)) : l;
   const bool empty = !(l > 0.0f) && l == l;
-  if (P.lse && lane < 32) P.lse[(int64_t)bh * P.padded + f.i] = f.i >= S || empty ? kInf : f.m * mul + (__builtin_amdgcn_logf(l) - (kLiftForward<T> + kLiftBackward<T>));
+  if (P.lse && lane < 32) P.lse[(int64_t)bh * P.padded + f.i] = f.i >= S || empty ? kInf : __builtin_amdgcn_logf(l) - kLiftBackward<T> - off;
   const int64_t at = (((int64_t)b * S + f.i) * P.H + head) * P.D;
   const float inv = empty ? 0.0f : 1.0f / sum;
   store_own<T, HD>(f.o, inv, static_cast<T*>(P.o) + at, P.D, f.i < S);
@@ -840,7 +856,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn_dq(AttnParams P)
   f.i = f.row0 + (lane & 31);
   f.K = static_cast<const T*>(P.k) + b * P.kb + kv * P.kh;
   f.V = static_cast<const T*>(P.v) + b * P.vb + kv * P.vh;
-  f.slope = BIAS ? P.slopes[head] * P.slope_mul : 0.0f;
+  f.slope = BIAS ? slope_of(P, P.slopes[head]) : 0.0f;
   f.docs = P.docs ? P.docs + (int64_t)b * P.padded : nullptr;
   f.ranges = P.docs ? P.ranges + (int64_t)b * (P.padded / 32) : nullptr;
   f.doc = P.docs ? f.docs[f.i] : 0;
@@ -996,7 +1012,7 @@ struct AttnGradKV {
       for (int g = 0; g < 4; ++g) L[g] = *reinterpret_cast<const f4v*>(stat(slot, BLOCK, 0) + 32 * g);
       fr.cols(lds_at(grows(slot, BLOCK)), cf);
       float th[16], p[16];
-      scores<CAP, BIAS>(x, th, P, BIAS ? slopes[t.head] * P.slope_mul : 0.0f, key - at);
+      scores<CAP, BIAS>(x, th, P, BIAS ? slope_of(P, slopes[t.head]) : 0.0f, key - at);
       if (t.part(BLOCK)) hide<false>(x, bound, docs, ranges, at, doc);
       const float mul = CAP ? 1.0f : P.scale_log2;
 #pragma unroll
@@ -1225,7 +1241,7 @@ struct AttnGradBoth {
     fetch(gt, rows);
     fr.cols(lds_at(gt), cf);
     float th[16], p[16];
-    scores<CAP, BIAS>(x, th, P, BIAS ? slopes[t.head] * P.slope_mul : 0.0f, key - at);
+    scores<CAP, BIAS>(x, th, P, BIAS ? slope_of(P, slopes[t.head]) : 0.0f, key - at);
     if (t.part(BLOCK)) hide<false>(x, bound, docs, ranges, at, doc);
     const float mul = CAP ? 1.0f : P.scale_log2;
 #pragma unroll

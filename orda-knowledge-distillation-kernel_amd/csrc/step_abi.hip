@@ -217,6 +217,9 @@ AttnParams attn_params(const orda_attention_t* p, const void* q, const void* k, 
   a.scale = (float)p->scale;
   a.scale_log2 = (float)(size * log2e);
   a.slope_mul = (float)(p->softcap > 0.0 ? log2e : 1.0 / size);
+  const double far = p->length * (p->softcap > 0.0 ? 1.0 : size * log2e);
+  a.slope_low = (float)std::fmax(-0x1p22 / far, -1e30);
+  a.slope_high = (float)std::fmin(0x1p30 / far, 1e30);
   a.cap = CAP_NONE;
   if (p->softcap > 0.0) {
     // (a cap below 1e-24 leaves scores of 0 and one past 1e30 the scores as they are, in fp32)

@@ -103,6 +103,7 @@ struct AttnParams {
   int parts, share;         // workgroups that take the heads of a tile of keys, heads of each
   float scale, scale_log2;  // scale_log2 = |scale| log2(e)
   float slope_mul;          // 1 / |scale|, with a cap log2(e)
+  float slope_low, slope_high;  // what it is then taken for at least and at most
   float cap_in, cap_out;    // 2 |scale| log2(e) / cap and cap log2(e)
 };
 enum AttnCap { CAP_NONE, CAP_SMALL, CAP_ANY };  // (attn.hpp: scores)
