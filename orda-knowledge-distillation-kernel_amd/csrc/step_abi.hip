@@ -127,7 +127,7 @@ int check_attention(const char* what, const orda_attention_t* p) {
   if (p->head_dim < 8 || p->head_dim > 128 || p->head_dim % 8 != 0)
     return fail(ORDA_EINVAL, "%s: head_dim must be a multiple of 8 in [8, 128], got %d", what, p->head_dim);
   if (p->causal != 0 && p->causal != 1) return fail(ORDA_EINVAL, "%s: causal must be 0 or 1, got %d", what, p->causal);
-  if (!std::isfinite(p->scale)) return fail(ORDA_EINVAL, "%s: scale must be finite, got %g", what, p->scale);
+  if (!(std::fabs(p->scale) <= 1e38)) return fail(ORDA_EINVAL, "%s: scale must be finite in fp32, up to 1e38, got %g", what, p->scale);
   if (!(p->softcap >= 0.0) || !std::isfinite(p->softcap)) return fail(ORDA_EINVAL, "%s: softcap must be finite and >= 0, got %g", what, p->softcap);
   // (a launch has fewer than 2^32 threads, a tile 256 of them, of dk and dv 512)
   if (padded_length(p) / 128 * p->batch * std::max(p->heads, 2 * p->kv_heads) >= (1ll << 24))

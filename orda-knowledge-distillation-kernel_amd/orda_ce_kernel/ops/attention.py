@@ -103,8 +103,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causa
     prefix = _integers(entry, "prefix", prefix, (B,), q.device)
     scale = D ** -0.5 if scale is None else float(scale)
     softcap = float(softcap)
-    if not math.isfinite(scale):
-        raise ValueError(f"{entry}: scale must be finite, got {scale}")
+    if not abs(scale) <= 1e38:
+        raise ValueError(f"{entry}: scale must be finite in fp32, up to 1e38, got {scale}")
     if not (softcap >= 0.0 and math.isfinite(softcap)):
         raise ValueError(f"{entry}: softcap must be finite and >= 0, got {softcap}")
     if softcap:  # (a cap below the one leaves scores of 0 and one past the other the scores as they are, in fp32)

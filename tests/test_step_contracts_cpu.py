@@ -1,12 +1,14 @@
 """What the docstrings of a student's operators promise beside their formulas, on the CPU."""
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 import orda_ce_kernel as orda
+from orda_ce_kernel import _native
 
 
 @pytest.mark.parametrize("call", [lambda x: orda.counter_dropout(x, 0.5), lambda x: orda.layer_norm(x, x[0], None, x, p=0.5)[1]],
@@ -48,3 +50,17 @@ def test_caps_past_the_range_of_fp32():
         y = orda.masked_attention(q, k, v, softcap=cap)
         assert torch.allclose(y, want, rtol=1e-6, atol=1e-6)
         assert all(torch.isfinite(a).all() for a in torch.autograd.grad(y.sum(), (q, k, v)))
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e300, math.inf, math.nan])
+def test_scales_past_the_range_of_fp32_are_refused(scale):
+    """As infinities in fp32 they would leave NaN everywhere."""
+    q = torch.zeros(1, 3, 1, 8)
+    with pytest.raises(ValueError, match="scale must be finite in fp32"):
+        orda.masked_attention(q, q, q, scale=scale)
+    dense = (ctypes.c_int64 * 3)(24, 8, 8)
+    p = _native.Attention(abi_version=_native.ABI_VERSION, dtype=0, heads=1, kv_heads=1, head_dim=8, causal=1, batch=1, length=3, q_stride=dense,
+                          k_stride=dense, v_stride=dense, g_stride=dense, documents_stride=3, scale=scale, softcap=0.0)
+    lib = _native.library()
+    assert lib.orda_attention_workspace_bytes(ctypes.byref(p)) == 0 and "scale must be finite in fp32" in lib.orda_last_error().decode()
+    assert orda.masked_attention(q, q, q, scale=-1e38).isfinite().all()
