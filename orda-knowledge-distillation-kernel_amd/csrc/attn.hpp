@@ -645,13 +645,13 @@ struct AttnForward {
     for (int r = 2; r < 16; ++r) top = fmaxf(top, x[r]);
     top = halves_max(top);
     const float mul = CAP ? 1.0f : P.scale_log2;
-    // The maximum follows only where it grows by more than 2^8: sums and products of
+    // The wave's maxima follow only where one grows by more than 2^8: sums and products of
     // probabilities up to 2^8 lose nothing in fp32.  Past 2^20 (far keys behind a steep
     // slope) fp32 holds no eighth of a score, and the maximum's own exponent is the
     // rounding of m mul: in fp16 it follows there wherever it grows, and is taken for 2
     // to 4 steps more, so that no probability passes the type's largest value.
     if (__any(top > bar)) {
-      const bool more = top > bar, far = kNarrow<T> && fabsf(top * mul) > 0x1p20f;
+      const bool more = top > m, far = kNarrow<T> && fabsf(top * mul) > 0x1p20f;
       const float to = more ? (far ? fmaf(fabsf(top), 0x1p-22f, top) : top) : m;
       const float by = more ? __builtin_amdgcn_exp2f((m - to) * mul) : 1.0f;
       bar = more ? (far ? top : fmaf(8.0f, __builtin_amdgcn_rcpf(mul), top)) : bar;
@@ -1202,6 +1202,7 @@ struct AttnGradBoth {
   Frag k[HD / 16], v[HD / 16];
   f32x16 dk[kBlocks], dv[kBlocks];
   float lift;  // of dz beside P's
+  float slope;  // the tile's head's
   int row0, key, bound, doc;
   __device__ __forceinline__ AttnGradBoth(const AttnParams& p) : P(p) {}
   __device__ __forceinline__ void issue(const AttnTile& t, int slot) {
@@ -1214,6 +1215,7 @@ struct AttnGradBoth {
                                                (threadIdx.x & 63) * 4, 0, 0, 0);
   }
   __device__ __forceinline__ void ready(const AttnTile& t, int slot) {
+    if constexpr (BIAS) slope = slope_of(P, slopes[t.head]);
     if (t.pad()) clear_padding<kAttnLd<HD>>(docs + t.first, qlds + slot * kTile, glds + slot * kTile);
   }
   template <int BLOCK>
@@ -1241,7 +1243,7 @@ struct AttnGradBoth {
     fetch(gt, rows);
     fr.cols(lds_at(gt), cf);
     float th[16], p[16];
-    scores<CAP, BIAS>(x, th, P, BIAS ? slope_of(P, slopes[t.head]) : 0.0f, key - at);
+    scores<CAP, BIAS>(x, th, P, slope, key - at);
     if (t.part(BLOCK)) hide<false>(x, bound, docs, ranges, at, doc);
     const float mul = CAP ? 1.0f : P.scale_log2;
 #pragma unroll
