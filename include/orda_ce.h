@@ -571,6 +571,8 @@ int orda_layer_norm_backward(const orda_layer_norm_t* p, const orda_dropout_t* d
 
 /* Masked self-attention on (batch, length, heads, head_dim) tensors.
  *   z = scale q.k; with softcap > 0 softcap tanh(z / softcap); less slopes[h] |i - j|
+ * (fp32: caps outside [1e-24, 1e30] are taken for its ends, slopes for what keeps a
+ * sequence's scores below 2^30 in log2, negative ones below 2^22).
  * Query i sees key j if (not causal, or j <= i, or j < prefix[b]) and, with
  * documents, both have the same number, 0 or above.  A query that sees nothing
  * gives zeros and no gradient.  Query head h reads key and value head h /
@@ -582,11 +584,11 @@ typedef struct orda_attention {
   int32_t heads, kv_heads;
   int32_t head_dim;    /* a multiple of 8 up to 128                             */
   int32_t causal;
-  int64_t batch, length; /* length up to 2^24                                   */
+  int64_t batch, length; /* up to 65535 and 2^24                                */
   int64_t q_stride[3], k_stride[3], v_stride[3]; /* of batch, position, head    */
   int64_t g_stride[3]; /* of grad_output                                        */
   int64_t documents_stride; /* of the batch                                     */
-  double scale, softcap;
+  double scale, softcap; /* scale up to 1e38 either way                         */
 } orda_attention_t;
 /* What a call keeps for its backward pass (in `saved`; without one it needs
  * orda_attention_saved_bytes(p, with_documents, 0) of it as a workspace). */

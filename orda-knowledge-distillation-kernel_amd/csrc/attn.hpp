@@ -232,7 +232,8 @@ __device__ __forceinline__ void as_operand(const float (&x)[16], typename Traits
   }
 }
 
-// What x's rounding to f left, as operands of their own: FINE, for short sequences.
+// What x's rounding to f left, as operands of their own: FINE, for short sequences
+// (step_abi.hip, where `fine` is set, has both sides measured).
 template <class T>
 __device__ __forceinline__ void rest_operand(const float (&x)[16], const typename Traits<T>::Frag (&f)[2], typename Traits<T>::Frag (&rest)[2]) {
   float y[16];
@@ -737,8 +738,12 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_attn(AttnParams P) {
   const float inv = empty ? 0.0f : 1.0f / sum;
   store_own<T, HD>(f.o, inv, static_cast<T*>(P.o) + at, P.D, f.i < S);
   // dz = P (dP - delta) cancels where P is near 1, and delta = sum(do o) would be
-  // as far off as o's rounding: for the backward pass o is kept in both halves
-  // (8 short rows: dq and dk off by 2.5e-3 of their norm instead of 3.4e-3 in bf16).
+  // as far off as o's rounding: for the backward pass o is kept in both halves, at
+  // the price of a second tensor of its size, written here and read with dq (67 MB
+  // each for 2 x 4096 rows of 32 heads of 128).  dq in bf16 is off by, of its norm,
+  //   4096 rows, scores of order 1, 4, 16: 2.4e-3, 2.9e-3, 3.5e-3; without the lower
+  //   half 2.5e-3, 3.6e-3, 6.3e-3;  8 rows: 1.7e-3, 1.8e-3, 2.0e-3 for 2.1e-3, 5.4e-3,
+  //   3.8e-3  (fp16 alike: 4096 rows 3.0e-4, 3.5e-4, 4.4e-4 for 3.2e-4, 4.4e-4, 8.2e-4)
   if (P.o_low) store_own<T, HD, true>(f.o, inv, static_cast<T*>(P.o_low) + at, P.D, f.i < S);
 }
 

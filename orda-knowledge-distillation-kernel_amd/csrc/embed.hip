@@ -24,7 +24,9 @@
 // Memory bounds both passes.  16384 tokens over 128256 rows of 4096 in bf16: forward
 // 268 MB in 53 us; backward 1.3 GB in 241 us (sort 23 and merge 21, with 128 MB of
 // zeros each, sums and the other 750 MB of zeros 181, join 16), where a fill of all
-// rows first and the sums behind it took 277.
+// rows first and the sums behind it took 277.  Small batches are the sort's: 1999
+// tokens in one workgroup take 10 us over a gradient of 0.8 MB, 14 with 78 MB of zeros
+// beside it (11 at a fill's rate).
 #include <algorithm>
 
 #include "pieces.hpp"

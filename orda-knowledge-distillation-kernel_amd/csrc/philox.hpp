@@ -8,7 +8,9 @@
 // threshold = p in steps of 2^-16.  (32 bits an element would be two calls for 8
 // elements: 40 quarter-rate multiplications, 640 cycles of a wave for 512
 // elements, more than the 512 elements' bytes take in bf16.  16 bits make it
-// 320.)
+// 320.  In rows of odd lengths a piece of 8 starts inside a block, as 7 of 8 rows do
+// there, and takes two: 640 again.  1999 rows of 1111 in fp16 take a norm 10.3 us
+// forward and 15.1 backward, of 1112 8.1 and 12.1.)
 #pragma once
 #include "orda_core.hpp"
 

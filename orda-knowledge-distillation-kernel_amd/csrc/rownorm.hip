@@ -488,7 +488,13 @@ static int64_t threads_of(int64_t cols) { return cols <= 4096 ? 256 : 1024; }
 
 // Workgroups of a pass: at 16384 x 4096 any number from 256 to 1024 backward and
 // from 1024 to 16384 forward takes the same time (130 to 143 us, 92 to 96); fewer
-// backward are fewer sums to add up.
+// backward are fewer sums to add up.  Chosen at that width only; rows of more than
+// 4096 have 1024 threads and fewer workgroups, of which 5120 columns leave 6 waves of
+// 16 without a piece.  Forward and backward with dropout and residual in bf16:
+// 16384 x 5120 162 to 191 and 169 to 209 us (its bytes at 6.2 TB/s: 108 and 135), 8192 x
+// 8192 102 and 126 (87 and 108), 4096 x 16384, by the long kernels, 189 and 606 (87
+// and 108: rows are read three times forward and twice backward, and dw and db added
+// up in memory for every row, 4 bytes at a time).
 constexpr int64_t kGradGroups = 512, kNormGroups = 2048;
 int64_t layer_norm_groups(int64_t rows, int64_t cols) {
   const int64_t steps = (rows + rows_per_group(cols) - 1) / rows_per_group(cols);

@@ -200,11 +200,13 @@ AttnParams attn_params(const orda_attention_t* p, const void* q, const void* k, 
   a.H = p->heads;
   a.KV = p->kv_heads;
   a.group = p->heads / p->kv_heads;
-  // The rounding of dz does not average out over a few keys, and there is time for
-  // two products more: dq and dk of 8 rows in bf16 are off by 1.8e-3 of their norm
-  // instead of 2.5e-3, of 64 by 1.7e-3 instead of 2.4e-3 (1.7e-3 is their own
-  // rounding).  Over long sequences dq would take 200 us instead of 124 (8 heads of
-  // 128, 4096: the registers do not hold both).
+  // dz rounded to 16 bits as an operand leaves dq and dk in bf16 off by 2.4e-3 of their
+  // norm at any length (1.7e-3 are their own rounding), in two halves by 1.7e-3 to
+  // 1.8e-3.  The second halves' products cost 0.3 us of 6 to 9 while a call is one
+  // tile of keys, from there on 3 to 15 % of either kernel (16 x 256 rows, 8 heads of
+  // 64 and of 128), up to 19 to 28 % of dq and 12 to 21 % of dk and dv (8 heads of 128,
+  // 4096 rows: 106 -> 136 and 135 -> 155 us).  Documents packed into longer rows have
+  // the one operand, however short they are.
   a.fine = p->length <= 64;
   a.parts = parts_of(p).count;
   a.share = parts_of(p).share;

@@ -75,15 +75,20 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causa
     ``q`` is ``(batch, length, heads, head_dim)``, ``k`` and ``v`` ``(batch, length, kv_heads, head_dim)`` with ``heads`` a
     multiple of ``kv_heads`` (query head h reads head ``h // (heads // kv_heads)``); slices of one projection's output serve
     as they are.  The result is ``(batch, length, heads, head_dim)``.  ``scale`` (default ``head_dim ** -0.5``) multiplies the
-    products; ``softcap`` > 0 caps them to ``softcap * tanh(z / softcap)``; ``slopes`` (``(heads,)``) takes ``slopes[h] *
-    |i - j|`` off.  ``causal``: query i sees the keys up to i, and with ``prefix`` (``(batch,)``) also those below
+    products; ``softcap`` > 0 caps them to ``softcap * tanh(z / softcap)``, at any cap with the precision of the score;
+    ``slopes`` (``(heads,)``) takes ``slopes[h] * |i - j|`` off.  ``causal``: query i sees the keys up to i, and with ``prefix`` (``(batch,)``) also those below
     ``prefix[b]`` (without ``causal`` it sees them all).  ``documents`` (``(batch, length)``): only keys with the query's own
     number (int64 numbers past 2^31 - 1 count as that one); a negative number is padding, which sees nothing and is not
     seen, whatever it holds: zeros come out, and zero gradients.
 
-    On the kernels bf16 and fp16 with head_dim up to 128 (multiples of 8 are read in place, others are copied).  The compute
-    dtype is the loss's rule; fp32 tensors run on ``backend="torch"`` or under autocast.  Probabilities and their gradients
-    are rounded to the compute dtype as operands of products (the latter in two parts up to a length of 64); sums are fp32.
+    On the kernels bf16 and fp16 with head_dim up to 128 (multiples of 8 are read in place, others are copied) and batches
+    up to 65535.  The compute dtype is the loss's rule; fp32 tensors run on ``backend="torch"`` or under autocast.  Scores and
+    sums are fp32 (a score's size times 2^-24 is what its probability may be off in the backward pass).  Probabilities and
+    their gradients are rounded to the compute dtype as operands of products, in fp16 lifted so that small ones keep its 11
+    bits; the gradients in two parts up to a length of 64, beyond in one (documents of any length in longer rows too), which
+    leaves the gradients of q and k off by 2.4e-3 of their norm in bf16 instead of the 1.7e-3 of their own rounding, and by
+    3e-4 instead of 2e-4 in fp16.  A training call keeps q, k, v, the result, what its rounding left (a second tensor of its
+    size) and an fp32 number a query and head.
     A value that is not finite, in a row that a query does not see, may still reach it where a query of the same 128 (from
     the sequence's start) sees a row of the value's 64 (padding excepted).  Once differentiable, in q, k and v.
     ``backend`` as :func:`distillation_loss` has it."""
